@@ -220,6 +220,104 @@ int pf_scan_exec(const void* w, const void* u, const void* k, const float* decay
                  const float* h0, void* h_out, float* final_state, int B, int H, int nc, int C,
                  int D, int dtype, int perdim, int out_dtype, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Serving operators around the chunked forwards: the short causal convolution, the selective state
+ * space scan, single tokens of the recurrences, and the norm with the residual's addition.  No
+ * counterpart in the reference, whose path ends at the chunked forward.
+ *
+ * Each exec takes a struct by pointer, read during the call only.  `size` is sizeof the struct
+ * (another value is PF_ERR_ARG: a caller built against another header).  Strides are in elements
+ * and >= 0; the innermost dimension is contiguous where no stride is named for it.  `dtype` is the
+ * type of the operands named E; a parameter (w, bias, dt) is E or fp32, by its own `*_f32` flag.
+ * Addresses need an element's alignment only.  Outputs may not overlap inputs unless stated.
+ * `slots` [B] (or NULL: sequence b in slot b) names each sequence's state in a pool of S: no two may
+ * be the same; one outside 0 .. S-1 is skipped (its state untouched, its output row zero).
+ * ------------------------------------------------------------------------------------------ */
+
+/* Short causal depthwise convolution along the tokens of x [B,T,W]:
+ *   y[b,t,c] = act( bias[c] + sum_k w[c,k] x[b, t-(K-1)+k, c] ),  act: 1 = silu, 0 = none
+ * Tokens before the first are state_in [B,K-1,W] (NULL: zero).  lengths [B] (NULL: all T): the tokens
+ * of each sequence; later ones are not read and y is zero there.  state_out [B,K-1,W] (or NULL): the
+ * last K-1 inputs, for the next call; it may be state_in.  Supported: K 2 to 4, T >= 0. */
+typedef struct pf_conv_args {
+  size_t size;
+  const void* x;         /* E, [B,T,W] */
+  const void* w;         /* [W,K] contiguous, E or fp32 */
+  const void* bias;      /* [W], the type of w, or NULL */
+  const void* state_in;  /* E or NULL */
+  const int* lengths;
+  void* y;               /* E */
+  void* state_out;       /* E or NULL */
+  long long x_b, x_t, y_b, y_t, state_in_b, state_out_b;   /* state rows are W apart */
+  int B, T, W, K, dtype, w_f32, act;
+} pf_conv_args;
+int pf_conv_exec(const pf_conv_args* args, void* stream);
+
+/* One token of each of B sequences: x [B,W], state [S,K-1,W] shifted in place, y [B,W]. */
+typedef struct pf_conv_step_args {
+  size_t size;
+  const void* x;
+  const void* w;
+  const void* bias;
+  void* state;
+  const int* slots;
+  void* y;
+  long long x_b, y_b, state_b;
+  int B, S, W, K, dtype, w_f32, act;
+} pf_conv_step_args;
+int pf_conv_step_exec(const pf_conv_step_args* args, void* stream);
+
+/* One token of the state space recurrence, for head h of group h / (H / G):
+ *   dt = softplus?(dt + dt_bias),  S <- e^{dt A} S + B (dt x)^T,  y = (C^T S + D x) * silu(z)?
+ * (DELTA = pf_ssm_step_exec: v = x, k = B, q = C) and of the gated delta rule (pf_gdn_step_exec; KDA
+ * with g_rows = 1):
+ *   S <- e^g S,  r = beta (v - k^T S),  S <- S + k r^T,  y = scale q^T S
+ * state [S,H,N,P] fp32 contiguous within a slot, updated in place.  Supported: N <= 256, P % 4 == 0;
+ * the delta rule: G = H. */
+typedef struct pf_step_args {
+  size_t size;
+  float* state;
+  const int* slots;
+  const void* v;         /* E [B,H,P] */
+  const void* k;         /* E [B,G,N] */
+  const void* q;         /* E [B,G,N] */
+  void* y;               /* [B,H,P]: E (state space), fp32 (delta rule) */
+  const void* dt;        /* state space: [B,H] */
+  const void* z;         /* state space: E [B,H,P] or NULL */
+  const float* a;        /* state space: A [H] */
+  const float* d;        /* state space: D [H] or NULL */
+  const float* dt_bias;  /* state space: [H] or NULL */
+  const float* beta;     /* delta rule: [B,H] contiguous */
+  const float* g;        /* delta rule: log decay [B,H], or [B,H,N] (g_rows), contiguous, or NULL */
+  long long v_b, v_h, k_b, k_h, q_b, q_h, y_b, y_h, dt_b, dt_h, z_b, z_h, state_b;
+  int B, S, H, G, N, P, dtype, dt_f32, softplus, g_rows;
+  float scale;
+} pf_step_args;
+int pf_ssm_step_exec(const pf_step_args* args, void* stream);
+int pf_gdn_step_exec(const pf_step_args* args, void* stream);
+
+/* Root-mean-square norm of `rows` rows of D, with the residual's addition:
+ *   h = x + residual (h = x without one),  n = h * rsqrt(mean(h^2) + eps) * w
+ * y = n in y_dtype (PF_DTYPE_*), or PF_NORM_FP8: codes e4m3(n * (448 / top)) with scales = top / 448, top the
+ * largest |n| of the row (scale_block = 0: scales [rows]) or of each 128 columns (scale_block = 128,
+ * D % 128 == 0: scales [rows, D / 128]).  h_out (with a residual; or NULL) takes h, rounded to the residual's
+ * type; it may be x or residual.  The norm is of h before that rounding.
+ * Supported: D <= 32768; y_dtype E, or bf16 of fp32 rows. */
+#define PF_NORM_FP8 2
+typedef struct pf_norm_args {
+  size_t size;
+  const void* x;         /* E */
+  const void* residual;  /* E or fp32 (r_f32), or NULL */
+  const void* w;         /* [D], E or fp32 (w_f32) */
+  void* y;
+  float* scales;         /* PF_NORM_FP8 only */
+  void* h_out;           /* type of residual, or NULL */
+  long long x_row, residual_row, y_row, h_row;
+  int rows, D, dtype, y_dtype, r_f32, w_f32, scale_block;
+  float eps;
+} pf_norm_args;
+int pf_norm_exec(const pf_norm_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

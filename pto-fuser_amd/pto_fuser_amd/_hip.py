@@ -18,6 +18,7 @@ from . import _build
 
 PF_DTYPE_F32 = 0
 PF_DTYPE_BF16 = 1
+PF_NORM_FP8 = 2            # y_dtype of pf_norm_exec
 PF_OK = 0
 PF_ERR_ARG = -1
 PF_ERR_WORKSPACE = -2
@@ -57,6 +58,12 @@ SIGNATURES = {
     "pf_qkv_flash_teardown": (None, [c_void_p]),
     "pf_scan_setup": (c_void_p, []),
     "pf_scan_teardown": (None, [c_void_p]),
+    # one packed argument struct (bytes, read during the call) and the stream
+    "pf_conv_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_conv_step_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_ssm_step_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_gdn_step_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_norm_exec": (c_int, [c_void_p, c_void_p]),
 }
 
 

@@ -1,0 +1,369 @@
+"""The short convolution, single tokens of the recurrences and the norm on the GPU, against their definitions in
+float64: odd sizes, views, lengths of zero and one, pools of states, rows of zeros and of infinities."""
+import pytest
+import torch
+
+import serving_refs as ref
+from conftest import announce
+from pto_fuser_amd import (add_rms_norm, add_rms_norm_fp8, causal_conv, causal_conv_step, gdn_chunk_forward, gdn_step,
+                           ssm_step)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+NAN, INF = float("nan"), float("inf")
+
+
+def _rand(seed):
+    gen = torch.Generator().manual_seed(seed)
+    return lambda *shape: torch.randn(*shape, generator=gen)
+
+
+def _dev(t, dtype=None):
+    return None if t is None else t.to(DEV, dtype)
+
+
+def _wide(t, extra):
+    """The same values as a view of rows that are ``extra`` wider, starting one element in; NaN around them."""
+    buf = torch.full((*t.shape[:-1], t.shape[-1] + extra), NAN, dtype=t.dtype, device=t.device)
+    view = buf[..., 1:1 + t.shape[-1]]
+    view.copy_(t)
+    return view
+
+
+# ------------------------------------------------------------------------------------------
+#  Convolution.  32-bit operations on a term: its product, at most K + 1 additions, and the activation's six.
+# ------------------------------------------------------------------------------------------
+CONV_OPS = 16
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,W,K", [(1, 1, 8, 4), (2, 2, 64, 4), (3, 3, 24, 3), (1, 8, 7, 2), (2, 9, 1, 4), (2, 37, 520, 4),
+                                     (1, 131, 40, 3), (5, 16, 13, 2)])
+@pytest.mark.parametrize("plain", [True, False])
+def test_conv(dtype, B, T, W, K, plain):
+    announce(f"causal_conv {dtype} B{B} T{T} W{W} K{K} plain={plain}")
+    r = _rand(B * T + W)
+    x, w = _dev(r(B, T, W), dtype), _dev(0.5 * r(W, K), dtype if plain else F32)
+    bias = None if plain else _dev(0.2 * r(W), F32)
+    state = None if plain else _dev(r(B, K - 1, W), dtype)
+    xin = x if plain else _wide(x, 5)
+    y, final = causal_conv(xin, w, bias, activation=None if plain else "silu", initial_state=state)
+    want, mag, last = ref.conv(ref.f64(x), ref.f64(w), ref.f64(bias), not plain, ref.f64(state))
+    ref.check(y, want, mag, CONV_OPS, "y")
+    assert torch.equal(ref.f64(final), last)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("K", [2, 3, 4])
+def test_conv_lengths(dtype, K):
+    """Sequences of 0, 1, 2, .. tokens in one batch: what follows them is NaN and is not read; the state is of the last
+    live token, written over the one that came in."""
+    announce(f"causal_conv lengths {dtype} K{K}")
+    T, W = 19, 48
+    lengths = [0, 1, 2, 3, T - 1, T]
+    B, r = len(lengths), _rand(K)
+    x, w, bias = _dev(r(B, T, W), dtype), _dev(0.5 * r(W, K), dtype), _dev(0.2 * r(W), dtype)
+    state = _dev(r(B, K - 1, W), dtype)
+    want, mag, last = ref.conv(ref.f64(x), ref.f64(w), ref.f64(bias), True, ref.f64(state), lengths)
+    for b, n in enumerate(lengths):
+        x[b, n:] = NAN
+    y, final = causal_conv(x, w, bias, initial_state=state, lengths=torch.tensor(lengths, dtype=torch.int32, device=DEV),
+                           final_out=state)
+    assert final is state
+    ref.check(y, want, mag, CONV_OPS, "y")
+    assert torch.equal(ref.f64(final), last)
+
+
+def test_conv_of_no_tokens():
+    announce("causal_conv T=0, B=0")
+    state = torch.randn(2, 3, 16, device=DEV)
+    w = torch.randn(16, 4, device=DEV)
+    y, final = causal_conv(torch.empty(2, 0, 16, device=DEV), w, initial_state=state)
+    assert y.shape == (2, 0, 16) and torch.equal(final, state)
+    y, final = causal_conv(torch.empty(2, 0, 16, device=DEV), w)
+    assert not final.any()
+    y, final = causal_conv(torch.empty(0, 5, 16, device=DEV), w)
+    assert y.shape == (0, 5, 16) and final.shape == (0, 3, 16)
+
+
+def test_conv_keeps_nan_where_it_is():
+    """A NaN or infinity reaches the K tokens that read it and no other, and no other channel."""
+    announce("causal_conv NaN")
+    x = torch.ones(1, 40, 64, device=DEV, dtype=BF)
+    x[0, 11, 3], x[0, 20, 5] = NAN, INF
+    y, _ = causal_conv(x, torch.ones(64, 4, device=DEV, dtype=BF), activation=None)
+    bad = ~torch.isfinite(y[0].cpu())
+    want = torch.zeros(40, 64, dtype=torch.bool)
+    want[11:15, 3] = want[20:24, 5] = True
+    assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("W,K", [(64, 4), (520, 3), (7, 2), (24, 4)])
+def test_conv_step_continues_the_prompt(dtype, W, K):
+    """A prompt, then single tokens from its state: the bits of the whole prompt at once."""
+    announce(f"causal_conv_step {dtype} W{W} K{K}")
+    B, T, n, r = 3, 12, 5, _rand(W)
+    x, w, bias = _dev(r(B, T, W), dtype), _dev(0.5 * r(W, K), dtype), _dev(0.2 * r(W), F32).to(dtype)
+    whole, last = causal_conv(x, w, bias)
+    first, state = causal_conv(x[:, :n], w, bias)
+    rest = [causal_conv_step(x[:, t], state, w, bias) for t in range(n, T)]
+    assert torch.equal(torch.cat([first, torch.stack(rest, 1)], 1), whole)
+    assert torch.equal(state, last)
+
+
+def test_conv_step_slots():
+    """States in a pool: the named ones move, all others keep their bits, and a slot outside the pool is skipped."""
+    announce("causal_conv_step slots")
+    r = _rand(2)
+    pool, x, w = _dev(r(9, 3, 40)), _dev(r(4, 40)), _dev(r(40, 4))
+    before = pool.clone()
+    slots = torch.tensor([7, -1, 0, 9], dtype=torch.int32, device=DEV)
+    y = causal_conv_step(x, pool, w, slots=slots)
+    picked = before[[7, 0]].clone()
+    want = causal_conv_step(x[[0, 2]], picked, w)
+    assert torch.equal(y[[0, 2]], want) and not y[[1, 3]].any()
+    before[[7, 0]] = picked
+    assert torch.equal(pool, before)
+
+
+# ------------------------------------------------------------------------------------------
+#  Single tokens.  Operations on a term: decay (with the exponential's and its argument's), products, and sums over up
+#  to 256 rows: at most 32 additions on a term's way (eight rows of a thread, a tree, four waves), with 12 more.
+# ------------------------------------------------------------------------------------------
+STEP_OPS = 48
+
+
+def _step_case(seed, dtype, B, H, P, G, N, z=True):
+    r = _rand(seed)
+    s = {"x": _dev(r(B, H, P), dtype), "dt": _dev(r(B, H), dtype), "A": _dev(-1 - r(H).abs()), "B": _dev(r(B, G, N), dtype),
+         "C": _dev(r(B, G, N), dtype), "D": _dev(r(H)), "z": _dev(r(B, H, P), dtype) if z else None, "dt_bias": _dev(r(H) - 3)}
+    return s, _dev(r(B, H, N, P))
+
+
+def _one_token(s, state):
+    add = lambda t: None if t is None else ref.f64(t).unsqueeze(2)  # noqa: E731
+    y, mag, S, M = ref.ssm(add(s["x"]), add(s["dt"]), ref.f64(s["A"]), add(s["B"]), add(s["C"]), ref.f64(s["D"]), add(s["z"]),
+                           ref.f64(s["dt_bias"]), True, ref.f64(state))
+    return y[:, :, 0], mag[:, :, 0], S, M
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,H,P,G,N", [(1, 1, 4, 1, 1), (2, 6, 64, 2, 128), (3, 5, 36, 5, 17), (1, 8, 96, 1, 64), (2, 3, 128, 1, 200),
+                                       (1, 2, 260, 2, 256)])
+def test_ssm_step(dtype, B, H, P, G, N):
+    announce(f"ssm_step {dtype} B{B} H{H} P{P} G{G} N{N}")
+    s, state = _step_case(B + N, dtype, B, H, P, G, N)
+    want, mag, S, M = _one_token(s, state)
+    y = ssm_step(state, dt_softplus=True, **s)
+    ref.check(y, want, mag, STEP_OPS, "y")
+    ref.check(state, S, M, STEP_OPS, "state")
+
+
+def test_ssm_step_views_and_plain_dt():
+    """Operands as slices of one projected row, dt in float32 and used as it is, no D, no z."""
+    announce("ssm_step views")
+    r = _rand(3)
+    row = _dev(r(4, 3 * 64 + 2 * 2 * 16 + 3), BF)
+    s = {"x": row[:, :192].unflatten(-1, (3, 64)), "B": row[:, 192:208].unflatten(-1, (1, 16)),
+         "C": row[:, 208:224].unflatten(-1, (1, 16)), "dt": _dev(r(4, 6).abs() * 0.1)[:, ::2], "A": _dev(-r(3).abs())}
+    state = _dev(r(4, 3, 16, 64))
+    add = lambda t: ref.f64(t).unsqueeze(2)  # noqa: E731
+    want, mag, S, M = ref.ssm(add(s["x"]), add(s["dt"]), ref.f64(s["A"]), add(s["B"]), add(s["C"]), h0=ref.f64(state))
+    out = torch.empty(4, 3, 80, device=DEV, dtype=BF)[..., 8:72]
+    y = ssm_step(state, out=out, **s)
+    assert y.data_ptr() == out.data_ptr()
+    ref.check(y, want[:, :, 0], mag[:, :, 0], STEP_OPS, "y")
+    ref.check(state, S, M, STEP_OPS, "state")
+
+
+def test_ssm_step_slots():
+    announce("ssm_step slots")
+    s, _ = _step_case(11, F32, 4, 2, 64, 1, 32)
+    pool = _dev(_rand(12)(6, 2, 32, 64))
+    before = pool.clone()
+    y = ssm_step(pool, dt_softplus=True, slots=torch.tensor([5, 6, 2, -3], dtype=torch.int32, device=DEV), **s)
+    picked = before[[5, 2]].clone()
+    want = ssm_step(picked, dt_softplus=True, **{k: v if k in ("A", "D", "dt_bias") else v[[0, 2]] for k, v in s.items()})
+    assert torch.equal(y[[0, 2]], want) and not y[[1, 3]].any()
+    before[[5, 2]] = picked
+    assert torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("gate", ["none", "head", "channel"])
+@pytest.mark.parametrize("B,H,DK,DV", [(1, 1, 128, 128), (2, 3, 128, 128), (2, 2, 64, 128), (1, 3, 256, 36), (3, 1, 5, 4)])
+def test_gdn_step(dtype, gate, B, H, DK, DV):
+    announce(f"gdn_step {dtype} {gate} B{B} H{H} DK{DK} DV{DV}")
+    r = _rand(DK + DV)
+    unit = torch.nn.functional.normalize
+    q, k = _dev(unit(r(B, H, DK), dim=-1), dtype), _dev(unit(r(B, H, DK), dim=-1), dtype)
+    v, beta = _dev(r(B, H, DV), dtype), _dev(torch.sigmoid(r(B, H)))
+    g = {"none": None, "head": -r(B, H).abs(), "channel": -r(B, H, DK).abs()}[gate]
+    g, state = _dev(g), _dev(r(B, H, DK, DV))
+    want, mag, S, M = ref.delta_step(*(ref.f64(t) for t in (state, q, k, v, beta, g)))
+    o = gdn_step(state, q, k, v, beta, g)
+    assert o.dtype is F32
+    ref.check(o, want, mag, 2 * STEP_OPS, "o")            # the two sums follow one another
+    ref.check(state, S, M, 2 * STEP_OPS, "state")
+
+
+def test_gdn_step_continues_the_chunked_forward():
+    """64 tokens through the chunked forward, four more one by one: the float64 recurrence over all 68."""
+    announce("gdn_step after gdn_chunk_forward")
+    B, H, T, n, D = 1, 2, 68, 64, 128
+    r = _rand(5)
+    unit = torch.nn.functional.normalize
+    q, k, v = unit(r(B, H, T, D), dim=-1), unit(r(B, H, T, D), dim=-1), r(B, H, T, D)
+    beta, g = torch.sigmoid(r(B, H, T)), -0.1 * r(B, H, T).abs()
+    S, M = (torch.zeros(B, H, D, D, dtype=torch.float64) for _ in range(2))
+    want = []
+    for t in range(T):
+        o, _, S, _ = ref.delta_step(S, *(a[:, :, t].double() for a in (q, k, v, beta, g)))
+        want.append(o)
+    d = [_dev(a) for a in (q, k, v, beta, g)]
+    _, state = gdn_chunk_forward(*(a[:, :, :n].contiguous() for a in d))
+    got = [gdn_step(state, *(a[:, :, t].contiguous() for a in d)) for t in range(n, T)]
+    # the chunked forward in fp32 is within 1e-4 of the largest value (its documented parity); the steps keep that
+    want = torch.stack(want[n:], 2)
+    assert (ref.f64(torch.stack(got, 2)) - want).abs().max() <= 1e-4 * want.abs().max()
+    assert (ref.f64(state) - S).abs().max() <= 1e-4 * S.abs().max()
+
+
+# ------------------------------------------------------------------------------------------
+#  Norm.  A value carries the residual's addition, half the relative error of the mean of squares (a tree over at most
+#  64 values of a thread: under 80 additions, halved by the root), the root, the quotient and two products.
+# ------------------------------------------------------------------------------------------
+NORM_OPS = 56
+WIDTHS = [1, 7, 8, 100, 513, 1024, 2048, 2056, 4096, 6144, 9000, 16384, 32768]
+
+
+def _norm_case(seed, dtype, rows, D, residual, w_dtype):
+    r = _rand(seed)
+    return (_dev(r(rows, D), dtype), _dev(1 + 0.1 * r(D), w_dtype), None if residual is None else _dev(3 * r(rows, D), residual))
+
+
+def _check_norm(y, h, x, w, res, what):
+    want, sums = ref.norm(ref.f64(x), ref.f64(w), ref.f64(res))
+    mag = want.abs()
+    if res is not None:      # the sum's own rounding, carried by the row's factor
+        mag = mag + ref.norm(ref.f64(x).abs() + ref.f64(res).abs(), ref.f64(w).abs())[0]
+        ref.check(h, sums, ref.f64(x).abs() + ref.f64(res).abs(), 1, what + " h")
+    ref.check(y, want, mag, NORM_OPS, what + " y")
+
+
+@pytest.mark.parametrize("D", WIDTHS)
+@pytest.mark.parametrize("dtype,residual,w_dtype", [(BF, None, BF), (BF, BF, F32), (BF, F32, BF), (F32, F32, F32), (F32, None, F32)])
+def test_norm(D, dtype, residual, w_dtype):
+    announce(f"add_rms_norm {dtype} residual {residual} D{D}")
+    x, w, res = _norm_case(D, dtype, 5, D, residual, w_dtype)
+    y, h = add_rms_norm(x, w, res)
+    assert y.dtype is dtype and (h is None) == (res is None) and (h is None or h.dtype is residual)
+    _check_norm(y, h, x, w, res, f"D{D}")
+
+
+def test_norm_layouts():
+    """Rows that are slices of wider ones, several leading dimensions, float32 rows to bfloat16, the stream in place."""
+    announce("add_rms_norm layouts")
+    x, w, res = _norm_case(1, F32, 12, 200, F32, F32)
+    want, sums = add_rms_norm(x, w, res)
+    y, h = add_rms_norm(_wide(x, 9), w, _wide(res, 3))
+    assert torch.equal(y, want) and torch.equal(h, sums)
+    y, _ = add_rms_norm(x.view(3, 4, 200), w, res.view(3, 4, 200))
+    assert y.shape == (3, 4, 200) and torch.equal(y.view(12, 200), want)
+    y, _ = add_rms_norm(x, w, res, out_dtype=BF)
+    assert torch.equal(y, want.to(BF))
+    stream = res.clone()
+    y, h = add_rms_norm(x, w, stream, residual_out=stream)
+    assert h is stream and torch.equal(stream, sums) and torch.equal(y, want)
+    y, h = add_rms_norm(x[:0], w, res[:0])
+    assert y.shape == (0, 200) and h.shape == (0, 200)
+
+
+def test_norm_rows_of_their_own():
+    """Rows of zeros, an infinity, a NaN, values whose squares overflow: each keeps to itself."""
+    announce("add_rms_norm special rows")
+    x = torch.ones(6, 96, device=DEV)
+    x[1] = 0
+    x[2, 5] = INF
+    x[3, 7] = NAN
+    x[4] = 1e30
+    w = torch.full((96,), 2.0, device=DEV)
+    y = add_rms_norm(x, w)[0].cpu()
+    assert torch.allclose(y[[0, 5]], torch.full((2, 96), 2.0), rtol=1e-6) and not y[1].any()
+    assert torch.isnan(y[2, 5]) and not y[2, :5].any() and torch.isnan(y[3]).all() and not y[4].any()
+    codes, scales, _ = add_rms_norm_fp8(x, w)
+    codes, scales = codes.float().cpu(), scales.cpu()
+    assert (codes[[0, 5]] == 448).all() and not codes[1].any() and scales[1] == 0
+    assert torch.isnan(codes[3]).all() and torch.isnan(scales[3])
+    assert torch.allclose(scales[[0, 5]], torch.full((2, 1), 2 / 448), rtol=1e-6)
+
+
+def _check_fp8(codes, scales, want, block, what):
+    """Each code is the value's nearest, up to the value's own 32-bit error: off by half a step (a sixteenth of the
+    power of two below, at least 2^-10 for the smallest) and NORM_OPS roundings."""
+    rows, D = want.shape
+    top = want.view(rows, -1, block).abs().amax(-1)
+    ref.check(scales, top / 448, top / 448, NORM_OPS + 2, what + " scales")
+    scaled = want.view(rows, -1, block) * torch.where(top > 0, 448 / top, 0.0)[..., None]
+    got = codes.float().cpu().double().view_as(scaled)
+    step = torch.maximum(2.0 ** torch.floor(torch.log2(scaled.abs().clamp(min=1e-30))) / 16, torch.tensor(2.0 ** -10, dtype=torch.float64))
+    over = (got - scaled).abs() - step - 2 * (NORM_OPS + 4) * ref.EPS32 * 448
+    assert over.max() <= 0, f"{what}: a code is {over.max():.3e} further off than half a step"
+
+
+@pytest.mark.parametrize("D,block", [(7, None), (128, None), (513, None), (2048, None), (6144, None), (16384, None), (128, 128),
+                                     (640, 128), (2048, 128), (6144, 128), (16384, 128), (32768, 128)])
+@pytest.mark.parametrize("dtype,residual", [(BF, None), (BF, BF), (BF, F32), (F32, F32)])
+def test_norm_fp8(D, block, dtype, residual):
+    announce(f"add_rms_norm_fp8 {dtype} residual {residual} D{D} block {block}")
+    x, w, res = _norm_case(D, dtype, 5, D, residual, dtype)
+    x[2] = 0
+    if res is not None:
+        res[2] = 0
+    codes, scales, h = add_rms_norm_fp8(x, w, res, scale_block=block)
+    assert codes.dtype is torch.float8_e4m3fn and scales.shape == (5, D // block if block else 1)
+    want, sums = ref.norm(ref.f64(x), ref.f64(w), ref.f64(res))
+    _check_fp8(codes, scales, want, block or D, f"D{D}")
+    if res is not None:
+        ref.check(h, sums, ref.f64(x).abs() + ref.f64(res).abs(), 1, "h")
+
+
+# ------------------------------------------------------------------------------------------
+#  Streams and graphs
+# ------------------------------------------------------------------------------------------
+def test_steps_in_a_graph():
+    """One decode step (norm, convolution, state space, delta rule) captured on a stream of its own and replayed, with
+    eager work between: every replay is the eager step's bits."""
+    announce("captured decode step")
+    s, state = _step_case(21, BF, 2, 4, 64, 1, 32)
+    r = _rand(22)
+    conv_x, conv_w, conv_s = _dev(r(2, 64), BF), _dev(r(64, 4), BF), _dev(r(2, 3, 64), BF)
+    rows, w = _dev(r(2, 96), BF), _dev(r(96), BF)
+    q = _dev(torch.nn.functional.normalize(r(2, 4, 32), dim=-1), BF)
+    beta, S2 = _dev(torch.sigmoid(r(2, 4))), _dev(r(2, 4, 32, 64))
+
+    def step(states):
+        return (add_rms_norm_fp8(rows, w, rows), causal_conv_step(conv_x, states[0], conv_w),
+                ssm_step(states[1], dt_softplus=True, **s), gdn_step(states[2], q, q, s["x"], beta))
+
+    def flat(outs):
+        return [t.float() for o in outs for t in (o if isinstance(o, tuple) else (o,))]
+
+    eager, captured = ([t.clone() for t in (conv_s, state, S2)] for _ in range(2))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        step([t.clone() for t in captured])
+        with torch.cuda.graph(graph, stream=stream):
+            outs = step(captured)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        want = flat(step(eager))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(flat(outs), want))
+        assert all(torch.equal(a, b) for a, b in zip(captured, eager))

@@ -1,0 +1,196 @@
+"""Refusals of the serving operators, without a GPU: the C entry points' statuses, the argument structs' sizes, and the
+Python operators' checks (device tensors are stood in for by CPU ones where a check comes after the device's)."""
+import os
+import subprocess
+
+import pytest
+import torch
+
+import pto_fuser_amd as pf
+from pto_fuser_amd import _build, _hip, ops, serving
+
+STRUCTS = {"pf_conv_args": serving._CONV_SIZE, "pf_conv_step_args": serving._CONV_STEP_SIZE, "pf_step_args": serving._STEP_SIZE,
+           "pf_norm_args": serving._NORM_SIZE}
+
+
+@pytest.fixture(scope="module")
+def lib():
+    _build.ensure_built()
+    return _hip.load()
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """CPU tensors pass for device ones, and a launch is recorded."""
+    made = []
+    on = lambda t, name: t.device  # noqa: E731
+    monkeypatch.setattr(serving, "_on_device", on)
+    monkeypatch.setattr(serving, "_exec", lambda name, dev, layout, *fields: made.append((name, layout.pack(*fields))))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: None)
+    return made
+
+
+def test_struct_sizes_are_the_header_s(tmp_path):
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "pto_fuser_hip.h"\nint main(void) {' +
+                   "".join(f'printf("{n} %zu\\n", sizeof({n}));' for n in STRUCTS) + "return 0; }\n")
+    subprocess.run(["gcc", "-I", _build.INCLUDE, str(src), "-o", str(tmp_path / "sizes")], check=True)
+    out = subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, check=True).stdout
+    assert dict((n, int(s)) for n, s in (line.split() for line in out.splitlines())) == STRUCTS
+
+
+def _conv(**kw):
+    f = dict(size=serving._CONV_SIZE, x=64, w=64, bias=0, state_in=0, lengths=0, y=64, state_out=0, x_b=0, x_t=0, y_b=0, y_t=0,
+             si=0, so=0, B=1, T=4, W=8, K=4, dtype=1, w_f32=0, act=1)
+    assert not set(kw) - set(f)
+    return serving._CONV.pack(*{**f, **kw}.values())
+
+
+@pytest.mark.parametrize("bad", [dict(size=8), dict(dtype=2), dict(K=1), dict(K=5), dict(W=0), dict(T=-1), dict(B=-1), dict(w=0),
+                                 dict(x=0), dict(y=0), dict(x_t=-1), dict(B=2 ** 31 - 1, W=2 ** 24, T=2 ** 20)])
+def test_conv_statuses(lib, bad):
+    assert lib.pf_conv_exec(_conv(**bad), None) == _hip.PF_ERR_ARG
+
+
+def test_empty_calls_launch_nothing(lib):
+    assert lib.pf_conv_exec(_conv(B=0, x=0, y=0), None) == _hip.PF_OK
+    assert lib.pf_conv_exec(None, None) == _hip.PF_ERR_ARG
+    assert lib.pf_norm_exec(_norm(rows=0, x=0, y=0), None) == _hip.PF_OK
+    assert lib.pf_ssm_step_exec(_step(B=0), None) == _hip.PF_OK
+    assert lib.pf_gdn_step_exec(_step(B=0, G=2, beta=64), None) == _hip.PF_OK
+    assert lib.pf_conv_step_exec(_conv_step(B=0), None) == _hip.PF_OK
+
+
+def _conv_step(**kw):
+    f = dict(size=serving._CONV_STEP_SIZE, x=64, w=64, bias=0, state=64, slots=0, y=64, x_b=0, y_b=0, s_b=0, B=1, S=1, W=8, K=4,
+             dtype=1, w_f32=0, act=1)
+    return serving._CONV_STEP.pack(*{**f, **kw}.values())
+
+
+@pytest.mark.parametrize("bad", [dict(size=0), dict(dtype=-1), dict(K=1), dict(K=5), dict(W=0), dict(state=0), dict(B=2), dict(x_b=-1)])
+def test_conv_step_statuses(lib, bad):
+    assert lib.pf_conv_step_exec(_conv_step(**bad), None) == _hip.PF_ERR_ARG
+
+
+def _step(**kw):
+    f = dict(size=serving._STEP_SIZE, state=64, slots=0, v=64, k=64, q=64, y=64, dt=64, z=0, a=64, d=0, dt_bias=0, beta=0, g=0)
+    f.update({f"s{i}": 0 for i in range(13)})
+    f.update(B=1, S=1, H=2, G=1, N=16, P=8, dtype=1, dt_f32=0, softplus=0, g_rows=0, scale=1.0)
+    return serving._STEP.pack(*{**f, **kw}.values())
+
+
+@pytest.mark.parametrize("bad", [dict(size=4), dict(dtype=3), dict(H=3, G=2), dict(N=257), dict(N=0), dict(P=6), dict(P=0), dict(dt=0),
+                                 dict(a=0), dict(state=0), dict(B=2), dict(s0=-1), dict(G=0)])
+def test_step_statuses(lib, bad):
+    assert lib.pf_ssm_step_exec(_step(**bad), None) == _hip.PF_ERR_ARG
+
+
+@pytest.mark.parametrize("bad", [dict(beta=0, G=2), dict(beta=64, G=1), dict(beta=64, G=2, N=300)])
+def test_gdn_step_statuses(lib, bad):
+    assert lib.pf_gdn_step_exec(_step(**bad), None) == _hip.PF_ERR_ARG
+
+
+def _norm(**kw):
+    f = dict(size=serving._NORM_SIZE, x=64, residual=0, w=64, y=64, scales=0, h=0, x_row=8, r_row=8, y_row=8, h_row=8, rows=1, D=256,
+             dtype=1, y_dtype=1, r_f32=0, w_f32=0, block=0, eps=1e-6)
+    return serving._NORM.pack(*{**f, **kw}.values())
+
+
+@pytest.mark.parametrize("bad", [dict(size=1), dict(dtype=2), dict(D=0), dict(D=32769), dict(y_dtype=0), dict(y_dtype=2), dict(block=128),
+                                 dict(y_dtype=2, scales=64, block=64), dict(y_dtype=2, scales=64, block=128, D=200), dict(h=64),
+                                 dict(x=0), dict(rows=-1), dict(x_row=-1)])
+def test_norm_statuses(lib, bad):
+    assert lib.pf_norm_exec(_norm(**bad), None) == _hip.PF_ERR_ARG
+
+
+def test_operators_want_a_device():
+    x = torch.zeros(1, 4, 8)
+    with pytest.raises(ValueError, match="HIP device"):
+        pf.causal_conv(x, torch.zeros(8, 4))
+    with pytest.raises(ValueError, match="HIP device"):
+        pf.causal_conv_step(x[0], torch.zeros(4, 3, 8), torch.zeros(8, 4))
+    with pytest.raises(ValueError, match="HIP device"):
+        pf.ssm_step(torch.zeros(1, 4, 2, 8), x, torch.zeros(1, 4), torch.zeros(4), x[:, :1, :2], x[:, :1, :2])
+    with pytest.raises(ValueError, match="HIP device"):
+        pf.gdn_step(torch.zeros(1, 4, 8, 8), x, x, x, torch.zeros(1, 4))
+    with pytest.raises(ValueError, match="HIP device"):
+        pf.add_rms_norm(x, torch.zeros(8))
+
+
+def test_conv_refusals(on_cpu):
+    x, w = torch.zeros(2, 4, 8), torch.zeros(8, 4)
+    pf.causal_conv(x, w, torch.zeros(8), initial_state=torch.zeros(2, 3, 8))
+    assert on_cpu.pop()[0] == "pf_conv_exec"
+    for match, call in (
+            (r"\[B,T,W\]", lambda: pf.causal_conv(x[0], w)),
+            ("taps", lambda: pf.causal_conv(x, torch.zeros(8, 5))),
+            ("dtype", lambda: pf.causal_conv(x.half(), w)),
+            ("weight has shape", lambda: pf.causal_conv(x, torch.zeros(7, 4))),
+            ("weight has dtype", lambda: pf.causal_conv(x, w.double())),
+            ("bias has dtype", lambda: pf.causal_conv(x.bfloat16(), w, torch.zeros(8, dtype=torch.bfloat16))),
+            ("last dimension", lambda: pf.causal_conv(torch.zeros(2, 8, 4).transpose(1, 2), w)),
+            ("initial_state has shape", lambda: pf.causal_conv(x, w, initial_state=torch.zeros(2, 4, 8))),
+            ("lengths has dtype", lambda: pf.causal_conv(x, w, lengths=torch.zeros(2, dtype=torch.int64))),
+            ("activation", lambda: pf.causal_conv(x, w, activation="gelu")),
+            ("out may not be x", lambda: pf.causal_conv(x, w, out=x)),
+            ("state holds 3", lambda: pf.causal_conv_step(x[0, :2], torch.zeros(3, 3, 8), w)),
+            ("slots has dtype", lambda: pf.causal_conv_step(x[0, :2], torch.zeros(3, 3, 8), w, slots=torch.zeros(2))),
+            ("state has shape", lambda: pf.causal_conv_step(x[0, :2], torch.zeros(2, 2, 8), w))):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not on_cpu
+
+
+def test_step_refusals(on_cpu):
+    x, b, S = torch.zeros(2, 4, 8), torch.zeros(2, 2, 16), torch.zeros(2, 4, 16, 8)
+    dt, A = torch.zeros(2, 4), torch.zeros(4)
+    pf.ssm_step(S, x, dt, A, b, b)
+    pf.gdn_step(S, torch.zeros(2, 4, 16), torch.zeros(2, 4, 16), x, dt, torch.zeros(2, 4, 16))
+    assert [n for n, _ in on_cpu] == ["pf_ssm_step_exec", "pf_gdn_step_exec"]
+    on_cpu.clear()
+    q = torch.zeros(2, 4, 16)
+    for match, call in (
+            ("multiple of G", lambda: pf.ssm_step(S, x, dt, A, torch.zeros(2, 3, 16), b)),
+            ("multiple of 4", lambda: pf.ssm_step(S, torch.zeros(2, 4, 6), dt, A, b, b)),
+            ("up to 256", lambda: pf.ssm_step(S, x, dt, A, torch.zeros(2, 2, 257), b)),
+            ("C has shape", lambda: pf.ssm_step(S, x, dt, A, b, b[:, :1])),
+            ("dt is", lambda: pf.ssm_step(S, x, dt[:1], A, b, b)),
+            ("dt has dtype", lambda: pf.ssm_step(S, x, dt.double(), A, b, b)),
+            ("A must", lambda: pf.ssm_step(S, x, dt, None, b, b)),
+            ("state has shape", lambda: pf.ssm_step(S[:, :, :8], x, dt, A, b, b)),
+            ("state has dtype", lambda: pf.ssm_step(S.bfloat16(), x, dt, A, b, b)),
+            ("z has shape", lambda: pf.ssm_step(S, x, dt, A, b, b, z=x[:1])),
+            ("beta", lambda: pf.gdn_step(S, q, q, x, None)),
+            ("g has shape", lambda: pf.gdn_step(S, q, q, x, dt, dt[:1])),
+            ("k has shape", lambda: pf.gdn_step(S, q, q[:, :2], x, dt)),
+            ("out has dtype", lambda: pf.gdn_step(S, q.bfloat16(), q.bfloat16(), x.bfloat16(), dt, out=x.bfloat16()))):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not on_cpu
+
+
+def test_norm_refusals(on_cpu):
+    x, w = torch.zeros(3, 256), torch.zeros(256)
+    pf.add_rms_norm(x, w, x)
+    assert on_cpu.pop()[0] == "pf_norm_exec"
+    for match, call in (
+            (r"\[\.\.\., D\]", lambda: pf.add_rms_norm(torch.zeros(2, 32769), w)),
+            ("weight has shape", lambda: pf.add_rms_norm(x, w[:8])),
+            ("residual is", lambda: pf.add_rms_norm(x, w, x[:2])),
+            ("residual has dtype", lambda: pf.add_rms_norm(x, w, x.half())),
+            ("without a residual", lambda: pf.add_rms_norm(x, w, residual_out=x)),
+            ("evenly spaced", lambda: pf.add_rms_norm(torch.zeros(256, 3).t(), w)),
+            ("out_dtype", lambda: pf.add_rms_norm(x.bfloat16(), w, out_dtype=torch.float32)),
+            ("scale_block", lambda: pf.add_rms_norm_fp8(x, w, scale_block=64)),
+            ("scale_block", lambda: pf.add_rms_norm_fp8(torch.zeros(3, 200), w[:200], scale_block=128)),
+            ("scales_out has shape", lambda: pf.add_rms_norm_fp8(x, w, scales_out=torch.zeros(3)))):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not on_cpu
+
+
+def test_sizes_past_32_bits_are_refused(monkeypatch):
+    """A size that does not fit its field is a ValueError, not a struct's."""
+    monkeypatch.setattr(_hip, "load", lambda: type("Lib", (), {"pf_norm_exec": None}))
+    with pytest.raises(ValueError, match="past what pf_norm_exec takes"):
+        serving._exec("pf_norm_exec", torch.device("cuda", 0), serving._NORM, serving._NORM_SIZE, *[0] * 10, 1 << 31, *[0] * 6, 0.0)
