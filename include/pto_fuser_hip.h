@@ -296,6 +296,40 @@ typedef struct pf_step_args {
 int pf_ssm_step_exec(const pf_step_args* args, void* stream);
 int pf_gdn_step_exec(const pf_step_args* args, void* stream);
 
+/* Selective state space scan over prompts, for head h of group h / (H / G):
+ *   dt = softplus?(dt + dt_bias),  S_t = e^{dt A} S_{t-1} + B_t (dt x_t)^T,  y_t = (C_t^T S_t + D x_t) * silu(z_t)?
+ * x, z, y [B,H,T,P], b, c [B,G,T,N], dt [B,H,T] with free strides; A, D, dt_bias [H] fp32; h0, h_final
+ * [B,H,N,P] fp32 contiguous (h_final may be h0).  lengths [B] (NULL: all T): the tokens of each sequence;
+ * later ones are not read, y is zero there, and the state is that after the last one.  Any T >= 0.
+ * The scan runs 64-token chunks; a non-finite operand reaches all of its chunk's rows.
+ * Supported: P a multiple of 32 up to 256, N a multiple of 16 up to 128.
+ * Few sequences run as segments side by side when `workspace` holds their states
+ * (pf_ssm_workspace_bytes: arithmetic, 0 where whole sequences fill the chip or the shape is not supported);
+ * on a smaller one, or NULL, the same call runs whole sequences.  The number of segments follows from the
+ * call's shape, so the same sequence alone and in a batch may differ by bf16 rounding.  The workspace is
+ * read and written by the launches of the call only. */
+typedef struct pf_ssm_args {
+  size_t size;
+  const void* x;         /* E */
+  const void* dt;        /* E or fp32 (dt_f32) */
+  const void* b;         /* E */
+  const void* c;         /* E */
+  const void* z;         /* E or NULL */
+  const float* a;
+  const float* d;        /* or NULL */
+  const float* dt_bias;  /* or NULL */
+  const float* h0;       /* or NULL: zero */
+  const int* lengths;
+  void* y;               /* E */
+  float* h_final;        /* or NULL */
+  void* workspace;       /* device memory, 16-byte aligned */
+  size_t workspace_bytes;
+  long long x_b, x_h, x_t, dt_b, dt_h, dt_t, b_b, b_g, b_t, c_b, c_g, c_t, z_b, z_h, z_t, y_b, y_h, y_t;
+  int B, H, G, T, N, P, dtype, dt_f32, softplus;
+} pf_ssm_args;
+size_t pf_ssm_workspace_bytes(int B, int H, int G, int T, int N, int P, int dtype);
+int pf_ssm_exec(const pf_ssm_args* args, void* stream);
+
 /* Root-mean-square norm of `rows` rows of D, with the residual's addition:
  *   h = x + residual (h = x without one),  n = h * rsqrt(mean(h^2) + eps) * w
  * y = n in y_dtype (PF_DTYPE_*), or PF_NORM_FP8: codes e4m3(n * (448 / top)) with scales = top / 448, top the

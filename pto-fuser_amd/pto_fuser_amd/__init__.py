@@ -23,7 +23,7 @@ from .policy import PlannedTransform, Policy
 from .registry import OpaqueContract, OpaqueRegistry, capture_mode, default_registry
 from .report import CompilationReport, TransformRecord
 from .serving import (add_rms_norm, add_rms_norm_fp8, causal_conv, causal_conv_step, gdn_step,
-                      ssm_step)
+                      ssm_chunk_forward, ssm_step)
 from .template import (EpilogueUnit, FuseChunkOFlash, FuseContractionEpilogue,
                        FusePerDimChunkOFlash, ScoreTemplate, Template, default_templates,
                        epilogue_report, extract_epilogue_unit)
@@ -33,7 +33,7 @@ from .transform import (EnableDirectReads, EnableFusedStore, Transform, Transfor
 __all__ = [
     "gdn_chunk_forward", "kda_chunk_forward", "kkt_inverse", "tri_inv", "gated_qk", "qkv_flash",
     "chunk_scan",
-    "causal_conv", "causal_conv_step", "ssm_step", "gdn_step", "add_rms_norm", "add_rms_norm_fp8",
+    "causal_conv", "causal_conv_step", "ssm_chunk_forward", "ssm_step", "gdn_step", "add_rms_norm", "add_rms_norm_fp8",
     "TensorRef", "Node", "EinsumNode", "OpaqueNode", "VecGlueNode", "TensorOp", "FusedNode",
     "Program", "Dataflow", "ProgramEdit", "StagedExecutor", "OpaqueRegistry", "OpaqueContract",
     "default_registry", "capture_mode", "GateResult", "FusedContract", "FusedKernel",

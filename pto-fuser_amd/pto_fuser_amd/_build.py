@@ -38,7 +38,7 @@ ARCH = os.environ.get("PF_OFFLOAD_ARCH", "gfx950")
 HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 ILP_FLAGS = ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]
-DEFAULT_SCHED_SOURCES = ("pf_seg.hip", "pf_serving.hip", "pf_stages.hip")
+DEFAULT_SCHED_SOURCES = ("pf_seg.hip", "pf_serving.hip", "pf_ssm.hip", "pf_stages.hip")
 OBJ_DIR = os.path.join(ROOT, "_build")
 
 

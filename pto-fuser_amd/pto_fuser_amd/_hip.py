@@ -61,6 +61,8 @@ SIGNATURES = {
     # one packed argument struct (bytes, read during the call) and the stream
     "pf_conv_exec": (c_int, [c_void_p, c_void_p]),
     "pf_conv_step_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_ssm_workspace_bytes": (c_size_t, [c_int] * 7),
+    "pf_ssm_exec": (c_int, [c_void_p, c_void_p]),
     "pf_ssm_step_exec": (c_int, [c_void_p, c_void_p]),
     "pf_gdn_step_exec": (c_int, [c_void_p, c_void_p]),
     "pf_norm_exec": (c_int, [c_void_p, c_void_p]),

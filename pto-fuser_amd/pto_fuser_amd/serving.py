@@ -3,7 +3,7 @@ tokens.
 
 * :func:`causal_conv`, :func:`causal_conv_step` — the short depthwise convolution along the tokens, for prompts and for
   single tokens, with its state.
-* :func:`ssm_step` — one token of the selective state space recurrence.
+* :func:`ssm_chunk_forward`, :func:`ssm_step` — the selective state space scan, over prompts and for single tokens.
 * :func:`gdn_step` — one token of the gated delta rule (GDN; DeltaNet with ``g is None``; KDA with a gate per channel):
   continues the final state of ``gdn_chunk_forward`` and ``kda_chunk_forward``.
 * :func:`add_rms_norm`, :func:`add_rms_norm_fp8` — the norm with the residual's addition, in the rows' type or in 8 bits
@@ -13,8 +13,9 @@ No counterpart in the reference, whose path ends at the chunked forward.  Forwar
 
 Unlike those, the operands may be views: batch, head and token strides are free (a slice of a projection's output, a
 transposed head layout); only the innermost dimension is contiguous.  Every operator raises ``ValueError`` before
-launching for what it does not support, launches once on the current stream of the operands' device, and neither
-allocates beyond its outputs nor synchronises, so each can be captured in a HIP graph.
+launching for what it does not support, works on the current stream of the operands' device, and neither synchronises nor
+allocates anything but its outputs and (the scan) a workspace, from torch's allocator: each can be captured in a HIP
+graph.
 """
 from __future__ import annotations
 
@@ -30,6 +31,7 @@ from .ops import _dtype_code, _on_device, _require
 _CONV = struct.Struct("@N7P6q7i")
 _CONV_STEP = struct.Struct("@N6P3q7i")
 _STEP = struct.Struct("@N13P13q10if")
+_SSM = struct.Struct("@N13PN18q9i")
 _NORM = struct.Struct("@N6P4q7if")
 
 
@@ -38,10 +40,12 @@ def _size(layout: struct.Struct) -> int:
     return (layout.size + 7) & ~7
 
 
-_CONV_SIZE, _CONV_STEP_SIZE, _STEP_SIZE, _NORM_SIZE = (_size(s) for s in (_CONV, _CONV_STEP, _STEP, _NORM))
+_CONV_SIZE, _CONV_STEP_SIZE, _STEP_SIZE, _SSM_SIZE, _NORM_SIZE = (
+    _size(s) for s in (_CONV, _CONV_STEP, _STEP, _SSM, _NORM))
 
 CONV_TAPS = (2, 3, 4)
 STEP_MAX_ROWS = 256
+SSM_MAX_ROWS, SSM_MAX_COLS = 128, 256
 NORM_MAX_WIDTH = 32768
 _ACTIVATIONS = {None: 0, "silu": 1}
 
@@ -189,6 +193,75 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
           state.data_ptr(), _ptr(slots), y.data_ptr(), x.stride(0), y.stride(0), (K - 1) * W, B,
           state.shape[0], W, K, code, w_f32, _act(activation))
     return y
+
+
+# ------------------------------------------------------------------------------------------
+#  Selective state space scan
+# ------------------------------------------------------------------------------------------
+def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                      D: Optional[torch.Tensor] = None, *, z: Optional[torch.Tensor] = None,
+                      dt_bias: Optional[torch.Tensor] = None, dt_softplus: bool = False,
+                      h0: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                      output_final_state: bool = True, out: Optional[torch.Tensor] = None,
+                      final_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Selective state space scan over prompts, in chunks of 64 tokens:
+
+        dt = softplus(dt + dt_bias),  S_t = e^{dt·A} S_{t-1} + B_t (dt·x_t)ᵀ,  y_t = C_tᵀ S_t + D·x_t  (times silu(z_t))
+
+    x, z [B,H,T,P] float32 or bfloat16, P a multiple of 32 up to 256; dt [B,H,T] in x's type or float32; B, C [B,G,T,N], N a
+    multiple of 16 up to 128, head h reading group h // (H // G); A, D, dt_bias [H] float32 (A < 0: it decays); h0
+    [B,H,N,P] float32.  Any T.  Batch, head and token strides are free: ``xbc[..., :H*P].unflatten(-1, (H, P)).transpose(1,
+    2)`` of a convolved row [B,T,..] is read in place.  ``lengths`` [B] int32 (None: all T): tokens of each sequence; what
+    follows them is not read, y is zero there, and the state is that after the last one.
+
+    Returns (y [B,H,T,P] in x's type, token-major in memory where x is; the final state [B,H,N,P] float32 or None).
+    ``final_out`` may be h0.  Few sequences run as segments side by side, whose number follows from the call's shape: the
+    same bfloat16 sequence alone and in a batch differs by its rounding."""
+    dev = _on_device(x, "x")
+    _dim(x, "x", 4, "[B,H,T,P]")
+    _dim(B, "B", 4, "[B,G,T,N]")
+    nb, H, T, P = x.shape
+    G, N = B.shape[1], B.shape[3]
+    code, dtype = _dtype_code(x.dtype), x.dtype
+    if H == 0 or G == 0 or H % G or not 0 < P <= SSM_MAX_COLS or P % 32 or not 0 < N <= SSM_MAX_ROWS or N % 16:
+        raise ValueError(f"unsupported shape H={H} G={G} N={N} P={P} (H a multiple of G, N of 16 up to {SSM_MAX_ROWS}, "
+                         f"P of 32 up to {SSM_MAX_COLS})")
+    _require_view(x, "x", (nb, H, T, P), dtype, dev)
+    _require_view(B, "B", (nb, G, T, N), dtype, dev)
+    _require_view(C, "C", (nb, G, T, N), dtype, dev)
+    _dim(dt, "dt", 3, "[B,H,T]")
+    dt_f32 = _param_f32(dt, "dt", dtype)
+    if tuple(dt.shape) != (nb, H, T) or dt.device != dev:
+        raise ValueError(f"dt is {tuple(dt.shape)} on {dt.device}, expected {(nb, H, T)} on {dev}")
+    if A is None:
+        raise ValueError("A must be a tensor")
+    for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
+        _require(t, name, (H,), torch.float32, dev)
+    if z is not None:
+        _require_view(z, "z", (nb, H, T, P), dtype, dev)
+    _require(h0, "h0", (nb, H, N, P), torch.float32, dev)
+    _require(lengths, "lengths", (nb,), torch.int32, dev)
+    sx = x.stride()
+    if out is not None:
+        _require_view(out, "out", (nb, H, T, P), dtype, dev)
+        y = out
+    elif sx[1] < sx[2]:
+        y = torch.empty(nb, T, H, P, device=dev, dtype=dtype).transpose(1, 2)
+    else:
+        y = torch.empty(nb, H, T, P, device=dev, dtype=dtype)
+    final = None
+    if output_final_state:
+        _require(final_out, "final_out", (nb, H, N, P), torch.float32, dev)
+        final = torch.empty(nb, H, N, P, device=dev, dtype=torch.float32) if final_out is None else final_out
+    need = _hip.load().pf_ssm_workspace_bytes(nb, H, G, T, N, P, code)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    sb, sc, sy, st = B.stride(), C.stride(), y.stride(), dt.stride()
+    sz = (0, 0, 0) if z is None else z.stride()
+    _exec("pf_ssm_exec", dev, _SSM, _SSM_SIZE, x.data_ptr(), dt.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(z),
+          A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(h0), _ptr(lengths), y.data_ptr(), _ptr(final), _ptr(ws), need,
+          sx[0], sx[1], sx[2], st[0], st[1], st[2], sb[0], sb[1], sb[2], sc[0], sc[1], sc[2], sz[0], sz[1], sz[2],
+          sy[0], sy[1], sy[2], nb, H, G, T, N, P, code, dt_f32, int(bool(dt_softplus)))
+    return y, final
 
 
 # ------------------------------------------------------------------------------------------

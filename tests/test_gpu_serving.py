@@ -367,3 +367,171 @@ def test_steps_in_a_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(flat(outs), want))
         assert all(torch.equal(a, b) for a, b in zip(captured, eager))
+
+
+# ------------------------------------------------------------------------------------------
+#  State space scan over prompts.  32-bit operations on a term of the state or of y: the step and its softplus, the chunk's
+#  decay (an exponential of a sum of up to 64 gates, whose own error is relative to its size: the tests keep a chunk's
+#  under 2^4, so 64 gates' roundings cost 2^4 of the 2^-24), a product a chunk from there on, and additions in a tree over
+#  64 tokens and 128 rows.  bfloat16 operands besides: the score's and the entering state's rounding to 8 bits, of each
+#  term, by at most 2^-9 (the state's update has its weighted x in 16 bits or more, 2^-17 of each term).
+# ------------------------------------------------------------------------------------------
+def _ssm_ops(T):
+    return 160 + (T + 63) // 64
+
+
+def _ssm_case(seed, dtype, B, H, T, P, G, N, z=True, h0=True, D=True):
+    r = _rand(seed)
+    s = {"x": _dev(r(B, H, T, P), dtype), "dt": _dev(0.5 * r(B, H, T), dtype), "A": _dev(-1 - r(H).abs()),
+         "B": _dev(r(B, G, T, N), dtype), "C": _dev(r(B, G, T, N), dtype), "D": _dev(r(H)) if D else None,
+         "z": _dev(r(B, H, T, P), dtype) if z else None, "dt_bias": _dev(0.3 * r(H) - 3.5)}
+    s["h0"] = _dev(r(B, H, N, P)) if h0 else None
+    return s
+
+
+def _check_ssm(s, y, final, lengths=None, what="", softplus=True):
+    args = {k: ref.f64(v) for k, v in s.items()}
+    want, mag, S, M = ref.ssm(args["x"], args["dt"], args["A"], args["B"], args["C"], args["D"], args["z"], args["dt_bias"],
+                              softplus, args["h0"], lengths)
+    ops = _ssm_ops(s["x"].shape[2])
+    if y.dtype is BF:
+        # the roundings to 8 bits are independent from term to term: over n terms their sum is some sqrt(n) of one, and
+        # far below the sum of their bounds, which is what is allowed here
+        ops += 2 * 2 ** 24 / 2 ** 9
+    ref.check(y, want, mag, ops, what + " y")
+    if final is not None:
+        # of the state's terms nothing is rounded below 24 bits
+        ref.check(final, S, M, _ssm_ops(s["x"].shape[2]), what + " state")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,H,T,P,G,N", [(1, 1, 1, 32, 1, 16), (1, 2, 5, 64, 1, 128), (2, 3, 64, 64, 1, 64), (1, 4, 65, 32, 2, 128),
+                                         (1, 4, 131, 64, 1, 128), (2, 2, 200, 128, 2, 32), (1, 5, 333, 96, 1, 48), (1, 1, 300, 256, 1, 112),
+                                         (3, 6, 90, 64, 3, 80), (1, 9, 520, 64, 1, 128)])
+def test_ssm(dtype, B, H, T, P, G, N):
+    announce(f"ssm_chunk_forward {dtype} B{B} H{H} T{T} P{P} G{G} N{N}")
+    s = _ssm_case(T + N, dtype, B, H, T, P, G, N)
+    y, final = pf_ssm(s)
+    _check_ssm(s, y, final)
+
+
+def pf_ssm(s, **kw):
+    from pto_fuser_amd import ssm_chunk_forward
+    return ssm_chunk_forward(s["x"], s["dt"], s["A"], s["B"], s["C"], s["D"], z=s["z"], dt_bias=s["dt_bias"],
+                             dt_softplus=True, h0=s["h0"], **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_ssm_views(dtype):
+    """x, B and C in place in one convolved row per token, dt and z of projections; no state in, no D; y comes token-major."""
+    announce(f"ssm_chunk_forward views {dtype}")
+    B, T, H, P, G, N = 2, 150, 4, 64, 2, 32
+    r = _rand(1)
+    row = _wide(_dev(r(B, T, H * P + 2 * G * N), dtype), 9)
+    x, b, c = row.split([H * P, G * N, G * N], dim=-1)
+    s = {"x": x.unflatten(-1, (H, P)).transpose(1, 2), "B": b.unflatten(-1, (G, N)).transpose(1, 2),
+         "C": c.unflatten(-1, (G, N)).transpose(1, 2), "dt": _dev(0.5 * r(B, T, H)).transpose(1, 2), "A": _dev(-1 - r(H).abs()),
+         "D": None, "z": _wide(_dev(r(B, T, H, P), dtype), 3).transpose(1, 2), "dt_bias": _dev(r(H) - 4), "h0": None}
+    y, final = pf_ssm(s)
+    assert y.transpose(1, 2).is_contiguous()
+    _check_ssm(s, y, final)
+    again, none = pf_ssm(s, output_final_state=False, out=torch.empty(B, H, T, P + 4, device=DEV, dtype=dtype)[..., :P])
+    assert none is None and torch.equal(again, y)
+    packed = {k: None if v is None else v.contiguous() for k, v in s.items()}
+    assert all(torch.equal(a, b) for a, b in zip(pf_ssm(packed), (y, final)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_ssm_lengths(dtype):
+    """Sequences of 0, 1, 63, 64, 65 .. tokens in one batch of segments: what follows them is NaN and is not read."""
+    announce(f"ssm_chunk_forward lengths {dtype}")
+    lengths = [0, 1, 63, 64, 65, 128, 200, 299, 300]
+    B, H, T, P, G, N = len(lengths), 2, 300, 32, 1, 32
+    s = _ssm_case(7, dtype, B, H, T, P, G, N)
+    clean = {k: None if v is None else v.clone() for k, v in s.items()}
+    for i, n in enumerate(lengths):
+        for k in ("x", "dt", "B", "C", "z"):
+            s[k][i, :, n:] = NAN
+    final = s["h0"]
+    y, got = pf_ssm(s, lengths=torch.tensor(lengths, dtype=torch.int32, device=DEV), final_out=final)
+    assert got is final
+    _check_ssm(clean, y, got, lengths)
+    for i, n in enumerate(lengths):
+        assert not y[i, :, n:].any()
+    assert torch.equal(final[0], clean["h0"][0])
+
+
+def test_ssm_of_no_tokens():
+    announce("ssm_chunk_forward T=0, B=0")
+    s = _ssm_case(1, F32, 2, 2, 0, 32, 1, 16)
+    y, final = pf_ssm(s)
+    assert y.shape == (2, 2, 0, 32) and torch.equal(final, s["h0"])
+    y, final = pf_ssm(_ssm_case(1, F32, 0, 2, 5, 32, 1, 16))
+    assert y.shape == (0, 2, 5, 32) and final.shape == (0, 2, 16, 32)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_ssm_strong_and_no_decay(dtype):
+    """Heads whose state is gone within a token, heads that never decay, and one that grows: no overflow where the result
+    has none."""
+    announce(f"ssm_chunk_forward decays {dtype}")
+    s = _ssm_case(3, dtype, 1, 4, 200, 32, 1, 32)
+    s["dt_bias"] = torch.tensor([3.0, -4.0, -4.0, 1.0], device=DEV)
+    s["A"] = torch.tensor([-60.0, 0.0, 0.01, -3.0], device=DEV)
+    y, final = pf_ssm(s)
+    args = {k: ref.f64(v) for k, v in s.items()}
+    want, mag, S, M = ref.ssm(args["x"], args["dt"], args["A"], args["B"], args["C"], args["D"], args["z"], args["dt_bias"], True,
+                              args["h0"])
+    # a chunk's gates sum to 64 * 4 * 60 at most here, 2^14: 10 bits more than the tests above allow for
+    ops = _ssm_ops(200) + 64 * 2 ** 10 + (2 ** 16 if dtype is BF else 0)
+    ref.check(y, want, mag, ops, "y")
+    ref.check(final, S, M, ops, "state")
+
+
+def test_ssm_workspace_is_optional():
+    """Through the C entry without a workspace: whole sequences, within rounding of the segments."""
+    from pto_fuser_amd import _hip, serving
+    announce("pf_ssm_exec without a workspace")
+    s = _ssm_case(5, F32, 1, 2, 1000, 64, 1, 64)
+    assert _hip.load().pf_ssm_workspace_bytes(1, 2, 1, 1000, 64, 64, 0) > 0
+    y, final = pf_ssm(s)
+    y2, final2 = torch.empty_like(y), torch.empty_like(final)
+    st = lambda t: t.stride()[:3]  # noqa: E731
+    serving._exec("pf_ssm_exec", s["x"].device, serving._SSM, serving._SSM_SIZE, s["x"].data_ptr(), s["dt"].data_ptr(),
+                  s["B"].data_ptr(), s["C"].data_ptr(), s["z"].data_ptr(), s["A"].data_ptr(), s["D"].data_ptr(),
+                  s["dt_bias"].data_ptr(), s["h0"].data_ptr(), 0, y2.data_ptr(), final2.data_ptr(), 0, 0, *st(s["x"]),
+                  *s["dt"].stride(), *st(s["B"]), *st(s["C"]), *st(s["z"]), *st(y2), 1, 2, 1, 1000, 64, 64, 0, 0, 1)
+    _check_ssm(s, y, final, what="segments")
+    _check_ssm(s, y2, final2, what="whole")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_ssm_step_continues_the_prompt(dtype):
+    announce(f"ssm_step after ssm_chunk_forward {dtype}")
+    s = _ssm_case(9, dtype, 2, 4, 71, 64, 2, 64, h0=False)
+    cut = {k: v[:, :, :67] if k in ("x", "dt", "B", "C", "z") else v for k, v in s.items()}
+    first, state = pf_ssm(cut)
+    rest = [ssm_step(state, *(s[k][:, :, t] for k in ("x", "dt")), s["A"], s["B"][:, :, t], s["C"][:, :, t], s["D"],
+                     z=s["z"][:, :, t], dt_bias=s["dt_bias"], dt_softplus=True) for t in range(67, 71)]
+    _check_ssm(s, torch.cat([first, torch.stack(rest, 2)], 2), state)
+
+
+def test_ssm_in_a_graph():
+    """Captured, segments and all, and replayed on changing inputs with eager calls between."""
+    announce("captured ssm_chunk_forward")
+    s = _ssm_case(13, BF, 1, 4, 700, 64, 1, 128)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        pf_ssm(s)
+        with torch.cuda.graph(graph, stream=stream):
+            y, final = pf_ssm(s)
+    torch.cuda.synchronize()
+    for i in range(4):
+        s["x"].copy_(_dev(_rand(100 + i)(*s["x"].shape), BF))
+        want = pf_ssm(s)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(final, want[1])

@@ -10,7 +10,7 @@ import pto_fuser_amd as pf
 from pto_fuser_amd import _build, _hip, ops, serving
 
 STRUCTS = {"pf_conv_args": serving._CONV_SIZE, "pf_conv_step_args": serving._CONV_STEP_SIZE, "pf_step_args": serving._STEP_SIZE,
-           "pf_norm_args": serving._NORM_SIZE}
+           "pf_ssm_args": serving._SSM_SIZE, "pf_norm_args": serving._NORM_SIZE}
 
 
 @pytest.fixture(scope="module")
@@ -90,6 +90,35 @@ def test_gdn_step_statuses(lib, bad):
     assert lib.pf_gdn_step_exec(_step(**bad), None) == _hip.PF_ERR_ARG
 
 
+def _ssm(**kw):
+    f = dict(size=serving._SSM_SIZE, x=64, dt=64, b=64, c=64, z=0, a=64, d=0, dt_bias=0, h0=0, lengths=0, y=64, h_final=0, ws=0,
+             ws_bytes=0)
+    f.update({f"s{i}": 0 for i in range(18)})
+    f.update(B=1, H=4, G=2, T=100, N=64, P=64, dtype=1, dt_f32=0, softplus=0)
+    assert not set(kw) - set(f)
+    return serving._SSM.pack(*{**f, **kw}.values())
+
+
+@pytest.mark.parametrize("bad", [dict(size=0), dict(dtype=2), dict(H=3), dict(H=0), dict(G=0), dict(N=144), dict(N=24), dict(N=0),
+                                 dict(P=48), dict(P=288), dict(P=0), dict(T=-1), dict(B=-1), dict(x=0), dict(dt=0), dict(b=0), dict(c=0),
+                                 dict(y=0), dict(a=0), dict(s0=-1), dict(s17=-1), dict(B=1 << 30, H=1 << 20, G=1)])
+def test_ssm_statuses(lib, bad):
+    assert lib.pf_ssm_exec(_ssm(**bad), None) == _hip.PF_ERR_ARG
+
+
+def test_ssm_workspace_sizes(lib):
+    """Whole sequences need none; segments a state and a decay each, never more than a generation of workgroups' worth;
+    an unsupported shape, or one past any memory, reports 0."""
+    size = lib.pf_ssm_workspace_bytes
+    assert lib.pf_ssm_exec(_ssm(B=0), None) == _hip.PF_OK
+    assert size(1, 4, 1, 64, 128, 64, 1) == 0 and size(64, 64, 1, 8192, 128, 64, 1) == 0
+    assert size(1, 4, 1, 8192, 100, 64, 1) == 0 and size(1 << 20, 1 << 20, 1, 8192, 128, 64, 1) == 0
+    for H, G, T, N, P in ((4, 1, 8192, 128, 64), (32, 1, 32768, 128, 64), (32, 32, 4096, 64, 128), (1, 1, 1 << 30, 16, 32)):
+        n = size(1, H, G, T, N, P, 1)
+        one = H * (N * P + 1) * 4
+        assert n and n % one == 0 and 2 <= n // one <= 512 and n == size(1, H, G, T, N, P, 0)
+
+
 def _norm(**kw):
     f = dict(size=serving._NORM_SIZE, x=64, residual=0, w=64, y=64, scales=0, h=0, x_row=8, r_row=8, y_row=8, h_row=8, rows=1, D=256,
              dtype=1, y_dtype=1, r_f32=0, w_f32=0, block=0, eps=1e-6)
@@ -164,6 +193,32 @@ def test_step_refusals(on_cpu):
             ("g has shape", lambda: pf.gdn_step(S, q, q, x, dt, dt[:1])),
             ("k has shape", lambda: pf.gdn_step(S, q, q[:, :2], x, dt)),
             ("out has dtype", lambda: pf.gdn_step(S, q.bfloat16(), q.bfloat16(), x.bfloat16(), dt, out=x.bfloat16()))):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not on_cpu
+
+
+def test_ssm_refusals(on_cpu):
+    x, b = torch.zeros(2, 4, 9, 32), torch.zeros(2, 2, 9, 16)
+    dt, A, h0 = torch.zeros(2, 4, 9), torch.zeros(4), torch.zeros(2, 4, 16, 32)
+    pf.ssm_chunk_forward(x, dt, A, b, b, A, z=x, dt_bias=A, h0=h0)
+    assert on_cpu.pop()[0] == "pf_ssm_exec"
+    for match, call in (
+            (r"\[B,H,T,P\]", lambda: pf.ssm_chunk_forward(x[0], dt, A, b, b)),
+            ("multiple of G", lambda: pf.ssm_chunk_forward(x, dt, A, torch.zeros(2, 3, 9, 16), b)),
+            ("P of 32", lambda: pf.ssm_chunk_forward(x[..., :16], dt, A, b, b)),
+            ("N of 16", lambda: pf.ssm_chunk_forward(x, dt, A, torch.zeros(2, 2, 9, 144), b)),
+            ("dtype", lambda: pf.ssm_chunk_forward(x.half(), dt, A, b, b)),
+            ("B has shape", lambda: pf.ssm_chunk_forward(x, dt, A, b[:, :, :8], b)),
+            ("C has dtype", lambda: pf.ssm_chunk_forward(x, dt, A, b, b.bfloat16())),
+            ("dt is", lambda: pf.ssm_chunk_forward(x, dt[:, :, :8], A, b, b)),
+            ("A has shape", lambda: pf.ssm_chunk_forward(x, dt, A[:2], b, b)),
+            ("last dimension", lambda: pf.ssm_chunk_forward(torch.zeros(2, 4, 32, 9).transpose(2, 3), dt, A, b, b)),
+            ("z has shape", lambda: pf.ssm_chunk_forward(x, dt, A, b, b, z=x[:1])),
+            ("h0 has shape", lambda: pf.ssm_chunk_forward(x, dt, A, b, b, h0=h0.transpose(2, 3))),
+            ("lengths has dtype", lambda: pf.ssm_chunk_forward(x, dt, A, b, b, lengths=torch.zeros(2))),
+            ("final_out has shape", lambda: pf.ssm_chunk_forward(x, dt, A, b, b, final_out=h0[:1])),
+            ("out has dtype", lambda: pf.ssm_chunk_forward(x, dt, A, b, b, out=x.bfloat16()))):
         with pytest.raises(ValueError, match=match):
             call()
     assert not on_cpu
