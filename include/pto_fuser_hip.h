@@ -302,7 +302,8 @@ int pf_gdn_step_exec(const pf_step_args* args, void* stream);
  * [B,H,N,P] fp32 contiguous (h_final may be h0).  lengths [B] (NULL: all T): the tokens of each sequence;
  * later ones are not read, y is zero there, and the state is that after the last one.  Any T >= 0.
  * The scan runs 64-token chunks; a non-finite operand reaches all of its chunk's rows.
- * Supported: P a multiple of 32 up to 256, N a multiple of 16 up to 128.
+ * Supported: P a multiple of 32 up to 256, N a multiple of 16 up to 128; token strides of x, b, c, z and y of a
+ * row at least and 2^22 elements at most.
  * Few sequences run as segments side by side when `workspace` holds their states
  * (pf_ssm_workspace_bytes: arithmetic, 0 where whole sequences fill the chip or the shape is not supported);
  * on a smaller one, or NULL, the same call runs whole sequences.  The number of segments follows from the

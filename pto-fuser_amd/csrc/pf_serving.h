@@ -13,9 +13,13 @@ __device__ __forceinline__ long block_id() { return (long)blockIdx.y * gridDim.x
 // sigmoid(v) v.  exp(-v) = inf gives v * 0, so the far negative side ends in -0 and not in NaN.
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
-// log(1 + e^v), to full precision where e^v is small: a step of 1e-3 is e^v = 1e-3, of which 1 + e^v would
-// keep four digits.
-__device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1pf(expf(v)); }
+// log(1 + e^v) = max(v, 0) + log(1 + u), u = e^-|v|.  1 + u keeps few digits of a small u (a step of 1e-3 would have
+// four): the logarithm of the rounded w = 1 + u is scaled by u / (w - 1), which is exact to first order (Kahan's log1p).
+__device__ __forceinline__ float softplus(float v) {
+  const float u = __expf(-fabsf(v)), w = 1.f + u, d = w - 1.f;
+  const float l = __logf(w) * (u * __builtin_amdgcn_rcpf(d));
+  return fmaxf(v, 0.f) + (d == 0.f ? u : l);
+}
 
 // One value of a tensor that is fp32 or the operands' type.
 template <typename E>

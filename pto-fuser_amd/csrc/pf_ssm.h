@@ -4,8 +4,8 @@
 //   S  <- e^{G_last} S + sum_t B_t (e^{G_last - G_t} dt_t x_t)^T
 // B and C belong to a group of heads, so the score C B^T is the same for all of them.
 //
-// A workgroup walks the chunks of one (sequence, group, block of heads): NW waves, each the owner of 32 columns of one
-// head.  A wave's state stays in its registers as MFMA results S[n, p] (rows n, column p a lane), which are at once the
+// A workgroup walks the chunks of one (sequence, group, block of columns): NW waves, each the owner of 16 or 32 columns
+// of one head.  A wave's state stays in its registers as MFMA results S[n, p] (rows n, column p a lane), which are at once the
 // operand of y^T = S^T C^T; y^T = x^T P^T takes the score tiles the same way, so the only exchanges are the staged rows
 // of B and C and the score tiles, which the waves compute together.  (Permuted K: see pf_device.h.)
 //
@@ -19,9 +19,9 @@
 
 namespace pf {
 
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kSsmChunk = 64;
+// A thread's offset inside a chunk is 32-bit: 64 tokens of this many 4-byte elements.
+constexpr long kMaxTokenStride = 1L << 22;
 
 struct SsmArgs {
   const void* x;
@@ -39,15 +39,39 @@ struct SsmArgs {
   float* seg_state;        // [B, H, segs, N, P]: what a segment adds, then what enters it
   float* seg_decay;        // [B, H, segs]: log2 of a segment's decay
   long x_b, x_h, x_t, dt_b, dt_h, dt_t, b_b, b_g, b_t, c_b, c_g, c_t, z_b, z_h, z_t, y_b, y_h, y_t;
-  long tasks;              // B * G * head blocks * segments
+  uint32_t tasks;          // B * G * column blocks * segments
   int B, H, G, T, N, P;
-  int heads;               // heads of a workgroup
-  int blocks;              // blocks of heads of a group
+  int blocks;              // blocks of columns of a group's heads
   int segs, seg_chunks;
   int dt_f32, softplus;
 };
 
 enum class SsmMode { kStates, kOutput };
+
+// A buffer offset past the end of any: reads as zero, is not written.
+constexpr uint32_t kPastEnd = 0x80000000u;
+
+template <typename E> __device__ __forceinline__ void buf_load4(__amdgpu_buffer_rsrc_t r, uint32_t off, float (&v)[4]);
+template <> __device__ __forceinline__ void buf_load4<bf16>(__amdgpu_buffer_rsrc_t r, uint32_t off, float (&v)[4]) {
+  const bf16x4 x = __builtin_bit_cast(bf16x4, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
+}
+template <> __device__ __forceinline__ void buf_load4<float>(__amdgpu_buffer_rsrc_t r, uint32_t off, float (&v)[4]) {
+  const floatx4 x = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = x[i];
+}
+template <typename E> __device__ __forceinline__ void buf_store4(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&v)[4]);
+template <> __device__ __forceinline__ void buf_store4<bf16>(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&v)[4]) {
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  const bf16x4 x = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), r, off, 0, 0);
+}
+template <> __device__ __forceinline__ void buf_store4<float>(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&v)[4]) {
+  const floatx4 x = {v[0], v[1], v[2], v[3]};
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), r, off, 0, 0);
+}
 
 // ---- one MFMA operand of 32 contraction rows: eight values a lane ---------------------------
 template <typename E> struct Frag;
@@ -70,39 +94,34 @@ template <typename E> __device__ __forceinline__ Frag<E> frag_of(const floatx4& 
 template <> __device__ __forceinline__ Frag<bf16> frag_of<bf16>(const floatx4& lo, const floatx4& hi) { return {pack8(lo, hi)}; }
 template <> __device__ __forceinline__ Frag<float> frag_of<float>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
 
-// ---- LDS tiles ------------------------------------------------------------------------------
-// Rows of B or C, [64][NT].  bf16: within each 32 columns the eight 4-column units are stored in the order 0 4 1 5 2 6 3 7,
-// so that lane group g finds its two units (4g.., 16 + 4g..) side by side; the rows are 16 bytes apart modulo the banks.
-template <typename E, int NT> struct RowTile {
-  static constexpr int LD = NT + 16 / (int)sizeof(E);
+template <typename E, typename V> __device__ __forceinline__ Frag<E> frag_cat(const V& lo, const V& hi);
+template <> __device__ __forceinline__ Frag<bf16> frag_cat<bf16, bf16x4>(const bf16x4& lo, const bf16x4& hi) { return {cat8(lo, hi)}; }
+template <> __device__ __forceinline__ Frag<float> frag_cat<float, floatx4>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
+
+// ---- LDS tiles: 64 token rows, PAD elements longer than they are ----------------------------
+// Rows 16 bytes apart modulo the banks suit the operand that reads sixteen rows at one place; 32 bytes the transposed one,
+// which reads eight rows at four neighbouring 8-byte places in half a wave.  fp32 rows are 16 bytes apart.
+template <typename E, int W, int PAD> struct Tile {
+  static constexpr int LD = W + PAD;
   static constexpr int ELEMS = kSsmChunk * LD;
-  // 16 bytes of row `row`, column vector `vec`
-  __device__ __forceinline__ static void put(E* s, int row, int vec, const u32x4& v) {
-    if constexpr (sizeof(E) == 2) {
-      const int q = vec & 3;                               // units 2q and 2q + 1
-      E* p = s + row * LD + (vec >> 2) * 32 + 4 * ((q & 1) * 4 + (q >> 1));
-      *reinterpret_cast<u32x2*>(p) = u32x2{v[0], v[1]};
-      *reinterpret_cast<u32x2*>(p + 8) = u32x2{v[2], v[3]};
-    } else {
-      *reinterpret_cast<u32x4*>(s + row * LD + vec * 4) = v;
-    }
-  }
-  // operand: lane c holds row `row`, lane group g its eight of columns 32 kb ..
+  // operand: lane c holds row `row`, lane group g the eight columns 32 kb + 8g ..
   __device__ __forceinline__ static Frag<E> rows(const E* s, int row, int kb, int g) {
+    const E* p = s + row * LD + kb * 32 + g * 8;
     if constexpr (sizeof(E) == 2) {
-      return {*reinterpret_cast<const bf16x8*>(s + row * LD + kb * 32 + g * 8)};
+      return {*reinterpret_cast<const bf16x8*>(p)};
     } else {
-      const E* p = s + row * LD + kb * 32 + g * 4;
-      return {*reinterpret_cast<const floatx4*>(p), *reinterpret_cast<const floatx4*>(p + 16)};
+      return {*reinterpret_cast<const floatx4*>(p), *reinterpret_cast<const floatx4*>(p + 4)};
     }
   }
-  // transposed operand: lane c holds column 16 nt + c, lane group g its eight of rows 32 kb ..
-  __device__ __forceinline__ static Frag<E> cols(const E* s, int nt, int kb, int c, int g) {
+  // transposed operand: lane c holds column col + c (APART = 4), or col + 8 (c / 4) + c % 4 (APART = 8); lane group g rows
+  // 32 kb + 4g .. and 32 kb + 16 + 4g ..
+  template <int APART>
+  __device__ __forceinline__ static Frag<E> cols(const E* s, int col, int kb, int c, int g) {
     if constexpr (sizeof(E) == 2) {
-      const E* p = s + (32 * kb + 4 * g + (c >> 2)) * LD + (nt >> 1) * 32 + 4 * (2 * (c & 3) + (nt & 1));
+      const E* p = s + (32 * kb + 4 * g + (c >> 2)) * LD + col + APART * (c & 3);
       return {cat8(lds_read_tr(p), lds_read_tr(p + 16 * LD))};
     } else {
-      const E* p = s + (32 * kb + 4 * g) * LD + 16 * nt + c;
+      const E* p = s + (32 * kb + 4 * g) * LD + col + APART * (c >> 2) + (c & 3);
       Frag<E> f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -113,309 +132,395 @@ template <typename E, int NT> struct RowTile {
     }
   }
 };
+// Row of the state that lane group g holds as register r of tile nt.  The tiles of a pair interleave, four rows each, so
+// that a lane group's rows in the two are the eight neighbouring columns of B or C it reads as one vector.
+__device__ __forceinline__ constexpr int state_row(int nt, int g, int r) { return 32 * (nt >> 1) + 8 * g + 4 * (nt & 1) + r; }
 
-// A wave's 32 columns of x, [64][32].
-template <typename E> struct XTile {
-  static constexpr int LD = 32 + 16 / (int)sizeof(E);
-  static constexpr int ELEMS = kSsmChunk * LD;
-  // operand: lane c holds column 16 pt + c, lane group g its eight of rows 32 kb ..
-  __device__ __forceinline__ static Frag<E> cols(const E* s, int pt, int kb, int c, int g) {
-    if constexpr (sizeof(E) == 2) {
-      const E* p = s + (32 * kb + 4 * g + (c >> 2)) * LD + 16 * pt + 4 * (c & 3);
-      return {cat8(lds_read_tr(p), lds_read_tr(p + 16 * LD))};
-    } else {
-      const E* p = s + (32 * kb + 4 * g) * LD + 16 * pt + c;
-      Frag<E> f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f.lo[i] = p[i * LD];
-        f.hi[i] = p[(16 + i) * LD];
-      }
-      return f;
-    }
-  }
-};
+template <typename E> struct TileVec4;        // an MFMA result as four operand values
+template <> struct TileVec4<bf16> { typedef bf16x4 T; };
+template <> struct TileVec4<float> { typedef floatx4 T; };
 
-// acc += A (x scaled by its rows' weights): the weighted operand in SPLIT bf16 terms, each the rounding of what the ones
-// before it left (8, 16 or 24 bits of the product); fp32 needs none.
-template <int SPLIT> struct Weighted {
-  Frag<bf16> t[SPLIT];
-  __device__ __forceinline__ Weighted(const Frag<bf16>& x, const floatx4& w0, const floatx4& w1) {
+// x scaled by its rows' weights, in SPLIT bf16 terms: each the rounding of what the ones before it left (8, 16 or 24 bits
+// of the product); fp32 needs one.
+template <int SPLIT>
+__device__ __forceinline__ void weigh(const Frag<bf16>& x, const floatx4& w0, const floatx4& w1, Frag<bf16> (&t)[SPLIT]) {
+  const u32x4 xb = __builtin_bit_cast(u32x4, x.v);
+  u32x4 o[SPLIT];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = (float)x.v[i] * (i < 4 ? w0[i & 3] : w1[i & 3]);
+  for (int i = 0; i < 4; ++i) {                  // pairs: one conversion makes two
+    float lo = __uint_as_float(xb[i] << 16) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
+    float hi = __uint_as_float(xb[i] & 0xffff0000u) * (i < 2 ? w0[2 * i + 1] : w1[2 * i - 3]);
 #pragma unroll
-      for (int k = 0; k < SPLIT; ++k) {
-        const bf16 r = (bf16)v;
-        t[k].v[i] = r;
-        v -= (float)r;
+    for (int k = 0; k < SPLIT; ++k) {
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      o[k][i] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)lo, (bf16)hi});
+      if (k + 1 < SPLIT) {
+        lo -= __uint_as_float(o[k][i] << 16);
+        hi -= __uint_as_float(o[k][i] & 0xffff0000u);
       }
     }
   }
-  __device__ __forceinline__ floatx4 times(const Frag<bf16>& a, floatx4 acc) const {
 #pragma unroll
-    for (int k = SPLIT - 1; k >= 0; --k) acc = mfma32(a, t[k], acc);
-    return acc;
-  }
-};
-struct WeightedF32 {
-  Frag<float> t;
-  __device__ __forceinline__ WeightedF32(const Frag<float>& x, const floatx4& w0, const floatx4& w1) : t{x.lo * w0, x.hi * w1} {}
-  __device__ __forceinline__ floatx4 times(const Frag<float>& a, floatx4 acc) const { return mfma32(a, t, acc); }
-};
-template <typename E, int SPLIT> struct WeightedOf { typedef Weighted<SPLIT> T; };
-template <int SPLIT> struct WeightedOf<float, SPLIT> { typedef WeightedF32 T; };
+  for (int k = 0; k < SPLIT; ++k) t[k].v = __builtin_bit_cast(bf16x8, o[k]);
+}
+__device__ __forceinline__ void weigh(const Frag<float>& x, const floatx4& w0, const floatx4& w1, Frag<float> (&t)[1]) {
+  t[0] = {x.lo * w0, x.hi * w1};
+}
 
-template <typename E, int NT, int NW> struct SsmLds {
-  E b[RowTile<E, NT>::ELEMS];
-  E c[RowTile<E, NT>::ELEMS];
-  E x[NW][XTile<E>::ELEMS];
-  floatx4 score[10][64];            // C B^T, tile (ib, jb): lane (c, g) holds rows j = 16 jb + 4 g .. of column i = 16 ib + c
-  float tab[NW][4][kSsmChunk];      // per token: G, dt, dt 2^(G_m - G) (m: last token of its 16), dt 2^(G_last - G)
+// 2^x of the hardware: results below 2^-126 are zero.
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// v of the lane N before (SHR) or behind (SHL) within a row of 16 lanes, zero past its end.
+template <int CTRL> __device__ __forceinline__ float row_move(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// Sums over the wave's lanes up to and from each on (inclusive).  The second is summed from its own end: as the total less
+// the first it would keep the total's error where it is small.
+__device__ __forceinline__ void wave_sums(float v, int g, float& up_to, float& from) {
+  float a = v, b = v;
+  a += row_move<0x111>(a); b += row_move<0x101>(b);
+  a += row_move<0x112>(a); b += row_move<0x102>(b);
+  a += row_move<0x114>(a); b += row_move<0x104>(b);
+  a += row_move<0x118>(a); b += row_move<0x108>(b);
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(a), 16 * i + 15));
+  up_to = a + (g == 0 ? 0.f : g == 1 ? r[0] : g == 2 ? r[0] + r[1] : r[0] + r[1] + r[2]);
+  from = b + (g == 3 ? 0.f : g == 2 ? r[3] : g == 1 ? r[2] + r[3] : r[1] + (r[2] + r[3]));
+}
+
+// The outputs keep one chunk and what only they need; the states' kernel two chunks.
+template <typename E, int NT, int NW, int PT, bool OUT> struct SsmLds {
+  static constexpr int SLOTS = 4 * NW, BUF = OUT ? 1 : 2;
+  typedef Tile<E, NT, 32 / (int)sizeof(E)> B;
+  typedef Tile<E, NT, 16 / (int)sizeof(E)> C;
+  typedef Tile<E, 16 * PT, 16 / (int)sizeof(E)> X;
+  E b[BUF][B::ELEMS];
+  E x[BUF][NW][X::ELEMS];
+  E c[OUT ? C::ELEMS : 1];
+  // C B^T, tile (ib, jb) transposed: lane (c, g) holds rows j = 16 jb + 4g .. of column i = 16 ib + c.
+  floatx4 score[OUT ? 10 : 1][64];
+  // Per (chunk, head) of a batch and token: dt 2^(G_last - G), G, dt, dt 2^(G_m - G) (m: the last token of its 16).
+  float tab[SLOTS][OUT ? 4 : 1][kSsmChunk];
+  float total[SLOTS];                                  // G_last
 };
 
 // SPLIT: bf16 terms of the weighted x in the state's update.  Three keep the state a sum in 24 bits, as it has to be where
 // it is returned; two where it only enters y, whose operand S is rounded to 8 bits anyway.
-template <typename E, int NT, int NW, SsmMode MODE, int SPLIT>
-__global__ __launch_bounds__(NW * 64) void ssm_kernel(SsmArgs a) {
-  using Rows = RowTile<E, NT>;
-  using Xs = XTile<E>;
-  constexpr int Q = kSsmChunk, V = 16 / (int)sizeof(E), TH = NW * 64;
+// PT: 16-column tiles of a wave.
+template <typename E, int NT, int NW, int PT, SsmMode MODE, int SPLIT, bool HAS_Z>
+__global__ __launch_bounds__(NW * 64) __attribute__((
+    amdgpu_waves_per_eu(sizeof(E) == 4 || NW * 16 * PT < 256 ? 1 : 2))) void ssm_kernel(SsmArgs a) {
+  constexpr int Q = kSsmChunk, ES = (int)sizeof(E), V = 16 / ES, TH = NW * 64, NTS = NT / 16;
+  constexpr int COLS = NW * 16 * PT;           // columns of a workgroup
   constexpr int RV = NT / V;                   // vectors of a row of B or C
-  constexpr int NB = Q * RV / TH;              // of them a thread
-  constexpr int XV = 32 / V;                   // vectors of a row of a wave's x
+  constexpr int NB = Q * RV < TH ? 1 : Q * RV / TH;   // of them a thread, TH / RV rows apart
+  constexpr int XV = 16 * PT / V;              // vectors of a row of a wave's x
   constexpr int NX = Q * XV / 64;
   constexpr bool OUT = MODE == SsmMode::kOutput;
-  __shared__ __attribute__((aligned(16))) SsmLds<E, NT, NW> s;
+  using Lds = SsmLds<E, NT, NW, PT, OUT>;
+  using Bs = typename Lds::B;
+  using Cs = typename Lds::C;
+  using Xs = typename Lds::X;
+  __shared__ __attribute__((aligned(16))) Lds s;
 
-  // Workgroups go round robin over the eight XCDs: each XCD takes a run of tasks, whose neighbours (the blocks of heads
+  // Workgroups go round robin over the eight XCDs: each XCD takes a run of tasks, whose neighbours (the blocks of columns
   // of one group's segment) read the same B and C through its L2.
-  const long per = (a.tasks + 7) / 8;
-  const long task = (block_id() % 8) * per + block_id() / 8;
-  if (block_id() / 8 >= per || task >= a.tasks) return;
-  const int hb = (int)(task % a.blocks);
-  long rest = task / a.blocks;
-  const int seg = (int)(rest % a.segs);
-  rest /= a.segs;
-  const int grp = (int)(rest % a.G);
-  const long bi = rest / a.G;
+  const uint32_t per = (a.tasks + 7) / 8, task = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (blockIdx.x >> 3 >= per || task >= a.tasks) return;
+  const int cb = (int)(task % (uint32_t)a.blocks);
+  uint32_t rest = task / (uint32_t)a.blocks;
+  const int seg = (int)(rest % (uint32_t)a.segs);
+  rest /= (uint32_t)a.segs;
+  const int grp = (int)(rest % (uint32_t)a.G);
+  const long bi = rest / (uint32_t)a.G;
 
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int R = a.H / a.G;
-  const int hl = w * 32 / a.P, p0 = w * 32 % a.P;
-  const bool active = hl < a.heads && hb * a.heads + hl < R;
-  const int h = grp * R + (active ? hb * a.heads + hl : 0);
+  // The columns of a group's heads lie end to end, and the workgroup has COLS of them: P is a multiple of 32, so that a
+  // wave's are of one head.
+  const int col = cb * COLS + w * 16 * PT;
+  const bool active = col < R * a.P;
+  const int hr = active ? col / a.P : 0, p0 = active ? col % a.P : 0;
+  const int h = grp * R + hr, hl = active ? hr - cb * COLS / a.P : 0;
   const int N = a.N, P = a.P;
   int len = a.T;
-  if (a.lengths) len = min(max(a.lengths[bi], 0), a.T);
+  if (a.lengths) len = __builtin_amdgcn_readfirstlane(min(max(a.lengths[bi], 0), a.T));
 
-  const E* xg = static_cast<const E*>(a.x) + bi * a.x_b + h * a.x_h + p0;
-  const E* bg = static_cast<const E*>(a.b) + bi * a.b_b + grp * a.b_g;
-  const E* cg = static_cast<const E*>(a.c) + bi * a.c_b + grp * a.c_g;
-  const float a2 = active ? a.a[h] * 1.44269504f : 0.f;
-  const float dbias = active && a.dt_bias ? a.dt_bias[h] : 0.f;
+  const int chunks = (a.T + Q - 1) / Q;
+  const int first = seg * a.seg_chunks, end = min(first + a.seg_chunks, chunks);
 
-  // ---- what a chunk loads: rows of B and C by all threads, its x by each wave, dt a token a lane
+  // ---- what a chunk loads: rows of B and C by all threads, its own columns of x by each wave.  The buffers end after the
+  // last live token of the chunk (a token's stride covers its row), so that what lies past it reads as zero.
+  const char* xg = reinterpret_cast<const char*>(static_cast<const E*>(a.x) + bi * a.x_b + h * a.x_h + p0);
+  const char* bg = reinterpret_cast<const char*>(static_cast<const E*>(a.b) + bi * a.b_b + grp * a.b_g);
+  const char* cg = reinterpret_cast<const char*>(static_cast<const E*>(a.c) + bi * a.c_b + grp * a.c_g);
+  const int xt = (int)a.x_t * ES, bt = (int)a.b_t * ES, ct = (int)a.c_t * ES;
+  const int b_row = threadIdx.x / RV, b_col = threadIdx.x % RV * V, x_row = lane / XV, x_col = lane % XV * V;
+  const bool stages = Q * RV >= TH || threadIdx.x < Q * RV;
+  const uint32_t b_off = b_col < N ? (uint32_t)(b_row * bt + b_col * ES) : kPastEnd;
+  const uint32_t c_off = b_col < N ? (uint32_t)(b_row * ct + b_col * ES) : kPastEnd;
+  const uint32_t x_off = active ? (uint32_t)(x_row * xt + x_col * ES) : kPastEnd;
   u32x4 rb[NB], rc[NB], rx[NX];
-  float rdt = 0.f;
   auto load = [&](int t0) {
-    const int valid = len - t0;
+    const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
+    const auto xr = make_rsrc(xg + (long)t0 * xt, (uint32_t)(valid * xt)), br = make_rsrc(bg + (long)t0 * bt, (uint32_t)(valid * bt)),
+               cr = make_rsrc(cg + (long)t0 * ct, (uint32_t)(valid * ct));
+    if (stages) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int v = threadIdx.x + i * TH, row = v / RV, col = (v % RV) * V;
-      rb[i] = u32x4{0, 0, 0, 0};
-      if (OUT) rc[i] = u32x4{0, 0, 0, 0};
-      if (row < valid && col < N) {
-        rb[i] = *reinterpret_cast<const u32x4_any*>(bg + (t0 + row) * a.b_t + col);
-        if (OUT) rc[i] = *reinterpret_cast<const u32x4_any*>(cg + (t0 + row) * a.c_t + col);
+      for (int i = 0; i < NB; ++i) {
+        rb[i] = __builtin_amdgcn_raw_buffer_load_b128(br, b_off + i * (TH / RV) * bt, 0, 0);
+        if (OUT) rc[i] = __builtin_amdgcn_raw_buffer_load_b128(cr, c_off + i * (TH / RV) * ct, 0, 0);
       }
     }
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      const int v = lane + i * 64, row = v / XV, col = (v % XV) * V;
-      rx[i] = u32x4{0, 0, 0, 0};
-      if (active && row < valid) rx[i] = *reinterpret_cast<const u32x4_any*>(xg + (t0 + row) * a.x_t + col);
-    }
-    rdt = 0.f;
-    if (active && lane < valid) rdt = load_any<E>(a.dt, bi * a.dt_b + h * a.dt_h + (t0 + lane) * a.dt_t, a.dt_f32);
+    for (int i = 0; i < NX; ++i) rx[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, x_off + i * (64 / XV) * xt, 0, 0);
   };
+  auto stage = [&](int buf) {
+    if (stages) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int row = b_row + i * (TH / RV);
+        *reinterpret_cast<u32x4*>(&s.b[buf][row * Bs::LD + b_col]) = rb[i];
+        if (OUT) *reinterpret_cast<u32x4*>(&s.c[row * Cs::LD + b_col]) = rc[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NX; ++i) *reinterpret_cast<u32x4*>(&s.x[buf][w][(x_row + i * (64 / XV)) * Xs::LD + x_col]) = rx[i];
+  };
+  // ---- the chunks' step sizes and decays, a token a lane, in log2.  A batch of chunks at a time: its (chunk, head) pairs
+  // are dealt over the waves, four each, the steps loaded a batch ahead.
+  const int h_first = cb * COLS / P, heads = min(R, (cb * COLS + COLS - 1) / P + 1) - h_first, batch = Lds::SLOTS / heads;
+  float rdt[4];
+  auto load_dt = [&](int ch) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int slot = w + i * NW, t = (ch + slot / heads) * Q + lane;
+      rdt[i] = 0.f;
+      if (slot / heads < batch && t < len)
+        rdt[i] = load_any<E>(a.dt, bi * a.dt_b + (grp * R + h_first + slot % heads) * a.dt_h + t * a.dt_t, a.dt_f32);
+    }
+  };
+  auto tabulate = [&](int ch) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int slot = w + i * NW, head = grp * R + h_first + slot % heads;
+      if (slot / heads >= batch) continue;
+      float dt = rdt[i];
+      if (a.dt_bias) dt += a.dt_bias[head];
+      if (a.softplus) dt = softplus(dt);
+      if ((ch + slot / heads) * Q + lane >= len) dt = 0.f;
+      const float gate = dt * (a.a[head] * 1.44269504f);
+      float G, after;
+      wave_sums(gate, g, G, after);
+      s.tab[slot][0][lane] = dt * pow2(after - gate);
+      if constexpr (OUT) {
+        s.tab[slot][1][lane] = G;
+        s.tab[slot][2][lane] = dt;
+        s.tab[slot][3][lane] = dt * pow2(row_move<0x15f>(G) - G);
+      }
+      if (lane == 63) s.total[slot] = G;
+    }
+  };
+  float decay2 = 0.f;                          // log2 of the segment's decay
 
-  floatx4 S[NT / 16][2];
+  floatx4 S[NTS][PT];
 #pragma unroll
-  for (int nt = 0; nt < NT / 16; ++nt)
+  for (int nt = 0; nt < NTS; ++nt)
 #pragma unroll
-    for (int pt = 0; pt < 2; ++pt) S[nt][pt] = zero4();
+    for (int pt = 0; pt < PT; ++pt) S[nt][pt] = zero4();
   if (OUT && active) {
     const float* in = a.segs > 1 ? a.seg_state + (((long)bi * a.H + h) * a.segs + seg) * N * P
                                  : (a.h0 ? a.h0 + ((long)bi * a.H + h) * N * P : nullptr);
     if (in) {
 #pragma unroll
-      for (int nt = 0; nt < NT / 16; ++nt)
+      for (int nt = 0; nt < NTS; ++nt)
 #pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
+        for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int n = 16 * nt + 4 * g + r;
+            const int n = state_row(nt, g, r);
             if (n < N) S[nt][pt][r] = in[(long)n * P + p0 + 16 * pt + c];
           }
     }
   }
 
-  const int chunks = (a.T + Q - 1) / Q;
-  const int first = seg * a.seg_chunks, end = min(first + a.seg_chunks, chunks);
-  float decay2 = 0.f;                          // kStates: log2 of the segment's decay
-  if (first < end) load(first * Q);
-  for (int ch = first; ch < end; ++ch) {
-    const int t0 = ch * Q;
-    lds_barrier();                             // the last chunk's reads are done
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int v = threadIdx.x + i * TH;
-      Rows::put(s.b, v / RV, v % RV, rb[i]);
-      if (OUT) Rows::put(s.c, v / RV, v % RV, rc[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      const int v = lane + i * 64;
-      *reinterpret_cast<u32x4*>(&s.x[w][(v / XV) * Xs::LD + (v % XV) * V]) = rx[i];
-    }
-    // the chunk's step sizes and decays, a token a lane, in log2
-    float dt = rdt + dbias;
-    if (a.softplus) dt = softplus(dt);
-    if (t0 + lane >= len) dt = 0.f;
-    const float gate = dt * a2;
-    float G = gate, after = gate;              // sums up to here, and from here on
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const float up = __shfl_up(G, m), down = __shfl_down(after, m);
-      if (lane >= m) G += up;
-      if (lane + m < 64) after += down;
-    }
-    const float total = __shfl(G, 63);
-    s.tab[w][0][lane] = G;
-    s.tab[w][1][lane] = dt;
-    s.tab[w][2][lane] = dt * exp2f(__shfl(G, lane | 15) - G);
-    s.tab[w][3][lane] = dt * exp2f(after - gate);
-    lds_barrier();
-    if (ch + 1 < end) load(t0 + Q);
+  const int yt = (int)a.y_t * ES, zt = (int)a.z_t * ES;
+  char* yg = reinterpret_cast<char*>(static_cast<E*>(a.y) + bi * a.y_b + h * a.y_h + p0);
+  const char* zg = reinterpret_cast<const char*>(static_cast<const E*>(a.z) + bi * a.z_b + h * a.z_h + p0);
+  const uint32_t y_off = active ? (uint32_t)(c * yt + 4 * g * ES) : kPastEnd, z_off = (uint32_t)(c * zt + 4 * g * ES);
+  const float dd = active && a.d ? a.d[h] : 0.f;
 
-    Frag<E> xf[2][2];
+  // Added to an exponent on the score's diagonal tiles: 2^-inf above the diagonal, whatever the sums are there.  (Opaque to
+  // the compiler, which would branch around each exponential.)
+  floatx4 above;
 #pragma unroll
-    for (int pt = 0; pt < 2; ++pt)
+  for (int r = 0; r < 4; ++r) {
+    above[r] = 4 * g + r <= c ? 0.f : -__builtin_inff();
+    __asm__("" : "+v"(above[r]));
+  }
+
+  int slot0 = -heads;                          // of this chunk's tables
+  if (first < end) {
+    load_dt(first);
+    load(first * Q);
+    if (!OUT) {
+      tabulate(first);
+      load_dt(first + batch);
+      stage(first & 1);
+      load((first + 1) * Q);                   // past the last chunk: nothing is valid, nothing is read
+      lds_barrier();
+    }
+  }
+  for (int ch = first; ch < end; ++ch) {
+    const int t0 = ch * Q, buf = OUT ? 0 : ch & 1;
+    slot0 += heads;
+    if (slot0 + heads > Lds::SLOTS) slot0 = 0;
+    const float(*tab)[Q] = s.tab[slot0 + hl];
+    if (OUT) {
+      lds_barrier();                           // the last chunk's reads are done
+      stage(0);
+      if (slot0 == 0) {
+        tabulate(ch);
+        load_dt(ch + batch);
+      }
+      lds_barrier();
+      if (ch + 1 < end) load(t0 + Q);
+    }
+    const E* sb = s.b[buf];
+    const E* sx = s.x[buf][w];
+
+    Frag<E> xf[PT][2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) xf[pt][kb] = Xs::cols(s.x[w], pt, kb, c, g);
+    for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) xf[pt][kb] = Xs::template cols<4>(sx, 16 * pt, kb, c, g);
 
     if constexpr (OUT) {
       // the score's tiles, dealt over the waves
 #pragma unroll
       for (int k = 0; k < (10 + NW - 1) / NW; ++k) {
         const int tile = w + k * NW;
-        if (tile < 10) {
+        if ((k + 1) * NW <= 10 || tile < 10) {
           const int ib = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, jb = tile - ib * (ib + 1) / 2;
           floatx4 acc = zero4();
 #pragma unroll
           for (int kb = 0; kb < NT / 32; ++kb)
-            acc = mfma32(Rows::rows(s.b, 16 * jb + c, kb, g), Rows::rows(s.c, 16 * ib + c, kb, g), acc);
+            acc = mfma32(Bs::rows(sb, 16 * jb + c, kb, g), Cs::rows(s.c, 16 * ib + c, kb, g), acc);
           s.score[tile][lane] = acc;
         }
       }
       // y^T = S^T C^T
-      floatx4 y[2][4];
+      floatx4 y[PT][4];
 #pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
+      for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
         for (int ib = 0; ib < 4; ++ib) y[pt][ib] = zero4();
 #pragma unroll
       for (int kb = 0; kb < NT / 32; ++kb) {
-        const Frag<E> s0 = frag_of<E>(S[2 * kb][0], S[2 * kb + 1][0]), s1 = frag_of<E>(S[2 * kb][1], S[2 * kb + 1][1]);
+        Frag<E> sf[PT];
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt) sf[pt] = frag_of<E>(S[2 * kb][pt], S[2 * kb + 1][pt]);
 #pragma unroll
         for (int ib = 0; ib < 4; ++ib) {
-          const Frag<E> cf = Rows::rows(s.c, 16 * ib + c, kb, g);
-          y[0][ib] = mfma32(s0, cf, y[0][ib]);
-          y[1][ib] = mfma32(s1, cf, y[1][ib]);
+          const Frag<E> cf = Cs::rows(s.c, 16 * ib + c, kb, g);
+#pragma unroll
+          for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(sf[pt], cf, y[pt][ib]);
         }
       }
       lds_barrier();                           // the score is whole
       floatx4 u[4];
 #pragma unroll
-      for (int jb = 0; jb < 4; ++jb) u[jb] = *reinterpret_cast<const floatx4*>(&s.tab[w][2][16 * jb + 4 * g]);
+      for (int jb = 0; jb < 4; ++jb) u[jb] = *reinterpret_cast<const floatx4*>(&tab[3][16 * jb + 4 * g]);
 #pragma unroll
       for (int ib = 0; ib < 4; ++ib) {
-        const float Gi = s.tab[w][0][16 * ib + c];
-        const float e = exp2f(Gi);
-        y[0][ib] *= e;
-        y[1][ib] *= e;
+        const float Gi = tab[1][16 * ib + c];
+        const float e = pow2(Gi);
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt) y[pt][ib] *= e;
         floatx4 pr[4];
 #pragma unroll
         for (int jb = 0; jb < 4; ++jb) {
           pr[jb] = zero4();
           if (jb < ib) {
-            const float f = exp2f(Gi - s.tab[w][0][16 * jb + 15]);
+            const float f = pow2(Gi - tab[1][16 * jb + 15]);
             pr[jb] = s.score[ib * (ib + 1) / 2 + jb][lane] * (u[jb] * f);
           } else if (jb == ib) {
             const floatx4 sc = s.score[ib * (ib + 1) / 2 + jb][lane];
-            const floatx4 Gj = *reinterpret_cast<const floatx4*>(&s.tab[w][0][16 * jb + 4 * g]);
-            const floatx4 dj = *reinterpret_cast<const floatx4*>(&s.tab[w][1][16 * jb + 4 * g]);
+            const floatx4 Gj = *reinterpret_cast<const floatx4*>(&tab[1][16 * jb + 4 * g]);
+            const floatx4 dj = *reinterpret_cast<const floatx4*>(&tab[2][16 * jb + 4 * g]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) pr[jb][r] = 4 * g + r <= c ? sc[r] * (dj[r] * exp2f(Gi - Gj[r])) : 0.f;
+            for (int r = 0; r < 4; ++r) pr[jb][r] = sc[r] * (dj[r] * pow2(Gi - Gj[r] + above[r]));
           }
         }
 #pragma unroll
         for (int kb = 0; kb <= ib / 2; ++kb) {
           const Frag<E> pf = frag_of<E>(pr[2 * kb], pr[2 * kb + 1]);
-          y[0][ib] = mfma32(xf[0][kb], pf, y[0][ib]);
-          y[1][ib] = mfma32(xf[1][kb], pf, y[1][ib]);
+#pragma unroll
+          for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(xf[pt][kb], pf, y[pt][ib]);
         }
       }
       // y out: lane c's token, four columns of each tile
-      if (active) {
-        const float dd = a.d ? a.d[h] : 0.f;
+      const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
+      const auto yr = make_rsrc(yg + (long)t0 * yt, (uint32_t)(min(a.T - t0, Q) * yt));
+      const auto zr = make_rsrc(zg + (long)t0 * zt, HAS_Z ? (uint32_t)(valid * zt) : 0);
 #pragma unroll
-        for (int ib = 0; ib < 4; ++ib) {
-          const int t = t0 + 16 * ib + c;
-          if (t < a.T) {
+      for (int ib = 0; ib < 4; ++ib)
 #pragma unroll
-            for (int pt = 0; pt < 2; ++pt) {
-              float v[4], xr[4];
+        for (int pt = 0; pt < PT; ++pt) {
+          float v[4];
+          load_vec<4>(&sx[(16 * ib + c) * Xs::LD + 16 * pt + 4 * g], v);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) xr[r] = to_f32(s.x[w][(16 * ib + c) * Xs::LD + 16 * pt + 4 * g + r]);
+          for (int r = 0; r < 4; ++r) v[r] = fmaf(dd, v[r], y[pt][ib][r]);
+          if (HAS_Z) {
+            float z[4];
+            buf_load4<E>(zr, z_off + 16 * ib * zt + 16 * pt * ES, z);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) v[r] = fmaf(dd, xr[r], y[pt][ib][r]);
-              if (a.z) {
-                float z[4];
-                load_vec<4>(static_cast<const E*>(a.z) + bi * a.z_b + h * a.z_h + t * a.z_t + p0 + 16 * pt + 4 * g, z);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] *= silu(z[r]);
-              }
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (t >= len) v[r] = 0.f;
-              store_vec<4>(static_cast<E*>(a.y) + bi * a.y_b + h * a.y_h + t * a.y_t + p0 + 16 * pt + 4 * g, v);
-            }
+            for (int r = 0; r < 4; ++r) v[r] *= silu(z[r]);
           }
+          if (valid < Q) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = 16 * ib + c < valid ? v[r] : 0.f;
+          }
+          buf_store4<E>(yr, y_off + 16 * ib * yt + 16 * pt * ES, v);
         }
-      }
     }
-
     // S <- e^{G_last} S + B^T (w x)
-    const float e = exp2f(total);
+    const float total = s.total[slot0 + hl], e = pow2(total);
     decay2 += total;
 #pragma unroll
-    for (int nt = 0; nt < NT / 16; ++nt) {
-      S[nt][0] *= e;
-      S[nt][1] *= e;
-    }
+    for (int nt = 0; nt < NTS; ++nt)
+#pragma unroll
+      for (int pt = 0; pt < PT; ++pt) S[nt][pt] *= e;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const floatx4 w0 = *reinterpret_cast<const floatx4*>(&s.tab[w][3][32 * kb + 4 * g]);
-      const floatx4 w1 = *reinterpret_cast<const floatx4*>(&s.tab[w][3][32 * kb + 16 + 4 * g]);
-      const typename WeightedOf<E, SPLIT>::T wx0(xf[0][kb], w0, w1), wx1(xf[1][kb], w0, w1);
+      const floatx4 w0 = *reinterpret_cast<const floatx4*>(&tab[0][32 * kb + 4 * g]);
+      const floatx4 w1 = *reinterpret_cast<const floatx4*>(&tab[0][32 * kb + 16 + 4 * g]);
+      Frag<E> wx[PT][SPLIT];
 #pragma unroll
-      for (int nt = 0; nt < NT / 16; ++nt) {
-        const Frag<E> bf = Rows::cols(s.b, nt, kb, c, g);
-        S[nt][0] = wx0.times(bf, S[nt][0]);
-        S[nt][1] = wx1.times(bf, S[nt][1]);
+      for (int pt = 0; pt < PT; ++pt) weigh(xf[pt][kb], w0, w1, wx[pt]);
+#pragma unroll
+      for (int np = 0; np < NTS; np += 2) {
+        const Frag<E> b0 = Bs::template cols<8>(sb, 16 * np, kb, c, g), b1 = Bs::template cols<8>(sb, 16 * np + 4, kb, c, g);
+#pragma unroll
+        for (int k = SPLIT - 1; k >= 0; --k)
+#pragma unroll
+          for (int pt = 0; pt < PT; ++pt) {
+            S[np][pt] = mfma32(b0, wx[pt][k], S[np][pt]);
+            S[np + 1][pt] = mfma32(b1, wx[pt][k], S[np + 1][pt]);
+          }
       }
+    }
+    if (!OUT && ch + 1 < end) {
+      stage((ch + 1) & 1);
+      load(t0 + 2 * Q);
+      if (slot0 + 2 * heads > Lds::SLOTS) {    // the next chunk begins a batch
+        lds_barrier();                         // the last batch's reads are done
+        tabulate(ch + 1);
+        load_dt(ch + 1 + batch);
+      }
+      lds_barrier();
     }
   }
 
@@ -428,12 +533,12 @@ __global__ __launch_bounds__(NW * 64) void ssm_kernel(SsmArgs a) {
   }
   if (active && out) {
 #pragma unroll
-    for (int nt = 0; nt < NT / 16; ++nt)
+    for (int nt = 0; nt < NTS; ++nt)
 #pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
+      for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int n = 16 * nt + 4 * g + r;
+          const int n = state_row(nt, g, r);
           if (n < N) out[(long)n * P + p0 + 16 * pt + c] = S[nt][pt][r];
         }
   }
@@ -458,7 +563,7 @@ __global__ __launch_bounds__(256) void ssm_prefix_kernel(SsmArgs a) {
     for (int i = 0; i < AHEAD; ++i)
       if (s0 + i < a.segs) {
         D[i] = *reinterpret_cast<const floatx4*>(st + (s0 + i) * step);
-        e[i] = exp2f(decay[s0 + i]);
+        e[i] = pow2(decay[s0 + i]);
       }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)

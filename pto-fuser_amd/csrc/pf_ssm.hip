@@ -12,9 +12,9 @@ namespace {
 using pf::bf16;
 using pf::SsmMode;
 
-// How a shape is cut: waves of a workgroup, heads of a workgroup, blocks of heads of a group, segments of a sequence.
+// How a shape is cut: columns of a workgroup, blocks of them in a group's heads, segments of a sequence.
 struct SsmPlan {
-  int waves, heads, blocks, segs, seg_chunks;
+  int cols, blocks, segs, seg_chunks;
   size_t bytes;              // workspace of the segments
 };
 
@@ -27,13 +27,12 @@ size_t state_bytes(long chains, int segs, int N, int P) {
   return (size_t)chains * segs * N * P * sizeof(float) + (size_t)chains * segs * sizeof(float);
 }
 
-SsmPlan plan(int B, int H, int G, int T, int N, int P) {
+SsmPlan plan(int B, int H, int G, int T, int N, int P, int dtype) {
   SsmPlan p{};
-  const int R = H / G, per_head = P / 32;
-  const long need = (long)R * per_head;
-  p.waves = need <= 2 && per_head <= 2 ? 2 : need <= 4 && per_head <= 4 ? 4 : 8;
-  p.heads = p.waves / per_head < R ? p.waves / per_head : R;
-  p.blocks = (R + p.heads - 1) / p.heads;
+  const long cols = (long)(H / G) * P;
+  p.cols = 64;
+  while (p.cols < cols && p.cols < (dtype == PF_DTYPE_BF16 ? 256 : 128)) p.cols *= 2;
+  p.blocks = (int)((cols + p.cols - 1) / p.cols);
   const int chunks = (T + pf::kSsmChunk - 1) / pf::kSsmChunk;
   const long units = (long)B * G * p.blocks;
   // Segments while they fit one generation of workgroups, of two chunks at least.
@@ -46,6 +45,8 @@ SsmPlan plan(int B, int H, int G, int T, int N, int P) {
   return p;
 }
 
+constexpr double kMaxTasks = 1 << 22;   // workgroups of up to 1024 threads in one grid dimension
+
 bool grid_of(double workgroups, dim3& grid) {
   if (workgroups > (double)pf::kGridX * (pf::kGridY - 1)) return false;
   const long n = (long)workgroups;
@@ -53,32 +54,38 @@ bool grid_of(double workgroups, dim3& grid) {
   return true;
 }
 
-template <typename E, int NT, int NW, SsmMode MODE, int SPLIT>
-void scan(const pf::SsmArgs& a, dim3 grid, hipStream_t s) {
-  pf::ssm_kernel<E, NT, NW, MODE, SPLIT><<<grid, dim3(NW * 64), 0, s>>>(a);
+template <typename E, int NT, int NW, int PT, int SPLIT>
+void outputs(const pf::SsmArgs& a, dim3 grid, hipStream_t s) {
+  if (a.z) pf::ssm_kernel<E, NT, NW, PT, SsmMode::kOutput, SPLIT, true><<<grid, dim3(NW * 64), 0, s>>>(a);
+  else pf::ssm_kernel<E, NT, NW, PT, SsmMode::kOutput, SPLIT, false><<<grid, dim3(NW * 64), 0, s>>>(a);
 }
 
-template <typename E, int NT, int NW>
+template <typename E, int NT, int COLS>
 int launch(pf::SsmArgs& a, hipStream_t s) {
   constexpr bool kF32 = std::is_same<E, float>::value;
-  a.tasks = (long)a.B * a.G * a.blocks * a.segs;
-  const long per = (a.tasks + 7) / 8;
-  dim3 grid, prefix;
-  if (!grid_of(8. * per, grid) || !grid_of(((double)a.N * a.P / 4 * a.B * a.H + 255) / 256, prefix)) return PF_ERR_ARG;
+  constexpr int PT = kF32 ? 1 : 2, NW = COLS / (16 * PT);
+  const double tasks = (double)a.B * a.G * a.blocks * a.segs;
+  if (tasks > kMaxTasks) return PF_ERR_ARG;
+  a.tasks = (uint32_t)tasks;
+  const dim3 grid((a.tasks + 7) / 8 * 8);
+  dim3 prefix;
+  if (!grid_of(((double)a.N * a.P / 4 * a.B * a.H + 255) / 256, prefix)) return PF_ERR_ARG;
   pf::LaunchScope scope;
   if (a.segs > 1) {
-    scan<E, NT, NW, SsmMode::kStates, kF32 ? 1 : 3>(a, grid, s);
+    pf::ssm_kernel<E, NT, NW, PT, SsmMode::kStates, kF32 ? 1 : 3, false><<<grid, dim3(NW * 64), 0, s>>>(a);
     pf::ssm_prefix_kernel<<<prefix, dim3(256), 0, s>>>(a);
-    scan<E, NT, NW, SsmMode::kOutput, kF32 ? 1 : 2>(a, grid, s);
+    outputs<E, NT, NW, PT, kF32 ? 1 : 2>(a, grid, s);
   } else {
-    scan<E, NT, NW, SsmMode::kOutput, kF32 ? 1 : 3>(a, grid, s);
+    outputs<E, NT, NW, PT, kF32 ? 1 : 3>(a, grid, s);
   }
   return scope.status();
 }
 
 template <typename E, int NT>
-int launch_waves(pf::SsmArgs& a, int waves, hipStream_t s) {
-  return waves == 2 ? launch<E, NT, 2>(a, s) : waves == 4 ? launch<E, NT, 4>(a, s) : launch<E, NT, 8>(a, s);
+int launch_cols(pf::SsmArgs& a, int cols, hipStream_t s) {
+  if constexpr (std::is_same<E, bf16>::value)
+    if (cols == 256) return launch<E, NT, 256>(a, s);
+  return cols == 128 ? launch<E, NT, 128>(a, s) : launch<E, NT, 64>(a, s);
 }
 
 }  // namespace
@@ -87,7 +94,7 @@ extern "C" {
 
 size_t pf_ssm_workspace_bytes(int B, int H, int G, int T, int N, int P, int dtype) {
   if (!shape_ok(B, H, G, T, N, P, dtype) || (double)B * H * N * P > 1e12) return 0;
-  return plan(B, H, G, T, N, P).bytes;
+  return plan(B, H, G, T, N, P, dtype).bytes;
 }
 
 int pf_ssm_exec(const pf_ssm_args* p, void* stream) {
@@ -97,8 +104,15 @@ int pf_ssm_exec(const pf_ssm_args* p, void* stream) {
   for (long long st : {p->x_b, p->x_h, p->x_t, p->dt_b, p->dt_h, p->dt_t, p->b_b, p->b_g, p->b_t, p->c_b, p->c_g, p->c_t,
                        p->z_b, p->z_h, p->z_t, p->y_b, p->y_h, p->y_t})
     if (st < 0) return PF_ERR_ARG;
+  // A chunk's rows are read up to the end of the last live one: a token's stride covers its row, whatever it is of one token.
+  const bool many = p->T > 1;
+  const long long x_t = many ? p->x_t : p->P, y_t = many ? p->y_t : p->P, z_t = many && p->z ? p->z_t : p->P,
+                  b_t = many ? p->b_t : p->N, c_t = many ? p->c_t : p->N;
+  if (x_t < p->P || y_t < p->P || z_t < p->P || b_t < p->N || c_t < p->N) return PF_ERR_ARG;
+  for (long long st : {x_t, y_t, z_t, b_t, c_t})
+    if (st > pf::kMaxTokenStride) return PF_ERR_ARG;
   if (p->B == 0) return PF_OK;
-  SsmPlan pl = plan(p->B, p->H, p->G, p->T, p->N, p->P);
+  SsmPlan pl = plan(p->B, p->H, p->G, p->T, p->N, p->P, p->dtype);
   if (!p->workspace || p->workspace_bytes < pl.bytes || ((size_t)p->workspace & 15)) {   // whole sequences
     pl.segs = 1;
     pl.seg_chunks = (p->T + pf::kSsmChunk - 1) / pf::kSsmChunk;
@@ -108,16 +122,16 @@ int pf_ssm_exec(const pf_ssm_args* p, void* stream) {
   a.h0 = p->h0; a.lengths = p->lengths; a.y = p->y; a.h_final = p->h_final;
   a.seg_state = static_cast<float*>(p->workspace);
   a.seg_decay = a.seg_state + (size_t)p->B * p->H * pl.segs * p->N * p->P;
-  a.x_b = p->x_b; a.x_h = p->x_h; a.x_t = p->x_t; a.dt_b = p->dt_b; a.dt_h = p->dt_h; a.dt_t = p->dt_t;
-  a.b_b = p->b_b; a.b_g = p->b_g; a.b_t = p->b_t; a.c_b = p->c_b; a.c_g = p->c_g; a.c_t = p->c_t;
-  a.z_b = p->z_b; a.z_h = p->z_h; a.z_t = p->z_t; a.y_b = p->y_b; a.y_h = p->y_h; a.y_t = p->y_t;
+  a.x_b = p->x_b; a.x_h = p->x_h; a.x_t = x_t; a.dt_b = p->dt_b; a.dt_h = p->dt_h; a.dt_t = p->dt_t;
+  a.b_b = p->b_b; a.b_g = p->b_g; a.b_t = b_t; a.c_b = p->c_b; a.c_g = p->c_g; a.c_t = c_t;
+  a.z_b = p->z_b; a.z_h = p->z_h; a.z_t = z_t; a.y_b = p->y_b; a.y_h = p->y_h; a.y_t = y_t;
   a.B = p->B; a.H = p->H; a.G = p->G; a.T = p->T; a.N = p->N; a.P = p->P;
-  a.heads = pl.heads; a.blocks = pl.blocks; a.segs = pl.segs; a.seg_chunks = pl.seg_chunks;
+  a.blocks = pl.blocks; a.segs = pl.segs; a.seg_chunks = pl.seg_chunks;
   a.dt_f32 = p->dt_f32; a.softplus = p->softplus;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p->dtype == PF_DTYPE_BF16)
-    return p->N <= 64 ? launch_waves<bf16, 64>(a, pl.waves, s) : launch_waves<bf16, 128>(a, pl.waves, s);
-  return p->N <= 64 ? launch_waves<float, 64>(a, pl.waves, s) : launch_waves<float, 128>(a, pl.waves, s);
+    return p->N <= 64 ? launch_cols<bf16, 64>(a, pl.cols, s) : launch_cols<bf16, 128>(a, pl.cols, s);
+  return p->N <= 64 ? launch_cols<float, 64>(a, pl.cols, s) : launch_cols<float, 128>(a, pl.cols, s);
 }
 
 }  // extern "C"

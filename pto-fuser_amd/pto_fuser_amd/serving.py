@@ -241,9 +241,13 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
         _require_view(z, "z", (nb, H, T, P), dtype, dev)
     _require(h0, "h0", (nb, H, N, P), torch.float32, dev)
     _require(lengths, "lengths", (nb,), torch.int32, dev)
+    if T > 1:      # rows that overlap (a token expanded along the sequence) are laid out first
+        x, B, C, z = (t if t is None or t.stride(2) >= t.shape[3] else t.contiguous() for t in (x, B, C, z))
     sx = x.stride()
     if out is not None:
         _require_view(out, "out", (nb, H, T, P), dtype, dev)
+        if T > 1 and out.stride(2) < P:
+            raise ValueError("out has overlapping rows")
         y = out
     elif sx[1] < sx[2]:
         y = torch.empty(nb, T, H, P, device=dev, dtype=dtype).transpose(1, 2)

@@ -93,7 +93,7 @@ def test_gdn_step_statuses(lib, bad):
 def _ssm(**kw):
     f = dict(size=serving._SSM_SIZE, x=64, dt=64, b=64, c=64, z=0, a=64, d=0, dt_bias=0, h0=0, lengths=0, y=64, h_final=0, ws=0,
              ws_bytes=0)
-    f.update({f"s{i}": 0 for i in range(18)})
+    f.update({f"s{i}": 64 for i in range(18)})
     f.update(B=1, H=4, G=2, T=100, N=64, P=64, dtype=1, dt_f32=0, softplus=0)
     assert not set(kw) - set(f)
     return serving._SSM.pack(*{**f, **kw}.values())
@@ -101,7 +101,8 @@ def _ssm(**kw):
 
 @pytest.mark.parametrize("bad", [dict(size=0), dict(dtype=2), dict(H=3), dict(H=0), dict(G=0), dict(N=144), dict(N=24), dict(N=0),
                                  dict(P=48), dict(P=288), dict(P=0), dict(T=-1), dict(B=-1), dict(x=0), dict(dt=0), dict(b=0), dict(c=0),
-                                 dict(y=0), dict(a=0), dict(s0=-1), dict(s17=-1), dict(B=1 << 30, H=1 << 20, G=1)])
+                                 dict(y=0), dict(a=0), dict(s0=-1), dict(s17=-1), dict(s2=63),
+                                 dict(s8=0), dict(s11=1 << 23), dict(z=64, s14=8), dict(B=1 << 30, H=1 << 20, G=1)])
 def test_ssm_statuses(lib, bad):
     assert lib.pf_ssm_exec(_ssm(**bad), None) == _hip.PF_ERR_ARG
 
@@ -114,9 +115,10 @@ def test_ssm_workspace_sizes(lib):
     assert size(1, 4, 1, 64, 128, 64, 1) == 0 and size(64, 64, 1, 8192, 128, 64, 1) == 0
     assert size(1, 4, 1, 8192, 100, 64, 1) == 0 and size(1 << 20, 1 << 20, 1, 8192, 128, 64, 1) == 0
     for H, G, T, N, P in ((4, 1, 8192, 128, 64), (32, 1, 32768, 128, 64), (32, 32, 4096, 64, 128), (1, 1, 1 << 30, 16, 32)):
-        n = size(1, H, G, T, N, P, 1)
         one = H * (N * P + 1) * 4
-        assert n and n % one == 0 and 2 <= n // one <= 512 and n == size(1, H, G, T, N, P, 0)
+        for dtype in (0, 1):
+            n = size(1, H, G, T, N, P, dtype)
+            assert n and n % one == 0 and 2 <= n // one <= 512
 
 
 def _norm(**kw):
