@@ -22,15 +22,44 @@ struct ConvArgs {
   long x_b, x_t, y_b, y_t;
   long si_b, so_b;
   long threads;           // B * tiles * vectors
+  long blocks;            // of 256 threads
   int B, T, W;
   int vectors, tiles;
   int w_f32, act;
 };
 
+// The filters of VEC neighbouring channels: their K taps lie side by side, K vectors of VEC values.
+template <typename E, int K, int VEC>
+__device__ __forceinline__ void load_taps(const void* w, int c, bool f32, float (&tap)[K][VEC]) {
+  float flat[K][VEC];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    if (f32) load_vec<VEC>(static_cast<const float*>(w) + (size_t)c * K + j * VEC, flat[j]);
+    else load_vec<VEC>(static_cast<const E*>(w) + (size_t)c * K + j * VEC, flat[j]);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+#pragma unroll
+    for (int k = 0; k < K; ++k) tap[k][i] = flat[(i * K + k) / VEC][(i * K + k) % VEC];
+}
+template <typename E, int VEC>
+__device__ __forceinline__ void load_bias(const void* bias, int c, bool f32, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+  if (bias) {
+    if (f32) load_vec<VEC>(static_cast<const float*>(bias) + c, v);
+    else load_vec<VEC>(static_cast<const E*>(bias) + c, v);
+  }
+}
+
 template <typename E, int K, int VEC, int TT>
 __global__ __launch_bounds__(256) void conv_kernel(ConvArgs a) {
-  const long id = block_id() * 256 + threadIdx.x;
-  if (id >= a.threads) return;
+  typedef typename VecAny<E, VEC>::T Vec;
+  // Workgroups go round robin over the eight XCDs: each takes a run of them, so that the rows that two neighbouring
+  // tiles both read come through one L2.
+  const long per = (a.blocks + 7) / 8, block = (block_id() & 7) * per + (block_id() >> 3);
+  const long id = block * 256 + threadIdx.x;
+  if (block_id() >> 3 >= per || id >= a.threads) return;
   const int cv = (int)(id % a.vectors);
   const long rest = id / a.vectors;
   const int tile = (int)(rest % a.tiles), b = (int)(rest / a.tiles);
@@ -41,41 +70,48 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvArgs a) {
   const E* x = static_cast<const E*>(a.x) + b * a.x_b + c;
   const E* si = a.state_in ? static_cast<const E*>(a.state_in) + b * a.si_b + c : nullptr;
 
-  // rows t0 - (K-1) .. t0 + TT - 1
-  float row[TT + K - 1][VEC];
+  // rows t0 - (K-1) .. t0 + TT - 1, as they are stored
+  Vec row[TT + K - 1];
+  if (t0 >= K - 1 && t0 + TT <= n) {
+    const E* p = x + (long)(t0 - (K - 1)) * a.x_t;
 #pragma unroll
-  for (int j = 0; j < TT + K - 1; ++j) {
-    const int t = t0 - (K - 1) + j;
+    for (int j = 0; j < TT + K - 1; ++j) row[j] = *reinterpret_cast<const Vec*>(p + j * a.x_t);
+  } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) row[j][i] = 0.f;
-    if (t >= 0) {
-      if (t < n) load_vec<VEC>(x + t * a.x_t, row[j]);
-    } else if (si) {
-      load_vec<VEC>(si + (long)(t + K - 1) * a.W, row[j]);
+    for (int j = 0; j < TT + K - 1; ++j) {
+      const int t = t0 - (K - 1) + j;
+      row[j] = Vec{};
+      if (t >= 0) {
+        if (t < n) row[j] = *reinterpret_cast<const Vec*>(x + t * a.x_t);
+      } else if (si) {
+        row[j] = *reinterpret_cast<const Vec*>(si + (long)(t + K - 1) * a.W);
+      }
     }
   }
   float w[K][VEC], bias[VEC];
+  load_taps<E, K, VEC>(a.w, c, a.w_f32, w);
+  load_bias<E, VEC>(a.bias, c, a.w_f32, bias);
+  float win[K][VEC];                            // the K rows of a token, in 32 bits; row j is at j % K
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) w[k][i] = load_any<E>(a.w, (size_t)(c + i) * K + k, a.w_f32);
-    bias[i] = a.bias ? load_any<E>(a.bias, c + i, a.w_f32) : 0.f;
-  }
+  for (int j = 0; j < K - 1; ++j) expand<E, VEC>(row[j], win[j]);
   E* y = static_cast<E*>(a.y) + b * a.y_b + c;
 #pragma unroll
   for (int j = 0; j < TT; ++j) {
     const int t = t0 + j;
-    if (t >= a.T) break;
+    expand<E, VEC>(row[j + K - 1], win[(j + K - 1) % K]);
     float o[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       o[i] = bias[i];
 #pragma unroll
-      for (int k = 0; k < K; ++k) o[i] = fmaf(w[k][i], row[j + k][i], o[i]);
+      for (int k = 0; k < K; ++k) o[i] = fmaf(w[k][i], win[(j + k) % K][i], o[i]);
       if (a.act) o[i] = silu(o[i]);
-      if (t >= n) o[i] = 0.f;
     }
-    store_vec<VEC>(y + t * a.y_t, o);
+    if (t >= n) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[i] = 0.f;
+    }
+    if (t < a.T) store_vec<VEC>(y + t * a.y_t, o);
   }
   // The state after the last token.  The thread of the first tile writes it: it is the only one that reads the state
   // before, whose rows a prompt shorter than K-1 tokens still needs, and has them in its first registers.
@@ -84,20 +120,15 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvArgs a) {
 #pragma unroll
     for (int r = 0; r < K - 1; ++r) {
       const int t = n - (K - 1) + r;
-      float v[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+      Vec v{};
       if (t >= 0) {
-        load_vec<VEC>(x + t * a.x_t, v);
+        v = *reinterpret_cast<const Vec*>(x + t * a.x_t);
       } else {
 #pragma unroll
         for (int j = 0; j < K - 1; ++j)
-          if (j == t + K - 1) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = row[j][i];
-          }
+          if (j == t + K - 1) v = row[j];
       }
-      store_vec<VEC>(so + (long)r * a.W, v);
+      *reinterpret_cast<Vec*>(so + (long)r * a.W) = v;
     }
   }
 }
@@ -133,11 +164,13 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvStepArgs a) {
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) load_vec<VEC>(s + (long)k * a.W, row[k]);
     load_vec<VEC>(static_cast<const E*>(a.x) + b * a.x_b + c, row[K - 1]);
+    float w[K][VEC];
+    load_taps<E, K, VEC>(a.w, c, a.w_f32, w);
+    load_bias<E, VEC>(a.bias, c, a.w_f32, o);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      o[i] = a.bias ? load_any<E>(a.bias, c + i, a.w_f32) : 0.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k) o[i] = fmaf(load_any<E>(a.w, (size_t)(c + i) * K + k, a.w_f32), row[k][i], o[i]);
+      for (int k = 0; k < K; ++k) o[i] = fmaf(w[k][i], row[k][i], o[i]);
       if (a.act) o[i] = silu(o[i]);
     }
 #pragma unroll

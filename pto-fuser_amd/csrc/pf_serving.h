@@ -33,6 +33,16 @@ template <typename E, int V> struct VecAny {
 };
 template <typename E> struct VecAny<E, 1> { typedef E T; };
 
+template <typename E, int V>
+__device__ __forceinline__ void expand(const typename VecAny<E, V>::T& x, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32((E)x[i]);
+  }
+}
+
 template <int V, typename E>
 __device__ __forceinline__ void load_vec(const E* p, float (&v)[V]) {
   if constexpr (V == 1) {

@@ -33,8 +33,9 @@ int conv_launch(pf::ConvArgs& a, hipStream_t s) {
   a.vectors = a.W / VEC;
   a.tiles = a.T ? (a.T + kConvTokens - 1) / kConvTokens : 1;
   dim3 grid;
-  long blocks;
-  if (!grid_of(a.B, a.tiles, a.vectors, 256, grid, blocks)) return PF_ERR_ARG;
+  long launched;
+  if (!grid_of(a.B, a.tiles, a.vectors, 256, grid, a.blocks)) return PF_ERR_ARG;
+  grid_of((double)((a.blocks + 7) / 8 * 8), 1, 1, 1, grid, launched);
   a.threads = (long)a.B * a.tiles * a.vectors;
   pf::LaunchScope scope;
   pf::conv_kernel<E, K, VEC, kConvTokens><<<grid, dim3(256), 0, s>>>(a);

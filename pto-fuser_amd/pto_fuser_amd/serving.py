@@ -25,7 +25,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _hip
-from .ops import _dtype_code, _on_device, _require
+from .ops import _dtype_code, _require
 
 # The argument structs of include/pto_fuser_hip.h: pointers, strides, then sizes and flags, in C's own layout.
 _CONV = struct.Struct("@N7P6q7i")
@@ -50,19 +50,32 @@ NORM_MAX_WIDTH = 32768
 _ACTIVATIONS = {None: 0, "silu": 1}
 
 
+_FUNCTIONS = {}
+
+
 def _exec(name: str, dev: torch.device, layout: struct.Struct, *fields) -> None:
-    """One launch on the current stream of ``dev``, with it as the current device."""
-    fn = getattr(_hip.load(), name)
+    """One call on the current stream of ``dev``, with it as the current device."""
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_hip.load(), name)
     try:
         args = layout.pack(*fields)
     except struct.error as e:
         raise ValueError(f"a size of this call is past what {name} takes: {e}") from None
-    if torch.cuda.current_device() == dev.index:
-        st = fn(args, _hip.current_stream_handle(dev))
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        st = fn(args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            st = fn(args, _hip.current_stream_handle(dev))
-    _hip.check(name, st)
+            st = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        _hip.check(name, st)
+
+
+def _device_of(t, name: str) -> torch.device:
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        return t.device
+    raise ValueError(f"{name} must be a tensor on a HIP device")
 
 
 def _require_view(t, name: str, shape, dtype, dev) -> None:
@@ -130,7 +143,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     ``lengths`` [B] int32 (None: all T): tokens of each sequence; what follows them is not read, and y is zero there.
     Returns (y [B,T,W] in x's type, the state after the last token [B,K-1,W] or None).  ``final_out`` may be
     ``initial_state``; ``out`` may not overlap x."""
-    dev = _on_device(x, "x")
+    dev = _device_of(x, "x")
     _dim(x, "x", 3, "[B,T,W]")
     _dim(weight, "weight", 2, "[W,K]")
     B, T, W = x.shape
@@ -141,9 +154,12 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     _require_view(x, "x", (B, T, W), dtype, dev)
     w_f32 = _param_f32(weight, "weight", dtype)
     _require(weight, "weight", (W, K), weight.dtype, dev)
-    _require(bias, "bias", (W,), weight.dtype, dev)
-    _require(initial_state, "initial_state", (B, K - 1, W), dtype, dev)
-    _require(lengths, "lengths", (B,), torch.int32, dev)
+    if bias is not None:
+        _require(bias, "bias", (W,), weight.dtype, dev)
+    if initial_state is not None:
+        _require(initial_state, "initial_state", (B, K - 1, W), dtype, dev)
+    if lengths is not None:
+        _require(lengths, "lengths", (B,), torch.int32, dev)
     if out is None:
         y = torch.empty(B, T, W, device=dev, dtype=dtype)
     else:
@@ -153,8 +169,11 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         y = out
     final = None
     if output_final_state:
-        _require(final_out, "final_out", (B, K - 1, W), dtype, dev)
-        final = torch.empty(B, K - 1, W, device=dev, dtype=dtype) if final_out is None else final_out
+        final = final_out
+        if final is None:
+            final = torch.empty((B, K - 1, W), device=dev, dtype=dtype)
+        else:
+            _require(final, "final_out", (B, K - 1, W), dtype, dev)
     sx, sy, state = x.stride(), y.stride(), (K - 1) * W
     _exec("pf_conv_exec", dev, _CONV, _CONV_SIZE, x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(initial_state),
           _ptr(lengths), y.data_ptr(), _ptr(final), sx[0], sx[1], sy[0], sy[1], state, state, B, T, W, K,
@@ -169,7 +188,7 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
 
     ``state`` [S,K-1,W] in x's type is updated in place.  Sequence b's is ``state[slots[b]]`` (``slots`` [B] int32, no two
     the same; one outside the pool is skipped and its y zero), or ``state[b]`` with S = B."""
-    dev = _on_device(x, "x")
+    dev = _device_of(x, "x")
     _dim(x, "x", 2, "[B,W]")
     _dim(weight, "weight", 2, "[W,K]")
     _dim(state, "state", 3, "[S,K-1,W]")
@@ -181,7 +200,8 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     _require_view(x, "x", (B, W), dtype, dev)
     w_f32 = _param_f32(weight, "weight", dtype)
     _require(weight, "weight", (W, K), weight.dtype, dev)
-    _require(bias, "bias", (W,), weight.dtype, dev)
+    if bias is not None:
+        _require(bias, "bias", (W,), weight.dtype, dev)
     _require(state, "state", (state.shape[0], K - 1, W), dtype, dev)
     _pool(state, slots, B, dev)
     if out is None:
@@ -217,7 +237,7 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
     Returns (y [B,H,T,P] in x's type, token-major in memory where x is; the final state [B,H,N,P] float32 or None).
     ``final_out`` may be h0.  Few sequences run as segments side by side, whose number follows from the call's shape: the
     same bfloat16 sequence alone and in a batch differs by its rounding."""
-    dev = _on_device(x, "x")
+    dev = _device_of(x, "x")
     _dim(x, "x", 4, "[B,H,T,P]")
     _dim(B, "B", 4, "[B,G,T,N]")
     nb, H, T, P = x.shape
@@ -231,16 +251,21 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
     _require_view(C, "C", (nb, G, T, N), dtype, dev)
     _dim(dt, "dt", 3, "[B,H,T]")
     dt_f32 = _param_f32(dt, "dt", dtype)
-    if tuple(dt.shape) != (nb, H, T) or dt.device != dev:
+    if dt.shape != (nb, H, T) or dt.get_device() != dev.index:
         raise ValueError(f"dt is {tuple(dt.shape)} on {dt.device}, expected {(nb, H, T)} on {dev}")
     if A is None:
         raise ValueError("A must be a tensor")
-    for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
-        _require(t, name, (H,), torch.float32, dev)
+    _require(A, "A", (H,), torch.float32, dev)
+    if D is not None:
+        _require(D, "D", (H,), torch.float32, dev)
+    if dt_bias is not None:
+        _require(dt_bias, "dt_bias", (H,), torch.float32, dev)
     if z is not None:
         _require_view(z, "z", (nb, H, T, P), dtype, dev)
-    _require(h0, "h0", (nb, H, N, P), torch.float32, dev)
-    _require(lengths, "lengths", (nb,), torch.int32, dev)
+    if h0 is not None:
+        _require(h0, "h0", (nb, H, N, P), torch.float32, dev)
+    if lengths is not None:
+        _require(lengths, "lengths", (nb,), torch.int32, dev)
     if T > 1:      # rows that overlap (a token expanded along the sequence) are laid out first
         x, B, C, z = (t if t is None or t.stride(2) >= t.shape[3] else t.contiguous() for t in (x, B, C, z))
     sx = x.stride()
@@ -255,8 +280,11 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
         y = torch.empty(nb, H, T, P, device=dev, dtype=dtype)
     final = None
     if output_final_state:
-        _require(final_out, "final_out", (nb, H, N, P), torch.float32, dev)
-        final = torch.empty(nb, H, N, P, device=dev, dtype=torch.float32) if final_out is None else final_out
+        final = final_out
+        if final is None:
+            final = torch.empty((nb, H, N, P), device=dev, dtype=torch.float32)
+        else:
+            _require(final, "final_out", (nb, H, N, P), torch.float32, dev)
     need = _hip.load().pf_ssm_workspace_bytes(nb, H, G, T, N, P, code)
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     sb, sc, sy, st = B.stride(), C.stride(), y.stride(), dt.stride()
@@ -282,7 +310,7 @@ def ssm_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.Te
     x, z [B,H,P] float32 or bfloat16 (P a multiple of 4); dt [B,H] in x's type or float32; B, C [B,G,N], N up to 256, head
     h reading group h // (H // G); A, D, dt_bias [H] float32 (A < 0: it decays).  ``state`` [S,H,N,P] float32 is updated
     in place, with ``slots`` as in :func:`causal_conv_step`.  Returns y [B,H,P] in x's type."""
-    dev = _on_device(x, "x")
+    dev = _device_of(x, "x")
     _dim(x, "x", 3, "[B,H,P]")
     _dim(B, "B", 3, "[B,G,N]")
     _dim(state, "state", 4, "[S,H,N,P]")
@@ -297,12 +325,15 @@ def ssm_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.Te
     _require_view(C, "C", (nb, G, N), dtype, dev)
     _dim(dt, "dt", 2, "[B,H]")
     dt_f32 = _param_f32(dt, "dt", dtype)
-    if tuple(dt.shape) != (nb, H) or dt.device != dev:
+    if dt.shape != (nb, H) or dt.get_device() != dev.index:
         raise ValueError(f"dt is {tuple(dt.shape)} on {dt.device}, expected {(nb, H)} on {dev}")
     if A is None:
         raise ValueError("A must be a tensor")
-    for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
-        _require(t, name, (H,), torch.float32, dev)
+    _require(A, "A", (H,), torch.float32, dev)
+    if D is not None:
+        _require(D, "D", (H,), torch.float32, dev)
+    if dt_bias is not None:
+        _require(dt_bias, "dt_bias", (H,), torch.float32, dev)
     if z is not None:
         _require_view(z, "z", (nb, H, P), dtype, dev)
     _require(state, "state", (state.shape[0], H, N, P), torch.float32, dev)
@@ -332,7 +363,7 @@ def gdn_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     [B,H] (GDN), [B,H,DK] (KDA: row d of S decays by g[..., d]) or None (DeltaNet).  ``state`` [S,H,DK,DV] float32 — the
     chunked forwards' ``h_final`` — is updated in place, with ``slots`` as in :func:`causal_conv_step`.  Returns
     o [B,H,DV] float32 scaled by ``scale`` (default DK^-1/2), as the chunked forwards do."""
-    dev = _on_device(q, "q")
+    dev = _device_of(q, "q")
     _dim(q, "q", 3, "[B,H,DK]")
     _dim(v, "v", 3, "[B,H,DV]")
     _dim(state, "state", 4, "[S,H,DK,DV]")
@@ -347,8 +378,10 @@ def gdn_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     if beta is None:
         raise ValueError("beta must be a tensor")
     _require(beta, "beta", (nb, H), torch.float32, dev)
-    rows = g is not None and g.dim() == 3
-    _require(g, "g", (nb, H, N) if rows else (nb, H), torch.float32, dev)
+    rows = False
+    if g is not None:
+        rows = isinstance(g, torch.Tensor) and g.dim() == 3
+        _require(g, "g", (nb, H, N) if rows else (nb, H), torch.float32, dev)
     _require(state, "state", (state.shape[0], H, N, P), torch.float32, dev)
     _pool(state, slots, nb, dev)
     if out is None:
@@ -389,7 +422,7 @@ def _norm(x, weight, residual, eps, y, y_code, block, scales, residual_out):
     h, r_f32, r_row, h_row = None, 0, 0, 0
     if residual is not None:
         r_f32 = _param_f32(residual, "residual", dtype)
-        if residual.shape != x.shape or residual.device != dev:
+        if residual.shape != x.shape or residual.get_device() != dev.index:
             raise ValueError(f"residual is {tuple(residual.shape)} on {residual.device}, expected {tuple(x.shape)} on {dev}")
         r_row = _rows_of(residual, "residual", D)
         if residual_out is None:
@@ -410,8 +443,7 @@ def _norm(x, weight, residual, eps, y, y_code, block, scales, residual_out):
 
 
 def _norm_operand(x) -> None:
-    _on_device(x, "x")
-    _dtype_code(x.dtype)
+    _device_of(x, "x")
     if x.dim() == 0 or not 0 < x.shape[-1] <= NORM_MAX_WIDTH:
         raise ValueError(f"x must be [..., D] with D in 1..{NORM_MAX_WIDTH}, got {tuple(x.shape)}")
 
@@ -454,8 +486,9 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
         out = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     elif out.shape != x.shape or out.dtype != torch.float8_e4m3fn or out.device != x.device:
         raise ValueError(f"out is {tuple(out.shape)} {out.dtype} on {out.device}, expected {tuple(x.shape)} float8_e4m3fn on {x.device}")
-    _require(scales_out, "scales_out", shape, torch.float32, x.device)
     if scales_out is None:
         scales_out = torch.empty(shape, device=x.device, dtype=torch.float32)
+    else:
+        _require(scales_out, "scales_out", shape, torch.float32, x.device)
     h = _norm(x, weight, residual, eps, out, _hip.PF_NORM_FP8, 128 if scale_block else 0, scales_out, residual_out)
     return out, scales_out, h

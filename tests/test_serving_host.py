@@ -24,7 +24,7 @@ def on_cpu(monkeypatch):
     """CPU tensors pass for device ones, and a launch is recorded."""
     made = []
     on = lambda t, name: t.device  # noqa: E731
-    monkeypatch.setattr(serving, "_on_device", on)
+    monkeypatch.setattr(serving, "_device_of", on)
     monkeypatch.setattr(serving, "_exec", lambda name, dev, layout, *fields: made.append((name, layout.pack(*fields))))
     monkeypatch.setattr(torch.Tensor, "get_device", lambda self: None)
     return made
@@ -248,6 +248,6 @@ def test_norm_refusals(on_cpu):
 
 def test_sizes_past_32_bits_are_refused(monkeypatch):
     """A size that does not fit its field is a ValueError, not a struct's."""
-    monkeypatch.setattr(_hip, "load", lambda: type("Lib", (), {"pf_norm_exec": None}))
+    monkeypatch.setattr(serving, "_FUNCTIONS", {"pf_norm_exec": None})
     with pytest.raises(ValueError, match="past what pf_norm_exec takes"):
         serving._exec("pf_norm_exec", torch.device("cuda", 0), serving._NORM, serving._NORM_SIZE, *[0] * 10, 1 << 31, *[0] * 6, 0.0)
