@@ -36,7 +36,7 @@ struct SsmArgs {
   const int* lengths;      // [B] or null
   void* y;
   float* h_final;          // or null; may be h0
-  float* seg_state;        // [B, H, segs, N, P]: what a segment adds, then what enters it
+  float* seg_state;        // what a segment adds, then what enters it: per task the registers of its waves, as they lie
   float* seg_decay;        // [B, H, segs]: log2 of a segment's decay
   long x_b, x_h, x_t, dt_b, dt_h, dt_t, b_b, b_g, b_t, c_b, c_g, c_t, z_b, z_h, z_t, y_b, y_h, y_t;
   uint32_t tasks;          // B * G * column blocks * segments
@@ -50,28 +50,6 @@ enum class SsmMode { kStates, kOutput };
 
 // A buffer offset past the end of any: reads as zero, is not written.
 constexpr uint32_t kPastEnd = 0x80000000u;
-
-template <typename E> __device__ __forceinline__ void buf_load4(__amdgpu_buffer_rsrc_t r, uint32_t off, float (&v)[4]);
-template <> __device__ __forceinline__ void buf_load4<bf16>(__amdgpu_buffer_rsrc_t r, uint32_t off, float (&v)[4]) {
-  const bf16x4 x = __builtin_bit_cast(bf16x4, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
-}
-template <> __device__ __forceinline__ void buf_load4<float>(__amdgpu_buffer_rsrc_t r, uint32_t off, float (&v)[4]) {
-  const floatx4 x = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = x[i];
-}
-template <typename E> __device__ __forceinline__ void buf_store4(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&v)[4]);
-template <> __device__ __forceinline__ void buf_store4<bf16>(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&v)[4]) {
-  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-  const bf16x4 x = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
-  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), r, off, 0, 0);
-}
-template <> __device__ __forceinline__ void buf_store4<float>(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&v)[4]) {
-  const floatx4 x = {v[0], v[1], v[2], v[3]};
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), r, off, 0, 0);
-}
 
 // ---- one MFMA operand of 32 contraction rows: eight values a lane ---------------------------
 template <typename E> struct Frag;
@@ -136,9 +114,9 @@ template <typename E, int W, int PAD> struct Tile {
 // that a lane group's rows in the two are the eight neighbouring columns of B or C it reads as one vector.
 __device__ __forceinline__ constexpr int state_row(int nt, int g, int r) { return 32 * (nt >> 1) + 8 * g + 4 * (nt & 1) + r; }
 
-template <typename E> struct TileVec4;        // an MFMA result as four operand values
-template <> struct TileVec4<bf16> { typedef bf16x4 T; };
-template <> struct TileVec4<float> { typedef floatx4 T; };
+// Column, of a wave's 16 PT, that lane c holds in tile pt: interleaved the same way, so that the rows 4g .. of the PT tiles
+// of y^T are 4 PT neighbouring columns, one vector.
+template <int PT> __device__ __forceinline__ constexpr int state_col(int pt, int c) { return 4 * PT * (c >> 2) + 4 * pt + (c & 3); }
 
 // x scaled by its rows' weights, in SPLIT bf16 terms: each the rounding of what the ones before it left (8, 16 or 24 bits
 // of the product); fp32 needs one.
@@ -189,10 +167,13 @@ __device__ __forceinline__ void wave_sums(float v, int g, float& up_to, float& f
   from = b + (g == 3 ? 0.f : g == 2 ? r[3] : g == 1 ? r[2] + r[3] : r[1] + (r[2] + r[3]));
 }
 
+// (chunk, head) pairs of a batch of tables that a wave makes.
+constexpr int kSsmShare = 2;
+
 // The outputs keep one chunk and what only they need; the states' kernel two chunks.
 template <typename E, int NT, int NW, int PT, bool OUT> struct SsmLds {
-  static constexpr int SLOTS = 4 * NW, BUF = OUT ? 1 : 2;
-  typedef Tile<E, NT, 32 / (int)sizeof(E)> B;
+  static constexpr int SLOTS = kSsmShare * NW, BUF = OUT ? 1 : 2;
+  typedef Tile<E, NT, (OUT ? 32 : 16) / (int)sizeof(E)> B;
   typedef Tile<E, NT, 16 / (int)sizeof(E)> C;
   typedef Tile<E, 16 * PT, 16 / (int)sizeof(E)> X;
   E b[BUF][B::ELEMS];
@@ -224,14 +205,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   using Xs = typename Lds::X;
   __shared__ __attribute__((aligned(16))) Lds s;
 
-  // Workgroups go round robin over the eight XCDs: each XCD takes a run of tasks, whose neighbours (the blocks of columns
-  // of one group's segment) read the same B and C through its L2.
+  // Workgroups go round robin over the eight XCDs: each XCD takes a run of tasks, so that the segments of one block of
+  // columns, and the sum along them, meet in its L2.
   const uint32_t per = (a.tasks + 7) / 8, task = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (blockIdx.x >> 3 >= per || task >= a.tasks) return;
-  const int cb = (int)(task % (uint32_t)a.blocks);
-  uint32_t rest = task / (uint32_t)a.blocks;
-  const int seg = (int)(rest % (uint32_t)a.segs);
-  rest /= (uint32_t)a.segs;
+  const int seg = (int)(task % (uint32_t)a.segs);
+  uint32_t rest = task / (uint32_t)a.segs;
+  const int cb = (int)(rest % (uint32_t)a.blocks);
+  rest /= (uint32_t)a.blocks;
   const int grp = (int)(rest % (uint32_t)a.G);
   const long bi = rest / (uint32_t)a.G;
 
@@ -290,12 +271,18 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
     for (int i = 0; i < NX; ++i) *reinterpret_cast<u32x4*>(&s.x[buf][w][(x_row + i * (64 / XV)) * Xs::LD + x_col]) = rx[i];
   };
   // ---- the chunks' step sizes and decays, a token a lane, in log2.  A batch of chunks at a time: its (chunk, head) pairs
-  // are dealt over the waves, four each, the steps loaded a batch ahead.
+  // are dealt over the waves, the steps loaded a batch ahead.
   const int h_first = cb * COLS / P, heads = min(R, (cb * COLS + COLS - 1) / P + 1) - h_first, batch = Lds::SLOTS / heads;
-  float rdt[4];
+  float rdt[kSsmShare], ra[kSsmShare], rbias[kSsmShare];
+#pragma unroll
+  for (int i = 0; i < kSsmShare; ++i) {
+    const int head = grp * R + h_first + (w + i * NW) % heads;
+    ra[i] = a.a[head];
+    rbias[i] = a.dt_bias ? a.dt_bias[head] : 0.f;
+  }
   auto load_dt = [&](int ch) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kSsmShare; ++i) {
       const int slot = w + i * NW, t = (ch + slot / heads) * Q + lane;
       rdt[i] = 0.f;
       if (slot / heads < batch && t < len)
@@ -304,14 +291,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   };
   auto tabulate = [&](int ch) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int slot = w + i * NW, head = grp * R + h_first + slot % heads;
+    for (int i = 0; i < kSsmShare; ++i) {
+      const int slot = w + i * NW;
       if (slot / heads >= batch) continue;
-      float dt = rdt[i];
-      if (a.dt_bias) dt += a.dt_bias[head];
+      float dt = rdt[i] + rbias[i];
       if (a.softplus) dt = softplus(dt);
       if ((ch + slot / heads) * Q + lane >= len) dt = 0.f;
-      const float gate = dt * (a.a[head] * 1.44269504f);
+      const float gate = dt * (ra[i] * 1.44269504f);
       float G, after;
       wave_sums(gate, g, G, after);
       s.tab[slot][0][lane] = dt * pow2(after - gate);
@@ -330,10 +316,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   for (int nt = 0; nt < NTS; ++nt)
 #pragma unroll
     for (int pt = 0; pt < PT; ++pt) S[nt][pt] = zero4();
+  floatx4* const slab = reinterpret_cast<floatx4*>(a.seg_state) + ((size_t)task * NW + w) * NTS * PT * 64 + lane;
   if (OUT && active) {
-    const float* in = a.segs > 1 ? a.seg_state + (((long)bi * a.H + h) * a.segs + seg) * N * P
-                                 : (a.h0 ? a.h0 + ((long)bi * a.H + h) * N * P : nullptr);
-    if (in) {
+    if (a.segs > 1) {
+#pragma unroll
+      for (int nt = 0; nt < NTS; ++nt)
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt) S[nt][pt] = slab[(nt * PT + pt) * 64];
+    } else if (a.h0) {
+      const float* in = a.h0 + ((long)bi * a.H + h) * N * P + p0;
 #pragma unroll
       for (int nt = 0; nt < NTS; ++nt)
 #pragma unroll
@@ -341,7 +332,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int n = state_row(nt, g, r);
-            if (n < N) S[nt][pt][r] = in[(long)n * P + p0 + 16 * pt + c];
+            if (n < N) S[nt][pt][r] = in[n * P + state_col<PT>(pt, c)];
           }
     }
   }
@@ -349,7 +340,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   const int yt = (int)a.y_t * ES, zt = (int)a.z_t * ES;
   char* yg = reinterpret_cast<char*>(static_cast<E*>(a.y) + bi * a.y_b + h * a.y_h + p0);
   const char* zg = reinterpret_cast<const char*>(static_cast<const E*>(a.z) + bi * a.z_b + h * a.z_h + p0);
-  const uint32_t y_off = active ? (uint32_t)(c * yt + 4 * g * ES) : kPastEnd, z_off = (uint32_t)(c * zt + 4 * g * ES);
+  const uint32_t y_off = active ? (uint32_t)(c * yt + 4 * PT * g * ES) : kPastEnd;
+  const uint32_t z_off = active ? (uint32_t)(c * zt + 4 * PT * g * ES) : kPastEnd;
+  static_assert(4 * PT == V, "a lane's columns of y are one vector");
   const float dd = active && a.d ? a.d[h] : 0.f;
 
   // Added to an exponent on the score's diagonal tiles: 2^-inf above the diagonal, whatever the sums are there.  (Opaque to
@@ -395,7 +388,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 #pragma unroll
     for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) xf[pt][kb] = Xs::template cols<4>(sx, 16 * pt, kb, c, g);
+      for (int kb = 0; kb < 2; ++kb) xf[pt][kb] = Xs::template cols<4 * PT>(sx, 4 * pt, kb, c, g);
 
     if constexpr (OUT) {
       // the score's tiles, dealt over the waves
@@ -429,6 +422,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
           for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(sf[pt], cf, y[pt][ib]);
         }
       }
+      // z of this chunk, for the epilogue
+      const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
+      u32x4 rz[HAS_Z ? 4 : 1];
+      if (HAS_Z) {
+        const auto zr = make_rsrc(zg + (long)t0 * zt, (uint32_t)(valid * zt));
+#pragma unroll
+        for (int ib = 0; ib < 4; ++ib) rz[ib] = __builtin_amdgcn_raw_buffer_load_b128(zr, z_off + 16 * ib * zt, 0, 0);
+      }
       lds_barrier();                           // the score is whole
       floatx4 u[4];
 #pragma unroll
@@ -461,56 +462,54 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
           for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(xf[pt][kb], pf, y[pt][ib]);
         }
       }
-      // y out: lane c's token, four columns of each tile
-      const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
+      // y out: lane c's token, the lane group's 4 PT columns as one vector
       const auto yr = make_rsrc(yg + (long)t0 * yt, (uint32_t)(min(a.T - t0, Q) * yt));
-      const auto zr = make_rsrc(zg + (long)t0 * zt, HAS_Z ? (uint32_t)(valid * zt) : 0);
 #pragma unroll
-      for (int ib = 0; ib < 4; ++ib)
+      for (int ib = 0; ib < 4; ++ib) {
+        float v[4 * PT];
+        load_vec<4 * PT>(&sx[(16 * ib + c) * Xs::LD + 4 * PT * g], v);
 #pragma unroll
-        for (int pt = 0; pt < PT; ++pt) {
-          float v[4];
-          load_vec<4>(&sx[(16 * ib + c) * Xs::LD + 16 * pt + 4 * g], v);
+        for (int i = 0; i < 4 * PT; ++i) v[i] = fmaf(dd, v[i], y[i / 4][ib][i % 4]);
+        if (HAS_Z) {
+          float z[4 * PT];
+          expand<E, V>(__builtin_bit_cast(typename VecAny<E, V>::T, rz[ib]), z);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = fmaf(dd, v[r], y[pt][ib][r]);
-          if (HAS_Z) {
-            float z[4];
-            buf_load4<E>(zr, z_off + 16 * ib * zt + 16 * pt * ES, z);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] *= silu(z[r]);
-          }
-          if (valid < Q) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = 16 * ib + c < valid ? v[r] : 0.f;
-          }
-          buf_store4<E>(yr, y_off + 16 * ib * yt + 16 * pt * ES, v);
+          for (int i = 0; i < 4 * PT; ++i) v[i] *= silu(z[i]);
         }
+        typename VecAny<E, V>::T o;
+#pragma unroll
+        for (int i = 0; i < 4 * PT; ++i) o[i] = from_f32<E>(v[i]);
+        u32x4 bits = __builtin_bit_cast(u32x4, o);
+        if (valid < Q && 16 * ib + c >= valid) bits = u32x4{0, 0, 0, 0};
+        __builtin_amdgcn_raw_buffer_store_b128(bits, yr, y_off + 16 * ib * yt, 0, 0);
+      }
     }
-    // S <- e^{G_last} S + B^T (w x)
+    // S <- e^{G_last} S + B^T (w x), a tile column and half of the chunk at a time: the products of one while the next one's
+    // x is weighed.
     const float total = s.total[slot0 + hl], e = pow2(total);
     decay2 += total;
+    floatx4 wt[4];
 #pragma unroll
-    for (int nt = 0; nt < NTS; ++nt)
+    for (int q = 0; q < 4; ++q) wt[q] = *reinterpret_cast<const floatx4*>(&tab[0][16 * q + 4 * g]);
+    Frag<E> bf[NTS], wx[2][SPLIT];
 #pragma unroll
-      for (int pt = 0; pt < PT; ++pt) S[nt][pt] *= e;
+    for (int nt = 0; nt < NTS; ++nt) bf[nt] = Bs::template cols<8>(sb, 32 * (nt >> 1) + 4 * (nt & 1), 0, c, g);
+    weigh(xf[0][0], wt[0], wt[1], wx[0]);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const floatx4 w0 = *reinterpret_cast<const floatx4*>(&tab[0][32 * kb + 4 * g]);
-      const floatx4 w1 = *reinterpret_cast<const floatx4*>(&tab[0][32 * kb + 16 + 4 * g]);
-      Frag<E> wx[PT][SPLIT];
+    for (int st = 0; st < 2 * PT; ++st) {
+      const int kb = st / PT, pt = st % PT, nx = st + 1;
+      if (nx < 2 * PT) weigh(xf[nx % PT][nx / PT], wt[2 * (nx / PT)], wt[2 * (nx / PT) + 1], wx[nx & 1]);
+      if (kb == 0) {
 #pragma unroll
-      for (int pt = 0; pt < PT; ++pt) weigh(xf[pt][kb], w0, w1, wx[pt]);
-#pragma unroll
-      for (int np = 0; np < NTS; np += 2) {
-        const Frag<E> b0 = Bs::template cols<8>(sb, 16 * np, kb, c, g), b1 = Bs::template cols<8>(sb, 16 * np + 4, kb, c, g);
-#pragma unroll
-        for (int k = SPLIT - 1; k >= 0; --k)
-#pragma unroll
-          for (int pt = 0; pt < PT; ++pt) {
-            S[np][pt] = mfma32(b0, wx[pt][k], S[np][pt]);
-            S[np + 1][pt] = mfma32(b1, wx[pt][k], S[np + 1][pt]);
-          }
+        for (int nt = 0; nt < NTS; ++nt) S[nt][pt] *= e;
       }
+#pragma unroll
+      for (int k = SPLIT - 1; k >= 0; --k)
+#pragma unroll
+        for (int nt = 0; nt < NTS; ++nt) {
+          S[nt][pt] = mfma32(bf[nt], wx[st & 1][k], S[nt][pt]);
+          if (k == 0 && pt == PT - 1 && kb == 0) bf[nt] = Bs::template cols<8>(sb, 32 * (nt >> 1) + 4 * (nt & 1), 1, c, g);
+        }
     }
     if (!OUT && ch + 1 < end) {
       stage((ch + 1) & 1);
@@ -524,14 +523,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
     }
   }
 
-  float* out = nullptr;
-  if (OUT) {
-    if (a.segs == 1 && a.h_final) out = a.h_final + ((long)bi * a.H + h) * N * P;
-  } else {
-    out = a.seg_state + (((long)bi * a.H + h) * a.segs + seg) * N * P;
-    if (active && p0 == 0 && lane == 0) a.seg_decay[((long)bi * a.H + h) * a.segs + seg] = decay2;
-  }
-  if (active && out) {
+  if (!active) return;
+  if (!OUT) {
+    if (p0 == 0 && lane == 0) a.seg_decay[((long)bi * a.H + h) * a.segs + seg] = decay2;
+#pragma unroll
+    for (int nt = 0; nt < NTS; ++nt)
+#pragma unroll
+      for (int pt = 0; pt < PT; ++pt) slab[(nt * PT + pt) * 64] = S[nt][pt];
+  } else if (a.segs == 1 && a.h_final) {
+    float* out = a.h_final + ((long)bi * a.H + h) * N * P + p0;
 #pragma unroll
     for (int nt = 0; nt < NTS; ++nt)
 #pragma unroll
@@ -539,22 +539,36 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int n = state_row(nt, g, r);
-          if (n < N) out[(long)n * P + p0 + 16 * pt + c] = S[nt][pt][r];
+          if (n < N) out[n * P + state_col<PT>(pt, c)] = S[nt][pt][r];
         }
   }
 }
 
 // The states that enter the segments, in place of what each adds: H_0 = h0, H_{s+1} = decay_s H_s + D_s; the last is the
-// final state.  A thread owns four neighbouring elements; the segments' values are loaded eight ahead of the sum.
+// final state.  A thread owns the four elements of one register of a segment's waves (four rows of one column); the
+// segments' values are loaded eight ahead of the sum.  The workgroups of one column block run where its segments' did.
+template <int NT, int PT, int COLS>
 __global__ __launch_bounds__(256) void ssm_prefix_kernel(SsmArgs a) {
-  const long vecs = (long)a.N * a.P / 4, id = block_id() * 256 + threadIdx.x;
-  if (id >= vecs * a.B * a.H) return;
-  const long bh = id / vecs, at = id % vecs * 4;
-  const long step = (long)a.N * a.P;
-  float* st = a.seg_state + bh * a.segs * step + at;
+  constexpr int SLAB = COLS * NT / 4, NTS = NT / 16;       // vectors of a segment
+  const long blocks = (long)(a.tasks / (uint32_t)a.segs) * (SLAB / 256), per = (blocks + 7) / 8;
+  const long block = (block_id() & 7) * per + (block_id() >> 3);
+  if (block_id() >> 3 >= per || block >= blocks) return;
+  const int at = (int)(block % (SLAB / 256)) * 256 + threadIdx.x;
+  const long unit = block / (SLAB / 256);
+  const int lane = at & 63, c = lane & 15, g = lane >> 4, pt = at / 64 % PT, nt = at / (64 * PT) % NTS, w = at / (64 * PT * NTS);
+  const int col = (int)(unit % a.blocks) * COLS + w * 16 * PT + state_col<PT>(pt, c), R = a.H / a.G;
+  if (col >= R * a.P) return;
+  const long bg = unit / a.blocks, bh = bg / a.G * a.H + bg % a.G * R + col / a.P;
+  const long h_at = bh * a.N * a.P + col % a.P;
+  const int n = state_row(nt, g, 0);                       // and the three after it
   const float* decay = a.seg_decay + bh * a.segs;
+  floatx4* st = reinterpret_cast<floatx4*>(a.seg_state) + (size_t)unit * a.segs * SLAB + at;
   floatx4 H = zero4();
-  if (a.h0) H = *reinterpret_cast<const floatx4_any*>(a.h0 + bh * step + at);
+  if (a.h0) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < a.N) H[r] = a.h0[h_at + (long)(n + r) * a.P];
+  }
   constexpr int AHEAD = 8;
   for (int s0 = 0; s0 < a.segs; s0 += AHEAD) {
     floatx4 D[AHEAD];
@@ -562,17 +576,21 @@ __global__ __launch_bounds__(256) void ssm_prefix_kernel(SsmArgs a) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
       if (s0 + i < a.segs) {
-        D[i] = *reinterpret_cast<const floatx4*>(st + (s0 + i) * step);
+        D[i] = st[(size_t)(s0 + i) * SLAB];
         e[i] = pow2(decay[s0 + i]);
       }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
       if (s0 + i < a.segs) {
-        *reinterpret_cast<floatx4*>(st + (s0 + i) * step) = H;
+        st[(size_t)(s0 + i) * SLAB] = H;
         H = H * e[i] + D[i];
       }
   }
-  if (a.h_final) *reinterpret_cast<floatx4_any*>(a.h_final + bh * step + at) = H;
+  if (a.h_final) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < a.N) a.h_final[h_at + (long)(n + r) * a.P] = H[r];
+  }
 }
 
 }  // namespace pf

@@ -23,26 +23,55 @@ bool shape_ok(int B, int H, int G, int T, int N, int P, int dtype) {
          P <= 256 && P % 32 == 0 && (dtype == PF_DTYPE_F32 || dtype == PF_DTYPE_BF16);
 }
 
-size_t state_bytes(long chains, int segs, int N, int P) {
-  return (size_t)chains * segs * N * P * sizeof(float) + (size_t)chains * segs * sizeof(float);
-}
+int padded_rows(int N) { return N <= 64 ? 64 : 128; }
+
+// The segments' states lie as the waves hold them: whole blocks of columns, rows padded.
+size_t state_floats(long units, int segs, int cols, int N) { return (size_t)units * segs * cols * padded_rows(N); }
+
+// What a plan takes in microseconds, within some 15 % of what was measured (one workgroup a CU, N = 128): whole sequences a
+// fixed part and a step a chunk; segments a fixed part for three launches, a step of both kernels a chunk of a segment, the
+// sum along the segments and the traffic of their states.  A step of 64 columns takes nearly as long as one of 256 (it is
+// latency, not throughput), so wide blocks win once there are enough of them to fill the chip, narrow ones before.
+// 32 heads of 64, bf16, us at 64 / 128 / 256 columns: 1 x 512 tokens 24.3 / 24.7 / 28.9 (in segments; whole 51 / 50 / 57),
+// 4 x 2048 131 / 79 / 68 (whole 179 / 172 / 198), 16 x 256 whole 39 / 36 / 40 (two segments of 256 columns 54),
+// 16 x 1024 110 / 100 whole, 108 in two segments of 256.
+struct SsmCost {
+  int cols;
+  double whole0, whole_step, seg0, seg_step;
+};
+constexpr SsmCost kCost[2][3] = {{{64, 10, 8.5, 15, 11.5}, {128, 10, 12.5, 17, 17}, {0, 0, 0, 0, 0}},
+                                 {{64, 10, 5, 13, 8}, {128, 10, 5, 14, 8}, {256, 12, 6, 15, 8.5}}};
 
 SsmPlan plan(int B, int H, int G, int T, int N, int P, int dtype) {
-  SsmPlan p{};
-  const long cols = (long)(H / G) * P;
-  p.cols = 64;
-  while (p.cols < cols && p.cols < (dtype == PF_DTYPE_BF16 ? 256 : 128)) p.cols *= 2;
-  p.blocks = (int)((cols + p.cols - 1) / p.cols);
   const int chunks = (T + pf::kSsmChunk - 1) / pf::kSsmChunk;
-  const long units = (long)B * G * p.blocks;
-  // Segments while they fit one generation of workgroups, of two chunks at least.
-  long segs = units > 0 ? pf::kCus / units : 1;
-  if (segs > chunks / 2) segs = chunks / 2;
-  if (segs < 2) segs = 1;
-  p.seg_chunks = chunks ? (int)((chunks + segs - 1) / segs) : 1;
-  p.segs = chunks ? (chunks + p.seg_chunks - 1) / p.seg_chunks : 1;
-  p.bytes = p.segs > 1 ? state_bytes((long)B * H, p.segs, N, P) : 0;
-  return p;
+  const long width = (long)(H / G) * P;
+  SsmPlan best{};
+  double least = 0;
+  for (const SsmCost& c : kCost[dtype == PF_DTYPE_BF16]) {
+    if (!c.cols || (c.cols > 64 && width <= c.cols / 2)) continue;
+    SsmPlan p{};
+    p.cols = c.cols;
+    p.blocks = (int)((width + c.cols - 1) / c.cols);
+    const long units = (long)B * G * p.blocks;
+    const auto consider = [&](int seg_chunks, double us) {
+      if (best.cols && us >= least) return;
+      p.seg_chunks = seg_chunks;
+      p.segs = chunks ? (chunks + seg_chunks - 1) / seg_chunks : 1;
+      best = p;
+      least = us;
+    };
+    consider(chunks ? chunks : 1, (double)((units + pf::kCus - 1) / pf::kCus) * (c.whole0 + c.whole_step * chunks));
+    long most = units > 0 ? pf::kCus / units : 1;       // one generation of workgroups
+    if (most > chunks) most = chunks;
+    for (; most >= 2; most /= 2) {
+      const int each = (int)((chunks + most - 1) / most), segs = (chunks + each - 1) / each;
+      if (segs < 2) break;
+      consider(each, c.seg0 + c.seg_step * each + 0.35 * segs + (double)units * segs * c.cols * padded_rows(N) * 16 / 9e6);
+    }
+  }
+  const long units = (long)B * G * best.blocks;
+  best.bytes = best.segs > 1 ? (state_floats(units, best.segs, best.cols, N) + (size_t)B * H * best.segs) * sizeof(float) : 0;
+  return best;
 }
 
 constexpr double kMaxTasks = 1 << 22;   // workgroups of up to 1024 threads in one grid dimension
@@ -69,11 +98,12 @@ int launch(pf::SsmArgs& a, hipStream_t s) {
   a.tasks = (uint32_t)tasks;
   const dim3 grid((a.tasks + 7) / 8 * 8);
   dim3 prefix;
-  if (!grid_of(((double)a.N * a.P / 4 * a.B * a.H + 255) / 256, prefix)) return PF_ERR_ARG;
+  const double prefix_blocks = tasks / a.segs * (COLS * NT / 4 / 256);
+  if (!grid_of((double)((long)(prefix_blocks + 7) / 8 * 8), prefix)) return PF_ERR_ARG;
   pf::LaunchScope scope;
   if (a.segs > 1) {
     pf::ssm_kernel<E, NT, NW, PT, SsmMode::kStates, kF32 ? 1 : 3, false><<<grid, dim3(NW * 64), 0, s>>>(a);
-    pf::ssm_prefix_kernel<<<prefix, dim3(256), 0, s>>>(a);
+    pf::ssm_prefix_kernel<NT, PT, COLS><<<prefix, dim3(256), 0, s>>>(a);
     outputs<E, NT, NW, PT, kF32 ? 1 : 2>(a, grid, s);
   } else {
     outputs<E, NT, NW, PT, kF32 ? 1 : 3>(a, grid, s);
@@ -121,7 +151,7 @@ int pf_ssm_exec(const pf_ssm_args* p, void* stream) {
   a.x = p->x; a.dt = p->dt; a.b = p->b; a.c = p->c; a.z = p->z; a.a = p->a; a.d = p->d; a.dt_bias = p->dt_bias;
   a.h0 = p->h0; a.lengths = p->lengths; a.y = p->y; a.h_final = p->h_final;
   a.seg_state = static_cast<float*>(p->workspace);
-  a.seg_decay = a.seg_state + (size_t)p->B * p->H * pl.segs * p->N * p->P;
+  a.seg_decay = a.seg_state + state_floats((long)p->B * p->G * pl.blocks, pl.segs, pl.cols, p->N);
   a.x_b = p->x_b; a.x_h = p->x_h; a.x_t = x_t; a.dt_b = p->dt_b; a.dt_h = p->dt_h; a.dt_t = p->dt_t;
   a.b_b = p->b_b; a.b_g = p->b_g; a.b_t = b_t; a.c_b = p->c_b; a.c_g = p->c_g; a.c_t = c_t;
   a.z_b = p->z_b; a.z_h = p->z_h; a.z_t = z_t; a.y_b = p->y_b; a.y_h = p->y_h; a.y_t = y_t;
@@ -130,8 +160,8 @@ int pf_ssm_exec(const pf_ssm_args* p, void* stream) {
   a.dt_f32 = p->dt_f32; a.softplus = p->softplus;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p->dtype == PF_DTYPE_BF16)
-    return p->N <= 64 ? launch_cols<bf16, 64>(a, pl.cols, s) : launch_cols<bf16, 128>(a, pl.cols, s);
-  return p->N <= 64 ? launch_cols<float, 64>(a, pl.cols, s) : launch_cols<float, 128>(a, pl.cols, s);
+    return padded_rows(p->N) == 64 ? launch_cols<bf16, 64>(a, pl.cols, s) : launch_cols<bf16, 128>(a, pl.cols, s);
+  return padded_rows(p->N) == 64 ? launch_cols<float, 64>(a, pl.cols, s) : launch_cols<float, 128>(a, pl.cols, s);
 }
 
 }  // extern "C"

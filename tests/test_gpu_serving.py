@@ -415,6 +415,20 @@ def test_ssm(dtype, B, H, T, P, G, N):
     _check_ssm(s, y, final)
 
 
+@pytest.mark.parametrize("dtype,B,H,T,P,G,N,segments", [
+    (BF, 9, 64, 130, 64, 1, 16, False),        # whole sequences, blocks of 256 columns
+    (BF, 1, 32, 4096, 64, 1, 80, True),        # segments of 256 columns, batches of tables begun again
+    (BF, 4, 13, 700, 96, 1, 32, True),         # heads cut by the blocks' ends
+    (BF, 2, 48, 180, 32, 2, 16, True), (F32, 3, 24, 300, 32, 2, 32, True), (F32, 40, 12, 129, 64, 1, 16, False)])
+def test_ssm_of_many_columns(dtype, B, H, T, P, G, N, segments):
+    """Shapes that take the wide blocks of columns, with and without segments."""
+    from pto_fuser_amd import _hip
+    announce(f"ssm_chunk_forward {dtype} B{B} H{H} T{T} P{P} G{G} N{N}")
+    assert (_hip.load().pf_ssm_workspace_bytes(B, H, G, T, N, P, int(dtype is BF)) > 0) == segments
+    s = _ssm_case(T + P, dtype, B, H, T, P, G, N, z=False)
+    _check_ssm(s, *pf_ssm(s))
+
+
 def pf_ssm(s, **kw):
     from pto_fuser_amd import ssm_chunk_forward
     return ssm_chunk_forward(s["x"], s["dt"], s["A"], s["B"], s["C"], s["D"], z=s["z"], dt_bias=s["dt_bias"],

@@ -114,11 +114,22 @@ def test_ssm_workspace_sizes(lib):
     assert lib.pf_ssm_exec(_ssm(B=0), None) == _hip.PF_OK
     assert size(1, 4, 1, 64, 128, 64, 1) == 0 and size(64, 64, 1, 8192, 128, 64, 1) == 0
     assert size(1, 4, 1, 8192, 100, 64, 1) == 0 and size(1 << 20, 1 << 20, 1, 8192, 128, 64, 1) == 0
-    for H, G, T, N, P in ((4, 1, 8192, 128, 64), (32, 1, 32768, 128, 64), (32, 32, 4096, 64, 128), (1, 1, 1 << 30, 16, 32)):
+    for H, G, T, N, P in ((4, 1, 8192, 128, 64), (32, 1, 32768, 128, 64), (32, 32, 4096, 64, 128), (64, 2, 1 << 30, 64, 64)):
         one = H * (N * P + 1) * 4
         for dtype in (0, 1):
             n = size(1, H, G, T, N, P, dtype)
             assert n and n % one == 0 and 2 <= n // one <= 512
+    assert 0 < size(1, 1, 1, 1 << 30, 16, 32, 1) <= 256 * 256 * 64 * 4 + 1024      # narrow states: padded blocks
+
+
+@pytest.mark.parametrize("B,H,T,P,dtype,segments", [
+    (1, 4, 256, 64, 1, 4), (1, 4, 512, 64, 1, 8), (1, 32, 1024, 64, 1, 16), (1, 32, 4096, 64, 1, 32), (2, 32, 8192, 64, 1, 16),
+    (4, 32, 2048, 64, 1, 8), (4, 32, 512, 64, 1, 4), (16, 32, 256, 64, 1, 0), (16, 32, 1024, 64, 1, 0), (16, 64, 512, 64, 1, 0),
+    (8, 64, 192, 64, 1, 0), (1, 4, 512, 64, 0, 8), (8, 32, 256, 64, 0, 0), (2, 32, 1024, 64, 0, 8)])
+def test_ssm_plans_where_they_were_measured(lib, B, H, T, P, dtype, segments):
+    """The number of segments (0: whole sequences) at shapes measured every way; the times are beside the rule."""
+    n, one = lib.pf_ssm_workspace_bytes(B, H, 1, T, 128, P, dtype), B * H * (128 * P + 1) * 4
+    assert n == segments * one
 
 
 def _norm(**kw):
