@@ -251,7 +251,7 @@ const char* pf_status_string(int status) {
   return "unknown status";
 }
 
-int pf_abi_version(void) { return 2; }
+int pf_abi_version(void) { return 3; }
 
 #ifndef PF_SOURCE_HASH
 #define PF_SOURCE_HASH "unknown"

@@ -5,6 +5,9 @@
 // Memory bound: 2K + 5 operations for two elements moved.  A thread owns VEC neighbouring channels (16 bytes) and TT
 // consecutive tokens: all its rows are loaded before the first is used, the window of K rows slides through registers,
 // and the K-1 rows before its tokens are read again (from the caches: the neighbouring thread's rows).
+// Measured, 4 x 4096 x 6144 bf16, K = 4: 91 us, 4.4 TB/s of the 403 MB it cannot do without (a copy of that size reaches
+// 5.3).  4 / 8 / 16 tokens a thread 105 / 92 / 91 us there, 11.6 / 12.7 / 15.9 at 3 x 1471 x 1920 fp32: 8.  The
+// activation's exponential and quotient are what is left beside the memory.  One token of 64 sequences: 4.1 us, launch.
 #pragma once
 
 #include "pf_serving.h"

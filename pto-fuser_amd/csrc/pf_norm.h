@@ -6,6 +6,8 @@
 // One pass: a row stays in the registers of the threads that loaded it (VPT vectors of 16 bytes each), the sum of
 // squares and the maximum are reduced across them in fp32, and y and h leave from the same registers.  h is rounded
 // once, when it is stored; the norm is of the sum before that.
+// Memory bound.  Measured, bf16 with a residual: 16384 x 2048, a wave a row, 50.5 us, 5.3 TB/s, a copy's rate;
+// 8191 x 6144 to 8 bits in blocks of 128, a workgroup a row, 76 us, 4.7 TB/s.  Four rows: 5 us, latency.
 #pragma once
 
 #include "pf_serving.h"

@@ -12,6 +12,20 @@
 // Few sequences do not fill the chip with whole walks.  A sequence then runs as segments side by side, in three launches:
 // the state each segment adds by itself (kStates: no C, no score), the states that enter the segments (a sum along the
 // segments, ssm_prefix_kernel), and the outputs (kOutput from those states).
+//
+// Rounding, bf16 operands: S and the decayed score are rounded to 8 bits where they enter a product for y (which is
+// rounded to 8 bits itself); the state is a sum in fp32 of products whose weighted operand has 16 or 24 bits (SPLIT).
+// fp32 operands: fp32 matrix instructions throughout.
+//
+// Measured, bf16, N = 128, P = 64 (kernel times): 2 x 32 heads x 8192 tokens, 16 segments: states 40 us (67 MB of x and
+// 34 MB of states moved, 2.6 TB/s), sum 13.5 us (67 MB, 5.0 TB/s), outputs 60 us (170 MB, 2.8 TB/s).  Bound by the chunk
+// step, not the memory: 6 900 and 11 700 cycles a step of a workgroup, of which the matrix pipes work 3 070 and 3 700, the
+// vector port 5 000 and 6 000 and LDS 3 600 and 5 000.  Two waves share a SIMD (the states and the chunk in flight fill
+// its registers), and a wave's own vector instructions wait for its matrix instructions, so these add up more than they
+// overlap.  Measured and left out: 64 columns a wave with one wave a SIMD (states 50, outputs 75 us: the halved LDS
+// traffic is lost to moves between the register files), two workgroups of 128 columns a CU (outputs 88 us with the
+// score shared or not), 16 columns a wave (states 47 us), the waves of one SIMD in opposite phases (spills, 147 us),
+// operands fetched half a chunk ahead (states 39 us).
 #pragma once
 
 #include "pf_gfx950.h"
@@ -143,6 +157,11 @@ __device__ __forceinline__ void weigh(const Frag<bf16>& x, const floatx4& w0, co
 }
 __device__ __forceinline__ void weigh(const Frag<float>& x, const floatx4& w0, const floatx4& w1, Frag<float> (&t)[1]) {
   t[0] = {x.lo * w0, x.hi * w1};
+}
+
+// A value that all lanes hold, in a scalar register.
+__device__ __forceinline__ float wave_value(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
 }
 
 // 2^x of the hardware: results below 2^-126 are zero.
@@ -277,8 +296,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 #pragma unroll
   for (int i = 0; i < kSsmShare; ++i) {
     const int head = grp * R + h_first + (w + i * NW) % heads;
-    ra[i] = a.a[head];
-    rbias[i] = a.dt_bias ? a.dt_bias[head] : 0.f;
+    ra[i] = wave_value(a.a[head] * 1.44269504f);
+    rbias[i] = wave_value(a.dt_bias ? a.dt_bias[head] : 0.f);
   }
   auto load_dt = [&](int ch) {
 #pragma unroll
@@ -297,7 +316,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
       float dt = rdt[i] + rbias[i];
       if (a.softplus) dt = softplus(dt);
       if ((ch + slot / heads) * Q + lane >= len) dt = 0.f;
-      const float gate = dt * (ra[i] * 1.44269504f);
+      const float gate = dt * ra[i];
       float G, after;
       wave_sums(gate, g, G, after);
       s.tab[slot][0][lane] = dt * pow2(after - gate);
@@ -343,7 +362,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   const uint32_t y_off = active ? (uint32_t)(c * yt + 4 * PT * g * ES) : kPastEnd;
   const uint32_t z_off = active ? (uint32_t)(c * zt + 4 * PT * g * ES) : kPastEnd;
   static_assert(4 * PT == V, "a lane's columns of y are one vector");
-  const float dd = active && a.d ? a.d[h] : 0.f;
+  const float dd = wave_value(active && a.d ? a.d[h] : 0.f);
 
   // Added to an exponent on the score's diagonal tiles: 2^-inf above the diagonal, whatever the sums are there.  (Opaque to
   // the compiler, which would branch around each exponential.)
@@ -422,14 +441,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
           for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(sf[pt], cf, y[pt][ib]);
         }
       }
-      // z of this chunk, for the epilogue
       const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
-      u32x4 rz[HAS_Z ? 4 : 1];
-      if (HAS_Z) {
-        const auto zr = make_rsrc(zg + (long)t0 * zt, (uint32_t)(valid * zt));
-#pragma unroll
-        for (int ib = 0; ib < 4; ++ib) rz[ib] = __builtin_amdgcn_raw_buffer_load_b128(zr, z_off + 16 * ib * zt, 0, 0);
-      }
       lds_barrier();                           // the score is whole
       floatx4 u[4];
 #pragma unroll
@@ -461,6 +473,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 #pragma unroll
           for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(xf[pt][kb], pf, y[pt][ib]);
         }
+      }
+      // z of this chunk.  (Asked for before the barrier, its registers cost more in spills than its latency does here:
+      // 32768 tokens 186 us against 160.)
+      u32x4 rz[HAS_Z ? 4 : 1];
+      if (HAS_Z) {
+        const auto zr = make_rsrc(zg + (long)t0 * zt, (uint32_t)(valid * zt));
+#pragma unroll
+        for (int ib = 0; ib < 4; ++ib) rz[ib] = __builtin_amdgcn_raw_buffer_load_b128(zr, z_off + 16 * ib * zt, 0, 0);
       }
       // y out: lane c's token, the lane group's 4 PT columns as one vector
       const auto yr = make_rsrc(yg + (long)t0 * yt, (uint32_t)(min(a.T - t0, Q) * yt));
