@@ -18,7 +18,7 @@
 // fp32 operands: fp32 matrix instructions throughout.
 //
 // Measured, bf16, N = 128, P = 64 (kernel times): 2 x 32 heads x 8192 tokens, 16 segments: states 40 us (67 MB of x and
-// 34 MB of states moved, 2.6 TB/s), sum 13.5 us (67 MB, 5.0 TB/s), outputs 60 us (170 MB, 2.8 TB/s).  Bound by the chunk
+// 34 MB of states moved, 2.6 TB/s), sum 11.5 us (67 MB, 5.8 TB/s), outputs 60 us (170 MB, 2.8 TB/s).  Bound by the chunk
 // step, not the memory: 6 900 and 11 700 cycles a step of a workgroup, of which the matrix pipes work 3 070 and 3 700, the
 // vector port 5 000 and 6 000 and LDS 3 600 and 5 000.  Two waves share a SIMD (the states and the chunk in flight fill
 // its registers), and a wave's own vector instructions wait for its matrix instructions, so these add up more than they
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
         }
       }
       // z of this chunk.  (Asked for before the barrier, its registers cost more in spills than its latency does here:
-      // 32768 tokens 186 us against 160.)
+      // 32768 tokens 186 us against 150.)
       u32x4 rz[HAS_Z ? 4 : 1];
       if (HAS_Z) {
         const auto zr = make_rsrc(zg + (long)t0 * zt, (uint32_t)(valid * zt));
@@ -566,7 +566,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 
 // The states that enter the segments, in place of what each adds: H_0 = h0, H_{s+1} = decay_s H_s + D_s; the last is the
 // final state.  A thread owns the four elements of one register of a segment's waves (four rows of one column); the
-// segments' values are loaded eight ahead of the sum.  The workgroups of one column block run where its segments' did.
+// segments' values are loaded four ahead of the sum.  The workgroups of one column block run where its segments' did.
+// Bound by memory (2 x 32 heads x 8192 tokens: 67 MB, 5.8 TB/s, part of it from the cache).  One / two / four / eight / sixteen
+// ahead, us: that shape 13.4 / 11.4 / 11.5 / 11.8 / 11.7, 32 segments of one context 16.4 / 13.0 / 12.8 / 13.4 / 13.7, 12 of
+// small states 7.0 / 5.1 / 4.6 / 4.6 / 4.5.
 template <int NT, int PT, int COLS>
 __global__ __launch_bounds__(256) void ssm_prefix_kernel(SsmArgs a) {
   constexpr int SLAB = COLS * NT / 4, NTS = NT / 16;       // vectors of a segment
@@ -589,7 +592,7 @@ __global__ __launch_bounds__(256) void ssm_prefix_kernel(SsmArgs a) {
     for (int r = 0; r < 4; ++r)
       if (n + r < a.N) H[r] = a.h0[h_at + (long)(n + r) * a.P];
   }
-  constexpr int AHEAD = 8;
+  constexpr int AHEAD = 4;
   for (int s0 = 0; s0 < a.segs; s0 += AHEAD) {
     floatx4 D[AHEAD];
     float e[AHEAD];
@@ -597,13 +600,13 @@ __global__ __launch_bounds__(256) void ssm_prefix_kernel(SsmArgs a) {
     for (int i = 0; i < AHEAD; ++i)
       if (s0 + i < a.segs) {
         D[i] = st[(size_t)(s0 + i) * SLAB];
-        e[i] = pow2(decay[s0 + i]);
+        e[i] = decay[s0 + i];                              // raw: its power taken here would wait for each load in turn
       }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
       if (s0 + i < a.segs) {
         st[(size_t)(s0 + i) * SLAB] = H;
-        H = H * e[i] + D[i];
+        H = H * pow2(e[i]) + D[i];
       }
   }
   if (a.h_final) {
