@@ -2,9 +2,11 @@
  *
  * This is the drop-in boundary for pto-fuser's chunked delta-rule forward.  The reference
  * hosts its fused kernels as ctypes-bound `.so` recipes (src/pto_fuser/fused.py:83-162) and its
- * triangular inverse as an opaque kernel (src/pto_fuser/registry.py:96-127); every entry point
- * below replaces one of those bindings.  Conventions, all plain C:
- *   - pointers are device pointers (HBM) unless stated; layouts are row-major and contiguous;
+ * triangular inverse as an opaque kernel (src/pto_fuser/registry.py:96-127); the entry points
+ * below replace those bindings, but for the serving operators at the end, which stand around the
+ * forward and have none there.  Conventions, all plain C:
+ *   - pointers are device pointers (HBM) unless stated; layouts are row-major and contiguous (the
+ *     serving operators take strides);
  *   - `dtype` selects the element type of the q/k/v/w/u operands: PF_DTYPE_F32 or PF_DTYPE_BF16;
  *     gates (g, beta, decay) are always fp32, outputs are fp32 unless stated;
  *   - `stream` is a hipStream_t passed as void* (torch.cuda.current_stream().cuda_stream);

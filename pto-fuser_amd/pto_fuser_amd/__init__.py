@@ -3,7 +3,9 @@
 Direct operators over the C ABI (``ops``: the fused GDN/DeltaNet forward, kkt + inverse, the
 tri-inverse and the stage kernels) and the reference's compile stack rebuilt over them: the
 Program IR, staged and HIP-graph executors, opaque and fused-kernel registries, gates, cost model,
-policy, transforms, templates and ``compile_program``.
+policy, transforms, templates and ``compile_program``.  ``serving`` holds the operators around the
+recurrence in a layer that is served (short convolution, state space scan, norms) and the
+recurrences' forms for single tokens.
 """
 from . import _hip
 from .compile import CompileResult, compile_program
