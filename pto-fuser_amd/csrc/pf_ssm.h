@@ -17,15 +17,15 @@
 // rounded to 8 bits itself); the state is a sum in fp32 of products whose weighted operand has 16 or 24 bits (SPLIT).
 // fp32 operands: fp32 matrix instructions throughout.
 //
-// Measured, bf16, N = 128, P = 64 (kernel times): 2 x 32 heads x 8192 tokens, 16 segments: states 40 us (67 MB of x and
-// 34 MB of states moved, 2.6 TB/s), sum 11.5 us (67 MB, 5.8 TB/s), outputs 60 us (170 MB, 2.8 TB/s).  Bound by the chunk
+// Measured, bf16, N = 128, P = 64 (kernel times): 2 x 32 heads x 8192 tokens, 16 segments: states 39 us (67 MB of x and
+// 34 MB of states moved, 2.6 TB/s), sum 11.5 us (67 MB, 5.8 TB/s), outputs 58 us (170 MB, 2.9 TB/s).  Bound by the chunk
 // step, not the memory: 6 900 and 11 700 cycles a step of a workgroup, of which the matrix pipes work 3 070 and 3 700, the
 // vector port 5 000 and 6 000 and LDS 3 600 and 5 000.  Two waves share a SIMD (the states and the chunk in flight fill
 // its registers), and a wave's own vector instructions wait for its matrix instructions, so these add up more than they
 // overlap.  Measured and left out: 64 columns a wave with one wave a SIMD (states 50, outputs 75 us: the halved LDS
 // traffic is lost to moves between the register files), two workgroups of 128 columns a CU (outputs 88 us with the
 // score shared or not), 16 columns a wave (states 47 us), the waves of one SIMD in opposite phases (spills, 147 us),
-// operands fetched half a chunk ahead (states 39 us).
+// operands fetched half a chunk ahead (states 39 us), the first chunk's loads before the state's (outputs 63 us).
 #pragma once
 
 #include "pf_gfx950.h"
@@ -292,7 +292,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   // ---- the chunks' step sizes and decays, a token a lane, in log2.  A batch of chunks at a time: its (chunk, head) pairs
   // are dealt over the waves, the steps loaded a batch ahead.
   const int h_first = cb * COLS / P, heads = min(R, (cb * COLS + COLS - 1) / P + 1) - h_first, batch = Lds::SLOTS / heads;
-  float rdt[kSsmShare], ra[kSsmShare], rbias[kSsmShare];
+  // The steps' bits as stored: a conversion beside the load would wait for it and for all before it (2 x 32 heads x 8192
+  // tokens: states 40 us against 39, outputs 60 against 58).
+  uint32_t rdt[kSsmShare];
+  float ra[kSsmShare], rbias[kSsmShare];
 #pragma unroll
   for (int i = 0; i < kSsmShare; ++i) {
     const int head = grp * R + h_first + (w + i * NW) % heads;
@@ -303,9 +306,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 #pragma unroll
     for (int i = 0; i < kSsmShare; ++i) {
       const int slot = w + i * NW, t = (ch + slot / heads) * Q + lane;
-      rdt[i] = 0.f;
-      if (slot / heads < batch && t < len)
-        rdt[i] = load_any<E>(a.dt, bi * a.dt_b + (grp * R + h_first + slot % heads) * a.dt_h + t * a.dt_t, a.dt_f32);
+      rdt[i] = 0;
+      if (slot / heads < batch && t < len) {
+        const size_t at = bi * a.dt_b + (grp * R + h_first + slot % heads) * a.dt_h + t * a.dt_t;
+        if (ES == 4 || a.dt_f32) rdt[i] = static_cast<const uint32_t*>(a.dt)[at];
+        else rdt[i] = static_cast<const uint16_t*>(a.dt)[at];
+      }
     }
   };
   auto tabulate = [&](int ch) {
@@ -313,7 +319,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
     for (int i = 0; i < kSsmShare; ++i) {
       const int slot = w + i * NW;
       if (slot / heads >= batch) continue;
-      float dt = rdt[i] + rbias[i];
+      float dt = __uint_as_float(ES == 4 || a.dt_f32 ? rdt[i] : rdt[i] << 16) + rbias[i];
       if (a.softplus) dt = softplus(dt);
       if ((ch + slot / heads) * Q + lane >= len) dt = 0.f;
       const float gate = dt * ra[i];
