@@ -186,6 +186,8 @@ __device__ __forceinline__ void wave_sums(float v, int g, float& up_to, float& f
   from = b + (g == 3 ? 0.f : g == 2 ? r[3] : g == 1 ? r[2] + r[3] : r[1] + (r[2] + r[3]));
 }
 
+constexpr float kGateFloor = -256.f;                     // log2 of a token's decay
+
 // (chunk, head) pairs of a batch of tables that a wave makes.
 constexpr int kSsmShare = 2;
 
@@ -322,7 +324,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
       float dt = __uint_as_float(ES == 4 || a.dt_f32 ? rdt[i] : rdt[i] << 16) + rbias[i];
       if (a.softplus) dt = softplus(dt);
       if ((ch + slot / heads) * Q + lane >= len) dt = 0.f;
-      const float gate = dt * ra[i];
+      // 2^-256 of anything is zero: more than that would only cost the sums the gates of the tokens after it.
+      float gate = dt * ra[i];
+      gate = gate < kGateFloor ? kGateFloor : gate;
       float G, after;
       wave_sums(gate, g, G, after);
       s.tab[slot][0][lane] = dt * pow2(after - gate);

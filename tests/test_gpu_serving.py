@@ -502,6 +502,24 @@ def test_ssm_strong_and_no_decay(dtype):
     ref.check(final, S, M, ops, "state")
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("step", [300.0, 1e4, 1e30])
+def test_ssm_after_a_token_that_ends_the_state(dtype, step):
+    """A token whose step decays all that was (and adds nothing): those after it keep their own decays."""
+    announce(f"ssm_chunk_forward reset by a step of {step} {dtype}")
+    s = _ssm_case(8, dtype, 1, 3, 190, 32, 1, 32)
+    for t in (5, 70, 100):
+        s["x"][:, :, t], s["dt"][:, :, t] = 0.0, step
+    y, final = pf_ssm(s)
+    args = {k: ref.f64(v) for k, v in s.items()}
+    want, mag, S, M = ref.ssm(args["x"], args["dt"], args["A"], args["B"], args["C"], args["D"], args["z"], args["dt_bias"], True,
+                              args["h0"])
+    # two such tokens of a chunk sum to 2 * 2^8 in log2: 2^9, or 5 bits more than the tests above allow for
+    ops = _ssm_ops(190) + 64 * 2 ** 5 + (2 ** 16 if dtype is BF else 0)
+    ref.check(y, want, mag, ops, "y")
+    ref.check(final, S, M, ops, "state")
+
+
 def test_ssm_workspace_is_optional():
     """Through the C entry without a workspace: whole sequences, within rounding of the segments."""
     from pto_fuser_amd import _hip, serving
