@@ -171,22 +171,35 @@ __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x
 template <int CTRL> __device__ __forceinline__ float row_move(float v) {
   return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
-// Sums over the wave's lanes up to and from each on (inclusive).  The second is summed from its own end: as the total less
-// the first it would keep the total's error where it is small.
-__device__ __forceinline__ void wave_sums(float v, int g, float& up_to, float& from) {
-  float a = v, b = v;
-  a += row_move<0x111>(a); b += row_move<0x101>(b);
-  a += row_move<0x112>(a); b += row_move<0x102>(b);
-  a += row_move<0x114>(a); b += row_move<0x104>(b);
-  a += row_move<0x118>(a); b += row_move<0x108>(b);
-  float r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(a), 16 * i + 15));
-  up_to = a + (g == 0 ? 0.f : g == 1 ? r[0] : g == 2 ? r[0] + r[1] : r[0] + r[1] + r[2]);
-  from = b + (g == 3 ? 0.f : g == 2 ? r[3] : g == 1 ? r[2] + r[3] : r[1] + (r[2] + r[3]));
+// Sums over a row's lanes up to each (inclusive).
+__device__ __forceinline__ float row_sums(float v) {
+  v += row_move<0x111>(v);
+  v += row_move<0x112>(v);
+  v += row_move<0x114>(v);
+  v += row_move<0x118>(v);
+  return v;
 }
+// The value of a row's last lane.
+__device__ __forceinline__ float row_last(float v) { return row_move<0x15f>(v); }
 
 constexpr float kGateFloor = -256.f;                     // log2 of a token's decay
+
+// The weight of one token for another is 2 to the sum of the gates between them, whose rounding has to be of its own size,
+// not of what came before it in the chunk (weak tokens behind strong ones).  Between 16s these are sums from a 16's end or
+// start; inside one, differences of the running sum, which is held in two parts for it: the high ones are multiples of 2^-10
+// and at most 16 * 2^8, so that they and their differences are exact, the low ones stay under 16 * 2^-11.
+constexpr float kGateGrain = 1.f / 1024;
+
+// The tables of a chunk and head.  Of each token: dt times the decay to the chunk's end; the running sum of gates within its
+// 16, in two parts; dt; dt times the decay to the end of its 16 (not of the last 16, where none comes after it); and the
+// decays over the 16s that end in it: its own up to it, and one, two or three before that, as far as there are any.
+enum SsmTab {
+  kToEnd = 0, kHigh = 64, kLow = 128, kStep = 192, kToTile = 256, kDecay1 = 304, kDecay2 = 368 - 16, kDecay3 = 416 - 32,
+  kDecay4 = 448 - 48, kTabEnd = 464
+};
+__device__ __forceinline__ constexpr int decay_over(int tiles) {
+  return tiles == 1 ? kDecay1 : tiles == 2 ? kDecay2 : tiles == 3 ? kDecay3 : kDecay4;
+}
 
 // (chunk, head) pairs of a batch of tables that a wave makes.
 constexpr int kSsmShare = 2;
@@ -202,9 +215,8 @@ template <typename E, int NT, int NW, int PT, bool OUT> struct SsmLds {
   E c[OUT ? C::ELEMS : 1];
   // C B^T, tile (ib, jb) transposed: lane (c, g) holds rows j = 16 jb + 4g .. of column i = 16 ib + c.
   floatx4 score[OUT ? 10 : 1][64];
-  // Per (chunk, head) of a batch and token: dt 2^(G_last - G), G, dt, dt 2^(G_m - G) (m: the last token of its 16).
-  float tab[SLOTS][OUT ? 4 : 1][kSsmChunk];
-  float total[SLOTS];                                  // G_last
+  float tab[SLOTS][OUT ? (int)kTabEnd : kSsmChunk];    // SsmTab, per (chunk, head) of a batch
+  float total[SLOTS];                                  // log2 of the chunk's decay
 };
 
 // SPLIT: bf16 terms of the weighted x in the state's update.  Three keep the state a sum in 24 bits, as it has to be where
@@ -324,18 +336,29 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
       float dt = __uint_as_float(ES == 4 || a.dt_f32 ? rdt[i] : rdt[i] << 16) + rbias[i];
       if (a.softplus) dt = softplus(dt);
       if ((ch + slot / heads) * Q + lane >= len) dt = 0.f;
-      // 2^-256 of anything is zero: more than that would only cost the sums the gates of the tokens after it.
+      // 2^-256 of anything is zero; the floor bounds the sums.
       float gate = dt * ra[i];
       gate = gate < kGateFloor ? kGateFloor : gate;
-      float G, after;
-      wave_sums(gate, g, G, after);
-      s.tab[slot][0][lane] = dt * pow2(after - gate);
+      const float coarse = rintf(gate * (1 / kGateGrain)) * kGateGrain;
+      const float high = row_sums(coarse), low = row_sums(gate - coarse), sum = high + low;
+      float t[4];                              // a 16's gates
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t[k] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sum), 16 * k + 15));
+      const float to_tile = (row_last(high) - high) + (row_last(low) - low);
+      const float after = g == 0 ? t[1] + t[2] + t[3] : g == 1 ? t[2] + t[3] : g == 2 ? t[3] : 0.f;
+      float* tab = s.tab[slot] + lane;
+      tab[kToEnd] = dt * pow2(to_tile + after);
       if constexpr (OUT) {
-        s.tab[slot][1][lane] = G;
-        s.tab[slot][2][lane] = dt;
-        s.tab[slot][3][lane] = dt * pow2(row_move<0x15f>(G) - G);
+        tab[kHigh] = high;
+        tab[kLow] = low;
+        tab[kStep] = dt;
+        tab[kDecay1] = pow2(sum);
+        if (g < 3) tab[kToTile] = dt * pow2(to_tile);
+        if (g > 0) tab[kDecay2] = pow2(sum + (g == 1 ? t[0] : g == 2 ? t[1] : t[2]));
+        if (g > 1) tab[kDecay3] = pow2(sum + (g == 2 ? t[0] + t[1] : t[1] + t[2]));
+        if (g > 2) tab[kDecay4] = pow2(sum + (t[0] + t[1] + t[2]));
       }
-      if (lane == 63) s.total[slot] = G;
+      if (lane == 63) s.total[slot] = t[0] + t[1] + t[2] + t[3];
     }
   };
   float decay2 = 0.f;                          // log2 of the segment's decay
@@ -374,15 +397,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   static_assert(4 * PT == V, "a lane's columns of y are one vector");
   const float dd = wave_value(active && a.d ? a.d[h] : 0.f);
 
-  // Added to an exponent on the score's diagonal tiles: 2^-inf above the diagonal, whatever the sums are there.  (Opaque to
-  // the compiler, which would branch around each exponential.)
-  floatx4 above;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    above[r] = 4 * g + r <= c ? 0.f : -__builtin_inff();
-    __asm__("" : "+v"(above[r]));
-  }
-
   int slot0 = -heads;                          // of this chunk's tables
   if (first < end) {
     load_dt(first);
@@ -399,7 +413,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
     const int t0 = ch * Q, buf = OUT ? 0 : ch & 1;
     slot0 += heads;
     if (slot0 + heads > Lds::SLOTS) slot0 = 0;
-    const float(*tab)[Q] = s.tab[slot0 + hl];
+    const float* tab = s.tab[slot0 + hl];
     if (OUT) {
       lds_barrier();                           // the last chunk's reads are done
       stage(0);
@@ -453,13 +467,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
       }
       const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
       lds_barrier();                           // the score is whole
-      floatx4 u[4];
-#pragma unroll
-      for (int jb = 0; jb < 4; ++jb) u[jb] = *reinterpret_cast<const floatx4*>(&tab[3][16 * jb + 4 * g]);
 #pragma unroll
       for (int ib = 0; ib < 4; ++ib) {
-        const float Gi = tab[1][16 * ib + c];
-        const float e = pow2(Gi);
+        const float e = tab[decay_over(ib + 1) + 16 * ib + c];
 #pragma unroll
         for (int pt = 0; pt < PT; ++pt) y[pt][ib] *= e;
         floatx4 pr[4];
@@ -467,14 +477,21 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
         for (int jb = 0; jb < 4; ++jb) {
           pr[jb] = zero4();
           if (jb < ib) {
-            const float f = pow2(Gi - tab[1][16 * jb + 15]);
-            pr[jb] = s.score[ib * (ib + 1) / 2 + jb][lane] * (u[jb] * f);
+            const float f = tab[decay_over(ib - jb) + 16 * ib + c];
+            const floatx4 u = *reinterpret_cast<const floatx4*>(&tab[kToTile + 16 * jb + 4 * g]);
+            pr[jb] = s.score[ib * (ib + 1) / 2 + jb][lane] * (u * f);
           } else if (jb == ib) {
             const floatx4 sc = s.score[ib * (ib + 1) / 2 + jb][lane];
-            const floatx4 Gj = *reinterpret_cast<const floatx4*>(&tab[1][16 * jb + 4 * g]);
-            const floatx4 dj = *reinterpret_cast<const floatx4*>(&tab[2][16 * jb + 4 * g]);
+            const float Gi = tab[kHigh + 16 * ib + c], li = tab[kLow + 16 * ib + c];
+            const floatx4 Gj = *reinterpret_cast<const floatx4*>(&tab[kHigh + 16 * jb + 4 * g]);
+            const floatx4 lj = *reinterpret_cast<const floatx4*>(&tab[kLow + 16 * jb + 4 * g]);
+            const floatx4 dj = *reinterpret_cast<const floatx4*>(&tab[kStep + 16 * jb + 4 * g]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) pr[jb][r] = sc[r] * (dj[r] * pow2(Gi - Gj[r] + above[r]));
+            for (int r = 0; r < 4; ++r) {
+              float v = sc[r] * (dj[r] * pow2((Gi - Gj[r]) + (li - lj[r])));
+              __asm__ volatile("" : "+v"(v));  // made here, or the select becomes a branch around the exponential
+              pr[jb][r] = 4 * g + r <= c ? v : 0.f;
+            }
           }
         }
 #pragma unroll
@@ -520,7 +537,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
     decay2 += total;
     floatx4 wt[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) wt[q] = *reinterpret_cast<const floatx4*>(&tab[0][16 * q + 4 * g]);
+    for (int q = 0; q < 4; ++q) wt[q] = *reinterpret_cast<const floatx4*>(&tab[kToEnd + 16 * q + 4 * g]);
     Frag<E> bf[NTS], wx[2][SPLIT];
 #pragma unroll
     for (int nt = 0; nt < NTS; ++nt) bf[nt] = Bs::template cols<8>(sb, 32 * (nt >> 1) + 4 * (nt & 1), 0, c, g);

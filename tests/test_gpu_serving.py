@@ -567,3 +567,37 @@ def test_ssm_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want[0]) and torch.equal(final, want[1])
+
+
+# ------------------------------------------------------------------------------------------
+#  The scan where its weights are differences of long sums: a weight is as exact as the gates between its two tokens,
+#  whatever came before them in the chunk.  The same operations as above, so the same count of roundings; a weight of
+#  2^-d has a relative error of some d roundings, and d 2^-d < 1.
+# ------------------------------------------------------------------------------------------
+def _steps_case(seed, dtype, T, strong, step, A, N=32):
+    """Steps as they are (no softplus): ``step`` at the ``strong`` tokens, 2^-7 to 2^-5 elsewhere; x everywhere."""
+    s = _ssm_case(seed, dtype, 2, 3, T, 32, 1, N)
+    s["A"] = torch.full((3,), A, device=DEV)
+    s["dt"] = _dev(2.0 ** -7 * (1 + 3 * torch.rand(2, 3, T, generator=torch.Generator().manual_seed(seed))), F32)
+    s["dt"][:, :, strong] = step
+    s["dt_bias"] = None
+    return s
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,h0", [(64, True), (64, False), (391, True)])
+@pytest.mark.parametrize("strong,step,A", [
+    (range(48), 1.0, -16.0), (range(8), 11.0, -16.0), (range(32), 11.0, -16.0), (range(48), 11.0, -16.0),
+    (range(0, 60, 3), 7.0, -20.0), ([5, 6, 21, 63], 1e4, -2.0), ([0], 3e30, -1.0)])
+def test_ssm_weak_tokens_between_strong_ones(dtype, T, h0, strong, step, A):
+    from pto_fuser_amd import ssm_chunk_forward
+    strong = [t + c for c in range(0, T, 64) for t in strong if t + c < T]
+    announce(f"ssm_chunk_forward {len(strong)} steps of {step} and weak ones {dtype} T{T} h0={h0}")
+    s = _steps_case(17, dtype, T, strong, step, A)
+    if step > 1e6:                       # the square of what such a step adds is past fp32
+        s["x"][:, :, strong] *= 1e-20
+        s["B"][:, :, strong] *= 1e-10
+    if not h0:
+        s["h0"] = None
+    y, final = ssm_chunk_forward(s["x"], s["dt"], s["A"], s["B"], s["C"], s["D"], z=s["z"], h0=s["h0"])
+    _check_ssm(s, y, final, softplus=False)
