@@ -303,7 +303,8 @@ int pf_gdn_step_exec(const pf_step_args* args, void* stream);
  * x, z, y [B,H,T,P], b, c [B,G,T,N], dt [B,H,T] with free strides; A, D, dt_bias [H] fp32; h0, h_final
  * [B,H,N,P] fp32 contiguous (h_final may be h0).  lengths [B] (NULL: all T): the tokens of each sequence;
  * later ones are not read, y is zero there, and the state is that after the last one.  Any T >= 0.
- * The scan runs 64-token chunks; a non-finite operand reaches all of its chunk's rows.
+ * The scan runs 64-token chunks.  A non-finite operand reaches what the recurrence takes it to, its own token and later ones,
+ * and nothing before; where a value of x is not finite, its column of y is NaN from there on.
  * Supported: P a multiple of 32 up to 256, N a multiple of 16 up to 128; token strides of x, b, c, z and y of a
  * row at least and 2^22 elements at most.
  * Few sequences run as segments side by side when `workspace` holds their states

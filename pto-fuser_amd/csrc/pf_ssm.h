@@ -86,6 +86,18 @@ template <typename E> __device__ __forceinline__ Frag<E> frag_of(const floatx4& 
 template <> __device__ __forceinline__ Frag<bf16> frag_of<bf16>(const floatx4& lo, const floatx4& hi) { return {pack8(lo, hi)}; }
 template <> __device__ __forceinline__ Frag<float> frag_of<float>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
 
+__device__ __forceinline__ void only_finite(Frag<bf16>& f) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f.v[i] = __builtin_isfinite((float)f.v[i]) ? f.v[i] : (bf16)0.f;
+}
+__device__ __forceinline__ void only_finite(Frag<float>& f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f.lo[i] = __builtin_isfinite(f.lo[i]) ? f.lo[i] : 0.f;
+    f.hi[i] = __builtin_isfinite(f.hi[i]) ? f.hi[i] : 0.f;
+  }
+}
+
 template <typename E, typename V> __device__ __forceinline__ Frag<E> frag_cat(const V& lo, const V& hi);
 template <> __device__ __forceinline__ Frag<bf16> frag_cat<bf16, bf16x4>(const bf16x4& lo, const bf16x4& hi) { return {cat8(lo, hi)}; }
 template <> __device__ __forceinline__ Frag<float> frag_cat<float, floatx4>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
@@ -159,7 +171,8 @@ __device__ __forceinline__ void weigh(const Frag<float>& x, const floatx4& w0, c
   t[0] = {x.lo * w0, x.hi * w1};
 }
 
-// A value that all lanes hold, in a scalar register.
+// A value that all lanes hold, in a scalar register.  (Quotients come in vector registers, and what is made of them stays there.)
+__device__ __forceinline__ int wave_int(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ float wave_value(float v) {
   return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
 }
@@ -222,9 +235,12 @@ template <typename E, int NT, int NW, int PT, bool OUT> struct SsmLds {
 // SPLIT: bf16 terms of the weighted x in the state's update.  Three keep the state a sum in 24 bits, as it has to be where
 // it is returned; two where it only enters y, whose operand S is rounded to 8 bits anyway.
 // PT: 16-column tiles of a wave.
-template <typename E, int NT, int NW, int PT, SsmMode MODE, int SPLIT, bool HAS_Z>
-__global__ __launch_bounds__(NW * 64) __attribute__((
-    amdgpu_waves_per_eu(sizeof(E) == 4 || NW * 16 * PT < 256 ? 1 : 2))) void ssm_kernel(SsmArgs a) {
+// One workgroup's walk.  Returns whether it has to be made AGAIN: a value of x that is not finite reaches the tokens before it
+// in its chunk, through the products with the zeros above the score's diagonal.  The second walk leaves such values out of the
+// products for y, and makes every token from theirs on NaN.
+template <typename E, int NT, int NW, int PT, SsmMode MODE, int SPLIT, bool HAS_Z, bool AGAIN>
+__device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT, MODE == SsmMode::kOutput>& s, const uint32_t tid,
+                                         const uint32_t bid) {
   constexpr int Q = kSsmChunk, ES = (int)sizeof(E), V = 16 / ES, TH = NW * 64, NTS = NT / 16;
   constexpr int COLS = NW * 16 * PT;           // columns of a workgroup
   constexpr int RV = NT / V;                   // vectors of a row of B or C
@@ -236,28 +252,27 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   using Bs = typename Lds::B;
   using Cs = typename Lds::C;
   using Xs = typename Lds::X;
-  __shared__ __attribute__((aligned(16))) Lds s;
 
   // Workgroups go round robin over the eight XCDs: each XCD takes a run of tasks, so that the segments of one block of
   // columns, and the sum along them, meet in its L2.
-  const uint32_t per = (a.tasks + 7) / 8, task = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (blockIdx.x >> 3 >= per || task >= a.tasks) return;
-  const int seg = (int)(task % (uint32_t)a.segs);
-  uint32_t rest = task / (uint32_t)a.segs;
-  const int cb = (int)(rest % (uint32_t)a.blocks);
-  rest /= (uint32_t)a.blocks;
-  const int grp = (int)(rest % (uint32_t)a.G);
-  const long bi = rest / (uint32_t)a.G;
+  const uint32_t per = (a.tasks + 7) / 8, task = (bid & 7) * per + (bid >> 3);
+  if (bid >> 3 >= per || task >= a.tasks) return false;
+  const int seg = wave_int(task % (uint32_t)a.segs);
+  uint32_t rest = wave_int(task / (uint32_t)a.segs);
+  const int cb = wave_int(rest % (uint32_t)a.blocks);
+  rest = wave_int(rest / (uint32_t)a.blocks);
+  const int grp = wave_int(rest % (uint32_t)a.G);
+  const long bi = wave_int(rest / (uint32_t)a.G);
 
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int R = a.H / a.G;
+  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int R = wave_int(a.H / a.G);
   // The columns of a group's heads lie end to end, and the workgroup has COLS of them: P is a multiple of 32, so that a
   // wave's are of one head.
   const int col = cb * COLS + w * 16 * PT;
   const bool active = col < R * a.P;
-  const int hr = active ? col / a.P : 0, p0 = active ? col % a.P : 0;
-  const int h = grp * R + hr, hl = active ? hr - cb * COLS / a.P : 0;
+  const int hr = wave_int(active ? col / a.P : 0), p0 = wave_int(active ? col - hr * a.P : 0);
+  const int h = grp * R + hr, hl = active ? hr - wave_int(cb * COLS / a.P) : 0;
   const int N = a.N, P = a.P;
   int len = a.T;
   if (a.lengths) len = __builtin_amdgcn_readfirstlane(min(max(a.lengths[bi], 0), a.T));
@@ -271,8 +286,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   const char* bg = reinterpret_cast<const char*>(static_cast<const E*>(a.b) + bi * a.b_b + grp * a.b_g);
   const char* cg = reinterpret_cast<const char*>(static_cast<const E*>(a.c) + bi * a.c_b + grp * a.c_g);
   const int xt = (int)a.x_t * ES, bt = (int)a.b_t * ES, ct = (int)a.c_t * ES;
-  const int b_row = threadIdx.x / RV, b_col = threadIdx.x % RV * V, x_row = lane / XV, x_col = lane % XV * V;
-  const bool stages = Q * RV >= TH || threadIdx.x < Q * RV;
+  const int b_row = tid / RV, b_col = tid % RV * V, x_row = lane / XV, x_col = lane % XV * V;
+  const bool stages = Q * RV >= TH || tid < Q * RV;
   const uint32_t b_off = b_col < N ? (uint32_t)(b_row * bt + b_col * ES) : kPastEnd;
   const uint32_t c_off = b_col < N ? (uint32_t)(b_row * ct + b_col * ES) : kPastEnd;
   const uint32_t x_off = active ? (uint32_t)(x_row * xt + x_col * ES) : kPastEnd;
@@ -305,7 +320,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
   };
   // ---- the chunks' step sizes and decays, a token a lane, in log2.  A batch of chunks at a time: its (chunk, head) pairs
   // are dealt over the waves, the steps loaded a batch ahead.
-  const int h_first = cb * COLS / P, heads = min(R, (cb * COLS + COLS - 1) / P + 1) - h_first, batch = Lds::SLOTS / heads;
+  const int h_first = wave_int(cb * COLS / P), heads = min(R, wave_int((cb * COLS + COLS - 1) / P) + 1) - h_first,
+            batch = wave_int(Lds::SLOTS / heads);
   // The steps' bits as stored: a conversion beside the load would wait for it and for all before it (2 x 32 heads x 8192
   // tokens: states 40 us against 39, outputs 60 against 58).
   uint32_t rdt[kSsmShare];
@@ -431,7 +447,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 #pragma unroll
     for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) xf[pt][kb] = Xs::template cols<4 * PT>(sx, 4 * pt, kb, c, g);
+      for (int kb = 0; kb < 2; ++kb) {
+        xf[pt][kb] = Xs::template cols<4 * PT>(sx, 4 * pt, kb, c, g);
+        if (AGAIN) only_finite(xf[pt][kb]);
+      }
 
     if constexpr (OUT) {
       // the score's tiles, dealt over the waves
@@ -500,6 +519,22 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
 #pragma unroll
           for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(xf[pt][kb], pf, y[pt][ib]);
         }
+      }
+      if (AGAIN) {                             // 0 x, summed along the tokens: NaN from a value that is not finite on
+#pragma unroll
+        for (int i = 0; i < 4 * PT; ++i) {
+          float before = 0.f;
+#pragma unroll
+          for (int ib = 0; ib < 4; ++ib) {
+            const float upto = row_sums(0.f * to_f32(sx[(16 * ib + c) * Xs::LD + 4 * PT * g + i]));
+            y[i / 4][ib][i % 4] += before + upto;
+            before += row_last(upto);
+          }
+        }
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) xf[pt][kb] = Xs::template cols<4 * PT>(sx, 4 * pt, kb, c, g);
       }
       // z of this chunk.  (Asked for before the barrier, its registers cost more in spills than its latency does here:
       // 32768 tokens 186 us against 150.)
@@ -570,7 +605,19 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
     }
   }
 
-  if (!active) return;
+  if (OUT && !AGAIN) {
+    // A value of x that is not finite stays in its column of the state, in all rows of it.
+    float bad = 0.f;
+#pragma unroll
+    for (int pt = 0; pt < PT; ++pt) bad += 0.f * S[0][pt][0];
+    bad = __any(bad != 0.f) ? 1.f : 0.f;
+    lds_barrier();                             // the last chunk's reads are done
+    if (lane == 0) s.total[w] = bad;
+    lds_barrier();
+    for (int i = 0; i < NW; ++i) bad += s.total[i];
+    if (__builtin_expect(wave_value(bad) != 0.f, 0)) return true;
+  }
+  if (!active) return false;
   if (!OUT) {
     if (p0 == 0 && lane == 0) a.seg_decay[((long)bi * a.H + h) * a.segs + seg] = decay2;
 #pragma unroll
@@ -588,6 +635,25 @@ __global__ __launch_bounds__(NW * 64) __attribute__((
           const int n = state_row(nt, g, r);
           if (n < N) out[n * P + state_col<PT>(pt, c)] = S[nt][pt][r];
         }
+  }
+  return false;
+}
+
+template <typename E, int NT, int NW, int PT, SsmMode MODE, int SPLIT, bool HAS_Z>
+__global__ __launch_bounds__(NW * 64) __attribute__((
+    amdgpu_waves_per_eu(sizeof(E) == 4 || NW * 16 * PT < 256 ? 1 : 2))) void ssm_kernel(SsmArgs a) {
+  __shared__ __attribute__((aligned(16))) SsmLds<E, NT, NW, PT, MODE == SsmMode::kOutput> s;
+  uint32_t tid = threadIdx.x, bid = blockIdx.x;
+  const bool again = ssm_walk<E, NT, NW, PT, MODE, SPLIT, HAS_Z, false>(a, s, tid, bid);
+  if constexpr (MODE == SsmMode::kOutput) {
+    if (__builtin_expect(again, 0)) {
+      __builtin_amdgcn_s_waitcnt(0);                   // the first walk's stores of y are done
+      // The second walk makes all it needs anew, arguments too: what it kept of the first would cost that one registers.
+      typedef const SsmArgs __attribute__((address_space(4)))* Args;
+      Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+      __asm__ volatile("" : "+v"(tid), "+s"(bid), "+s"(args));
+      ssm_walk<E, NT, NW, PT, MODE, SPLIT, HAS_Z, true>(*(const SsmArgs*)args, s, tid, bid);
+    }
   }
 }
 

@@ -232,7 +232,8 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
     multiple of 16 up to 128, head h reading group h // (H // G); A, D, dt_bias [H] float32 (A < 0: it decays); h0
     [B,H,N,P] float32.  Any T.  Batch, head and token strides are free: ``xbc[..., :H*P].unflatten(-1, (H, P)).transpose(1,
     2)`` of a convolved row [B,T,..] is read in place.  ``lengths`` [B] int32 (None: all T): tokens of each sequence; what
-    follows them is not read, y is zero there, and the state is that after the last one.
+    follows them is not read, y is zero there, and the state is that after the last one.  A NaN or infinity reaches
+    its own token and those after it, as in the recurrence, and none before.
 
     Returns (y [B,H,T,P] in x's type, token-major in memory where x is; the final state [B,H,N,P] float32 or None).
     ``final_out`` may be h0.  Few sequences run as segments side by side, whose number follows from the call's shape: the

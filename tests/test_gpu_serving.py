@@ -601,3 +601,40 @@ def test_ssm_weak_tokens_between_strong_ones(dtype, T, h0, strong, step, A):
         s["h0"] = None
     y, final = ssm_chunk_forward(s["x"], s["dt"], s["A"], s["B"], s["C"], s["D"], z=s["z"], h0=s["h0"])
     _check_ssm(s, y, final, softplus=False)
+
+
+# ------------------------------------------------------------------------------------------
+#  Values that are not finite: the recurrence takes one to its own token and to those after it.
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,H,T,P,N,t", [(1, 3, 64, 32, 32, 37), (2, 4, 150, 64, 128, 100), (1, 4, 700, 64, 64, 331),
+                                         (17, 16, 70, 64, 128, 66), (9, 64, 70, 32, 16, 13)])
+@pytest.mark.parametrize("bad", [NAN, INF])
+@pytest.mark.parametrize("name", ["x", "z", "dt", "B", "C", "h0"])
+def test_ssm_keeps_nan_where_it_is(dtype, B, H, T, P, N, t, bad, name):
+    announce(f"ssm_chunk_forward {bad} in {name} {dtype} B{B} H{H} T{T} P{P} N{N}")
+    s = _ssm_case(23, dtype, B, H, T, P, 1, N)
+    s["D"] = torch.ones(H, device=DEV)
+    clean, clean_state = pf_ssm(s)
+    b, h, p, n = B - 1, H - 2, P - 3, N // 2 + 1
+    at = {"x": (b, h, t, p), "z": (b, h, t, p), "dt": (b, h, t), "B": (b, 0, t, n), "C": (b, 0, t, n), "h0": (b, h, n, p)}[name]
+    s[name][at] = bad
+    y, state = pf_ssm(s)
+    # where the definition has it
+    want, want_state = torch.zeros(B, H, T, P, dtype=torch.bool), torch.zeros(B, H, N, P, dtype=torch.bool)
+    if name == "x":
+        want[b, h, t:, p] = want_state[b, h, :, p] = True
+    elif name == "dt":
+        want[b, h, t:] = want_state[b, h] = True
+    elif name == "B":
+        want[b, :, t:] = want_state[b, :, n] = True
+    elif name == "C":
+        want[b, :, t] = True
+    elif name == "h0":
+        want[b, h, :, p] = want_state[b, h, n, p] = True
+    else:
+        want[b, h, t, p] = True
+    assert torch.equal(~torch.isfinite(y.cpu()), want) and torch.equal(~torch.isfinite(state.cpu()), want_state)
+    # and the bits of everything else stay
+    assert torch.equal(torch.where(want, 0, y.float().cpu()), torch.where(want, 0, clean.float().cpu()))
+    assert torch.equal(torch.where(want_state, 0, state.cpu()), torch.where(want_state, 0, clean_state.cpu()))
