@@ -15,10 +15,12 @@ Unlike those, the operands may be views: batch, head and token strides are free 
 transposed head layout); only the innermost dimension is contiguous.  Every operator raises ``ValueError`` before
 launching for what it does not support, works on the current stream of the operands' device, and neither synchronises nor
 allocates anything but its outputs and (the scan) a workspace, from torch's allocator: each can be captured in a HIP
-graph.
+graph.  What a call is given to write (``out`` and the like) shares memory with no other operand, unless its description
+names one that it may be; slices of one buffer that lie side by side are apart.
 """
 from __future__ import annotations
 
+import math
 import struct
 from typing import Optional, Tuple
 
@@ -121,6 +123,45 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _span(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to the end of its last."""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors may have memory in common.  Blocks that lie side by side in one buffer (slices of a projection's
+    output) do not: all offsets of both are multiples of one pitch, apart from their start and their place in a block."""
+    at, bt = a.data_ptr(), b.data_ptr()
+    if not a.numel() or not b.numel() or at + _span(a) <= bt or bt + _span(b) <= at:
+        return False
+    pitch, widths = 0, []
+    for t in (a, b):
+        width, size = 1, t.element_size()
+        for stride, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+            if stride == width:
+                width *= n                        # the block goes on
+            else:
+                pitch = math.gcd(pitch, stride * size)
+        widths.append(width * size)
+    if not pitch:
+        return True
+    ahead = (bt - at) % pitch
+    return ahead < widths[0] or ahead + widths[1] > pitch
+
+
+def _apart(name: str, t: Optional[torch.Tensor], same=(), **others) -> None:
+    """``t``, which a call writes, has no memory in common with what other threads of it read or write.  It may be the very
+    view ``others`` name in ``same``: those elements are read by the thread that writes them."""
+    if t is None:
+        return
+    for other, u in others.items():
+        if u is None or not _share(t, u):
+            continue
+        if other in same and t.data_ptr() == u.data_ptr() and t.dtype == u.dtype and t.stride() == u.stride():
+            continue
+        raise ValueError(f"{name} may not be {other} nor share memory with it")
+
+
 def _pool(state: torch.Tensor, slots, B: int, dev) -> None:
     if slots is not None:
         _require(slots, "slots", (B,), torch.int32, dev)
@@ -142,7 +183,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     float32 (both in one).  ``initial_state`` [B,K-1,W] holds the last K-1 inputs of what came before (None: zeros).
     ``lengths`` [B] int32 (None: all T): tokens of each sequence; what follows them is not read, and y is zero there.
     Returns (y [B,T,W] in x's type, the state after the last token [B,K-1,W] or None).  ``final_out`` may be
-    ``initial_state``; ``out`` may not overlap x."""
+    ``initial_state``."""
     dev = _device_of(x, "x")
     _dim(x, "x", 3, "[B,T,W]")
     _dim(weight, "weight", 2, "[W,K]")
@@ -164,8 +205,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         y = torch.empty(B, T, W, device=dev, dtype=dtype)
     else:
         _require_view(out, "out", (B, T, W), dtype, dev)
-        if out.data_ptr() == x.data_ptr() and x.numel():
-            raise ValueError("out may not be x: a token's output would overwrite its neighbours' input")
+        _apart("out", out, x=x, weight=weight, bias=bias, initial_state=initial_state, lengths=lengths)
         y = out
     final = None
     if output_final_state:
@@ -174,6 +214,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
             final = torch.empty((B, K - 1, W), device=dev, dtype=dtype)
         else:
             _require(final, "final_out", (B, K - 1, W), dtype, dev)
+            _apart("final_out", final, ("initial_state",), x=x, weight=weight, bias=bias, initial_state=initial_state,
+                   lengths=lengths, out=y)
     sx, sy, state = x.stride(), y.stride(), (K - 1) * W
     _exec("pf_conv_exec", dev, _CONV, _CONV_SIZE, x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(initial_state),
           _ptr(lengths), y.data_ptr(), _ptr(final), sx[0], sx[1], sy[0], sy[1], state, state, B, T, W, K,
@@ -187,7 +229,7 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     """One token of :func:`causal_conv` for each of B sequences: x [B,W]; returns y [B,W].
 
     ``state`` [S,K-1,W] in x's type is updated in place.  Sequence b's is ``state[slots[b]]`` (``slots`` [B] int32, no two
-    the same; one outside the pool is skipped and its y zero), or ``state[b]`` with S = B."""
+    the same; one outside the pool is skipped and its y zero), or ``state[b]`` with S = B.  ``out`` may be x."""
     dev = _device_of(x, "x")
     _dim(x, "x", 2, "[B,W]")
     _dim(weight, "weight", 2, "[W,K]")
@@ -208,6 +250,7 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
         y = torch.empty(B, W, device=dev, dtype=dtype)
     else:
         _require_view(out, "out", (B, W), dtype, dev)
+        _apart("out", out, ("x",), x=x, state=state, weight=weight, bias=bias, slots=slots)
         y = out
     _exec("pf_conv_step_exec", dev, _CONV_STEP, _CONV_STEP_SIZE, x.data_ptr(), weight.data_ptr(), _ptr(bias),
           state.data_ptr(), _ptr(slots), y.data_ptr(), x.stride(0), y.stride(0), (K - 1) * W, B,
@@ -274,6 +317,7 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
         _require_view(out, "out", (nb, H, T, P), dtype, dev)
         if T > 1 and out.stride(2) < P:
             raise ValueError("out has overlapping rows")
+        _apart("out", out, x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, h0=h0, lengths=lengths)
         y = out
     elif sx[1] < sx[2]:
         y = torch.empty(nb, T, H, P, device=dev, dtype=dtype).transpose(1, 2)
@@ -286,6 +330,8 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
             final = torch.empty((nb, H, N, P), device=dev, dtype=torch.float32)
         else:
             _require(final, "final_out", (nb, H, N, P), torch.float32, dev)
+            _apart("final_out", final, ("h0",), x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, h0=h0,
+                   lengths=lengths, out=y)
     need = _hip.load().pf_ssm_workspace_bytes(nb, H, G, T, N, P, code)
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     sb, sc, sy, st = B.stride(), C.stride(), y.stride(), dt.stride()
@@ -310,7 +356,7 @@ def ssm_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.Te
 
     x, z [B,H,P] float32 or bfloat16 (P a multiple of 4); dt [B,H] in x's type or float32; B, C [B,G,N], N up to 256, head
     h reading group h // (H // G); A, D, dt_bias [H] float32 (A < 0: it decays).  ``state`` [S,H,N,P] float32 is updated
-    in place, with ``slots`` as in :func:`causal_conv_step`.  Returns y [B,H,P] in x's type."""
+    in place, with ``slots`` as in :func:`causal_conv_step`.  Returns y [B,H,P] in x's type; ``out`` may be x or z."""
     dev = _device_of(x, "x")
     _dim(x, "x", 3, "[B,H,P]")
     _dim(B, "B", 3, "[B,G,N]")
@@ -343,6 +389,7 @@ def ssm_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.Te
         y = torch.empty(nb, H, P, device=dev, dtype=dtype)
     else:
         _require_view(out, "out", (nb, H, P), dtype, dev)
+        _apart("out", out, ("x", "z"), x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, state=state, slots=slots)
         y = out
     sx, sb, sc, sy, st = x.stride(), B.stride(), C.stride(), y.stride(), dt.stride()
     sz = (0, 0) if z is None else z.stride()
@@ -363,7 +410,7 @@ def gdn_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     q, k [B,H,DK] (DK up to 256) and v [B,H,DV] (DV a multiple of 4) float32 or bfloat16; beta [B,H] float32; g float32:
     [B,H] (GDN), [B,H,DK] (KDA: row d of S decays by g[..., d]) or None (DeltaNet).  ``state`` [S,H,DK,DV] float32 — the
     chunked forwards' ``h_final`` — is updated in place, with ``slots`` as in :func:`causal_conv_step`.  Returns
-    o [B,H,DV] float32 scaled by ``scale`` (default DK^-1/2), as the chunked forwards do."""
+    o [B,H,DV] float32 scaled by ``scale`` (default DK^-1/2), as the chunked forwards do; ``out`` may be v."""
     dev = _device_of(q, "q")
     _dim(q, "q", 3, "[B,H,DK]")
     _dim(v, "v", 3, "[B,H,DV]")
@@ -389,6 +436,7 @@ def gdn_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
         o = torch.empty(nb, H, P, device=dev, dtype=torch.float32)
     else:
         _require_view(out, "out", (nb, H, P), torch.float32, dev)
+        _apart("out", out, ("v",), q=q, k=k, v=v, beta=beta, g=g, state=state, slots=slots)
         o = out
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), o.stride()
     _exec("pf_gdn_step_exec", dev, _STEP, _STEP_SIZE, state.data_ptr(), _ptr(slots), v.data_ptr(), k.data_ptr(),
@@ -414,7 +462,7 @@ def _rows_of(t: torch.Tensor, name: str, D: int) -> int:
     return flat.stride(0)
 
 
-def _norm(x, weight, residual, eps, y, y_code, block, scales, residual_out):
+def _norm(x, weight, residual, eps, y, y_code, block, scales, residual_out, given):
     dev, D, dtype = x.device, x.shape[-1], x.dtype
     if weight is None:
         raise ValueError("weight must be a tensor")
@@ -435,8 +483,12 @@ def _norm(x, weight, residual, eps, y, y_code, block, scales, residual_out):
                 raise ValueError(f"residual_out is {tuple(h.shape)} {h.dtype} on {h.device}, expected {tuple(x.shape)} "
                                  f"{residual.dtype} on {dev}")
             h_row = _rows_of(h, "residual_out", D)
+            _apart("residual_out", h, ("x", "residual"), x=x, residual=residual, weight=weight, out=y, scales_out=scales)
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
+    if given:
+        _apart("out", y, ("x", "residual"), x=x, residual=residual, weight=weight, scales_out=scales)
+        _apart("scales_out", scales, x=x, residual=residual, weight=weight)
     _exec("pf_norm_exec", dev, _NORM, _NORM_SIZE, x.data_ptr(), _ptr(residual), weight.data_ptr(), y.data_ptr(),
           _ptr(scales), _ptr(h), _rows_of(x, "x", D), r_row, _rows_of(y, "out", D), h_row, x.numel() // D,
           D, _dtype_code(dtype), y_code, r_f32, w_f32, block, float(eps))
@@ -456,16 +508,18 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
 
     x [..., D] float32 or bfloat16, D up to 32768; residual of x's shape and weight [D] in x's type or float32.  Returns
     (y, h): y in x's type (bfloat16 also of float32 rows: ``out_dtype``), h in the residual's, or None without one.  The
-    norm is of h before it is rounded.  ``residual_out`` may be ``residual`` (the stream updated in place) or x."""
+    norm is of h before it is rounded.  ``residual_out`` may be ``residual`` (the stream updated in place) or x, and ``out``
+    too, where it has their type; not both the same."""
     _norm_operand(x)
     dtype = x.dtype if out_dtype is None else out_dtype
     if dtype is not x.dtype and dtype is not torch.bfloat16:
         raise ValueError(f"out_dtype {dtype} of {x.dtype} rows ({x.dtype} or bfloat16)")
+    given = out is not None
     if out is None:
         out = torch.empty(x.shape, device=x.device, dtype=dtype)
     elif out.shape != x.shape or out.dtype != dtype or out.device != x.device:
         raise ValueError(f"out is {tuple(out.shape)} {out.dtype} on {out.device}, expected {tuple(x.shape)} {dtype} on {x.device}")
-    h = _norm(x, weight, residual, eps, out, _dtype_code(dtype), 0, None, residual_out)
+    h = _norm(x, weight, residual, eps, out, _dtype_code(dtype), 0, None, residual_out, given)
     return out, h
 
 
@@ -483,6 +537,7 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
     if scale_block is not None and (scale_block != 128 or D % 128):
         raise ValueError(f"scale_block must be None or 128, of rows of a multiple of 128: got {scale_block} of {D}")
     shape = (*x.shape[:-1], 1 if scale_block is None else D // 128)
+    given = out is not None or scales_out is not None
     if out is None:
         out = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     elif out.shape != x.shape or out.dtype != torch.float8_e4m3fn or out.device != x.device:
@@ -491,5 +546,6 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
         scales_out = torch.empty(shape, device=x.device, dtype=torch.float32)
     else:
         _require(scales_out, "scales_out", shape, torch.float32, x.device)
-    h = _norm(x, weight, residual, eps, out, _hip.PF_NORM_FP8, 128 if scale_block else 0, scales_out, residual_out)
+    h = _norm(x, weight, residual, eps, out, _hip.PF_NORM_FP8, 128 if scale_block else 0, scales_out, residual_out,
+              given)
     return out, scales_out, h

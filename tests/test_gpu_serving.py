@@ -638,3 +638,31 @@ def test_ssm_keeps_nan_where_it_is(dtype, B, H, T, P, N, t, bad, name):
     # and the bits of everything else stay
     assert torch.equal(torch.where(want, 0, y.float().cpu()), torch.where(want, 0, clean.float().cpu()))
     assert torch.equal(torch.where(want_state, 0, state.cpu()), torch.where(want_state, 0, clean_state.cpu()))
+
+
+def test_outputs_over_their_own_operands():
+    """What the descriptions let be one view: the bits of separate ones."""
+    announce("outputs over operands")
+    s, state = _step_case(31, BF, 5, 4, 64, 2, 32)
+    r = _rand(32)
+
+    def both(call, *over):
+        """call(out) with fresh memory, and with each of ``over`` (restored) as the output."""
+        want = call(None).clone()
+        for t in over:
+            kept = t.clone()
+            got = call(t)
+            assert got is t and torch.equal(got, want)
+            t.copy_(kept)
+
+    both(lambda o: ssm_step(state.clone(), dt_softplus=True, out=o, **s), s["x"], s["z"])
+    q, v, beta, S = _dev(0.1 * r(5, 4, 32)), _dev(r(5, 4, 64)), _dev(torch.sigmoid(r(5, 4))), _dev(r(5, 4, 32, 64))
+    both(lambda o: gdn_step(S.clone(), q, q, v, beta, out=o), v)
+    x, w, conv = _dev(r(5, 520), BF), _dev(r(520, 4), BF), _dev(r(5, 3, 520), BF)
+    both(lambda o: causal_conv_step(x, conv.clone(), w, out=o), x)
+    for D in (520, 4096):                    # a wave and a workgroup a row
+        rows, res, w = _dev(r(37, D), BF), _dev(r(37, D), BF), _dev(r(D), BF)
+        both(lambda o: add_rms_norm(rows, w, res, out=o)[0], rows, res)
+        both(lambda o: add_rms_norm(rows, w, res, residual_out=o)[1], rows, res)
+    wide = _dev(r(2, 33, 3 * 64), BF)
+    both(lambda o: causal_conv(wide[..., :64], _dev(torch.ones(64, 4), BF), out=o)[0], wide[..., 64:128])

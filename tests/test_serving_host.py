@@ -262,3 +262,79 @@ def test_sizes_past_32_bits_are_refused(monkeypatch):
     monkeypatch.setattr(serving, "_FUNCTIONS", {"pf_norm_exec": None})
     with pytest.raises(ValueError, match="past what pf_norm_exec takes"):
         serving._exec("pf_norm_exec", torch.device("cuda", 0), serving._NORM, serving._NORM_SIZE, *[0] * 10, 1 << 31, *[0] * 6, 0.0)
+
+
+def test_outputs_that_share_memory_are_refused(on_cpu):
+    """A workgroup may not write what another still reads; the very view that its writer reads may be written, and slices that
+    lie side by side in one buffer are apart."""
+    x, w = torch.zeros(2, 4, 8), torch.zeros(8, 4)
+    buf, state = torch.zeros(2, 5, 8), torch.zeros(2, 3, 8)
+    q, S, dt, A = torch.zeros(2, 4, 8), torch.zeros(2, 4, 8, 8), torch.zeros(2, 4), torch.zeros(4)
+    v, b = torch.zeros(2, 4, 8), torch.zeros(2, 2, 8)
+    px, pb, h0 = torch.zeros(2, 4, 9, 32), torch.zeros(2, 2, 9, 16), torch.zeros(2, 4, 16, 32)
+    pdt, pool = torch.zeros(2, 4, 9), torch.zeros(3, 4, 16, 32)
+    rows, nw = torch.zeros(6, 256), torch.zeros(256)
+    scales = torch.zeros(6, 1)
+    for match, call in (
+            ("out may not be x", lambda: pf.causal_conv(buf[:, :4], w, out=buf[:, 1:])),
+            ("out may not be initial_state", lambda: pf.causal_conv(x[:, :3], w, initial_state=state, out=state)),
+            ("final_out may not be x", lambda: pf.causal_conv(x, w, final_out=x.view(-1)[:48].view(2, 3, 8))),
+            ("final_out may not be initial_state", lambda: pf.causal_conv(x, w, initial_state=buf.view(-1)[:48].view(2, 3, 8),
+                                                                          final_out=buf.view(-1)[8:56].view(2, 3, 8))),
+            ("final_out may not be out", lambda: pf.causal_conv(x[:, :3], w, out=state, final_out=state)),
+            ("out may not be state", lambda: pf.causal_conv_step(x[:, 0], state, w, out=state[:, 0])),
+            ("out may not be x", lambda: pf.causal_conv_step(buf.view(-1)[:16].view(2, 8), state, w, out=buf.view(-1)[8:24].view(2, 8))),
+            ("out may not be q", lambda: pf.gdn_step(S, q, v, v, dt, out=q)),
+            ("out may not be k", lambda: pf.gdn_step(S, q, v, q + 1, dt, out=v)),
+            ("out may not be state", lambda: pf.gdn_step(S, q, q, v, dt, out=S[:, :, 0])),
+            ("out may not be B", lambda: pf.ssm_step(S, v, dt, A, q, q, out=q)),
+            ("out may not be x", lambda: pf.ssm_step(S, v, dt, A, b, b, out=v.view(4, 2, 8).transpose(0, 1))),
+            ("out may not be x", lambda: pf.ssm_chunk_forward(px, pdt, A, pb, pb, out=px)),
+            ("out may not be z", lambda: pf.ssm_chunk_forward(px + 1, pdt, A, pb, pb, z=px, out=px)),
+            ("final_out may not be h0", lambda: pf.ssm_chunk_forward(px, pdt, A, pb, pb, h0=pool[:2], final_out=pool[1:])),
+            ("out may not be x", lambda: pf.add_rms_norm(rows[:5], nw, out=rows[1:])),
+            ("out may not be x", lambda: pf.add_rms_norm(rows, nw, out_dtype=torch.bfloat16, out=rows.view(torch.bfloat16)[:, :256])),
+            ("residual_out may not be out", lambda: pf.add_rms_norm(rows + 1, nw, rows, out=rows, residual_out=rows)),
+            ("residual_out may not be residual", lambda: pf.add_rms_norm(rows[:5] + 1, nw, rows[:5], residual_out=rows[1:])),
+            ("scales_out may not be x", lambda: pf.add_rms_norm_fp8(rows, nw, scales_out=rows.view(-1)[:6].view(6, 1)))):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not on_cpu
+    wide = torch.zeros(2, 4, 24)
+    pf.causal_conv(wide[..., :8], w, out=wide[..., 8:16], initial_state=state, final_out=state)
+    pf.causal_conv_step(x[:, 0], state, w, out=x[:, 0])
+    pf.gdn_step(S, q, q, v, dt, out=v)
+    pf.ssm_step(S, v, dt, A, b, b, z=q, out=q)
+    pf.ssm_step(S, v, dt, A, b, b, out=v)
+    heads = torch.zeros(2, 9, 256)
+    one, two = (heads[..., i:i + 128].unflatten(-1, (4, 32)).transpose(1, 2) for i in (0, 128))
+    pf.ssm_chunk_forward(one, pdt, A, pb, pb, h0=h0, out=two, final_out=h0)
+    pf.add_rms_norm(rows, nw, rows + 1, out=rows)
+    pf.add_rms_norm(rows, nw, nw.expand(6, 256).contiguous(), out=rows[:, :256].view(6, 256))
+    pf.add_rms_norm(rows, nw, rows + 1, residual_out=rows)
+    pf.add_rms_norm_fp8(rows, nw, scales_out=scales)
+    assert len(on_cpu) == 10
+
+
+def test_memory_in_common_is_never_missed():
+    """Random views of one buffer against their elements' addresses."""
+    import random
+    rng, buf, found = random.Random(1), torch.zeros(400), 0
+
+    def view():
+        shape = [rng.randint(1, 4) for _ in range(rng.randint(1, 3))]
+        strides = [rng.choice([0, 1, 2, 3, 4, 6, 8, 12, 24, 48]) for _ in shape]
+        return torch.as_strided(buf, shape, strides[:-1] + [rng.choice([1, strides[-1]])], rng.randint(0, 50))
+
+    def cells(t):
+        at = {t.storage_offset()}
+        for n, s in zip(t.shape, t.stride()):
+            at = {o + i * s for o in at for i in range(n)}
+        return at
+
+    for _ in range(3000):
+        a, b = view(), view()
+        if cells(a) & cells(b):
+            assert serving._share(a, b)
+            found += 1
+    assert found > 100
