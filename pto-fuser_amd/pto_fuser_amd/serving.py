@@ -128,6 +128,17 @@ def _span(t: torch.Tensor) -> int:
     return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
+def _once(t: torch.Tensor, name: str) -> None:
+    """No two elements of ``t``, which a call writes, are one place (an expanded dimension, rows closer than they are long)."""
+    if t.is_contiguous():
+        return
+    end = 1
+    for stride, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if stride < end:
+            raise ValueError(f"{name} has overlapping rows")
+        end = stride * (n - 1) + end
+
+
 def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors may have memory in common.  Blocks that lie side by side in one buffer (slices of a projection's
     output) do not: all offsets of both are multiples of one pitch, apart from their start and their place in a block."""
@@ -150,10 +161,11 @@ def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _apart(name: str, t: Optional[torch.Tensor], same=(), **others) -> None:
-    """``t``, which a call writes, has no memory in common with what other threads of it read or write.  It may be the very
-    view ``others`` name in ``same``: those elements are read by the thread that writes them."""
+    """``t``, which a call writes, is written once an element and has no memory in common with what other threads of it read
+    or write.  It may be the very view ``others`` name in ``same``: those elements are read by the thread that writes them."""
     if t is None:
         return
+    _once(t, name)
     for other, u in others.items():
         if u is None or not _share(t, u):
             continue
@@ -315,8 +327,6 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
     sx = x.stride()
     if out is not None:
         _require_view(out, "out", (nb, H, T, P), dtype, dev)
-        if T > 1 and out.stride(2) < P:
-            raise ValueError("out has overlapping rows")
         _apart("out", out, x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, h0=h0, lengths=lengths)
         y = out
     elif sx[1] < sx[2]:

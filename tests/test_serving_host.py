@@ -338,3 +338,25 @@ def test_memory_in_common_is_never_missed():
             assert serving._share(a, b)
             found += 1
     assert found > 100
+
+
+def test_outputs_over_themselves_are_refused(on_cpu):
+    """An element is written by one thread: no expanded dimension, no rows closer than they are long."""
+    x, w, v, S = torch.zeros(2, 4, 8), torch.zeros(8, 4), torch.zeros(2, 4, 8), torch.zeros(2, 4, 8, 8)
+    dt, A, b, rows, nw = torch.zeros(2, 4), torch.zeros(4), torch.zeros(2, 2, 8), torch.zeros(6, 256), torch.zeros(256)
+    px, pb, pdt = torch.zeros(2, 4, 9, 32), torch.zeros(2, 2, 9, 16), torch.zeros(2, 4, 9)
+    for call in (lambda: pf.causal_conv(x, w, out=torch.zeros(4, 8).expand(2, 4, 8)),
+                 lambda: pf.causal_conv(x, w, out=torch.zeros(64).as_strided((2, 4, 8), (24, 7, 1))),
+                 lambda: pf.causal_conv_step(x[:, 0], torch.zeros(2, 3, 8), w, out=torch.zeros(8).expand(2, 8)),
+                 lambda: pf.gdn_step(S, v, v, v, dt, out=torch.zeros(2, 1, 8).expand(2, 4, 8)),
+                 lambda: pf.ssm_step(S, v, dt, A, b, b, out=torch.zeros(64).as_strided((2, 4, 8), (16, 8, 1))),
+                 lambda: pf.ssm_chunk_forward(px, pdt, A, pb, pb, out=torch.zeros(2, 1, 9, 32).expand(2, 4, 9, 32)),
+                 lambda: pf.ssm_chunk_forward(px, pdt, A, pb, pb, out=torch.zeros(2048).as_strided((2, 4, 9, 32), (1000, 32, 31, 1))),
+                 lambda: pf.add_rms_norm(rows, nw, out=torch.zeros(256).expand(6, 256)),
+                 lambda: pf.add_rms_norm(rows, nw, rows, residual_out=torch.zeros(2000).as_strided((6, 256), (255, 1)))):
+        with pytest.raises(ValueError, match="overlapping rows"):
+            call()
+    assert not on_cpu
+    pf.causal_conv(x, w, out=torch.zeros(100).as_strided((2, 4, 8), (8, 20, 1)))
+    pf.causal_conv(x[:1, :1], w, out=torch.zeros(8).as_strided((1, 1, 8), (0, 0, 1)))
+    assert len(on_cpu) == 2
