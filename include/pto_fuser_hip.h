@@ -240,7 +240,7 @@ int pf_scan_exec(const void* w, const void* u, const void* k, const float* decay
  *   y[b,t,c] = act( bias[c] + sum_k w[c,k] x[b, t-(K-1)+k, c] ),  act: 1 = silu, 0 = none
  * Tokens before the first are state_in [B,K-1,W] (NULL: zero).  lengths [B] (NULL: all T): the tokens
  * of each sequence; later ones are not read and y is zero there.  state_out [B,K-1,W] (or NULL): the
- * last K-1 inputs, for the next call; it may be state_in.  Supported: K 2 to 4, T >= 0. */
+ * last K-1 inputs, for the next call; it may be state_in.  Supported: K 2 to 4, T 0 to 2^30. */
 typedef struct pf_conv_args {
   size_t size;
   const void* x;         /* E, [B,T,W] */
@@ -274,7 +274,7 @@ int pf_conv_step_exec(const pf_conv_step_args* args, void* stream);
  * (DELTA = pf_ssm_step_exec: v = x, k = B, q = C) and of the gated delta rule (pf_gdn_step_exec; KDA
  * with g_rows = 1):
  *   S <- e^g S,  r = beta (v - k^T S),  S <- S + k r^T,  y = scale q^T S
- * state [S,H,N,P] fp32 contiguous within a slot, updated in place.  Supported: N <= 256, P % 4 == 0;
+ * state [S,H,N,P] fp32 contiguous within a slot, updated in place.  Supported: N <= 256, P % 4 == 0 up to 2^30;
  * the delta rule: G = H. */
 typedef struct pf_step_args {
   size_t size;
@@ -302,7 +302,7 @@ int pf_gdn_step_exec(const pf_step_args* args, void* stream);
  *   dt = softplus?(dt + dt_bias),  S_t = e^{dt A} S_{t-1} + B_t (dt x_t)^T,  y_t = (C_t^T S_t + D x_t) * silu(z_t)?
  * x, z, y [B,H,T,P], b, c [B,G,T,N], dt [B,H,T] with free strides; A, D, dt_bias [H] fp32; h0, h_final
  * [B,H,N,P] fp32 contiguous (h_final may be h0).  lengths [B] (NULL: all T): the tokens of each sequence;
- * later ones are not read, y is zero there, and the state is that after the last one.  Any T >= 0.
+ * later ones are not read, y is zero there, and the state is that after the last one.  T 0 to 2^30.
  * The scan runs 64-token chunks.  A non-finite operand reaches what the recurrence takes it to, its own token and later ones,
  * and nothing before; where a value of x is not finite, its column of y is NaN from there on.
  * Supported: P a multiple of 32 up to 256, N a multiple of 16 up to 128; token strides of x, b, c, z and y of a

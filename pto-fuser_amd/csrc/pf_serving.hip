@@ -14,6 +14,9 @@ using pf::bf16;
 
 bool known(int dtype) { return dtype == PF_DTYPE_F32 || dtype == PF_DTYPE_BF16; }
 
+// The largest prompt and head: what is rounded up to whole tiles and counted past the end stays an int.
+constexpr int kMaxSize = 1 << 30;
+
 template <typename... S>
 bool strides_ok(S... s) { return ((s >= 0) && ...); }
 
@@ -84,7 +87,7 @@ int step_rows(pf::StepArgs& a, int B, hipStream_t s) {
 template <bool DELTA>
 int step(const pf_step_args* p, void* stream) {
   if (!p || p->size != sizeof *p || !known(p->dtype)) return PF_ERR_ARG;
-  if (p->B < 0 || p->S < 0 || p->H <= 0 || p->G <= 0 || p->H % p->G || p->N <= 0 || p->N > 256 || p->P <= 0 || p->P % 4)
+  if (p->B < 0 || p->S < 0 || p->H <= 0 || p->G <= 0 || p->H % p->G || p->N <= 0 || p->N > 256 || p->P <= 0 || p->P % 4 || p->P > kMaxSize)
     return PF_ERR_ARG;
   if (DELTA ? p->G != p->H || !p->beta : !p->dt || !p->a) return PF_ERR_ARG;
   if (!p->state || !p->v || !p->k || !p->q || !p->y) return PF_ERR_ARG;
@@ -139,7 +142,7 @@ extern "C" {
 
 int pf_conv_exec(const pf_conv_args* p, void* stream) {
   if (!p || p->size != sizeof *p || !known(p->dtype)) return PF_ERR_ARG;
-  if (p->B < 0 || p->T < 0 || p->W <= 0 || p->K < 2 || p->K > 4 || !p->w) return PF_ERR_ARG;
+  if (p->B < 0 || p->T < 0 || p->T > kMaxSize || p->W <= 0 || p->K < 2 || p->K > 4 || !p->w) return PF_ERR_ARG;
   if (p->T > 0 && p->B > 0 && (!p->x || !p->y)) return PF_ERR_ARG;
   if (!strides_ok(p->x_b, p->x_t, p->y_b, p->y_t, p->state_in_b, p->state_out_b)) return PF_ERR_ARG;
   if (p->B == 0) return PF_OK;

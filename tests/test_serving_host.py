@@ -360,3 +360,16 @@ def test_outputs_over_themselves_are_refused(on_cpu):
     pf.causal_conv(x, w, out=torch.zeros(100).as_strided((2, 4, 8), (8, 20, 1)))
     pf.causal_conv(x[:1, :1], w, out=torch.zeros(8).as_strided((1, 1, 8), (0, 0, 1)))
     assert len(on_cpu) == 2
+
+
+@pytest.mark.parametrize("T", [2 ** 30 + 1, 2 ** 31 - 7, 2 ** 31 - 1])
+def test_prompts_past_the_counters_are_refused(lib, T):
+    """Rounded up to whole tiles they would pass 2^31."""
+    assert lib.pf_conv_exec(_conv(T=T), None) == _hip.PF_ERR_ARG
+    assert lib.pf_ssm_exec(_ssm(T=T), None) == _hip.PF_ERR_ARG
+
+
+@pytest.mark.parametrize("P", [2 ** 30 + 4, 2 ** 31 - 4])
+def test_heads_past_the_counters_are_refused(lib, P):
+    assert lib.pf_ssm_step_exec(_step(P=P), None) == _hip.PF_ERR_ARG
+    assert lib.pf_gdn_step_exec(_step(P=P, G=2, beta=64), None) == _hip.PF_ERR_ARG
