@@ -89,12 +89,13 @@ int step(const pf_step_args* p, void* stream) {
   if (!p || p->size != sizeof *p || !known(p->dtype)) return PF_ERR_ARG;
   if (p->B < 0 || p->S < 0 || p->H <= 0 || p->G <= 0 || p->H % p->G || p->N <= 0 || p->N > 256 || p->P <= 0 || p->P % 4 || p->P > kMaxSize)
     return PF_ERR_ARG;
-  if (DELTA ? p->G != p->H || !p->beta : !p->dt || !p->a) return PF_ERR_ARG;
-  if (!p->state || !p->v || !p->k || !p->q || !p->y) return PF_ERR_ARG;
+  if (DELTA && p->G != p->H) return PF_ERR_ARG;
   if (!strides_ok(p->v_b, p->v_h, p->k_b, p->k_h, p->q_b, p->q_h, p->y_b, p->y_h, p->dt_b, p->dt_h, p->z_b, p->z_h, p->state_b))
     return PF_ERR_ARG;
   if (!p->slots && p->B > p->S) return PF_ERR_ARG;
-  if (p->B == 0) return PF_OK;
+  if (p->B == 0) return PF_OK;                // (of no elements a pointer may be null)
+  if (DELTA ? !p->beta : !p->dt || !p->a) return PF_ERR_ARG;
+  if ((!p->state && p->S > 0) || !p->v || !p->k || !p->q || !p->y) return PF_ERR_ARG;
   pf::StepArgs a{};
   a.state = p->state; a.slots = p->slots; a.v = p->v; a.k = p->k; a.q = p->q; a.y = p->y;
   a.dt = p->dt; a.z = p->z; a.a = p->a; a.d = p->d; a.dt_bias = p->dt_bias; a.beta = p->beta; a.g = p->g;
@@ -158,7 +159,7 @@ int pf_conv_exec(const pf_conv_args* p, void* stream) {
 int pf_conv_step_exec(const pf_conv_step_args* p, void* stream) {
   if (!p || p->size != sizeof *p || !known(p->dtype)) return PF_ERR_ARG;
   if (p->B < 0 || p->S < 0 || p->W <= 0 || p->K < 2 || p->K > 4 || !p->w) return PF_ERR_ARG;
-  if (p->B > 0 && (!p->x || !p->y || !p->state)) return PF_ERR_ARG;
+  if (p->B > 0 && (!p->x || !p->y || (!p->state && p->S > 0))) return PF_ERR_ARG;
   if (!strides_ok(p->x_b, p->y_b, p->state_b) || (!p->slots && p->B > p->S)) return PF_ERR_ARG;
   if (p->B == 0) return PF_OK;
   pf::ConvStepArgs a{};

@@ -666,3 +666,23 @@ def test_outputs_over_their_own_operands():
         both(lambda o: add_rms_norm(rows, w, res, residual_out=o)[1], rows, res)
     wide = _dev(r(2, 33, 3 * 64), BF)
     both(lambda o: causal_conv(wide[..., :64], _dev(torch.ones(64, 4), BF), out=o)[0], wide[..., 64:128])
+
+
+def test_steps_of_empty_batches_and_pools():
+    announce("steps of no sequences, and of a pool of none")
+    s, state = _step_case(33, BF, 3, 4, 64, 1, 32)
+    none = {k: t[:0] if t is not None and t.shape[0] == 3 else t for k, t in s.items()}
+    before = state.clone()
+    slots = torch.zeros(0, dtype=torch.int32, device=DEV)
+    q, v, beta = torch.zeros(0, 4, 32, device=DEV, dtype=BF), none["x"], torch.zeros(0, 4, device=DEV)
+    x, conv, w = torch.zeros(0, 64, device=DEV, dtype=BF), torch.zeros(2, 3, 64, device=DEV, dtype=BF), torch.ones(64, 4, device=DEV, dtype=BF)
+    assert ssm_step(state, slots=slots, **none).shape == ssm_step(state[:0], **none).shape == (0, 4, 64)
+    assert gdn_step(state, q, q, v, beta, slots=slots).shape == gdn_step(state[:0], q, q, v, beta).shape == (0, 4, 64)
+    assert causal_conv_step(x, conv, w, slots=slots).shape == causal_conv_step(x, conv[:0], w).shape == (0, 64)
+    assert torch.equal(state, before)
+    # a pool of no states: every slot is outside it
+    slots = torch.tensor([0, 1, -1], dtype=torch.int32, device=DEV)
+    assert not ssm_step(state[:0], slots=slots, **s).any()
+    q, beta = torch.ones(3, 4, 32, device=DEV, dtype=BF), torch.ones(3, 4, device=DEV)
+    assert not gdn_step(state[:0], q, q, s["x"], beta, slots=slots).any()
+    assert not causal_conv_step(torch.ones(3, 64, device=DEV, dtype=BF), conv[:0], w, slots=slots).any()

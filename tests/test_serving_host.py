@@ -373,3 +373,13 @@ def test_prompts_past_the_counters_are_refused(lib, T):
 def test_heads_past_the_counters_are_refused(lib, P):
     assert lib.pf_ssm_step_exec(_step(P=P), None) == _hip.PF_ERR_ARG
     assert lib.pf_gdn_step_exec(_step(P=P, G=2, beta=64), None) == _hip.PF_ERR_ARG
+
+
+def test_empty_batches_launch_nothing(lib):
+    """Tensors of no elements have null pointers."""
+    null = dict(v=0, k=0, q=0, y=0, dt=0, beta=0)
+    for S, state in ((0, 0), (5, 64)):
+        assert lib.pf_ssm_step_exec(_step(B=0, S=S, state=state, **null), None) == _hip.PF_OK
+        assert lib.pf_gdn_step_exec(_step(B=0, S=S, state=state, G=2, **null), None) == _hip.PF_OK
+        assert lib.pf_conv_step_exec(_conv_step(B=0, S=S, state=state, x=0, y=0), None) == _hip.PF_OK
+    assert lib.pf_conv_exec(_conv(B=0, x=0, y=0), None) == lib.pf_ssm_exec(_ssm(B=0, x=0, dt=0, b=0, c=0, y=0), None) == _hip.PF_OK
