@@ -130,6 +130,7 @@ size_t pf_ssm_workspace_bytes(int B, int H, int G, int T, int N, int P, int dtyp
 int pf_ssm_exec(const pf_ssm_args* p, void* stream) {
   if (!p || p->size != sizeof *p || !shape_ok(p->B, p->H, p->G, p->T, p->N, p->P, p->dtype)) return PF_ERR_ARG;
   if ((double)p->B * p->H * p->N * p->P > 1e12 || !p->a) return PF_ERR_ARG;
+  if (p->B == 0) return PF_OK;
   if (p->T > 0 && p->B > 0 && (!p->x || !p->dt || !p->b || !p->c || !p->y)) return PF_ERR_ARG;
   for (long long st : {p->x_b, p->x_h, p->x_t, p->dt_b, p->dt_h, p->dt_t, p->b_b, p->b_g, p->b_t, p->c_b, p->c_g, p->c_t,
                        p->z_b, p->z_h, p->z_t, p->y_b, p->y_h, p->y_t})
@@ -141,7 +142,6 @@ int pf_ssm_exec(const pf_ssm_args* p, void* stream) {
   if (x_t < p->P || y_t < p->P || z_t < p->P || b_t < p->N || c_t < p->N) return PF_ERR_ARG;
   for (long long st : {x_t, y_t, z_t, b_t, c_t})
     if (st > pf::kMaxTokenStride) return PF_ERR_ARG;
-  if (p->B == 0) return PF_OK;
   SsmPlan pl = plan(p->B, p->H, p->G, p->T, p->N, p->P, p->dtype);
   if (!p->workspace || p->workspace_bytes < pl.bytes || ((size_t)p->workspace & 15)) {   // whole sequences
     pl.segs = 1;

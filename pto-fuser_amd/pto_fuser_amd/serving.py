@@ -14,8 +14,8 @@ No counterpart in the reference, whose path ends at the chunked forward.  Forwar
 Unlike those, the operands may be views: batch, head and token strides are free (a slice of a projection's output, a
 transposed head layout); only the innermost dimension is contiguous.  Every operator raises ``ValueError`` before
 launching for what it does not support, works on the current stream of the operands' device, and neither synchronises nor
-allocates anything but its outputs and (the scan) a workspace, from torch's allocator: each can be captured in a HIP
-graph.  What a call is given to write (``out`` and the like) shares memory with no other operand, unless its description
+allocates anything but its outputs and (the scan) a workspace and operands that it has to copy, from torch's allocator: each can
+be captured in a HIP graph.  What a call is given to write (``out`` and the like) shares memory with no other operand, unless its description
 names one that it may be; slices of one buffer that lie side by side are apart.
 """
 from __future__ import annotations
@@ -47,7 +47,7 @@ _CONV_SIZE, _CONV_STEP_SIZE, _STEP_SIZE, _SSM_SIZE, _NORM_SIZE = (
 
 CONV_TAPS = (2, 3, 4)
 STEP_MAX_ROWS = 256
-SSM_MAX_ROWS, SSM_MAX_COLS = 128, 256
+SSM_MAX_ROWS, SSM_MAX_COLS, SSM_MAX_STRIDE = 128, 256, 1 << 22
 NORM_MAX_WIDTH = 32768
 _ACTIVATIONS = {None: 0, "silu": 1}
 
@@ -70,6 +70,8 @@ def _exec(name: str, dev: torch.device, layout: struct.Struct, *fields) -> None:
     else:
         with torch.cuda.device(dev):
             st = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if st == _hip.PF_ERR_ARG:
+        raise ValueError(f"{name} does not take a call of this size: a stride or its grid is past what one launch covers")
     if st:
         _hip.check(name, st)
 
@@ -191,7 +193,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Depthwise causal convolution along the tokens: y[b,t,c] = act(bias[c] + Σ_k w[c,k] x[b,t-(K-1)+k,c]).
 
-    x [B,T,W] float32 or bfloat16, token and batch strides free; weight [W,K], K in 2..4, and bias [W] in x's type or
+    x [B,T,W] float32 or bfloat16, T up to 2^30, token and batch strides free; weight [W,K], K in 2..4, and bias [W] in x's type or
     float32 (both in one).  ``initial_state`` [B,K-1,W] holds the last K-1 inputs of what came before (None: zeros).
     ``lengths`` [B] int32 (None: all T): tokens of each sequence; what follows them is not read, and y is zero there.
     Returns (y [B,T,W] in x's type, the state after the last token [B,K-1,W] or None).  ``final_out`` may be
@@ -285,8 +287,9 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
 
     x, z [B,H,T,P] float32 or bfloat16, P a multiple of 32 up to 256; dt [B,H,T] in x's type or float32; B, C [B,G,T,N], N a
     multiple of 16 up to 128, head h reading group h // (H // G); A, D, dt_bias [H] float32 (A < 0: it decays); h0
-    [B,H,N,P] float32.  Any T.  Batch, head and token strides are free: ``xbc[..., :H*P].unflatten(-1, (H, P)).transpose(1,
-    2)`` of a convolved row [B,T,..] is read in place.  ``lengths`` [B] int32 (None: all T): tokens of each sequence; what
+    [B,H,N,P] float32.  T up to 2^30.  Batch, head and token strides are free: ``xbc[..., :H*P].unflatten(-1, (H,
+    P)).transpose(1, 2)`` of a convolved row [B,T,..] is read in place; tokens that overlap or lie more than 2^22 elements
+    apart are copied first, and not written (``out``).  ``lengths`` [B] int32 (None: all T): tokens of each sequence; what
     follows them is not read, y is zero there, and the state is that after the last one.  A NaN or infinity reaches
     its own token and those after it, as in the recurrence, and none before.
 
@@ -322,14 +325,17 @@ def ssm_chunk_forward(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: tor
         _require(h0, "h0", (nb, H, N, P), torch.float32, dev)
     if lengths is not None:
         _require(lengths, "lengths", (nb,), torch.int32, dev)
-    if T > 1:      # rows that overlap (a token expanded along the sequence) are laid out first
-        x, B, C, z = (t if t is None or t.stride(2) >= t.shape[3] else t.contiguous() for t in (x, B, C, z))
+    token_major = x.stride(1) < x.stride(2)
+    if T > 1:      # rows that overlap (a token expanded along the sequence) or lie far apart are laid out first
+        x, B, C, z = (t if t is None or t.shape[3] <= t.stride(2) <= SSM_MAX_STRIDE else t.contiguous() for t in (x, B, C, z))
     sx = x.stride()
     if out is not None:
         _require_view(out, "out", (nb, H, T, P), dtype, dev)
+        if T > 1 and out.stride(2) > SSM_MAX_STRIDE:
+            raise ValueError(f"out's tokens are {out.stride(2)} elements apart (up to {SSM_MAX_STRIDE})")
         _apart("out", out, x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, h0=h0, lengths=lengths)
         y = out
-    elif sx[1] < sx[2]:
+    elif token_major:
         y = torch.empty(nb, T, H, P, device=dev, dtype=dtype).transpose(1, 2)
     else:
         y = torch.empty(nb, H, T, P, device=dev, dtype=dtype)

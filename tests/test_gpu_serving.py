@@ -686,3 +686,19 @@ def test_steps_of_empty_batches_and_pools():
     q, beta = torch.ones(3, 4, 32, device=DEV, dtype=BF), torch.ones(3, 4, device=DEV)
     assert not gdn_step(state[:0], q, q, s["x"], beta, slots=slots).any()
     assert not causal_conv_step(torch.ones(3, 64, device=DEV, dtype=BF), conv[:0], w, slots=slots).any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_ssm_of_tokens_far_apart(dtype):
+    """Token strides at the kernel's bound, read in place, and past it: the bits of packed operands."""
+    announce(f"ssm_chunk_forward token strides of 2^22 {dtype}")
+    s = _ssm_case(41, dtype, 1, 2, 3, 32, 1, 16)
+    want = pf_ssm(s)
+    for stride in (1 << 22, (1 << 22) + 8):
+        far = dict(s)
+        for k in ("x", "B", "C", "z"):
+            t = s[k]
+            buf = torch.full((3 * stride,), NAN, device=DEV, dtype=dtype)
+            far[k] = buf.as_strided(t.shape, (0, t.shape[3], stride, 1))
+            far[k].copy_(t)
+        assert all(torch.equal(a, b) for a, b in zip(pf_ssm(far), want))

@@ -383,3 +383,31 @@ def test_empty_batches_launch_nothing(lib):
         assert lib.pf_gdn_step_exec(_step(B=0, S=S, state=state, G=2, **null), None) == _hip.PF_OK
         assert lib.pf_conv_step_exec(_conv_step(B=0, S=S, state=state, x=0, y=0), None) == _hip.PF_OK
     assert lib.pf_conv_exec(_conv(B=0, x=0, y=0), None) == lib.pf_ssm_exec(_ssm(B=0, x=0, dt=0, b=0, c=0, y=0), None) == _hip.PF_OK
+
+
+def test_calls_that_no_launch_covers_are_value_errors(monkeypatch):
+    """What an entry point does not take is refused as such; what fails in the launch is the library's error."""
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    for status, error in ((_hip.PF_ERR_ARG, ValueError), (719, _hip.HipKernelError)):
+        monkeypatch.setattr(serving, "_FUNCTIONS", {"pf_norm_exec": lambda args, stream: status})
+        with pytest.raises(error, match="pf_norm_exec"):
+            serving._exec("pf_norm_exec", torch.device("cuda", 0), serving._NORM, serving._NORM_SIZE, *[0] * 17, 0.0)
+
+
+def test_ssm_token_strides(on_cpu):
+    """Operands whose tokens overlap or lie past the kernel's offsets are laid out first, an output is refused."""
+    far = serving.SSM_MAX_STRIDE + 8
+    buf = torch.zeros(far + 256)
+    view = lambda n, stride: buf.as_strided((1, 1, 2, n), (0, 0, stride, 1))  # noqa: E731
+    dt, A = torch.zeros(1, 1, 2), torch.zeros(1)
+    for stride, same in ((32, True), (serving.SSM_MAX_STRIDE, True), (far, False), (0, False), (16, False)):
+        pf.ssm_chunk_forward(view(32, stride), dt, A, view(16, stride), view(16, stride), z=view(32, stride))
+        f = serving._SSM.unpack(on_cpu.pop()[1])
+        x_t, b_t, c_t, z_t = (f[i] for i in (17, 23, 26, 29))
+        want = [stride, stride, stride, stride] if same else [32, stride if stride == 16 else 16, stride if stride == 16 else 16, 32]
+        assert [x_t, b_t, c_t, z_t] == want
+        assert (f[1] == buf.data_ptr()) == same
+    with pytest.raises(ValueError, match="elements apart"):
+        pf.ssm_chunk_forward(view(32, 32) + 0, dt, A, view(16, 16) + 0, view(16, 16) + 0, out=view(32, far))
+    assert not on_cpu
