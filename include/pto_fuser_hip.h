@@ -269,10 +269,9 @@ typedef struct pf_conv_step_args {
 } pf_conv_step_args;
 int pf_conv_step_exec(const pf_conv_step_args* args, void* stream);
 
-/* One token of the state space recurrence, for head h of group h / (H / G):
+/* One token of the state space recurrence (pf_ssm_step_exec: v = x, k = B, q = C), for head h of group h / (H / G):
  *   dt = softplus?(dt + dt_bias),  S <- e^{dt A} S + B (dt x)^T,  y = (C^T S + D x) * silu(z)?
- * (DELTA = pf_ssm_step_exec: v = x, k = B, q = C) and of the gated delta rule (pf_gdn_step_exec; KDA
- * with g_rows = 1):
+ * and of the gated delta rule (pf_gdn_step_exec; KDA with g_rows = 1):
  *   S <- e^g S,  r = beta (v - k^T S),  S <- S + k r^T,  y = scale q^T S
  * state [S,H,N,P] fp32 contiguous within a slot, updated in place.  Supported: N <= 256, P % 4 == 0 up to 2^30;
  * the delta rule: G = H. */
