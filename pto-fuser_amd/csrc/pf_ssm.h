@@ -98,10 +98,6 @@ __device__ __forceinline__ void only_finite(Frag<float>& f) {
   }
 }
 
-template <typename E, typename V> __device__ __forceinline__ Frag<E> frag_cat(const V& lo, const V& hi);
-template <> __device__ __forceinline__ Frag<bf16> frag_cat<bf16, bf16x4>(const bf16x4& lo, const bf16x4& hi) { return {cat8(lo, hi)}; }
-template <> __device__ __forceinline__ Frag<float> frag_cat<float, floatx4>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
-
 // ---- LDS tiles: 64 token rows, PAD elements longer than they are ----------------------------
 // Rows 16 bytes apart modulo the banks suit the operand that reads sixteen rows at one place; 32 bytes the transposed one,
 // which reads eight rows at four neighbouring 8-byte places in half a wave.  fp32 rows are 16 bytes apart.
