@@ -13,8 +13,10 @@
 // the state each segment adds by itself (kStates: no C, no score), the states that enter the segments (a sum along the
 // segments, ssm_prefix_kernel), and the outputs (kOutput from those states).
 //
-// Rounding, bf16 operands: S and the decayed score are rounded to 8 bits where they enter a product for y (which is
-// rounded to 8 bits itself); the state is a sum in fp32 of products whose weighted operand has 16 or 24 bits (SPLIT).
+// Rounding, bf16 operands: S and the decayed score enter the products for y in two bf16 terms each, 16 bits, so that y is
+// off by its own rounding to 8 bits (1.66e-3 of its norm; with one term each 1.75e-3 where D x is most of y, 2.0e-3 to
+// 2.4e-3 else, at 101 and 205 us against 108 and 222 for 8192 and 32768 tokens); the state is a sum in fp32 of products
+// whose weighted operand has 16 or 24 bits (SPLIT).
 // fp32 operands: fp32 matrix instructions throughout.
 //
 // Measured, bf16, N = 128, P = 64 (kernel times): 2 x 32 heads x 8192 tokens, 16 segments: states 39 us (67 MB of x and
@@ -81,11 +83,6 @@ __device__ __forceinline__ floatx4 mfma32(const Frag<float>& a, const Frag<float
   return acc;
 }
 
-// Two MFMA results as the operand that contracts over their 32 rows.
-template <typename E> __device__ __forceinline__ Frag<E> frag_of(const floatx4& lo, const floatx4& hi);
-template <> __device__ __forceinline__ Frag<bf16> frag_of<bf16>(const floatx4& lo, const floatx4& hi) { return {pack8(lo, hi)}; }
-template <> __device__ __forceinline__ Frag<float> frag_of<float>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
-
 __device__ __forceinline__ void only_finite(Frag<bf16>& f) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) f.v[i] = __builtin_isfinite((float)f.v[i]) ? f.v[i] : (bf16)0.f;
@@ -97,6 +94,29 @@ __device__ __forceinline__ void only_finite(Frag<float>& f) {
     f.hi[i] = __builtin_isfinite(f.hi[i]) ? f.hi[i] : 0.f;
   }
 }
+
+template <typename E, typename V> __device__ __forceinline__ Frag<E> frag_cat(const V& lo, const V& hi);
+template <> __device__ __forceinline__ Frag<bf16> frag_cat<bf16, bf16x4>(const bf16x4& lo, const bf16x4& hi) { return {cat8(lo, hi)}; }
+template <> __device__ __forceinline__ Frag<float> frag_cat<float, floatx4>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
+
+// Two MFMA results as the operand that contracts over their 32 rows: in TERMS bf16 terms, each the rounding of what the ones
+// before it left; fp32 needs one.
+template <int TERMS>
+__device__ __forceinline__ void terms_of(const floatx4& lo, const floatx4& hi, Frag<bf16> (&t)[TERMS]) {
+  floatx4 l = lo, h = hi;
+#pragma unroll
+  for (int k = 0; k < TERMS; ++k) {
+    t[k].v = pack8(l, h);
+    if (k + 1 < TERMS) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        l[i] -= (float)t[k].v[i];
+        h[i] -= (float)t[k].v[4 + i];
+      }
+    }
+  }
+}
+__device__ __forceinline__ void terms_of(const floatx4& lo, const floatx4& hi, Frag<float> (&t)[1]) { t[0] = {lo, hi}; }
 
 // ---- LDS tiles: 64 token rows, PAD elements longer than they are ----------------------------
 // Rows 16 bytes apart modulo the banks suit the operand that reads sixteen rows at one place; 32 bytes the transposed one,
@@ -229,7 +249,7 @@ template <typename E, int NT, int NW, int PT, bool OUT> struct SsmLds {
 };
 
 // SPLIT: bf16 terms of the weighted x in the state's update.  Three keep the state a sum in 24 bits, as it has to be where
-// it is returned; two where it only enters y, whose operand S is rounded to 8 bits anyway.
+// it is returned; two where it only enters y, whose operand S has two terms itself.
 // PT: 16-column tiles of a wave.
 // One workgroup's walk.  Returns whether it has to be made AGAIN: a value of x that is not finite reaches the tokens before it
 // in its chunk, through the products with the zeros above the score's diagonal.  The second walk leaves such values out of the
@@ -463,6 +483,7 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
         }
       }
       // y^T = S^T C^T
+      constexpr int TERMS = sizeof(E) == 2 ? 2 : 1;      // of an fp32 operand
       floatx4 y[PT][4];
 #pragma unroll
       for (int pt = 0; pt < PT; ++pt)
@@ -470,14 +491,16 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
         for (int ib = 0; ib < 4; ++ib) y[pt][ib] = zero4();
 #pragma unroll
       for (int kb = 0; kb < NT / 32; ++kb) {
-        Frag<E> sf[PT];
+        Frag<E> sf[PT][TERMS];
 #pragma unroll
-        for (int pt = 0; pt < PT; ++pt) sf[pt] = frag_of<E>(S[2 * kb][pt], S[2 * kb + 1][pt]);
+        for (int pt = 0; pt < PT; ++pt) terms_of(S[2 * kb][pt], S[2 * kb + 1][pt], sf[pt]);
 #pragma unroll
         for (int ib = 0; ib < 4; ++ib) {
           const Frag<E> cf = Cs::rows(s.c, 16 * ib + c, kb, g);
 #pragma unroll
-          for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(sf[pt], cf, y[pt][ib]);
+          for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+            for (int k = TERMS - 1; k >= 0; --k) y[pt][ib] = mfma32(sf[pt][k], cf, y[pt][ib]);
         }
       }
       const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
@@ -511,9 +534,12 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
         }
 #pragma unroll
         for (int kb = 0; kb <= ib / 2; ++kb) {
-          const Frag<E> pf = frag_of<E>(pr[2 * kb], pr[2 * kb + 1]);
+          Frag<E> pf[TERMS];
+          terms_of(pr[2 * kb], pr[2 * kb + 1], pf);
 #pragma unroll
-          for (int pt = 0; pt < PT; ++pt) y[pt][ib] = mfma32(xf[pt][kb], pf, y[pt][ib]);
+          for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+            for (int k = TERMS - 1; k >= 0; --k) y[pt][ib] = mfma32(xf[pt][kb], pf[k], y[pt][ib]);
         }
       }
       if (AGAIN) {                             // 0 x, summed along the tokens: NaN from a value that is not finite on
