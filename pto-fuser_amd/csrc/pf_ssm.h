@@ -15,8 +15,8 @@
 //
 // Rounding, bf16 operands: S and the decayed score enter the products for y in two bf16 terms each, 16 bits, so that y is
 // off by its own rounding to 8 bits (1.66e-3 of its norm; with one term each 1.75e-3 where D x is most of y, 2.0e-3 to
-// 2.4e-3 else, at 101 and 205 us against 108 and 222 for 8192 and 32768 tokens); the state is a sum in fp32 of products
-// whose weighted operand has 16 or 24 bits (SPLIT).
+// 2.4e-3 else, at 100 and 204 us against 105 and 215 for 2 x 8192 and 32768 tokens); the state is a sum in fp32 of
+// products whose weighted operand has 16 or 24 bits (SPLIT).
 // fp32 operands: fp32 matrix instructions throughout.
 //
 // Measured, bf16, N = 128, P = 64 (kernel times): 2 x 32 heads x 8192 tokens, 16 segments: states 39 us (67 MB of x and
@@ -99,24 +99,38 @@ template <typename E, typename V> __device__ __forceinline__ Frag<E> frag_cat(co
 template <> __device__ __forceinline__ Frag<bf16> frag_cat<bf16, bf16x4>(const bf16x4& lo, const bf16x4& hi) { return {cat8(lo, hi)}; }
 template <> __device__ __forceinline__ Frag<float> frag_cat<float, floatx4>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
 
-// Two MFMA results as the operand that contracts over their 32 rows: in TERMS bf16 terms, each the rounding of what the ones
-// before it left; fp32 needs one.
-template <int TERMS>
-__device__ __forceinline__ void terms_of(const floatx4& lo, const floatx4& hi, Frag<bf16> (&t)[TERMS]) {
-  floatx4 l = lo, h = hi;
+// Two MFMA results as the operand that contracts over their 32 rows, in bf16 terms: each the rounding of what the ones before
+// it left (8, 16 or 24 bits); fp32 needs one.  A product with minus the identity takes a term off, exactly (one product and
+// zeros, which also is why a value that is not finite spoils its column, as it does in the sums to come).  The vector
+// port has more to do here than the matrix pipes: with subtractions there 2 x 32 heads x 8192 tokens took 108.5 us against 105.
+template <typename E> struct Terms;
+template <> struct Terms<bf16> {
+  static constexpr int N = 2;        // for y
+  Frag<bf16> lo, hi;                 // minus the identity for the first 16 and for the second 16 of 32 rows
+  __device__ __forceinline__ Terms(int c, int g) {
 #pragma unroll
-  for (int k = 0; k < TERMS; ++k) {
-    t[k].v = pack8(l, h);
-    if (k + 1 < TERMS) {
+    for (int i = 0; i < 4; ++i) {
+      lo.v[i] = hi.v[4 + i] = 4 * g + i == c ? (bf16)-1.f : (bf16)0.f;
+      lo.v[4 + i] = hi.v[i] = (bf16)0.f;
+    }
+  }
+  template <int COUNT>
+  __device__ __forceinline__ void of(floatx4 l, floatx4 h, Frag<bf16> (&t)[COUNT]) const {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        l[i] -= (float)t[k].v[i];
-        h[i] -= (float)t[k].v[4 + i];
+    for (int k = 0; k < COUNT; ++k) {
+      t[k].v = pack8(l, h);
+      if (k + 1 < COUNT) {
+        l = mfma32(lo, t[k], l);
+        h = mfma32(hi, t[k], h);
       }
     }
   }
-}
-__device__ __forceinline__ void terms_of(const floatx4& lo, const floatx4& hi, Frag<float> (&t)[1]) { t[0] = {lo, hi}; }
+};
+template <> struct Terms<float> {
+  static constexpr int N = 1;
+  __device__ __forceinline__ Terms(int, int) {}
+  __device__ __forceinline__ void of(const floatx4& l, const floatx4& h, Frag<float> (&t)[N]) const { t[0] = {l, h}; }
+};
 
 // ---- LDS tiles: 64 token rows, PAD elements longer than they are ----------------------------
 // Rows 16 bytes apart modulo the banks suit the operand that reads sixteen rows at one place; 32 bytes the transposed one,
@@ -160,30 +174,23 @@ __device__ __forceinline__ constexpr int state_row(int nt, int g, int r) { retur
 // of y^T are 4 PT neighbouring columns, one vector.
 template <int PT> __device__ __forceinline__ constexpr int state_col(int pt, int c) { return 4 * PT * (c >> 2) + 4 * pt + (c & 3); }
 
-// x scaled by its rows' weights, in SPLIT bf16 terms: each the rounding of what the ones before it left (8, 16 or 24 bits
-// of the product); fp32 needs one.
+// x scaled by its rows' weights, in SPLIT terms.
 template <int SPLIT>
-__device__ __forceinline__ void weigh(const Frag<bf16>& x, const floatx4& w0, const floatx4& w1, Frag<bf16> (&t)[SPLIT]) {
+__device__ __forceinline__ void weigh(const Terms<bf16>& terms, const Frag<bf16>& x, const floatx4& w0, const floatx4& w1,
+                                      Frag<bf16> (&t)[SPLIT]) {
   const u32x4 xb = __builtin_bit_cast(u32x4, x.v);
-  u32x4 o[SPLIT];
+  floatx4 l, h;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {                  // pairs: one conversion makes two
-    float lo = __uint_as_float(xb[i] << 16) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
-    float hi = __uint_as_float(xb[i] & 0xffff0000u) * (i < 2 ? w0[2 * i + 1] : w1[2 * i - 3]);
-#pragma unroll
-    for (int k = 0; k < SPLIT; ++k) {
-      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-      o[k][i] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)lo, (bf16)hi});
-      if (k + 1 < SPLIT) {
-        lo -= __uint_as_float(o[k][i] << 16);
-        hi -= __uint_as_float(o[k][i] & 0xffff0000u);
-      }
-    }
+  for (int i = 0; i < 2; ++i) {
+    l[2 * i] = __uint_as_float(xb[i] << 16) * w0[2 * i];
+    l[2 * i + 1] = __uint_as_float(xb[i] & 0xffff0000u) * w0[2 * i + 1];
+    h[2 * i] = __uint_as_float(xb[2 + i] << 16) * w1[2 * i];
+    h[2 * i + 1] = __uint_as_float(xb[2 + i] & 0xffff0000u) * w1[2 * i + 1];
   }
-#pragma unroll
-  for (int k = 0; k < SPLIT; ++k) t[k].v = __builtin_bit_cast(bf16x8, o[k]);
+  terms.of(l, h, t);
 }
-__device__ __forceinline__ void weigh(const Frag<float>& x, const floatx4& w0, const floatx4& w1, Frag<float> (&t)[1]) {
+__device__ __forceinline__ void weigh(const Terms<float>&, const Frag<float>& x, const floatx4& w0, const floatx4& w1,
+                                      Frag<float> (&t)[1]) {
   t[0] = {x.lo * w0, x.hi * w1};
 }
 
@@ -429,6 +436,7 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
   static_assert(4 * PT == V, "a lane's columns of y are one vector");
   const float dd = wave_value(active && a.d ? a.d[h] : 0.f);
 
+  const Terms<E> terms(c, g);
   int slot0 = -heads;                          // of this chunk's tables
   if (first < end) {
     load_dt(first);
@@ -483,7 +491,6 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
         }
       }
       // y^T = S^T C^T
-      constexpr int TERMS = sizeof(E) == 2 ? 2 : 1;      // of an fp32 operand
       floatx4 y[PT][4];
 #pragma unroll
       for (int pt = 0; pt < PT; ++pt)
@@ -491,16 +498,16 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
         for (int ib = 0; ib < 4; ++ib) y[pt][ib] = zero4();
 #pragma unroll
       for (int kb = 0; kb < NT / 32; ++kb) {
-        Frag<E> sf[PT][TERMS];
+        Frag<E> sf[PT][Terms<E>::N];
 #pragma unroll
-        for (int pt = 0; pt < PT; ++pt) terms_of(S[2 * kb][pt], S[2 * kb + 1][pt], sf[pt]);
+        for (int pt = 0; pt < PT; ++pt) terms.of(S[2 * kb][pt], S[2 * kb + 1][pt], sf[pt]);
 #pragma unroll
         for (int ib = 0; ib < 4; ++ib) {
           const Frag<E> cf = Cs::rows(s.c, 16 * ib + c, kb, g);
 #pragma unroll
           for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-            for (int k = TERMS - 1; k >= 0; --k) y[pt][ib] = mfma32(sf[pt][k], cf, y[pt][ib]);
+            for (int k = Terms<E>::N - 1; k >= 0; --k) y[pt][ib] = mfma32(sf[pt][k], cf, y[pt][ib]);
         }
       }
       const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
@@ -534,12 +541,12 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
         }
 #pragma unroll
         for (int kb = 0; kb <= ib / 2; ++kb) {
-          Frag<E> pf[TERMS];
-          terms_of(pr[2 * kb], pr[2 * kb + 1], pf);
+          Frag<E> pf[Terms<E>::N];
+          terms.of(pr[2 * kb], pr[2 * kb + 1], pf);
 #pragma unroll
           for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-            for (int k = TERMS - 1; k >= 0; --k) y[pt][ib] = mfma32(xf[pt][kb], pf[k], y[pt][ib]);
+            for (int k = Terms<E>::N - 1; k >= 0; --k) y[pt][ib] = mfma32(xf[pt][kb], pf[k], y[pt][ib]);
         }
       }
       if (AGAIN) {                             // 0 x, summed along the tokens: NaN from a value that is not finite on
@@ -598,11 +605,11 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
     Frag<E> bf[NTS], wx[2][SPLIT];
 #pragma unroll
     for (int nt = 0; nt < NTS; ++nt) bf[nt] = Bs::template cols<8>(sb, 32 * (nt >> 1) + 4 * (nt & 1), 0, c, g);
-    weigh(xf[0][0], wt[0], wt[1], wx[0]);
+    weigh(terms, xf[0][0], wt[0], wt[1], wx[0]);
 #pragma unroll
     for (int st = 0; st < 2 * PT; ++st) {
       const int kb = st / PT, pt = st % PT, nx = st + 1;
-      if (nx < 2 * PT) weigh(xf[nx % PT][nx / PT], wt[2 * (nx / PT)], wt[2 * (nx / PT) + 1], wx[nx & 1]);
+      if (nx < 2 * PT) weigh(terms, xf[nx % PT][nx / PT], wt[2 * (nx / PT)], wt[2 * (nx / PT) + 1], wx[nx & 1]);
       if (kb == 0) {
 #pragma unroll
         for (int nt = 0; nt < NTS; ++nt) S[nt][pt] *= e;
