@@ -19,15 +19,17 @@
 // products whose weighted operand has 16 or 24 bits (SPLIT).
 // fp32 operands: fp32 matrix instructions throughout.
 //
-// Measured, bf16, N = 128, P = 64 (kernel times): 2 x 32 heads x 8192 tokens, 16 segments: states 39 us (67 MB of x and
-// 34 MB of states moved, 2.6 TB/s), sum 11.5 us (67 MB, 5.8 TB/s), outputs 58 us (170 MB, 2.9 TB/s).  Bound by the chunk
-// step, not the memory: 6 900 and 11 700 cycles a step of a workgroup, of which the matrix pipes work 3 070 and 3 700, the
-// vector port 5 000 and 6 000 and LDS 3 600 and 5 000.  Two waves share a SIMD (the states and the chunk in flight fill
-// its registers), and a wave's own vector instructions wait for its matrix instructions, so these add up more than they
-// overlap.  Measured and left out: 64 columns a wave with one wave a SIMD (states 50, outputs 75 us: the halved LDS
-// traffic is lost to moves between the register files), two workgroups of 128 columns a CU (outputs 88 us with the
-// score shared or not), 16 columns a wave (states 47 us), the waves of one SIMD in opposite phases (spills, 147 us),
-// operands fetched half a chunk ahead (states 39 us), the first chunk's loads before the state's (outputs 63 us).
+// Measured, bf16, N = 128, P = 64 (kernel times of a trace; together they take 105 us): 2 x 32 heads x 8192 tokens, 16
+// segments: states 36.5 us (67 MB of x and 34 MB of states moved, 2.8 TB/s), sum 11.2 us (67 MB, 6.0 TB/s), outputs 67 us
+// (170 MB, 2.5 TB/s).  Bound by neither the memory nor the products: with every matrix instruction taken out the states'
+// kernel takes 26 us and the outputs' 50.  A chunk step of a workgroup takes some 8 500 and 16 800 cycles, of which the
+// matrix pipes work 3 580 and 6 180, the vector port 2 990 and 6 800 and LDS 2 670 and 5 460.  The rest is waiting, which
+// two waves a SIMD (the states and the chunk in flight fill its registers) do not fill for each other: the outputs have
+// three barriers a step, and the phases between them use one of the three at a time.  Measured and left out, in times of one bf16 term for y (states 39, outputs 58 us): 64 columns a wave with one
+// wave a SIMD (states 50, outputs 75 us: the halved LDS traffic is lost to moves between the register files), two workgroups
+// of 128 columns a CU (outputs 88 us with the score shared or not), 16 columns a wave (states 47 us), the waves of one SIMD in
+// opposite phases (spills, 147 us), operands fetched half a chunk ahead (states 39 us), the first chunk's loads before the
+// state's (outputs 63 us).
 #pragma once
 
 #include "pf_gfx950.h"
@@ -100,11 +102,13 @@ template <> __device__ __forceinline__ Frag<bf16> frag_cat<bf16, bf16x4>(const b
 template <> __device__ __forceinline__ Frag<float> frag_cat<float, floatx4>(const floatx4& lo, const floatx4& hi) { return {lo, hi}; }
 
 // Two MFMA results as the operand that contracts over their 32 rows, in bf16 terms: each the rounding of what the ones before
-// it left (8, 16 or 24 bits); fp32 needs one.  A product with minus the identity takes a term off, exactly (one product and
-// zeros, which also is why a value that is not finite spoils its column, as it does in the sums to come).  The vector
-// port has more to do here than the matrix pipes: with subtractions there 2 x 32 heads x 8192 tokens took 108.5 us against 105.
-template <typename E> struct Terms;
-template <> struct Terms<bf16> {
+// it left (8, 16 or 24 bits); fp32 needs one.  A term is taken off by subtractions, or (BY_PRODUCT) by a product with minus
+// the identity, exact as well: one product and zeros.  (That also spoils the column of a value that is not finite, as the sums
+// to come do.)  Where two waves share a SIMD the vector port is the fuller one: 2 x 32 heads x 8192 tokens 108.5 us by
+// subtractions, 105.5 by products.  A wave alone on its SIMD waits for its products: 64 columns, 1 x 512 tokens whole 47
+// against 53, 128 columns, 16 x 1024 92 against 97.
+template <typename E, bool BY_PRODUCT> struct Terms;
+template <bool BY_PRODUCT> struct Terms<bf16, BY_PRODUCT> {
   static constexpr int N = 2;        // for y
   Frag<bf16> lo, hi;                 // minus the identity for the first 16 and for the second 16 of 32 rows
   __device__ __forceinline__ Terms(int c, int g) {
@@ -119,14 +123,24 @@ template <> struct Terms<bf16> {
 #pragma unroll
     for (int k = 0; k < COUNT; ++k) {
       t[k].v = pack8(l, h);
-      if (k + 1 < COUNT) {
+      if (k + 1 == COUNT) break;
+      if constexpr (BY_PRODUCT) {
         l = mfma32(lo, t[k], l);
         h = mfma32(hi, t[k], h);
+      } else {
+        const u32x4 o = __builtin_bit_cast(u32x4, t[k].v);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          l[2 * i] -= __uint_as_float(o[i] << 16);
+          l[2 * i + 1] -= __uint_as_float(o[i] & 0xffff0000u);
+          h[2 * i] -= __uint_as_float(o[2 + i] << 16);
+          h[2 * i + 1] -= __uint_as_float(o[2 + i] & 0xffff0000u);
+        }
       }
     }
   }
 };
-template <> struct Terms<float> {
+template <bool BY_PRODUCT> struct Terms<float, BY_PRODUCT> {
   static constexpr int N = 1;
   __device__ __forceinline__ Terms(int, int) {}
   __device__ __forceinline__ void of(const floatx4& l, const floatx4& h, Frag<float> (&t)[N]) const { t[0] = {l, h}; }
@@ -175,8 +189,8 @@ __device__ __forceinline__ constexpr int state_row(int nt, int g, int r) { retur
 template <int PT> __device__ __forceinline__ constexpr int state_col(int pt, int c) { return 4 * PT * (c >> 2) + 4 * pt + (c & 3); }
 
 // x scaled by its rows' weights, in SPLIT terms.
-template <int SPLIT>
-__device__ __forceinline__ void weigh(const Terms<bf16>& terms, const Frag<bf16>& x, const floatx4& w0, const floatx4& w1,
+template <typename T, int SPLIT>
+__device__ __forceinline__ void weigh(const T& terms, const Frag<bf16>& x, const floatx4& w0, const floatx4& w1,
                                       Frag<bf16> (&t)[SPLIT]) {
   const u32x4 xb = __builtin_bit_cast(u32x4, x.v);
   floatx4 l, h;
@@ -189,7 +203,8 @@ __device__ __forceinline__ void weigh(const Terms<bf16>& terms, const Frag<bf16>
   }
   terms.of(l, h, t);
 }
-__device__ __forceinline__ void weigh(const Terms<float>&, const Frag<float>& x, const floatx4& w0, const floatx4& w1,
+template <typename T>
+__device__ __forceinline__ void weigh(const T&, const Frag<float>& x, const floatx4& w0, const floatx4& w1,
                                       Frag<float> (&t)[1]) {
   t[0] = {x.lo * w0, x.hi * w1};
 }
@@ -436,7 +451,7 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
   static_assert(4 * PT == V, "a lane's columns of y are one vector");
   const float dd = wave_value(active && a.d ? a.d[h] : 0.f);
 
-  const Terms<E> terms(c, g);
+  const Terms<E, NW * 16 * PT == 256> terms(c, g);
   int slot0 = -heads;                          // of this chunk's tables
   if (first < end) {
     load_dt(first);
@@ -498,7 +513,7 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
         for (int ib = 0; ib < 4; ++ib) y[pt][ib] = zero4();
 #pragma unroll
       for (int kb = 0; kb < NT / 32; ++kb) {
-        Frag<E> sf[PT][Terms<E>::N];
+        Frag<E> sf[PT][terms.N];
 #pragma unroll
         for (int pt = 0; pt < PT; ++pt) terms.of(S[2 * kb][pt], S[2 * kb + 1][pt], sf[pt]);
 #pragma unroll
@@ -507,7 +522,7 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
 #pragma unroll
           for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-            for (int k = Terms<E>::N - 1; k >= 0; --k) y[pt][ib] = mfma32(sf[pt][k], cf, y[pt][ib]);
+            for (int k = terms.N - 1; k >= 0; --k) y[pt][ib] = mfma32(sf[pt][k], cf, y[pt][ib]);
         }
       }
       const int valid = __builtin_amdgcn_readfirstlane(min(max(len - t0, 0), Q));
@@ -541,12 +556,12 @@ __device__ __forceinline__ bool ssm_walk(const SsmArgs& a, SsmLds<E, NT, NW, PT,
         }
 #pragma unroll
         for (int kb = 0; kb <= ib / 2; ++kb) {
-          Frag<E> pf[Terms<E>::N];
+          Frag<E> pf[terms.N];
           terms.of(pr[2 * kb], pr[2 * kb + 1], pf);
 #pragma unroll
           for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-            for (int k = Terms<E>::N - 1; k >= 0; --k) y[pt][ib] = mfma32(xf[pt][kb], pf[k], y[pt][ib]);
+            for (int k = terms.N - 1; k >= 0; --k) y[pt][ib] = mfma32(xf[pt][kb], pf[k], y[pt][ib]);
         }
       }
       if (AGAIN) {                             // 0 x, summed along the tokens: NaN from a value that is not finite on

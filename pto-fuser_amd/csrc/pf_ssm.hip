@@ -28,13 +28,16 @@ int padded_rows(int N) { return N <= 64 ? 64 : 128; }
 // The segments' states lie as the waves hold them: whole blocks of columns, rows padded.
 size_t state_floats(long units, int segs, int cols, int N) { return (size_t)units * segs * cols * padded_rows(N); }
 
-// What a plan takes in microseconds, within some 15 % of what was measured (one workgroup a CU, N = 128): whole sequences a
-// fixed part and a step a chunk; segments a fixed part for three launches, a step of both kernels a chunk of a segment, the
-// sum along the segments and the traffic of their states.  A step of 64 columns takes nearly as long as one of 256 (it is
-// latency, not throughput), so wide blocks win once there are enough of them to fill the chip, narrow ones before.
-// 32 heads of 64, bf16, us at 64 / 128 / 256 columns: 1 x 512 tokens 24.3 / 24.7 / 28.9 (in segments; whole 51 / 50 / 57),
-// 4 x 2048 131 / 79 / 68 (whole 179 / 172 / 198), 16 x 256 whole 39 / 36 / 40 (two segments of 256 columns 54),
-// 16 x 1024 110 / 100 whole, 108 in two segments of 256.
+// What a plan takes in microseconds, to choose among plans by (one workgroup a CU, N = 128): whole sequences a fixed part and
+// a step a chunk; segments a fixed part for three launches, a step of both kernels a chunk of a segment, the sum along the
+// segments and the traffic of their states.  A step of 64 columns takes nearly as long as one of 256 (it is latency, not
+// throughput), so wide blocks win once there are enough of them to fill the chip, narrow ones before.  32 heads of 64, bf16,
+// us at 64 / 128 / 256 columns: 1 x 512 tokens 24.4 / 24.3 / 25.1 (8 segments; whole 46 / 47 / 57), 4 x 2048 79 / 78 / 67
+// (whole 166 / 168 / 209), 16 x 256 whole 31 / 30 / 36 (two segments of 256 columns 49), 16 x 1024 92 / 91 / 111 whole, 105 in
+// two segments of 256, 2 x 8192 133 / 133 / 105 in 8, 8 and 16 segments.
+// As a time it is right to 5 % at the long ones of these (4 x 2048 67 for 67, 16 x 1024 90 for 91, 2 x 8192 104 for 105), and not
+// elsewhere: 28 for 24 at 1 x 512, 177 for 217 at 1 x 32768 with z, which it does not know, 44 for 31 at 3 x 1471 fp32 with
+// 64 rows, which it takes for 128.
 struct SsmCost {
   int cols;
   double whole0, whole_step, seg0, seg_step;
