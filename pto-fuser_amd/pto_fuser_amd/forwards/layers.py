@@ -6,8 +6,8 @@ Two layers over the package's operators, with torch's library products for the p
   over x, B and C in place, the scan, the norm of its output in 8 bits with a scale a token, and the projection of those;
 * a gated delta rule layer — the same around the chunked forward (``gdn_chunk_forward``) and ``gdn_step``.
 
-Sequences' states live in pools; ``slots`` names them.  No counterpart in the reference, whose path ends at the chunked
-forward.
+``prefill`` returns the states after each prompt; ``step`` moves states in a pool on, which its ``slots`` name.  No
+counterpart in the reference, whose path ends at the chunked forward.
 """
 from __future__ import annotations
 
