@@ -355,6 +355,108 @@ typedef struct pf_norm_args {
 } pf_norm_args;
 int pf_norm_exec(const pf_norm_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention of a served model: causal attention over prompts, one token over a cache of keys and values in pages, and the
+ * cache's bookkeeping.  Conventions as above.  H query heads share G heads of keys and values (head h reads h / (H / G));
+ * D is a multiple of 8 up to 128; scale > 0.  A row whose tokens are none, or whose scores are all minus infinity, is zero.
+ * A page holds `page` rows, a power of two from 16 to 65536; a row of the cache is page_index * page + offset.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Causal attention over B prompts whose rows lie in one buffer: prompt b has rows cu[b] .. cu[b+1]-1 (cu [B+1] rising; cut at
+ * N), of which the first lengths[b] are live (NULL: all):
+ *   o_i = sum_{j <= i} softmax_j(scale q_i . k_j) v_j
+ * q, o [N,H,D], k, v [N,G,D].  Rows of no live token are written zero (zero_rest) or not written.  A value that is not finite
+ * reaches its own token and later ones of its prompt, as in the formula, and nothing before.
+ * q, k, v: 16-byte aligned with strides of whole 16-byte vectors; token strides of k and v up to 2^22 elements. */
+typedef struct pf_attn_args {
+  size_t size;
+  const void* q;         /* E */
+  const void* k;         /* E */
+  const void* v;         /* E */
+  void* o;               /* E */
+  const int* cu;
+  const int* lengths;
+  long long q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h;
+  int N, B, H, G, D, dtype, zero_rest;
+  float scale;
+} pf_attn_args;
+int pf_attn_exec(const pf_attn_args* args, void* stream);
+
+/* One new token of each of B sequences, q, o [B,H,D], over its lengths[b] tokens (the new one among them) in a cache
+ * k, v [pages,page,G,D].  Sequence b's pages are tables[slots[b]] (tables [S,M] contiguous; slots NULL: tables[b]); entries
+ * past its length are not read; a page outside the pool holds no tokens, nor does a slot outside it.  lengths are cut at
+ * M * page, at most 2^30.  The walk is shared out over workgroups by the lengths of all B: the same sequence alone and in a
+ * batch may differ by rounding.  workspace: pf_attn_step_workspace_bytes (arithmetic; 0: none needed, or not supported),
+ * 16-byte aligned, used by the launches of the call only.  q, k, v as above; row strides of k and v up to 2^22 elements. */
+typedef struct pf_attn_step_args {
+  size_t size;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const int* tables;
+  const int* lengths;
+  const int* slots;
+  void* workspace;
+  size_t workspace_bytes;
+  long long q_b, q_h, o_b, o_h, k_p, k_r, k_h, v_p, v_r, v_h;
+  int B, S, H, G, D, M, pages, page, dtype;
+  float scale;
+} pf_attn_step_args;
+size_t pf_attn_step_workspace_bytes(int B, int H, int G, int D, int M, int page, int dtype);
+int pf_attn_step_exec(const pf_attn_step_args* args, void* stream);
+
+/* Pages for tokens[b] (NULL: one each) new tokens of B requests that have lengths[b] in the cache, served in order: request b's
+ * next pages are free[*taken ..], entered in its table.  One whose slot is outside the pool, whose tokens pass M * page (at most
+ * 2^30) or the capacity, or whose pages are more than free (F entries) has left is not served: its rows are -1, its length
+ * stays; after one that lacked pages, none that needs any is served.
+ * rows [capacity]: the cache row of each new token, -1 of none; cu [B+1]: the requests' new tokens in them (cut at capacity);
+ * lengths_out [B], taken_out [1]: lengths and taken after the call (they may not be lengths and taken).  place [B]: scratch. */
+typedef struct pf_assign_args {
+  size_t size;
+  int* tables;
+  const int* lengths;
+  const int* tokens;
+  const int* slots;
+  const int* free;
+  const int* taken;
+  long long* rows;
+  int* cu;
+  int* lengths_out;
+  int* taken_out;
+  int* place;
+  int B, S, M, F, capacity, page;
+} pf_assign_args;
+int pf_assign_exec(const pf_assign_args* args, void* stream);
+
+/* The pages of B requests go back: free[*taken - 1] and downwards, in order of the requests and of their tables.  A request
+ * before whose pages and its own more come than were taken keeps them.  taken_out may not be taken. */
+typedef struct pf_release_args {
+  size_t size;
+  const int* tables;
+  const int* lengths;
+  const int* slots;
+  int* free;
+  const int* taken;
+  int* taken_out;
+  int B, S, M, F, page;
+} pf_release_args;
+int pf_release_exec(const pf_release_args* args, void* stream);
+
+/* k, v [N,G,D] into rows[t] of k_cache, v_cache [pages,page,G,D]; a row outside the cache is skipped, no two may be the same.
+ * D a multiple of 8 up to 65536; addresses need an element's alignment. */
+typedef struct pf_store_args {
+  size_t size;
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const long long* rows;
+  long long k_t, k_h, v_t, v_h, kc_p, kc_r, kc_h, vc_p, vc_r, vc_h;
+  int N, G, D, pages, page, dtype;
+} pf_store_args;
+int pf_store_exec(const pf_store_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,361 @@
+// Causal attention over packed prompts.  For query row i of a prompt, over its rows j <= i, with c = scale log2(e):
+//   o_i = sum_j 2^{c (q_i . k_j - m_i)} v_j / l_i,     m_i a bound of q_i . k_j so far,  l_i = sum_j 2^{..}
+// in one pass over the keys: m_i, l_i and o_i are carried, and o_i and l_i are scaled down when m_i has to grow.
+//
+// A workgroup owns BM query rows of one head and walks the keys up to its last row in tiles.  The products are made
+// transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane holds ONE query's column of S^T: the maximum and the sum over
+// keys are sums over its registers (and one swap with the other half of the wave), and the registers of P^T are at once the
+// operand of the second product (permuted K: see pf_device.h).  K and V tiles go from global memory to LDS directly, double
+// buffered, one barrier a tile.
+#pragma once
+
+#include "pf_gfx950.h"
+#include "pf_serving.h"
+
+namespace pf {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+struct AttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const int* cu;           // [B + 1]: the prompts' rows
+  const int* lengths;      // [B] or null: live rows of each
+  long q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h;
+  int N, B, H, G, D;
+  int tiles;               // of BM rows, at most, plus one or more that find none
+  int zero_rest;           // rows of no live token are written zero
+  float scale_log2;
+};
+
+__device__ __forceinline__ floatx16 zero16() {
+  floatx16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// The larger / the sum of a value in the two halves of a wave.
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ void async_load16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
+}
+
+// Rows of DP elements in LDS, their 16-byte chunks permuted by XOR with a function of the row, so that sixteen rows at one
+// chunk (the operand of S^T) and four rows at four neighbouring chunks (the transposed one of O^T) meet no bank twice.
+template <typename E, int DP> struct Rows {
+  static constexpr int V = 16 / (int)sizeof(E), RB = DP * (int)sizeof(E), CHUNKS = RB / 16;
+  __device__ __forceinline__ static int swizzle(int row) {
+    if constexpr (RB >= 256) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  }
+  __device__ __forceinline__ static int at(int row, int col) { return row * DP + ((col / V) ^ swizzle(row)) * V + col % V; }
+};
+
+constexpr float kAttnRescale = 8.f;      // log2 by which scores may pass the carried maximum before it is moved
+
+// Where a tile of the grid lies: prompt, first row within it.  Every wave works it out for itself, 64 prompts at a time.
+struct AttnTile {
+  int start, extent, len, row0;          // extent: rows up to the next prompt; len: live ones
+  int excess, first, last;               // of a tile that found none: its number among those; the rows that prompts cover
+  bool found;
+};
+
+template <int BM>
+__device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int tile) {
+  const int lane = threadIdx.x & 63;
+  AttnTile t{};
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    int start = 0, extent = 0, n = 0;
+    if (b < a.B) {
+      start = min(max(a.cu[b], 0), a.N);
+      extent = min(max(a.cu[b + 1], start), a.N) - start;
+      n = (extent + BM - 1) / BM;
+    }
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int other = __shfl_up(upto, d);
+      if (lane >= d) upto += other;
+    }
+    const unsigned long long behind = __ballot(before + upto > tile);
+    if (behind) {
+      const int l = __builtin_ctzll(behind);
+      t.found = true;
+      t.start = __builtin_amdgcn_readlane(start, l);
+      t.extent = __builtin_amdgcn_readlane(extent, l);
+      const int rank = tile - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
+      t.row0 = ((t.extent + BM - 1) / BM - 1 - rank) * BM;      // the longest first
+      t.len = t.extent;
+      if (a.lengths) t.len = min(max(__builtin_amdgcn_readfirstlane(a.lengths[b0 + l]), 0), t.extent);
+      return t;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  t.excess = tile - before;
+  t.first = min(max(a.cu[0], 0), a.N);
+  t.last = min(max(a.cu[a.B], t.first), a.N);
+  return t;
+}
+
+// Zeros in rows [from, to) of the output's head h, by a workgroup.
+template <typename E>
+__device__ __forceinline__ void zero_rows(const AttnArgs& a, int h, long from, long to, long step, long rows) {
+  for (long r0 = from; r0 < to; r0 += step) {
+    const long n = min(to - r0, rows);
+    for (long i = threadIdx.x; i < n * a.D; i += blockDim.x)
+      static_cast<E*>(a.o)[(r0 + i / a.D) * a.o_t + h * a.o_h + i % a.D] = from_f32<E>(0.f);
+  }
+}
+
+template <typename E, int DP, int BN> struct AttnLds {
+  E k[2][BN * DP], v[2][BN * DP];
+};
+
+// One workgroup's walk.  Returns whether an output came out not finite.  A value of v that is not finite reaches the queries
+// before it through the products with the zeros above the diagonal: the walk is then made AGAIN, which leaves such values of
+// the diagonal's tiles out of the products and adds them to the queries that see them.
+template <typename E, int DP, int QT, int BN, bool AGAIN>
+__device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>& s, const AttnTile& t, const int h) {
+  using R = Rows<E, DP>;
+  constexpr bool kBf = sizeof(E) == 2;
+  constexpr int NW = 4, BM = NW * 32 * QT, KT = BN / 32, DT = DP / 32, ES = sizeof(E);
+  constexpr int LOADS = BN * R::RB / 1024 / NW;      // 1 KiB each, of a wave and operand
+  constexpr int QV = DP / (kBf ? 16 : 8);            // 16-byte vectors of a lane's query
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, hf = lane >> 5;
+  const int g = h / (a.H / a.G);
+  const int q0 = t.row0 + w * 32 * QT;               // the wave's first query
+
+  const char* kg = reinterpret_cast<const char*>(static_cast<const E*>(a.k) + (long)t.start * a.k_t + g * a.k_h);
+  const char* vg = reinterpret_cast<const char*>(static_cast<const E*>(a.v) + (long)t.start * a.v_t + g * a.v_h);
+  const uint32_t kt = (uint32_t)a.k_t * ES, vt = (uint32_t)a.v_t * ES;
+  const int rows_end = min(t.row0 + BM, t.len);      // keys that any query here sees
+  const int n_tiles = (rows_end + BN - 1) / BN;
+
+  // A lane's place in the loads of a tile: row and (swizzled) chunk.  Rows past the last live one repeat it: they are masked.
+  const auto load = [&](int tile, int buf) {
+    const int j0 = tile * BN, last = t.len - 1 - j0;
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kg + (long)j0 * kt, 0x7fffffffu), rv = make_rsrc(vg + (long)j0 * vt, 0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int first = (i * NW + w) * (1024 / R::RB), row = first + lane / R::CHUNKS;
+      const int chunk = (lane % R::CHUNKS) ^ R::swizzle(row);
+      const uint32_t from = min(row, last);
+      if (chunk * R::V < a.D) {                      // columns past D stay zero
+        async_load16(rk, &s.k[buf][first * DP], from * kt + chunk * 16);
+        async_load16(rv, &s.v[buf][first * DP], from * vt + chunk * 16);
+      }
+    }
+  };
+
+  if (n_tiles > 0) load(0, 0);
+
+  // Q: a lane has row q0 + 32 qt + c; columns 16 kb + 8 hf .. (fp32: 8 kb + 4 hf ..)
+  u32x4 q[QT][QV];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const long row = t.start + min(q0 + 32 * qt + c, t.len - 1);
+    const E* p = static_cast<const E*>(a.q) + row * a.q_t + h * a.q_h;
+#pragma unroll
+    for (int kb = 0; kb < QV; ++kb) {
+      const int col = (kb * 2 + hf) * R::V;
+      q[qt][kb] = col < a.D ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{0, 0, 0, 0};
+    }
+  }
+
+  floatx16 o[QT][DT];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m[qt] = -INFINITY;
+    l[qt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[qt][dt] = zero16();
+  }
+  const float sc = a.scale_log2;
+
+  for (int tile = 0; tile < n_tiles; ++tile) {
+    const int buf = tile & 1, j0 = tile * BN;
+    __asm__ __volatile__("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt 0, lgkmcnt 0
+    __builtin_amdgcn_s_barrier();
+    __asm__ __volatile__("" ::: "memory");
+    if (tile + 1 < n_tiles) load(tile + 1, buf ^ 1);
+    const E* ks = s.k[buf];
+    const E* vs = s.v[buf];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int qa = q0 + 32 * qt;
+      if (j0 > qa + 31) continue;                    // nothing of the tile is visible to these queries
+      floatx16 st[KT];
+#pragma unroll
+      for (int kt2 = 0; kt2 < KT; ++kt2) {
+        st[kt2] = zero16();
+#pragma unroll
+        for (int kb = 0; kb < QV; ++kb) {
+          const u32x4 f = *reinterpret_cast<const u32x4*>(ks + R::at(32 * kt2 + c, (kb * 2 + hf) * R::V));
+          if constexpr (kBf) {
+            st[kt2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, q[qt][kb]),
+                                                              st[kt2], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              st[kt2] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f[i]), __uint_as_float(q[qt][kb][i]), st[kt2], 0, 0, 0);
+          }
+        }
+      }
+      const bool masked = j0 + BN - 1 > qa;
+      if (masked) {
+#pragma unroll
+        for (int kt2 = 0; kt2 < KT; ++kt2)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (j0 + 32 * kt2 + 8 * (i / 4) + 4 * hf + i % 4 > qa + c) st[kt2][i] = -INFINITY;
+      }
+      float top = st[0][0];
+#pragma unroll
+      for (int kt2 = 0; kt2 < KT; ++kt2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, st[kt2][i]);
+      top = half_max(top);
+      if (__ballot((top - m[qt]) * sc > kAttnRescale)) {       // (-inf - -inf is no number and asks for nothing)
+        const float up = fmaxf(top, m[qt]);
+        const float f = m[qt] == -INFINITY ? 0.f : pow2((m[qt] - up) * sc);
+        m[qt] = up;
+        l[qt] *= f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[qt][dt] *= f;
+      }
+      const float off = m[qt] == -INFINITY ? 0.f : m[qt] * sc;
+      float p[KT][16];
+#pragma unroll
+      for (int kt2 = 0; kt2 < KT; ++kt2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          p[kt2][i] = pow2(__builtin_fmaf(st[kt2][i], sc, -off));
+          l[qt] += p[kt2][i];
+        }
+#pragma unroll
+      for (int kt2 = 0; kt2 < KT; ++kt2) {
+        if constexpr (kBf) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            bf16x8 pb;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pb[i] = (bf16)p[kt2][8 * j + i];
+            const int row = 32 * kt2 + 16 * j + 4 * hf + ((lane & 15) >> 2);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              const int col = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+              bf16x8 vf = cat8(lds_read_tr(vs + R::at(row, col)), lds_read_tr(vs + R::at(row + 8, col)));
+              if (AGAIN && masked) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) vf[i] = __builtin_isfinite((float)vf[i]) ? vf[i] : (bf16)0.f;
+              }
+              o[qt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[qt][dt], 0, 0, 0);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int row = 32 * kt2 + 8 * (i / 4) + 4 * hf + i % 4;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              float vf = vs[R::at(row, 32 * dt + c)];
+              if (AGAIN && masked) vf = __builtin_isfinite(vf) ? vf : 0.f;
+              o[qt][dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, p[kt2][i], o[qt][dt], 0, 0, 0);
+            }
+          }
+        }
+      }
+      if (AGAIN && masked) {
+        for (int j = 0; j < BN; ++j)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float x = to_f32(vs[R::at(j, 32 * dt + 8 * (i / 4) + 4 * hf + i % 4)]);
+              if (!__builtin_isfinite(x) && j0 + j <= qa + c) o[qt][dt][i] += x;
+            }
+      }
+    }
+  }
+
+  bool bad = false;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int row = q0 + 32 * qt + c;
+    const float total = half_sum(l[qt]);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (row >= t.extent || (row >= t.len && !a.zero_rest)) continue;
+    E* p = static_cast<E*>(a.o) + (long)(t.start + row) * a.o_t + h * a.o_h;
+    typedef typename VecAny<E, 4>::T Out;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const int col = 32 * dt + 8 * i4 + 4 * hf;
+        if (col >= a.D) continue;
+        Out out;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = row < t.len ? o[qt][dt][4 * i4 + i] * inv : 0.f;
+          bad |= !__builtin_isfinite(x);
+          out[i] = from_f32<E>(x);
+        }
+        *reinterpret_cast<Out*>(p + col) = out;
+      }
+  }
+  return bad;
+}
+
+template <typename E, int DP, int QT, int BN>
+__global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
+  constexpr int BM = 128 * QT;
+  __shared__ AttnLds<E, DP, BN> s;
+  __shared__ int again;
+  // Heads vary fastest, those of keys before those that share one, and go round robin over the eight XCDs: the workgroups that
+  // read the same keys at the same time meet in few L2s.
+  const uint32_t bid = block_id(), hi = bid % (uint32_t)a.H, tile = bid / (uint32_t)a.H;
+  if (tile >= (uint32_t)a.tiles) return;
+  const int h = wave_int(hi % (uint32_t)a.G * (a.H / a.G) + hi / (uint32_t)a.G);
+  const AttnTile t = find_tile<BM>(a, wave_int(tile));
+  if (!t.found) {
+    if (!a.zero_rest) return;
+    const long each = 64, step = (long)(a.tiles - ((int)tile - t.excess)) * each;
+    zero_rows<E>(a, h, t.excess * each, t.first, step, each);
+    zero_rows<E>(a, h, t.last + t.excess * each, a.N, step, each);
+    return;
+  }
+  if (t.row0 >= t.len) {
+    if (a.zero_rest) {
+      const long r = t.start + t.row0, n = min(t.extent - t.row0, BM);
+      zero_rows<E>(a, h, r, r + n, n, n);
+    }
+    return;
+  }
+  if (a.D < DP) {                                    // columns past D
+    u32x4* z = reinterpret_cast<u32x4*>(&s);
+    for (int i = threadIdx.x; i < (int)(sizeof(s) / 16); i += 256) z[i] = u32x4{0, 0, 0, 0};
+  }
+  if (threadIdx.x == 0) again = 0;
+  __syncthreads();
+  if (attn_walk<E, DP, QT, BN, false>(a, s, t, h)) again = 1;
+  __syncthreads();
+  if (again) attn_walk<E, DP, QT, BN, true>(a, s, t, h);
+}
+
+}  // namespace pf

@@ -1,0 +1,135 @@
+// extern "C" entry points of attention over prompts and over a paged cache (declared in include/pto_fuser_hip.h): checks on
+// the host, then one launch, or two where the walk over a cache is shared out.
+#include <hip/hip_runtime.h>
+
+#include "../../include/pto_fuser_hip.h"
+#include "pf_attn.h"
+#include "pf_attn_step.h"
+#include "pf_status.h"
+
+namespace {
+
+using pf::bf16;
+
+constexpr int kMaxRows = 1 << 30;
+constexpr long long kMaxRowStride = 1LL << 22;   // elements: offsets inside a tile are 32-bit
+
+bool heads_ok(int H, int G, int D, int dtype) {
+  return H > 0 && G > 0 && H % G == 0 && H <= 65536 && D > 0 && D <= 128 && D % 8 == 0 &&
+         (dtype == PF_DTYPE_F32 || dtype == PF_DTYPE_BF16);
+}
+
+// Whole 16-byte vectors: base addresses, and strides that are multiples of one.
+template <typename... S>
+bool vectors(int dtype, const void* p, S... strides) {
+  const long long v = dtype == PF_DTYPE_BF16 ? 8 : 4;
+  return ((size_t)p & 15) == 0 && ((strides >= 0 && strides % v == 0) && ...);
+}
+
+bool grid_of(double workgroups, dim3& grid) {
+  if (workgroups > (double)pf::kGridX * (pf::kGridY - 1)) return false;
+  const long n = (long)workgroups;
+  grid = dim3((unsigned)(n < pf::kGridX ? n : pf::kGridX), (unsigned)((n + pf::kGridX - 1) / pf::kGridX));
+  return true;
+}
+
+// ---- prompts -------------------------------------------------------------------------------
+template <typename E, int DP, int QT, int BN>
+int attn_launch(pf::AttnArgs& a, hipStream_t s) {
+  constexpr int BM = 128 * QT;
+  a.tiles = a.N / BM + a.B + 1;        // a prompt's last tile is ragged; and one that finds none
+  dim3 grid;
+  if ((double)a.tiles * a.H >= 2147483648.0 || !grid_of((double)a.tiles * a.H, grid)) return PF_ERR_ARG;
+  pf::LaunchScope scope;
+  pf::attn_kernel<E, DP, QT, BN><<<grid, dim3(256), 0, s>>>(a);
+  return scope.status();
+}
+
+// ---- single tokens -------------------------------------------------------------------------
+constexpr int kStepWgs = 512;          // workgroups that share a walk: two a CU
+
+struct StepPlan {
+  int rows, wgs, blocks;
+  size_t bytes;
+};
+
+bool step_plan(int B, int H, int G, int D, int M, int page, StepPlan& p) {
+  p.blocks = (H / G + 15) / 16;
+  const double rows = (double)B * G * p.blocks, tokens = (double)M * page;
+  const double units = rows * ((tokens + pf::kStepUnit - 1) / pf::kStepUnit + 1);
+  if (tokens > kMaxRows || units >= 2147483648.0) return false;
+  p.rows = (int)rows;
+  p.wgs = tokens <= 4 * pf::kStepUnit ? 0 : (int)(units < kStepWgs ? units : kStepWgs);
+  p.bytes = (size_t)p.wgs * 2 * 16 * ((D <= 64 ? 64 : 128) + 4) * sizeof(float);
+  return true;
+}
+
+template <typename E, int DP>
+int step_launch(const pf::AttnStepArgs& a, const StepPlan& p, hipStream_t s) {
+  dim3 grid, rows;
+  if (!grid_of(p.wgs ? p.wgs : p.rows, grid) || !grid_of(p.rows, rows)) return PF_ERR_ARG;
+  pf::LaunchScope scope;
+  pf::attn_step_kernel<E, DP><<<grid, dim3(256), 0, s>>>(a);
+  if (p.wgs) pf::attn_join_kernel<E, DP><<<rows, dim3(256), 0, s>>>(a);
+  return scope.status();
+}
+
+int log2_of(int page) {
+  if (page < 16 || page > 65536 || (page & (page - 1))) return -1;
+  return __builtin_ctz((unsigned)page);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pf_attn_exec(const pf_attn_args* p, void* stream) {
+  if (!p || p->size != sizeof *p || !heads_ok(p->H, p->G, p->D, p->dtype)) return PF_ERR_ARG;
+  if (p->N < 0 || p->N > kMaxRows || p->B < 0 || p->B > kMaxRows || !p->cu || !(p->scale > 0.f)) return PF_ERR_ARG;
+  if (p->N == 0) return PF_OK;
+  if (!p->q || !p->k || !p->v || !p->o) return PF_ERR_ARG;
+  if (!vectors(p->dtype, p->q, p->q_t, p->q_h) || !vectors(p->dtype, p->k, p->k_t, p->k_h) || !vectors(p->dtype, p->v, p->v_t, p->v_h))
+    return PF_ERR_ARG;
+  if (p->k_t > kMaxRowStride || p->v_t > kMaxRowStride || p->o_t < 0 || p->o_h < 0) return PF_ERR_ARG;
+  pf::AttnArgs a{};
+  a.q = p->q; a.k = p->k; a.v = p->v; a.o = p->o; a.cu = p->cu; a.lengths = p->lengths;
+  a.q_t = p->q_t; a.q_h = p->q_h; a.k_t = p->k_t; a.k_h = p->k_h; a.v_t = p->v_t; a.v_h = p->v_h; a.o_t = p->o_t; a.o_h = p->o_h;
+  a.N = p->N; a.B = p->B; a.H = p->H; a.G = p->G; a.D = p->D; a.zero_rest = p->zero_rest;
+  a.scale_log2 = p->scale * 1.44269504088896340736f;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p->dtype == PF_DTYPE_BF16) return p->D <= 64 ? attn_launch<bf16, 64, 1, 64>(a, s) : attn_launch<bf16, 128, 1, 64>(a, s);
+  return p->D <= 64 ? attn_launch<float, 64, 1, 32>(a, s) : attn_launch<float, 128, 1, 32>(a, s);
+}
+
+size_t pf_attn_step_workspace_bytes(int B, int H, int G, int D, int M, int page, int dtype) {
+  StepPlan pl;
+  if (B <= 0 || M < 0 || !heads_ok(H, G, D, dtype) || log2_of(page) < 0 || !step_plan(B, H, G, D, M, page, pl)) return 0;
+  return pl.bytes;
+}
+
+int pf_attn_step_exec(const pf_attn_step_args* p, void* stream) {
+  if (!p || p->size != sizeof *p || !heads_ok(p->H, p->G, p->D, p->dtype) || log2_of(p->page) < 0) return PF_ERR_ARG;
+  if (p->B < 0 || p->S < 0 || p->M < 0 || p->pages < 0 || !(p->scale > 0.f) || (!p->slots && p->B > p->S)) return PF_ERR_ARG;
+  StepPlan pl;
+  if (!step_plan(p->B, p->H, p->G, p->D, p->M, p->page, pl)) return PF_ERR_ARG;
+  if (p->B == 0) return PF_OK;
+  if (!p->q || !p->o || !p->lengths || (p->pages > 0 && (!p->k || !p->v)) || (!p->tables && p->S > 0 && p->M > 0)) return PF_ERR_ARG;
+  if (!vectors(p->dtype, p->q, p->q_b, p->q_h) || !vectors(p->dtype, p->k, p->k_p, p->k_r, p->k_h) ||
+      !vectors(p->dtype, p->v, p->v_p, p->v_r, p->v_h))
+    return PF_ERR_ARG;
+  if (p->k_r > kMaxRowStride || p->v_r > kMaxRowStride || p->o_b < 0 || p->o_h < 0) return PF_ERR_ARG;
+  if (pl.bytes && (!p->workspace || p->workspace_bytes < pl.bytes || ((size_t)p->workspace & 15))) return PF_ERR_WORKSPACE;
+  pf::AttnStepArgs a{};
+  a.q = p->q; a.k = p->k; a.v = p->v; a.o = p->o; a.tables = p->tables; a.lengths = p->lengths; a.slots = p->slots;
+  a.part = static_cast<float*>(p->workspace);
+  a.q_b = p->q_b; a.q_h = p->q_h; a.o_b = p->o_b; a.o_h = p->o_h;
+  a.k_p = p->k_p; a.k_r = p->k_r; a.k_h = p->k_h; a.v_p = p->v_p; a.v_r = p->v_r; a.v_h = p->v_h;
+  a.B = p->B; a.S = p->S; a.H = p->H; a.G = p->G; a.D = p->D; a.M = p->M; a.pages = p->pages; a.page_log = log2_of(p->page);
+  a.blocks = pl.blocks; a.wgs = pl.wgs;
+  a.scale_log2 = p->scale * 1.44269504088896340736f;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p->dtype == PF_DTYPE_BF16) return p->D <= 64 ? step_launch<bf16, 64>(a, pl, s) : step_launch<bf16, 128>(a, pl, s);
+  return p->D <= 64 ? step_launch<float, 64>(a, pl, s) : step_launch<float, 128>(a, pl, s);
+}
+
+}  // extern "C"

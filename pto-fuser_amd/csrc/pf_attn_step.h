@@ -1,0 +1,318 @@
+// One new token of each of B sequences over a cache of keys and values in pages:
+//   o = sum_j 2^{c (q . k_j - m)} v_j / l over the sequence's tokens j,  c = scale log2(e),  m a bound,  l the sum of weights.
+//
+// Bound by the bytes of the cache, each read once: the R query heads that share a head of keys are the columns of one 16-wide
+// product (transposed as in pf_attn.h: S^T = K Q^T, O^T = V^T P^T).  The walk is cut evenly, whatever the lengths: the keys
+// of all sequences and heads, in units of 128, are one line of which each workgroup takes an equal run.  A (sequence, head)
+// that ends up in several workgroups leaves partial sums there, which a second kernel joins.
+#pragma once
+
+#include "pf_attn.h"
+
+namespace pf {
+
+constexpr int kStepUnit = 128;           // keys: 32 of each wave
+
+struct AttnStepArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const int* tables;       // [S, M]: a sequence's pages
+  const int* lengths;      // [B]
+  const int* slots;        // [B] or null
+  float* part;             // [2 wgs][16][DP + 2]: sums, then the bound and the weights' sum
+  long q_b, q_h, o_b, o_h, k_p, k_r, k_h, v_p, v_r, v_h;
+  int B, S, H, G, D, M, pages, page_log;
+  int blocks;              // of 16 of a group's query heads
+  int wgs;                 // that share the walk; 0: a workgroup a (sequence, head, block)
+  float scale_log2;
+};
+
+// Tokens of a sequence that the cache holds.
+__device__ __forceinline__ int cached(const AttnStepArgs& a, int b) {
+  if (a.slots) {
+    const int s = a.slots[b];
+    if (s < 0 || s >= a.S) return 0;
+  }
+  return a.pages > 0 ? (int)min((long)max(a.lengths[b], 0), (long)a.M << a.page_log) : 0;
+}
+// Its units, one of them of an empty sequence, whose output somebody has to write.
+__device__ __forceinline__ int units_of(int len) { return max((len - 1) / kStepUnit + 1, 1); }
+
+// The sequences' units on the line, 64 sequences at a time by each wave.  (The host keeps the line under 2^31 units.)
+__device__ __forceinline__ int units_before(const AttnStepArgs& a, int b) {
+  int sum = 0;
+  for (int i = threadIdx.x & 63; i < b; i += 64) sum += units_of(cached(a, i));
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
+  return wave_int(sum) * a.G * a.blocks;
+}
+// The sequence that unit x lies in, and how many units come before that.
+__device__ __forceinline__ int sequence_at(const AttnStepArgs& a, int x, int& before) {
+  const int lane = threadIdx.x & 63;
+  before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    const int n = b < a.B ? units_of(cached(a, b)) * a.G * a.blocks : 0;
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int other = __shfl_up(upto, d);
+      if (lane >= d) upto += other;
+    }
+    const unsigned long long behind = __ballot(before + upto > x);
+    if (behind) {
+      const int l = __builtin_ctzll(behind);
+      before += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
+      return b0 + l;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return a.B;
+}
+// Units of a workgroup's run.
+__device__ __forceinline__ int run_of(const AttnStepArgs& a, int total) { return (total + a.wgs - 1) / a.wgs; }
+
+template <typename E, int DP> struct StepLds {
+  static constexpr int KEYS = sizeof(E) == 2 ? 32 : 16;    // of a wave's step
+  union {
+    E v[4][2][KEYS * DP];
+    float o[4][16 * (DP + 4)];                               // the waves' sums
+  };
+  float m[4][16], l[4][16];
+};
+
+// The keys [k0, k1) of one (sequence, head, block) by a workgroup; len: the sequence's.
+template <typename E, int DP>
+__device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, DP>& s, const int b, const int g, const int hb,
+                                             const int len, const int k0, const int k1, float* part) {
+  using R = Rows<E, DP>;
+  constexpr bool kBf = sizeof(E) == 2;
+  constexpr int ES = sizeof(E), KEYS = StepLds<E, DP>::KEYS, KG = KEYS / 16, DT = DP / 16;
+  constexpr int QV = DP / (kBf ? 32 : 16);
+  constexpr int LOADS = 16 * R::RB / 1024;           // of a 16-key group of V
+  const int tid = threadIdx.x, lane = tid & 63, w = wave_int(tid >> 6), c = lane & 15, gr = lane >> 4;
+  const int share = a.H / a.G, heads = min(16, share - 16 * hb);
+  const int slot = a.slots ? a.slots[b] : b;
+  const int* table = a.tables + (long)wave_int(slot) * a.M;
+
+  u32x4 q[QV];
+  const E* qp = static_cast<const E*>(a.q) + b * a.q_b + (g * share + 16 * hb + min(c, heads - 1)) * a.q_h;
+#pragma unroll
+  for (int kb = 0; kb < QV; ++kb) {
+    const int col = (kb * 4 + gr) * R::V;
+    q[kb] = col < a.D ? *reinterpret_cast<const u32x4*>(qp + col) : u32x4{0, 0, 0, 0};
+  }
+  floatx4 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = zero4();
+  float m = -INFINITY, l = 0.f;
+  const float sc = a.scale_log2;
+  const char* kg = static_cast<const char*>(a.k) + g * a.k_h * ES;
+  const char* vg = static_cast<const char*>(a.v) + g * a.v_h * ES;
+  const uint32_t kr = (uint32_t)a.k_r * ES, vr = (uint32_t)a.v_r * ES;
+
+  int buf = 0;
+  for (int j = k0 + w * KEYS; j < k1; j += 4 * KEYS, buf ^= 1) {
+    // The groups' pages.  A group past the end, or whose page is outside the pool, takes the other's rows and weighs nothing.
+    long at[KG];
+    bool ok[KG], any = false;
+#pragma unroll
+    for (int t = 0; t < KG; ++t) {
+      const int key = j + 16 * t;
+      const int page = key < len ? wave_int(table[key >> a.page_log]) : -1;
+      ok[t] = page >= 0 && page < a.pages;
+      at[t] = page;
+      any |= ok[t];
+    }
+    if (!any) continue;
+    int from[KG];
+#pragma unroll
+    for (int t = 0; t < KG; ++t) {
+      from[t] = ok[t] ? t : KG - 1 - t;
+    }
+    u32x4 kf[KG][QV];
+    E* vs = s.v[w][buf];
+#pragma unroll
+    for (int t = 0; t < KG; ++t) {
+      const int u = from[t], key = j + 16 * u;
+      const long page = ok[t] ? at[t] : at[KG - 1 - t];
+      const int row = key & ((1 << a.page_log) - 1), last = len - 1 - key;
+      const __amdgpu_buffer_rsrc_t rk = make_rsrc(kg + (page * a.k_p + row * a.k_r) * ES, 0x7fffffffu);
+      const __amdgpu_buffer_rsrc_t rv = make_rsrc(vg + (page * a.v_p + row * a.v_r) * ES, 0x7fffffffu);
+      const uint32_t ko = min(c, last) * kr;
+#pragma unroll
+      for (int kb = 0; kb < QV; ++kb) {
+        const int col = (kb * 4 + gr) * R::V;
+        const uint4 x = col < a.D ? buf_load16(rk, ko + col * ES, 0) : make_uint4(0, 0, 0, 0);
+        kf[t][kb] = u32x4{x.x, x.y, x.z, x.w};
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int first = i * (1024 / R::RB), r = first + lane / R::CHUNKS;
+        const int chunk = (lane % R::CHUNKS) ^ R::swizzle(16 * t + r);
+        if (chunk * R::V < a.D) async_load16(rv, vs + (16 * t + first) * DP, min(r, last) * vr + chunk * 16);
+      }
+    }
+    floatx4 st[KG];
+#pragma unroll
+    for (int t = 0; t < KG; ++t) {
+      st[t] = zero4();
+#pragma unroll
+      for (int kb = 0; kb < QV; ++kb) {
+        if constexpr (kBf) {
+          st[t] = mfma_bf16(__builtin_bit_cast(bf16x8, kf[t][kb]), __builtin_bit_cast(bf16x8, q[kb]), st[t]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[t][kb][i]), __uint_as_float(q[kb][i]), st[t], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!ok[t] || j + 16 * t + 4 * gr + i >= len) st[t][i] = -INFINITY;
+    }
+    float top = st[0][0];
+#pragma unroll
+    for (int t = 0; t < KG; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, st[t][i]);
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = half_max(top);
+    if (__ballot((top - m) * sc > kAttnRescale)) {
+      const float up = fmaxf(top, m), f = m == -INFINITY ? 0.f : pow2((m - up) * sc);
+      m = up;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+    }
+    const float off = m == -INFINITY ? 0.f : m * sc;
+    floatx4 p[KG];
+#pragma unroll
+    for (int t = 0; t < KG; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[t][i] = pow2(__builtin_fmaf(st[t][i], sc, -off));
+        l += p[t][i];
+      }
+    __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      if constexpr (kBf) {
+        const int row = 4 * gr + (c >> 2), col = 16 * dt + 4 * (c & 3);
+        o[dt] = mfma_bf16(cat8(lds_read_tr(vs + R::at(row, col)), lds_read_tr(vs + R::at(row + 16, col))), pack8(p[0], p[KG - 1]), o[dt]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vs[R::at(4 * gr + i, 16 * dt + c)], p[0][i], o[dt], 0, 0, 0);
+      }
+    }
+  }
+
+  // The waves' sums over their keys, at one bound.
+  l += __shfl_xor(l, 16);
+  l = half_sum(l);
+  __syncthreads();
+  if (gr == 0) {
+    s.m[w][c] = m;
+    s.l[w][c] = l;
+  }
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<floatx4*>(&s.o[w][c * (DP + 4) + 16 * dt + 4 * gr]) = o[dt];
+  __syncthreads();
+  for (int i = tid; i < heads * (DP / 4); i += 256) {
+    const int r = i / (DP / 4), col = i % (DP / 4) * 4;
+    float up = s.m[0][r];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) up = fmaxf(up, s.m[k][r]);
+    floatx4 sum = zero4();
+    float weight = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = s.m[k][r] == -INFINITY ? 1.f : pow2((s.m[k][r] - up) * sc);
+      sum += *reinterpret_cast<const floatx4*>(&s.o[k][r * (DP + 4) + col]) * f;
+      weight += s.l[k][r] * f;
+    }
+    if (part) {
+      *reinterpret_cast<floatx4*>(part + r * (DP + 4) + col) = sum;
+      if (col == 0) {
+        part[r * (DP + 4) + DP] = up;
+        part[r * (DP + 4) + DP + 1] = weight;
+      }
+    } else if (col < a.D) {
+      const float inv = weight == 0.f ? 0.f : 1.f / weight;
+      const float out[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
+      store_vec<4>(static_cast<E*>(a.o) + b * a.o_b + (g * share + 16 * hb + r) * a.o_h + col, out);
+    }
+  }
+  __syncthreads();
+}
+
+template <int DP> __device__ __forceinline__ float* part_of(const AttnStepArgs& a, long i) { return a.part + i * 16 * (DP + 4); }
+
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void attn_step_kernel(AttnStepArgs a) {
+  __shared__ StepLds<E, DP> s;
+  const int each = a.G * a.blocks, wg = (int)block_id();
+  if (!a.wgs) {
+    const int b = wg / each, u = wg % each;
+    if (b >= a.B) return;
+    const int len = wave_int(cached(a, b));
+    step_segment<E, DP>(a, s, b, u / a.blocks, u % a.blocks, len, 0, len, nullptr);
+    return;
+  }
+  if (wg >= a.wgs) return;
+  const int total = units_before(a, a.B), per = run_of(a, total);
+  if ((long)wg * per >= total) return;
+  int x = wg * per, before;
+  const int begin = x, end = min(x + per, total);
+  int b = sequence_at(a, x, before), off = x - before;
+  while (x < end) {
+    const int len = wave_int(cached(a, b)), n = units_of(len), u = off / n, i0 = off % n, count = min(n - i0, end - x);
+    float* part = count == n ? nullptr : part_of<DP>(a, 2 * wg + (x == begin ? 0 : 1));
+    step_segment<E, DP>(a, s, b, u / a.blocks, u % a.blocks, len, i0 * kStepUnit, min(len, (i0 + count) * kStepUnit), part);
+    x += count;
+    off += count;
+    if (off == n * each) {
+      off = 0;
+      ++b;
+    }
+  }
+}
+
+// A (sequence, head, block) in several workgroups' runs: their partial sums, joined.
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnStepArgs a) {
+  const int each = a.G * a.blocks;
+  const int row = (int)block_id(), b = row / each, u = row % each;
+  if (b >= a.B) return;
+  const int n = units_of(wave_int(cached(a, b)));
+  const int per = run_of(a, units_before(a, a.B));
+  const int x0 = units_before(a, b) + u * n, w0 = x0 / per, w1 = (x0 + n - 1) / per;
+  if (w0 == w1) return;
+  const int share = a.H / a.G, g = u / a.blocks, hb = u % a.blocks, heads = min(16, share - 16 * hb);
+  const float sc = a.scale_log2;
+  // The first of them is its workgroup's last piece, unless it begins that run; in the others it is the first.
+  const int p0 = 2 * w0 + (w0 * per == x0 ? 0 : 1);
+  for (int i = threadIdx.x; i < heads * (DP / 4); i += 256) {
+    const int r = i / (DP / 4), col = i % (DP / 4) * 4;
+    float up = -INFINITY;
+    for (int w = w0; w <= w1; ++w) up = fmaxf(up, part_of<DP>(a, w == w0 ? p0 : 2 * w)[r * (DP + 4) + DP]);
+    floatx4 sum = zero4();
+    float weight = 0.f;
+    for (int w = w0; w <= w1; ++w) {
+      const float* p = part_of<DP>(a, w == w0 ? p0 : 2 * w) + r * (DP + 4);
+      const float f = p[DP] == -INFINITY ? 1.f : pow2((p[DP] - up) * sc);
+      sum += *reinterpret_cast<const floatx4*>(p + col) * f;
+      weight += p[DP + 1] * f;
+    }
+    if (col < a.D) {
+      const float inv = weight == 0.f ? 0.f : 1.f / weight;
+      const float out[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
+      store_vec<4>(static_cast<E*>(a.o) + b * a.o_b + (g * share + 16 * hb + r) * a.o_h + col, out);
+    }
+  }
+}
+
+}  // namespace pf

@@ -10,6 +10,15 @@ constexpr long kGridX = 1L << 20, kGridY = 65535;
 
 __device__ __forceinline__ long block_id() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
 
+// A value that all lanes hold, in a scalar register.  (Quotients come in vector registers, and what is made of them stays there.)
+__device__ __forceinline__ int wave_int(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float wave_value(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
+
+// 2^x of the hardware: results below 2^-126 are zero.
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // sigmoid(v) v.  exp(-v) = inf gives v * 0, so the far negative side ends in -0 and not in NaN.
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 

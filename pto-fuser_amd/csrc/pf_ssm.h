@@ -209,15 +209,6 @@ __device__ __forceinline__ void weigh(const T&, const Frag<float>& x, const floa
   t[0] = {x.lo * w0, x.hi * w1};
 }
 
-// A value that all lanes hold, in a scalar register.  (Quotients come in vector registers, and what is made of them stays there.)
-__device__ __forceinline__ int wave_int(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ float wave_value(float v) {
-  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
-}
-
-// 2^x of the hardware: results below 2^-126 are zero.
-__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
-
 // v of the lane N before (SHR) or behind (SHL) within a row of 16 lanes, zero past its end.
 template <int CTRL> __device__ __forceinline__ float row_move(float v) {
   return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));

@@ -5,9 +5,12 @@ tri-inverse and the stage kernels) and the reference's compile stack rebuilt ove
 Program IR, staged and HIP-graph executors, opaque and fused-kernel registries, gates, cost model,
 policy, transforms, templates and ``compile_program``.  ``serving`` holds the operators around the
 recurrence in a layer that is served (short convolution, state space scan, norms) and the
-recurrences' forms for single tokens.
+recurrences' forms for single tokens; ``attention`` those of the attention layers among them, over
+prompts and over a paged cache.
 """
 from . import _hip
+from .attention import (PagePlan, assign_pages, attention_step, causal_attention, release_pages,
+                        store_kv)
 from .compile import CompileResult, compile_program
 from .cost import CostModel, Features, Prediction
 from .dataflow import Dataflow, ProgramEdit
@@ -36,6 +39,7 @@ __all__ = [
     "gdn_chunk_forward", "kda_chunk_forward", "kkt_inverse", "tri_inv", "gated_qk", "qkv_flash",
     "chunk_scan",
     "causal_conv", "causal_conv_step", "ssm_chunk_forward", "ssm_step", "gdn_step", "add_rms_norm", "add_rms_norm_fp8",
+    "causal_attention", "attention_step", "assign_pages", "release_pages", "store_kv", "PagePlan",
     "TensorRef", "Node", "EinsumNode", "OpaqueNode", "VecGlueNode", "TensorOp", "FusedNode",
     "Program", "Dataflow", "ProgramEdit", "StagedExecutor", "OpaqueRegistry", "OpaqueContract",
     "default_registry", "capture_mode", "GateResult", "FusedContract", "FusedKernel",

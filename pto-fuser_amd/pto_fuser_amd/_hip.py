@@ -66,6 +66,12 @@ SIGNATURES = {
     "pf_ssm_step_exec": (c_int, [c_void_p, c_void_p]),
     "pf_gdn_step_exec": (c_int, [c_void_p, c_void_p]),
     "pf_norm_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_attn_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_attn_step_workspace_bytes": (c_size_t, [c_int] * 7),
+    "pf_attn_step_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_assign_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_release_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_store_exec": (c_int, [c_void_p, c_void_p]),
 }
 
 

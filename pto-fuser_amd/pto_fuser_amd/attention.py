@@ -1,0 +1,265 @@
+"""Attention of a served model, for the attention layers that stand among recurrent ones.
+
+* :func:`causal_attention` — a whole prompt, or several of different lengths packed into one buffer.
+* :func:`attention_step` — one new token of each running sequence over a cache of keys and values in pages.
+* :func:`assign_pages`, :func:`release_pages` — which pages of the cache new tokens take and which row each has, and back.
+* :func:`store_kv` — keys and values into those rows.
+
+No counterpart in the reference.  Forward only.  As in ``serving``: operands may be views whose innermost dimension is
+contiguous, every operator raises ``ValueError`` before launching for what it does not support, works on the current stream of
+the operands' device, and neither synchronises nor allocates anything but its outputs, scratch and operands that it has to copy.
+
+A cache is two tensors [pages, page, G, D], views allowed; a page holds a power of two of rows from 16 to 65536, and a row of
+the cache is named by page · page_size + offset.  ``tables`` [S, M] int32 holds the pages of S sequences, ``slots`` [B] int32
+names each request's row of it as it names states elsewhere (no two the same; one outside the pool has no tokens; None: row b).
+"""
+from __future__ import annotations
+
+import struct
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _hip
+from .ops import _dtype_code, _require
+from .serving import _apart, _device_of, _dim, _exec, _pool, _ptr, _require_view, _size
+
+_ATTN = struct.Struct("@N6P8q7if")
+_ATTN_STEP = struct.Struct("@N8PN10q9if")
+_ASSIGN = struct.Struct("@N11P6i")
+_RELEASE = struct.Struct("@N6P5i")
+_STORE = struct.Struct("@N5P10q6i")
+_ATTN_SIZE, _ATTN_STEP_SIZE, _ASSIGN_SIZE, _RELEASE_SIZE, _STORE_SIZE = (
+    _size(s) for s in (_ATTN, _ATTN_STEP, _ASSIGN, _RELEASE, _STORE))
+
+HEAD_MAX = 128
+ROW_MAX_STRIDE = 1 << 22
+MAX_TOKENS = 1 << 30
+
+
+def _heads(H: int, G: int, D: int) -> None:
+    if H == 0 or G == 0 or H % G or not 0 < D <= HEAD_MAX or D % 8:
+        raise ValueError(f"unsupported shape H={H} G={G} D={D} (H a multiple of G, D of 8 up to {HEAD_MAX})")
+
+
+def _scale(scale: Optional[float], D: int) -> float:
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return scale
+
+
+def _page(page: int) -> None:
+    if not 16 <= page <= 65536 or page & (page - 1):
+        raise ValueError(f"a page holds a power of two of rows from 16 to 65536, got {page}")
+
+
+def _vectors(t: torch.Tensor) -> bool:
+    """Whether ``t``'s rows are whole 16-byte vectors."""
+    each = 16 // t.element_size()
+    return t.data_ptr() % 16 == 0 and all(s % each == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
+
+
+def _strides(t: torch.Tensor):
+    """Strides of all but the last dimension, 0 where there is nothing to step to."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+
+
+def _cache(k_cache, v_cache, dtype, dev):
+    _dim(k_cache, "k_cache", 4, "[pages,page,G,D]")
+    _page(k_cache.shape[1])
+    _require_view(k_cache, "k_cache", tuple(k_cache.shape), dtype, dev)
+    _require_view(v_cache, "v_cache", tuple(k_cache.shape), dtype, dev)
+    return k_cache.shape
+
+
+def _tables(tables, slots, B: int, dev):
+    _dim(tables, "tables", 2, "[S,M]")
+    _require(tables, "tables", tuple(tables.shape), torch.int32, dev)
+    _pool(tables, slots, B, dev)
+    return tables.shape
+
+
+def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *,
+                     lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention over prompts packed in one buffer: o_i = Σ_{j≤i} softmax_j(scale · q_i·k_j) v_j within each prompt.
+
+    q [N,H,D], k and v [N,G,D], float32 or bfloat16, D a multiple of 8 up to 128, query head h reading head h // (H // G) of
+    keys and values; token and head strides are free (operands whose rows are not whole 16-byte vectors, or whose tokens lie
+    more than 2^22 elements apart, are copied first).  ``cu_seqlens`` [B+1] int32, rising: prompt b has rows cu_seqlens[b] up
+    to cu_seqlens[b+1], of which the first ``lengths[b]`` (int32; None: all) are live; a padded batch [B,T] has cu_seqlens of
+    multiples of T.  Scores, maxima and sums are held in 32 bits; with bfloat16 operands the weights enter the product with v
+    in bfloat16.  A value that is not finite reaches its own token and later ones of its prompt, and none before.
+
+    Returns o [N,H,D] in q's type.  Rows of no live token are zero, or in a given ``out`` left as they were.  ``scale``
+    (positive) is D^-1/2 by default."""
+    dev = _device_of(q, "q")
+    _dim(q, "q", 3, "[N,H,D]")
+    _dim(k, "k", 3, "[N,G,D]")
+    N, H, D = q.shape
+    G, code, dtype = k.shape[1], _dtype_code(q.dtype), q.dtype
+    _heads(H, G, D)
+    if N > MAX_TOKENS:
+        raise ValueError(f"q has {N} rows (up to {MAX_TOKENS})")
+    _require_view(q, "q", (N, H, D), dtype, dev)
+    _require_view(k, "k", (N, G, D), dtype, dev)
+    _require_view(v, "v", (N, G, D), dtype, dev)
+    _dim(cu_seqlens, "cu_seqlens", 1, "[B+1]")
+    B = cu_seqlens.shape[0] - 1
+    if B < 0:
+        raise ValueError("cu_seqlens must have an entry more than there are prompts")
+    _require(cu_seqlens, "cu_seqlens", (B + 1,), torch.int32, dev)
+    if lengths is not None:
+        _require(lengths, "lengths", (B,), torch.int32, dev)
+    scale = _scale(scale, D)
+    if out is None:
+        o = torch.empty(N, H, D, device=dev, dtype=dtype)
+    else:
+        _require_view(out, "out", (N, H, D), dtype, dev)
+        _apart("out", out, q=q, k=k, v=v, cu_seqlens=cu_seqlens, lengths=lengths)
+        o = out
+    q, k, v = (t if _vectors(t) and _strides(t)[0] <= ROW_MAX_STRIDE else t.clone(memory_format=torch.contiguous_format)
+               for t in (q, k, v))
+    _exec("pf_attn_exec", dev, _ATTN, _ATTN_SIZE, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+          cu_seqlens.data_ptr(), _ptr(lengths), *_strides(q), *_strides(k), *_strides(v), *_strides(o), N, B, H, G, D,
+          code, int(out is None), scale)
+    return o
+
+
+def attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tables: torch.Tensor,
+                   lengths: torch.Tensor, *, slots: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One new token of each of B sequences over its cache: o = Σ_j softmax_j(scale · q·k_j) v_j over its ``lengths[b]`` tokens,
+    the new one (stored before) among them.
+
+    q [B,H,D] float32 or bfloat16; k_cache, v_cache [pages,page,G,D] in its type, whole 16-byte vectors; D, H and G as in
+    :func:`causal_attention`.  Sequence b's pages are ``tables[slots[b]]``; entries past its length are not read, and a page
+    outside the cache holds no tokens.  lengths [B] int32, cut at M · page.  A sequence of no tokens gives zeros.  The keys
+    of all sequences are shared out evenly over the chip, so the same sequence alone and in a batch may differ by rounding.
+    Returns o [B,H,D] in q's type."""
+    dev = _device_of(q, "q")
+    _dim(q, "q", 3, "[B,H,D]")
+    B, H, D = q.shape
+    code, dtype = _dtype_code(q.dtype), q.dtype
+    pages, page, G, Dk = _cache(k_cache, v_cache, dtype, dev)
+    if Dk != D:
+        raise ValueError(f"k_cache has heads of {Dk}, expected {D}")
+    _heads(H, G, D)
+    _require_view(q, "q", (B, H, D), dtype, dev)
+    S, M = _tables(tables, slots, B, dev)
+    _require(lengths, "lengths", (B,), torch.int32, dev)
+    if M * page > MAX_TOKENS:
+        raise ValueError(f"tables hold {M} pages of {page} (up to {MAX_TOKENS} tokens)")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.numel() and (not _vectors(t) or _strides(t)[1] > ROW_MAX_STRIDE):
+            raise ValueError(f"{name} must be whole 16-byte vectors, its rows up to {ROW_MAX_STRIDE} elements apart")
+    scale = _scale(scale, D)
+    if out is None:
+        o = torch.empty(B, H, D, device=dev, dtype=dtype)
+    else:
+        _require_view(out, "out", (B, H, D), dtype, dev)
+        _apart("out", out, q=q, k_cache=k_cache, v_cache=v_cache, tables=tables, lengths=lengths, slots=slots)
+        o = out
+    if not _vectors(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    need = _hip.load().pf_attn_step_workspace_bytes(B, H, G, D, M, page, code)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    _exec("pf_attn_step_exec", dev, _ATTN_STEP, _ATTN_STEP_SIZE, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+          o.data_ptr(), tables.data_ptr(), lengths.data_ptr(), _ptr(slots), _ptr(ws), need, *_strides(q), *_strides(o),
+          *_strides(k_cache), *_strides(v_cache), B, S, H, G, D, M, pages, page, code, scale)
+    return o
+
+
+class PagePlan(NamedTuple):
+    """Where the new tokens of a step or of arriving prompts go."""
+    rows: torch.Tensor          # [capacity] int64: the cache row of each new token, -1 of none
+    cu_seqlens: torch.Tensor    # [B+1] int32: the requests' new tokens among them
+    lengths: torch.Tensor       # [B] int32: tokens of each request in the cache, the new ones among them
+    taken: torch.Tensor         # [1] int32: pages taken from the pool
+
+
+def _pool_state(tables, lengths, free, taken, slots, page_size: int, dev):
+    _page(page_size)
+    _dim(lengths, "lengths", 1, "[B]")
+    B = lengths.shape[0]
+    _require(lengths, "lengths", (B,), torch.int32, dev)
+    S, M = _tables(tables, slots, B, dev)
+    if M * page_size > MAX_TOKENS:
+        raise ValueError(f"tables hold {M} pages of {page_size} (up to {MAX_TOKENS} tokens)")
+    _dim(free, "free", 1, "[F]")
+    _require(free, "free", tuple(free.shape), torch.int32, dev)
+    _require(taken, "taken", (1,), torch.int32, dev)
+    return B, S, M, free.shape[0]
+
+
+def assign_pages(tables: torch.Tensor, lengths: torch.Tensor, tokens: Optional[torch.Tensor], free: torch.Tensor,
+                 taken: torch.Tensor, *, page_size: int, capacity: Optional[int] = None,
+                 slots: Optional[torch.Tensor] = None) -> PagePlan:
+    """Pages and cache rows for the new tokens of B requests, without the host knowing their lengths.
+
+    ``lengths`` [B] int32: tokens of each request that the cache holds; ``tokens`` [B] int32: new ones of each (None: one
+    each, a decoding step).  Pages are taken from ``free`` [F] int32 at ``taken`` [1] int32 on, for the requests in their
+    order, and entered in ``tables`` (in place).  ``capacity`` (by default B, for a step): rows that the new tokens are
+    packed into.
+
+    A request is served whole or not at all: not where its slot is outside the pool, its tokens pass its table or the
+    capacity, or its pages are more than the pool has left (after which no request that needs any is served).  Its rows are
+    then -1, its length stays, and :func:`store_kv` skips it.  Returns a :class:`PagePlan`; lengths and taken are new tensors,
+    which the caller passes on the next time."""
+    dev = _device_of(tables, "tables")
+    B, S, M, F = _pool_state(tables, lengths, free, taken, slots, page_size, dev)
+    if tokens is not None:
+        _require(tokens, "tokens", (B,), torch.int32, dev)
+    if capacity is None:
+        if tokens is not None:
+            raise ValueError("capacity must be given with tokens")
+        capacity = B
+    if not 0 <= capacity <= MAX_TOKENS:
+        raise ValueError(f"capacity must be 0 to {MAX_TOKENS}, got {capacity}")
+    _apart("tables", tables, lengths=lengths, tokens=tokens, free=free, taken=taken, slots=slots)
+    rows = torch.empty(capacity, device=dev, dtype=torch.int64)
+    ints = torch.empty(3 * B + 2, device=dev, dtype=torch.int32)
+    cu, after, taken_after, place = ints.split([B + 1, B, 1, B])
+    _exec("pf_assign_exec", dev, _ASSIGN, _ASSIGN_SIZE, tables.data_ptr(), lengths.data_ptr(), _ptr(tokens), _ptr(slots),
+          free.data_ptr(), taken.data_ptr(), rows.data_ptr(), cu.data_ptr(), after.data_ptr(), taken_after.data_ptr(),
+          place.data_ptr(), B, S, M, F, capacity, page_size)
+    return PagePlan(rows, cu, after, taken_after)
+
+
+def release_pages(tables: torch.Tensor, lengths: torch.Tensor, free: torch.Tensor, taken: torch.Tensor, *, page_size: int,
+                  slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The pages of B requests that leave go back to ``free`` (in place), below ``taken``; returns taken afterwards [1].
+
+    ``lengths`` [B] int32: tokens that each request holds, whose pages its table names; the caller sets them to 0.  A
+    request is refused, and keeps its pages, where more would come back than were taken."""
+    dev = _device_of(tables, "tables")
+    B, S, M, F = _pool_state(tables, lengths, free, taken, slots, page_size, dev)
+    _apart("free", free, tables=tables, lengths=lengths, taken=taken, slots=slots)
+    after = torch.empty(1, device=dev, dtype=torch.int32)
+    _exec("pf_release_exec", dev, _RELEASE, _RELEASE_SIZE, tables.data_ptr(), lengths.data_ptr(), _ptr(slots),
+          free.data_ptr(), taken.data_ptr(), after.data_ptr(), B, S, M, F, page_size)
+    return after
+
+
+def store_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, rows: torch.Tensor) -> None:
+    """Keys and values k, v [N,G,D] of N tokens into their rows of the cache [pages,page,G,D] (in place), all of one type.
+
+    ``rows`` [N] int64, as :func:`assign_pages` gives them: one outside the cache (-1) is skipped, no two others are the same.
+    float32 or bfloat16, D a multiple of 8; token and head strides of k and v are free."""
+    dev = _device_of(k, "k")
+    _dim(k, "k", 3, "[N,G,D]")
+    N, G, D = k.shape
+    code, dtype = _dtype_code(k.dtype), k.dtype
+    if not 0 < G <= 65536 or not 0 < D <= 65536 or D % 8:
+        raise ValueError(f"unsupported shape G={G} D={D} (D a multiple of 8; both up to 65536)")
+    _require_view(k, "k", (N, G, D), dtype, dev)
+    _require_view(v, "v", (N, G, D), dtype, dev)
+    pages, page, Gc, Dc = _cache(k_cache, v_cache, dtype, dev)
+    if (Gc, Dc) != (G, D):
+        raise ValueError(f"k_cache has {Gc} heads of {Dc}, expected {G} of {D}")
+    _require(rows, "rows", (N,), torch.int64, dev)
+    _apart("k_cache", k_cache, k=k, v=v, v_cache=v_cache, rows=rows)
+    _apart("v_cache", v_cache, k=k, v=v, rows=rows)
+    _exec("pf_store_exec", dev, _STORE, _STORE_SIZE, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+          rows.data_ptr(), *_strides(k), *_strides(v), *_strides(k_cache), *_strides(v_cache), N, G, D, pages, page, code)
