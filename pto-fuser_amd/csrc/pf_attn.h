@@ -12,6 +12,8 @@
 #include "pf_gfx950.h"
 #include "pf_serving.h"
 
+#include <type_traits>
+
 namespace pf {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
@@ -47,16 +49,49 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-__device__ __forceinline__ void async_load16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
+// Loads from global memory to LDS, N of 1 KiB each by a wave, 16 bytes a lane in order of the lanes, APART bytes of LDS from one
+// to the next.  In assembly, since the compiler would wait for all of them before the next read of LDS, whatever buffer that is
+// of; the caller waits (wait_loads) before it reads what they bring.  They write no register.  (s_nop: the distance from a
+// scalar that a vector instruction has just written, and from m0, to a load.)
+template <int N, int APART>
+__device__ __forceinline__ void async_loads(const void* base, uint32_t lds, const uint32_t (&off)[N]) {
+  const uint64_t at = (uint64_t)base;
+  const u32x4 r = {(uint32_t)wave_int((int)at), (uint32_t)wave_int((int)(at >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
+  const uint32_t m = (uint32_t)wave_int((int)lds);
+  if constexpr (N == 4) {
+    __asm__ __volatile__(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds\n\t"
+        "s_add_u32 m0, %0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %1, 0 offen lds\n\t"
+        "s_add_u32 m0, %0, %7\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %1, 0 offen lds\n\t"
+        "s_add_u32 m0, %0, %8\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %1, 0 offen lds"
+        :: "s"(m), "s"(r), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "n"(APART), "n"(2 * APART), "n"(3 * APART)
+        : "memory", "m0", "scc");
+  } else {
+    static_assert(N == 2, "two or four loads");
+    __asm__ __volatile__(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds\n\t"
+        "s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %1, 0 offen lds"
+        :: "s"(m), "s"(r), "v"(off[0]), "v"(off[1]), "n"(APART) : "memory", "m0", "scc");
+  }
+}
+// All of them, and this wave's reads of LDS.
+__device__ __forceinline__ void wait_loads() {
+  __asm__ __volatile__("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);                // vmcnt 0, lgkmcnt 0
+  __asm__ __volatile__("" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
 
 // Rows of DP elements in LDS, their 16-byte chunks permuted by XOR with a function of the row, so that sixteen rows at one
 // chunk (the operand of S^T) and four rows at four neighbouring chunks (the transposed one of O^T) meet no bank twice.
 template <typename E, int DP> struct Rows {
   static constexpr int V = 16 / (int)sizeof(E), RB = DP * (int)sizeof(E), CHUNKS = RB / 16;
-  __device__ __forceinline__ static int swizzle(int row) {
-    if constexpr (RB >= 256) return ((row & 3) << 2) | ((row >> 2) & 3);
+  __device__ __forceinline__ static constexpr int swizzle(int row) {
+    if constexpr (RB > 256) return ((row & 3) << 2) | ((row >> 2) & 1);     // (fp32: twice is no loss beside its products)
+    if constexpr (RB == 256) return ((row & 3) << 2) | ((row >> 2) & 3);
     else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
   }
   __device__ __forceinline__ static int at(int row, int col) { return row * DP + ((col / V) ^ swizzle(row)) * V + col % V; }
@@ -113,8 +148,10 @@ __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int tile) {
 // Zeros in rows [from, to) of the output's head h, by a workgroup.
 template <typename E>
 __device__ __forceinline__ void zero_rows(const AttnArgs& a, int h, long from, long to, long step, long rows) {
+#pragma unroll 1
   for (long r0 = from; r0 < to; r0 += step) {
     const long n = min(to - r0, rows);
+#pragma unroll 1
     for (long i = threadIdx.x; i < n * a.D; i += blockDim.x)
       static_cast<E*>(a.o)[(r0 + i / a.D) * a.o_t + h * a.o_h + i % a.D] = from_f32<E>(0.f);
   }
@@ -136,7 +173,7 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
   constexpr int QV = DP / (kBf ? 16 : 8);            // 16-byte vectors of a lane's query
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hf = lane >> 5;
-  const int g = h / (a.H / a.G);
+  const int g = wave_int(h / (a.H / a.G));
   const int q0 = t.row0 + w * 32 * QT;               // the wave's first query
 
   const char* kg = reinterpret_cast<const char*>(static_cast<const E*>(a.k) + (long)t.start * a.k_t + g * a.k_h);
@@ -145,19 +182,34 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
   const int rows_end = min(t.row0 + BM, t.len);      // keys that any query here sees
   const int n_tiles = (rows_end + BN - 1) / BN;
 
-  // A lane's place in the loads of a tile: row and (swizzled) chunk.  Rows past the last live one repeat it: they are masked.
+  // A lane's place in the loads of a tile: row and (swizzled) chunk, the same chunk for all LOADS.  Rows past the last live one
+  // repeat it: they are masked.  Lanes whose columns lie past D stay out, and what they would fill stays zero.
+  constexpr int FIRST = 1024 / R::RB;                // rows of a load
+  const int l_row = w * FIRST + lane / R::CHUNKS, l_chunk = (lane % R::CHUNKS) ^ R::swizzle(l_row);
+  static_assert(R::swizzle(NW * FIRST) == 0, "the swizzle is the same for a lane's rows");
+  const uint32_t k_lds = lds_address(s.k[0]) + w * 1024, v_lds = lds_address(s.v[0]) + w * 1024;
+  uint32_t k_off[LOADS], v_off[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    k_off[i] = (l_row + i * NW * FIRST) * kt + l_chunk * 16;
+    v_off[i] = (l_row + i * NW * FIRST) * vt + l_chunk * 16;
+  }
   const auto load = [&](int tile, int buf) {
     const int j0 = tile * BN, last = t.len - 1 - j0;
-    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kg + (long)j0 * kt, 0x7fffffffu), rv = make_rsrc(vg + (long)j0 * vt, 0x7fffffffu);
+    if (l_chunk * R::V >= a.D) return;
+    if (last >= BN - 1) {
+      async_loads<LOADS, NW * 1024>(kg + (long)j0 * kt, k_lds + buf * BN * R::RB, k_off);
+      async_loads<LOADS, NW * 1024>(vg + (long)j0 * vt, v_lds + buf * BN * R::RB, v_off);
+    } else {
+      uint32_t ko[LOADS], vo[LOADS];
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int first = (i * NW + w) * (1024 / R::RB), row = first + lane / R::CHUNKS;
-      const int chunk = (lane % R::CHUNKS) ^ R::swizzle(row);
-      const uint32_t from = min(row, last);
-      if (chunk * R::V < a.D) {                      // columns past D stay zero
-        async_load16(rk, &s.k[buf][first * DP], from * kt + chunk * 16);
-        async_load16(rv, &s.v[buf][first * DP], from * vt + chunk * 16);
+      for (int i = 0; i < LOADS; ++i) {
+        const uint32_t row = min(l_row + i * NW * FIRST, last);
+        ko[i] = row * kt + l_chunk * 16;
+        vo[i] = row * vt + l_chunk * 16;
       }
+      async_loads<LOADS, NW * 1024>(kg + (long)j0 * kt, k_lds + buf * BN * R::RB, ko);
+      async_loads<LOADS, NW * 1024>(vg + (long)j0 * vt, v_lds + buf * BN * R::RB, vo);
     }
   };
 
@@ -187,10 +239,10 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
   }
   const float sc = a.scale_log2;
 
-  for (int tile = 0; tile < n_tiles; ++tile) {
-    const int buf = tile & 1, j0 = tile * BN;
-    __asm__ __volatile__("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt 0, lgkmcnt 0
+  const auto step = [&](const int tile, auto parity) {
+    constexpr int buf = decltype(parity)::value;
+    const int j0 = tile * BN;
+    wait_loads();
     __builtin_amdgcn_s_barrier();
     __asm__ __volatile__("" ::: "memory");
     if (tile + 1 < n_tiles) load(tile + 1, buf ^ 1);
@@ -292,6 +344,10 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
             }
       }
     }
+  };
+  for (int tile = 0; tile < n_tiles; tile += 2) {    // (twice, so that the buffers' addresses are constants)
+    step(tile, std::integral_constant<int, 0>{});
+    if (tile + 1 < n_tiles) step(tile + 1, std::integral_constant<int, 1>{});
   }
 
   bool bad = false;
@@ -323,7 +379,7 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
 }
 
 template <typename E, int DP, int QT, int BN>
-__global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   constexpr int BM = 128 * QT;
   __shared__ AttnLds<E, DP, BN> s;
   __shared__ int again;

@@ -152,7 +152,9 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
       for (int i = 0; i < LOADS; ++i) {
         const int first = i * (1024 / R::RB), r = first + lane / R::CHUNKS;
         const int chunk = (lane % R::CHUNKS) ^ R::swizzle(16 * t + r);
-        if (chunk * R::V < a.D) async_load16(rv, vs + (16 * t + first) * DP, min(r, last) * vr + chunk * 16);
+        if (chunk * R::V < a.D)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(vs + (16 * t + first) * DP), 16,
+                                                   min(r, last) * vr + chunk * 16, 0, 0, 0);
       }
     }
     floatx4 st[KG];
