@@ -81,6 +81,14 @@ __device__ __forceinline__ void wait_loads() {
   __asm__ __volatile__("" ::: "memory");
 }
 
+// All but the last N.
+template <int N> __device__ __forceinline__ void wait_all_but() {
+  static_assert(N < 64, "six bits");
+  __asm__ __volatile__("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+  __asm__ __volatile__("" ::: "memory");
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }

@@ -46,7 +46,7 @@ int attn_launch(pf::AttnArgs& a, hipStream_t s) {
 }
 
 // ---- single tokens -------------------------------------------------------------------------
-constexpr int kStepWgs = 512;          // workgroups that share a walk: two a CU
+constexpr int kStepWgs = 512;          // workgroups that share a walk: two a CU, which their LDS fills (heads up to 64: four)
 
 struct StepPlan {
   int rows, wgs, blocks;
@@ -59,7 +59,8 @@ bool step_plan(int B, int H, int G, int D, int M, int page, StepPlan& p) {
   const double units = rows * ((tokens + pf::kStepUnit - 1) / pf::kStepUnit + 1);
   if (tokens > kMaxRows || units >= 2147483648.0) return false;
   p.rows = (int)rows;
-  p.wgs = tokens <= 4 * pf::kStepUnit ? 0 : (int)(units < kStepWgs ? units : kStepWgs);
+  const double wgs = D <= 64 ? 2 * kStepWgs : kStepWgs;
+  p.wgs = tokens <= 512 ? 0 : (int)(units < wgs ? units : wgs);
   p.bytes = (size_t)p.wgs * 2 * 16 * ((D <= 64 ? 64 : 128) + 4) * sizeof(float);
   return true;
 }
@@ -67,9 +68,9 @@ bool step_plan(int B, int H, int G, int D, int M, int page, StepPlan& p) {
 template <typename E, int DP>
 int step_launch(const pf::AttnStepArgs& a, const StepPlan& p, hipStream_t s) {
   dim3 grid, rows;
-  if (!grid_of(p.wgs ? p.wgs : p.rows, grid) || !grid_of(p.rows, rows)) return PF_ERR_ARG;
+  if (!grid_of(p.wgs ? p.wgs : p.rows, grid) || !grid_of((double)a.B * a.H, rows)) return PF_ERR_ARG;
   pf::LaunchScope scope;
-  pf::attn_step_kernel<E, DP><<<grid, dim3(256), 0, s>>>(a);
+  pf::attn_step_kernel<E, DP><<<grid, dim3(64 * pf::kStepWaves), 0, s>>>(a);
   if (p.wgs) pf::attn_join_kernel<E, DP><<<rows, dim3(256), 0, s>>>(a);
   return scope.status();
 }

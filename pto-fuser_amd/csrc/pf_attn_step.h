@@ -11,7 +11,8 @@
 
 namespace pf {
 
-constexpr int kStepUnit = 128;           // keys: 32 of each wave
+constexpr int kStepWaves = 2;
+constexpr int kStepUnit = 32 * kStepWaves;           // keys: 32 of each wave
 
 struct AttnStepArgs {
   const void* q;
@@ -76,11 +77,12 @@ __device__ __forceinline__ int run_of(const AttnStepArgs& a, int total) { return
 
 template <typename E, int DP> struct StepLds {
   static constexpr int KEYS = sizeof(E) == 2 ? 32 : 16;    // of a wave's step
+  E k[kStepWaves][2][KEYS * DP];
   union {
-    E v[4][2][KEYS * DP];
-    float o[4][16 * (DP + 4)];                               // the waves' sums
+    E v[kStepWaves][2][KEYS * DP];
+    float o[kStepWaves][16 * (DP + 4)];                      // the waves' sums
   };
-  float m[4][16], l[4][16];
+  float m[kStepWaves][16], l[kStepWaves][16];
 };
 
 // The keys [k0, k1) of one (sequence, head, block) by a workgroup; len: the sequence's.
@@ -91,11 +93,13 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
   constexpr bool kBf = sizeof(E) == 2;
   constexpr int ES = sizeof(E), KEYS = StepLds<E, DP>::KEYS, KG = KEYS / 16, DT = DP / 16;
   constexpr int QV = DP / (kBf ? 32 : 16);
-  constexpr int LOADS = 16 * R::RB / 1024;           // of a 16-key group of V
+  constexpr int FIRST = 1024 / R::RB, LOADS = 16 / FIRST;   // rows of a load; loads of a 16-key group
+  constexpr int N = LOADS > 4 ? 4 : LOADS;
   const int tid = threadIdx.x, lane = tid & 63, w = wave_int(tid >> 6), c = lane & 15, gr = lane >> 4;
   const int share = a.H / a.G, heads = min(16, share - 16 * hb);
-  const int slot = a.slots ? a.slots[b] : b;
-  const int* table = a.tables + (long)wave_int(slot) * a.M;
+  const int slot = wave_int(a.slots ? a.slots[b] : b);
+  // (through the scalar cache, whose loads are not counted with those of keys and values)
+  const auto* table = (const __attribute__((address_space(4))) int*)(a.tables + (long)slot * a.M);
 
   u32x4 q[QV];
   const E* qp = static_cast<const E*>(a.q) + b * a.q_b + (g * share + 16 * hb + min(c, heads - 1)) * a.q_h;
@@ -113,67 +117,90 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
   const char* vg = static_cast<const char*>(a.v) + g * a.v_h * ES;
   const uint32_t kr = (uint32_t)a.k_r * ES, vr = (uint32_t)a.v_r * ES;
 
-  int buf = 0;
-  for (int j = k0 + w * KEYS; j < k1; j += 4 * KEYS, buf ^= 1) {
-    // The groups' pages.  A group past the end, or whose page is outside the pool, takes the other's rows and weighs nothing.
-    long at[KG];
-    bool ok[KG], any = false;
+  // A lane's place in a group's loads.  Columns past D repeat the first ones; they are left out where K is read.
+  uint32_t l_row[LOADS], l_chunk[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    l_row[i] = i * FIRST + lane / R::CHUNKS;
+    l_chunk[i] = (lane % R::CHUNKS) ^ R::swizzle(l_row[i]);
+    if ((int)l_chunk[i] * R::V >= a.D) l_chunk[i] = 0;
+  }
+
+  struct Stage {
+    int j;
+    bool ok[KG], any;
+  };
+  // The pages of a step's groups: -1 past the sequence's end and where a page is outside the pool.
+  const auto entries = [&](int j, int (&page)[KG]) {
 #pragma unroll
     for (int t = 0; t < KG; ++t) {
       const int key = j + 16 * t;
-      const int page = key < len ? wave_int(table[key >> a.page_log]) : -1;
-      ok[t] = page >= 0 && page < a.pages;
-      at[t] = page;
-      any |= ok[t];
+      page[t] = key < len ? table[key >> a.page_log] : -1;
+      if (page[t] >= a.pages) page[t] = -1;
     }
-    if (!any) continue;
-    int from[KG];
+  };
+  // A step's loads.  A group without a page takes the rows of the other, and weighs nothing; without either, page 0's.
+  const auto issue = [&](int j, const int (&page)[KG], int buf, Stage& st) {
+    st.j = j;
+    st.any = false;
 #pragma unroll
     for (int t = 0; t < KG; ++t) {
-      from[t] = ok[t] ? t : KG - 1 - t;
+      st.ok[t] = page[t] >= 0;
+      st.any |= st.ok[t];
     }
-    u32x4 kf[KG][QV];
-    E* vs = s.v[w][buf];
+    __builtin_amdgcn_s_waitcnt(0xc07f);              // this wave's reads of the buffer
 #pragma unroll
     for (int t = 0; t < KG; ++t) {
-      const int u = from[t], key = j + 16 * u;
-      const long page = ok[t] ? at[t] : at[KG - 1 - t];
-      const int row = key & ((1 << a.page_log) - 1), last = len - 1 - key;
-      const __amdgpu_buffer_rsrc_t rk = make_rsrc(kg + (page * a.k_p + row * a.k_r) * ES, 0x7fffffffu);
-      const __amdgpu_buffer_rsrc_t rv = make_rsrc(vg + (page * a.v_p + row * a.v_r) * ES, 0x7fffffffu);
-      const uint32_t ko = min(c, last) * kr;
-#pragma unroll
-      for (int kb = 0; kb < QV; ++kb) {
-        const int col = (kb * 4 + gr) * R::V;
-        const uint4 x = col < a.D ? buf_load16(rk, ko + col * ES, 0) : make_uint4(0, 0, 0, 0);
-        kf[t][kb] = u32x4{x.x, x.y, x.z, x.w};
-      }
+      const int u = st.ok[t] ? t : KG - 1 - t, key = j + 16 * u;
+      const long p = st.any ? page[st.ok[t] ? t : KG - 1 - t] : 0;
+      const int row = st.any ? key & ((1 << a.page_log) - 1) : 0, last = st.any ? len - 1 - key : 15;
+      const char* kp = kg + (p * a.k_p + row * a.k_r) * ES;
+      const char* vp = vg + (p * a.v_p + row * a.v_r) * ES;
+      uint32_t ko[LOADS], vo[LOADS];
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int first = i * (1024 / R::RB), r = first + lane / R::CHUNKS;
-        const int chunk = (lane % R::CHUNKS) ^ R::swizzle(16 * t + r);
-        if (chunk * R::V < a.D)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(vs + (16 * t + first) * DP), 16,
-                                                   min(r, last) * vr + chunk * 16, 0, 0, 0);
+        const uint32_t r = min((int)l_row[i], last);
+        ko[i] = r * kr + l_chunk[i] * 16;
+        vo[i] = r * vr + l_chunk[i] * 16;
+      }
+      const uint32_t kl = lds_address(&s.k[w][buf][16 * t * DP]), vl = lds_address(&s.v[w][buf][16 * t * DP]);
+#pragma unroll
+      for (int i = 0; i < LOADS; i += N) {
+        uint32_t kn[N], vn[N];
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+          kn[x] = ko[i + x];
+          vn[x] = vo[i + x];
+        }
+        async_loads<N, 1024>(kp, kl + i * 1024, kn);
+        async_loads<N, 1024>(vp, vl + i * 1024, vn);
       }
     }
+  };
+
+  const auto compute = [&](const Stage& stage, int buf) {
+    if (!stage.any) return;
+    const E* ks = s.k[w][buf];
+    const E* vs = s.v[w][buf];
     floatx4 st[KG];
 #pragma unroll
     for (int t = 0; t < KG; ++t) {
       st[t] = zero4();
 #pragma unroll
       for (int kb = 0; kb < QV; ++kb) {
+        u32x4 f = *reinterpret_cast<const u32x4*>(ks + R::at(16 * t + c, (kb * 4 + gr) * R::V));
+        if ((kb * 4 + gr) * R::V >= a.D) f = u32x4{0, 0, 0, 0};
         if constexpr (kBf) {
-          st[t] = mfma_bf16(__builtin_bit_cast(bf16x8, kf[t][kb]), __builtin_bit_cast(bf16x8, q[kb]), st[t]);
+          st[t] = mfma_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, q[kb]), st[t]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[t][kb][i]), __uint_as_float(q[kb][i]), st[t], 0, 0, 0);
+            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f[i]), __uint_as_float(q[kb][i]), st[t], 0, 0, 0);
         }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (!ok[t] || j + 16 * t + 4 * gr + i >= len) st[t][i] = -INFINITY;
+        if (!stage.ok[t] || stage.j + 16 * t + 4 * gr + i >= len) st[t][i] = -INFINITY;
     }
     float top = st[0][0];
 #pragma unroll
@@ -198,7 +225,6 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
         p[t][i] = pow2(__builtin_fmaf(st[t][i], sc, -off));
         l += p[t][i];
       }
-    __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       if constexpr (kBf) {
@@ -210,12 +236,36 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
           o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vs[R::at(4 * gr + i, 16 * dt + c)], p[0][i], o[dt], 0, 0, 0);
       }
     }
+  };
+
+  // Two steps in flight: while one is worked on the next is loaded, whose pages were asked for a step before.
+  const int first = k0 + w * KEYS, count = first < k1 ? (k1 - first + kStepWaves * KEYS - 1) / (kStepWaves * KEYS) : 0;
+  if (count > 0) {
+    int page[KG];
+    Stage now, next;
+    entries(first, page);
+    wait_loads();                                    // (the query: the compiler counts its own loads)
+    issue(first, page, 0, now);
+    if (count > 1) entries(first + kStepWaves * KEYS, page);
+    for (int i = 0; i < count; ++i) {
+      const int buf = i & 1;
+      if (i + 1 < count) {
+        const int j = first + (i + 1) * kStepWaves * KEYS;
+        issue(j, page, buf ^ 1, next);
+        if (i + 2 < count) entries(j + kStepWaves * KEYS, page);
+        wait_all_but<2 * KG * LOADS>();
+      } else {
+        wait_all_but<0>();
+      }
+      compute(now, buf);
+      now = next;
+    }
   }
 
   // The waves' sums over their keys, at one bound.
   l += __shfl_xor(l, 16);
   l = half_sum(l);
-  __syncthreads();
+  __syncthreads();                                   // (the sums take the place of V)
   if (gr == 0) {
     s.m[w][c] = m;
     s.l[w][c] = l;
@@ -223,15 +273,15 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<floatx4*>(&s.o[w][c * (DP + 4) + 16 * dt + 4 * gr]) = o[dt];
   __syncthreads();
-  for (int i = tid; i < heads * (DP / 4); i += 256) {
+  for (int i = tid; i < heads * (DP / 4); i += 64 * kStepWaves) {
     const int r = i / (DP / 4), col = i % (DP / 4) * 4;
     float up = s.m[0][r];
 #pragma unroll
-    for (int k = 1; k < 4; ++k) up = fmaxf(up, s.m[k][r]);
+    for (int k = 1; k < kStepWaves; ++k) up = fmaxf(up, s.m[k][r]);
     floatx4 sum = zero4();
     float weight = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kStepWaves; ++k) {
       const float f = s.m[k][r] == -INFINITY ? 1.f : pow2((s.m[k][r] - up) * sc);
       sum += *reinterpret_cast<const floatx4*>(&s.o[k][r * (DP + 4) + col]) * f;
       weight += s.l[k][r] * f;
@@ -254,7 +304,7 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
 template <int DP> __device__ __forceinline__ float* part_of(const AttnStepArgs& a, long i) { return a.part + i * 16 * (DP + 4); }
 
 template <typename E, int DP>
-__global__ __launch_bounds__(256) void attn_step_kernel(AttnStepArgs a) {
+__global__ __launch_bounds__(64 * kStepWaves) void attn_step_kernel(AttnStepArgs a) {
   __shared__ StepLds<E, DP> s;
   const int each = a.G * a.blocks, wg = (int)block_id();
   if (!a.wgs) {
@@ -283,37 +333,58 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnStepArgs a) {
   }
 }
 
-// A (sequence, head, block) in several workgroups' runs: their partial sums, joined.
+// A query head of a (sequence, head, block) that lies in several workgroups' runs: their partial sums, joined.  The parts are
+// shared out over eight groups of lanes, each of which holds a row, and the groups' sums meet in LDS.
 template <typename E, int DP>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnStepArgs a) {
-  const int each = a.G * a.blocks;
-  const int row = (int)block_id(), b = row / each, u = row % each;
+  constexpr int LANES = DP / 4, GROUPS = 256 / LANES;
+  __shared__ floatx4 sums[GROUPS][LANES];
+  __shared__ float bounds[GROUPS], weights[GROUPS];
+  const int share = a.H / a.G, each = a.G * a.blocks;
+  const int head = (int)block_id(), b = head / a.H, g = head % a.H / share, hr = head % share, hb = hr / 16, r = hr % 16;
   if (b >= a.B) return;
   const int n = units_of(wave_int(cached(a, b)));
   const int per = run_of(a, units_before(a, a.B));
-  const int x0 = units_before(a, b) + u * n, w0 = x0 / per, w1 = (x0 + n - 1) / per;
+  const int x0 = units_before(a, b) + (g * a.blocks + hb) * n, w0 = x0 / per, w1 = (x0 + n - 1) / per;
   if (w0 == w1) return;
-  const int share = a.H / a.G, g = u / a.blocks, hb = u % a.blocks, heads = min(16, share - 16 * hb);
   const float sc = a.scale_log2;
   // The first of them is its workgroup's last piece, unless it begins that run; in the others it is the first.
-  const int p0 = 2 * w0 + (w0 * per == x0 ? 0 : 1);
-  for (int i = threadIdx.x; i < heads * (DP / 4); i += 256) {
-    const int r = i / (DP / 4), col = i % (DP / 4) * 4;
-    float up = -INFINITY;
-    for (int w = w0; w <= w1; ++w) up = fmaxf(up, part_of<DP>(a, w == w0 ? p0 : 2 * w)[r * (DP + 4) + DP]);
-    floatx4 sum = zero4();
-    float weight = 0.f;
-    for (int w = w0; w <= w1; ++w) {
-      const float* p = part_of<DP>(a, w == w0 ? p0 : 2 * w) + r * (DP + 4);
-      const float f = p[DP] == -INFINITY ? 1.f : pow2((p[DP] - up) * sc);
-      sum += *reinterpret_cast<const floatx4*>(p + col) * f;
-      weight += p[DP + 1] * f;
-    }
-    if (col < a.D) {
-      const float inv = weight == 0.f ? 0.f : 1.f / weight;
-      const float out[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
-      store_vec<4>(static_cast<E*>(a.o) + b * a.o_b + (g * share + 16 * hb + r) * a.o_h + col, out);
-    }
+  const int p0 = 2 * w0 + (w0 * per == x0 ? 0 : 1), grp = threadIdx.x / LANES, col = threadIdx.x % LANES * 4;
+  floatx4 sum = zero4();
+  float up = -INFINITY, weight = 0.f;
+#pragma unroll 4
+  for (int w = w0 + grp; w <= w1; w += GROUPS) {
+    const float* p = part_of<DP>(a, w == w0 ? p0 : 2 * w) + r * (DP + 4);
+    const float m = p[DP], l = p[DP + 1];
+    const floatx4 x = *reinterpret_cast<const floatx4*>(p + col);
+    const float top = fmaxf(up, m);
+    const float f = up == -INFINITY ? 1.f : pow2((up - top) * sc), fw = m == -INFINITY ? 1.f : pow2((m - top) * sc);
+    sum = sum * f + x * fw;
+    weight = weight * f + l * fw;
+    up = top;
+  }
+  sums[grp][threadIdx.x % LANES] = sum;
+  if (col == 0) {
+    bounds[grp] = up;
+    weights[grp] = weight;
+  }
+  __syncthreads();
+  if (grp != 0) return;
+  float top = up;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) top = fmaxf(top, bounds[i]);
+  sum = zero4();
+  weight = 0.f;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const float f = bounds[i] == -INFINITY ? 1.f : pow2((bounds[i] - top) * sc);
+    sum += sums[i][threadIdx.x] * f;
+    weight += weights[i] * f;
+  }
+  if (col < a.D) {
+    const float inv = weight == 0.f ? 0.f : 1.f / weight;
+    const float out[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
+    store_vec<4>(static_cast<E*>(a.o) + b * a.o_b + (g * share + hr) * a.o_h + col, out);
   }
 }
 

@@ -22,7 +22,7 @@ import torch
 
 from . import _hip
 from .ops import _dtype_code, _require
-from .serving import _apart, _device_of, _dim, _exec, _pool, _ptr, _require_view, _size
+from .serving import _apart, _device_of, _dim, _exec, _pool, _ptr, _require_view, _size, _span
 
 _ATTN = struct.Struct("@N6P8q7if")
 _ATTN_STEP = struct.Struct("@N8PN10q9if")
@@ -54,30 +54,65 @@ def _page(page: int) -> None:
         raise ValueError(f"a page holds a power of two of rows from 16 to 65536, got {page}")
 
 
-def _vectors(t: torch.Tensor) -> bool:
-    """Whether ``t``'s rows are whole 16-byte vectors."""
+def _vectors(t: torch.Tensor, strides) -> bool:
+    """Whether rows with these strides, where ``t`` starts, are whole 16-byte vectors."""
     each = 16 // t.element_size()
-    return t.data_ptr() % 16 == 0 and all(s % each == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
+    if t.data_ptr() % 16:
+        return False
+    for s in strides:
+        if s % each:
+            return False
+    return True
 
 
 def _strides(t: torch.Tensor):
-    """Strides of all but the last dimension, 0 where there is nothing to step to."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+    """Strides of all but the last dimension; 0 where there is nothing to step to, whatever the tensor says."""
+    s = t.stride()[:-1]
+    return s if 1 not in t.shape else tuple(0 if n == 1 else x for x, n in zip(s, t.shape))
+
+
+def _bytes(t: torch.Tensor) -> int:
+    return t.numel() * t.element_size() if t.is_contiguous() else _span(t)
+
+
+def _clear(name: str, t: torch.Tensor, **others) -> None:
+    """``t``, which a call writes, overlaps neither itself nor ``others``: by their ends, and where that does not say, by
+    :func:`serving._apart`."""
+    if not t.is_contiguous():
+        return _apart(name, t, **others)
+    lo = t.data_ptr()
+    hi = lo + t.numel() * t.element_size()
+    for u in others.values():
+        if u is not None:
+            at = u.data_ptr()
+            if at < hi and (at >= lo or at + _bytes(u) > lo):
+                return _apart(name, t, **others)
 
 
 def _cache(k_cache, v_cache, dtype, dev):
     _dim(k_cache, "k_cache", 4, "[pages,page,G,D]")
-    _page(k_cache.shape[1])
-    _require_view(k_cache, "k_cache", tuple(k_cache.shape), dtype, dev)
-    _require_view(v_cache, "v_cache", tuple(k_cache.shape), dtype, dev)
-    return k_cache.shape
+    shape = k_cache.shape
+    _page(shape[1])
+    _require_view(k_cache, "k_cache", shape, dtype, dev)
+    _require_view(v_cache, "v_cache", shape, dtype, dev)
+    return shape
 
 
 def _tables(tables, slots, B: int, dev):
     _dim(tables, "tables", 2, "[S,M]")
-    _require(tables, "tables", tuple(tables.shape), torch.int32, dev)
+    shape = tables.shape
+    _require(tables, "tables", shape, torch.int32, dev)
     _pool(tables, slots, B, dev)
-    return tables.shape
+    return shape
+
+
+def _rows(t: torch.Tensor):
+    """``t`` as the kernels read it, copied where its rows are no whole vectors or lie too far apart, and its strides."""
+    s = _strides(t)
+    if s[0] <= ROW_MAX_STRIDE and _vectors(t, s):
+        return t, s
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, _strides(t)
 
 
 def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *,
@@ -117,13 +152,13 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         o = torch.empty(N, H, D, device=dev, dtype=dtype)
     else:
         _require_view(out, "out", (N, H, D), dtype, dev)
-        _apart("out", out, q=q, k=k, v=v, cu_seqlens=cu_seqlens, lengths=lengths)
+        _clear("out", out, q=q, k=k, v=v, cu_seqlens=cu_seqlens, lengths=lengths)
         o = out
-    q, k, v = (t if _vectors(t) and _strides(t)[0] <= ROW_MAX_STRIDE else t.clone(memory_format=torch.contiguous_format)
-               for t in (q, k, v))
+    q, sq = _rows(q)
+    k, sk = _rows(k)
+    v, sv = _rows(v)
     _exec("pf_attn_exec", dev, _ATTN, _ATTN_SIZE, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-          cu_seqlens.data_ptr(), _ptr(lengths), *_strides(q), *_strides(k), *_strides(v), *_strides(o), N, B, H, G, D,
-          code, int(out is None), scale)
+          cu_seqlens.data_ptr(), _ptr(lengths), *sq, *sk, *sv, *_strides(o), N, B, H, G, D, code, int(out is None), scale)
     return o
 
 
@@ -151,23 +186,22 @@ def attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _require(lengths, "lengths", (B,), torch.int32, dev)
     if M * page > MAX_TOKENS:
         raise ValueError(f"tables hold {M} pages of {page} (up to {MAX_TOKENS} tokens)")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.numel() and (not _vectors(t) or _strides(t)[1] > ROW_MAX_STRIDE):
+    sk, sv = _strides(k_cache), _strides(v_cache)
+    for name, t, s in (("k_cache", k_cache, sk), ("v_cache", v_cache, sv)):
+        if pages and (s[1] > ROW_MAX_STRIDE or not _vectors(t, s)):
             raise ValueError(f"{name} must be whole 16-byte vectors, its rows up to {ROW_MAX_STRIDE} elements apart")
     scale = _scale(scale, D)
     if out is None:
         o = torch.empty(B, H, D, device=dev, dtype=dtype)
     else:
         _require_view(out, "out", (B, H, D), dtype, dev)
-        _apart("out", out, q=q, k_cache=k_cache, v_cache=v_cache, tables=tables, lengths=lengths, slots=slots)
+        _clear("out", out, q=q, k_cache=k_cache, v_cache=v_cache, tables=tables, lengths=lengths, slots=slots)
         o = out
-    if not _vectors(q):
-        q = q.clone(memory_format=torch.contiguous_format)
+    q, sq = _rows(q)
     need = _hip.load().pf_attn_step_workspace_bytes(B, H, G, D, M, page, code)
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     _exec("pf_attn_step_exec", dev, _ATTN_STEP, _ATTN_STEP_SIZE, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-          o.data_ptr(), tables.data_ptr(), lengths.data_ptr(), _ptr(slots), _ptr(ws), need, *_strides(q), *_strides(o),
-          *_strides(k_cache), *_strides(v_cache), B, S, H, G, D, M, pages, page, code, scale)
+          o.data_ptr(), tables.data_ptr(), lengths.data_ptr(), _ptr(slots), _ptr(ws), need, *sq, *_strides(o), *sk, *sv, B, S, H, G, D, M, pages, page, code, scale)
     return o
 
 
@@ -188,7 +222,7 @@ def _pool_state(tables, lengths, free, taken, slots, page_size: int, dev):
     if M * page_size > MAX_TOKENS:
         raise ValueError(f"tables hold {M} pages of {page_size} (up to {MAX_TOKENS} tokens)")
     _dim(free, "free", 1, "[F]")
-    _require(free, "free", tuple(free.shape), torch.int32, dev)
+    _require(free, "free", free.shape, torch.int32, dev)
     _require(taken, "taken", (1,), torch.int32, dev)
     return B, S, M, free.shape[0]
 
@@ -217,7 +251,7 @@ def assign_pages(tables: torch.Tensor, lengths: torch.Tensor, tokens: Optional[t
         capacity = B
     if not 0 <= capacity <= MAX_TOKENS:
         raise ValueError(f"capacity must be 0 to {MAX_TOKENS}, got {capacity}")
-    _apart("tables", tables, lengths=lengths, tokens=tokens, free=free, taken=taken, slots=slots)
+    _clear("tables", tables, lengths=lengths, tokens=tokens, free=free, taken=taken, slots=slots)
     rows = torch.empty(capacity, device=dev, dtype=torch.int64)
     ints = torch.empty(3 * B + 2, device=dev, dtype=torch.int32)
     cu, after, taken_after, place = ints.split([B + 1, B, 1, B])
@@ -235,7 +269,7 @@ def release_pages(tables: torch.Tensor, lengths: torch.Tensor, free: torch.Tenso
     request is refused, and keeps its pages, where more would come back than were taken."""
     dev = _device_of(tables, "tables")
     B, S, M, F = _pool_state(tables, lengths, free, taken, slots, page_size, dev)
-    _apart("free", free, tables=tables, lengths=lengths, taken=taken, slots=slots)
+    _clear("free", free, tables=tables, lengths=lengths, taken=taken, slots=slots)
     after = torch.empty(1, device=dev, dtype=torch.int32)
     _exec("pf_release_exec", dev, _RELEASE, _RELEASE_SIZE, tables.data_ptr(), lengths.data_ptr(), _ptr(slots),
           free.data_ptr(), taken.data_ptr(), after.data_ptr(), B, S, M, F, page_size)
@@ -259,7 +293,7 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     if (Gc, Dc) != (G, D):
         raise ValueError(f"k_cache has {Gc} heads of {Dc}, expected {G} of {D}")
     _require(rows, "rows", (N,), torch.int64, dev)
-    _apart("k_cache", k_cache, k=k, v=v, v_cache=v_cache, rows=rows)
-    _apart("v_cache", v_cache, k=k, v=v, rows=rows)
+    _clear("k_cache", k_cache, k=k, v=v, v_cache=v_cache, rows=rows)
+    _clear("v_cache", v_cache, k=k, v=v, rows=rows)
     _exec("pf_store_exec", dev, _STORE, _STORE_SIZE, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-          rows.data_ptr(), *_strides(k), *_strides(v), *_strides(k_cache), *_strides(v_cache), N, G, D, pages, page, code)
+          rows.data_ptr(), *k.stride()[:2], *v.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3], N, G, D, pages, page, code)
