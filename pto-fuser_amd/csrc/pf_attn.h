@@ -58,7 +58,10 @@ __device__ __forceinline__ void async_loads(const void* base, uint32_t lds, cons
   const uint64_t at = (uint64_t)base;
   const u32x4 r = {(uint32_t)wave_int((int)at), (uint32_t)wave_int((int)(at >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
   const uint32_t m = (uint32_t)wave_int((int)lds);
-  if constexpr (N == 4) {
+  if constexpr (N == 1) {
+    __asm__ __volatile__("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds"
+                         :: "s"(m), "s"(r), "v"(off[0]) : "memory", "m0");
+  } else if constexpr (N == 4) {
     __asm__ __volatile__(
         "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds\n\t"
         "s_add_u32 m0, %0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %1, 0 offen lds\n\t"
@@ -66,8 +69,11 @@ __device__ __forceinline__ void async_loads(const void* base, uint32_t lds, cons
         "s_add_u32 m0, %0, %8\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %1, 0 offen lds"
         :: "s"(m), "s"(r), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "n"(APART), "n"(2 * APART), "n"(3 * APART)
         : "memory", "m0", "scc");
+  } else if constexpr (N == 8) {
+    async_loads<4, APART>(base, lds, {off[0], off[1], off[2], off[3]});
+    async_loads<4, APART>(base, lds + 4 * APART, {off[4], off[5], off[6], off[7]});
   } else {
-    static_assert(N == 2, "two or four loads");
+    static_assert(N == 2, "one, two, four or eight loads");
     __asm__ __volatile__(
         "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds\n\t"
         "s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %1, 0 offen lds"
@@ -107,49 +113,92 @@ template <typename E, int DP> struct Rows {
 
 constexpr float kAttnRescale = 8.f;      // log2 by which scores may pass the carried maximum before it is moved
 
-// Where a tile of the grid lies: prompt, first row within it.  Every wave works it out for itself, 64 prompts at a time.
+// Sums over the lanes of a wave up to each (inclusive): within rows of 16, then from row to row.
+__device__ __forceinline__ int wave_sums(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // a row's last lane to the next row, of rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // lane 31 to rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_sums(v), 63); }
+
+// Where a tile of the grid lies: prompt, first row within it.
 struct AttnTile {
   int start, extent, len, row0;          // extent: rows up to the next prompt; len: live ones
-  int excess, first, last;               // of a tile that found none: its number among those; the rows that prompts cover
-  bool found;
+  int excess, first, last;               // of a tile past all prompts: its number among those; the rows that prompts cover
+  bool found, past;
 };
 
+// The longest tiles are to come first, and the shortest last, when the chip runs empty.  Up to 64 prompts, a lane each: the
+// tiles are numbered by their place in the prompt, the last place first, over all prompts, and a search over places finds the
+// tile.  More prompts: prompt b has tiles from cu[b] / BM + b on, which leaves it as many as it needs and one too many at most,
+// so that a search in cu finds it.  (Offsets that fall find some prompt or none, inside the rows.)
 template <int BM>
 __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int tile) {
   const int lane = threadIdx.x & 63;
   AttnTile t{};
-  int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
-    int start = 0, extent = 0, n = 0;
-    if (b < a.B) {
-      start = min(max(a.cu[b], 0), a.N);
-      extent = min(max(a.cu[b + 1], start), a.N) - start;
-      n = (extent + BM - 1) / BM;
-    }
-    int upto = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int other = __shfl_up(upto, d);
-      if (lane >= d) upto += other;
-    }
-    const unsigned long long behind = __ballot(before + upto > tile);
-    if (behind) {
-      const int l = __builtin_ctzll(behind);
-      t.found = true;
-      t.start = __builtin_amdgcn_readlane(start, l);
-      t.extent = __builtin_amdgcn_readlane(extent, l);
-      const int rank = tile - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
-      t.row0 = ((t.extent + BM - 1) / BM - 1 - rank) * BM;      // the longest first
-      t.len = t.extent;
-      if (a.lengths) t.len = min(max(__builtin_amdgcn_readfirstlane(a.lengths[b0 + l]), 0), t.extent);
+  int b, place;
+  if (a.B <= 64) {
+    const int start = min(max(a.cu[min(lane, a.B)], 0), a.N), end = min(max(a.cu[min(lane + 1, a.B)], start), a.N);
+    const int n = lane < a.B ? (end - start + BM - 1) / BM : 0;
+    const auto from = [&](int p) { return wave_sum(max(n - p, 0)); };     // tiles at place p and later
+    const int all = from(0);
+    t.excess = tile - all;
+    if (t.excess >= 0) {
+      t.past = true;
+      t.first = __builtin_amdgcn_readlane(start, 0);
+      t.last = max(min(max(wave_int(a.cu[a.B]), 0), a.N), t.first);
       return t;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    int lo = 0, hi = a.N / BM + 1, behind = 0;       // tiles from lo on are more than this one's number, from hi on `behind`
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2, count = from(mid);
+      if (count > tile) {
+        lo = mid;
+      } else {
+        hi = mid;
+        behind = count;
+      }
+    }
+    const unsigned long long here = __ballot(n > lo);
+    const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(here >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)here, 0));
+    const unsigned long long mine = __ballot(n > lo && rank == tile - behind);
+    if (!mine) return t;
+    b = __builtin_ctzll(mine);
+    place = lo;
+    t.start = __builtin_amdgcn_readlane(start, b);
+    t.extent = __builtin_amdgcn_readlane(end, b) - t.start;
+    t.found = true;
+  } else {
+    int lo = 0, count = a.B + 1;                     // entries of cu, the last of which at or before the tile is sought
+    while (count > 1) {
+      const int run = (count + 63) / 64, i = lo + min(lane * run, count - 1);
+      const unsigned long long before = __ballot(min(max(a.cu[i], 0), a.N) / BM + i <= tile && lane * run < count);
+      const int l = before ? 63 - __builtin_clzll(before) : 0;
+      lo += l * run;
+      count = min(run, count - l * run);
+    }
+    const int start = min(max(wave_int(a.cu[lo]), 0), a.N), rank = tile - (start / BM + lo);
+    if (lo == a.B) {
+      t.past = true;
+      t.excess = max(rank, 0);
+      t.first = min(max(wave_int(a.cu[0]), 0), a.N);
+      t.last = max(start, t.first);
+      return t;
+    }
+    b = lo;
+    t.start = start;
+    t.extent = min(max(wave_int(a.cu[lo + 1]), start), a.N) - start;
+    const int tiles = (t.extent + BM - 1) / BM;
+    t.found = rank >= 0 && rank < tiles;
+    place = tiles - 1 - rank;
   }
-  t.excess = tile - before;
-  t.first = min(max(a.cu[0], 0), a.N);
-  t.last = min(max(a.cu[a.B], t.first), a.N);
+  t.row0 = place * BM;
+  t.len = t.extent;
+  if (a.lengths) t.len = min(max(wave_int(a.lengths[b]), 0), t.extent);
   return t;
 }
 
@@ -167,22 +216,23 @@ __device__ __forceinline__ void zero_rows(const AttnArgs& a, int h, long from, l
 
 template <typename E, int DP, int BN> struct AttnLds {
   E k[2][BN * DP], v[2][BN * DP];
+  float bounds[4][2][64];                            // of waves that share rows
 };
 
 // One workgroup's walk.  Returns whether an output came out not finite.  A value of v that is not finite reaches the queries
 // before it through the products with the zeros above the diagonal: the walk is then made AGAIN, which leaves such values of
 // the diagonal's tiles out of the products and adds them to the queries that see them.
-template <typename E, int DP, int QT, int BN, bool AGAIN>
+template <typename E, int DP, int KW, int BN, bool AGAIN>
 __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>& s, const AttnTile& t, const int h) {
   using R = Rows<E, DP>;
   constexpr bool kBf = sizeof(E) == 2;
-  constexpr int NW = 4, BM = NW * 32 * QT, KT = BN / 32, DT = DP / 32, ES = sizeof(E);
+  constexpr int NW = 4, RW = NW / KW, BM = RW * 32, KT = BN / KW / 32, DT = DP / 32, ES = sizeof(E);
   constexpr int LOADS = BN * R::RB / 1024 / NW;      // 1 KiB each, of a wave and operand
   constexpr int QV = DP / (kBf ? 16 : 8);            // 16-byte vectors of a lane's query
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hf = lane >> 5;
   const int g = wave_int(h / (a.H / a.G));
-  const int q0 = t.row0 + w * 32 * QT;               // the wave's first query
+  const int kw = w / RW, q0 = t.row0 + w % RW * 32;  // the wave's part of a tile's keys, its first query
 
   const char* kg = reinterpret_cast<const char*>(static_cast<const E*>(a.k) + (long)t.start * a.k_t + g * a.k_h);
   const char* vg = reinterpret_cast<const char*>(static_cast<const E*>(a.v) + (long)t.start * a.v_t + g * a.v_h);
@@ -223,28 +273,39 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
 
   if (n_tiles > 0) load(0, 0);
 
-  // Q: a lane has row q0 + 32 qt + c; columns 16 kb + 8 hf .. (fp32: 8 kb + 4 hf ..)
-  u32x4 q[QT][QV];
+  // Q: a lane has row q0 + 32 qt + c; columns 16 kb + 8 hf .. (fp32: 8 kb + 4 hf ..).  Whole bf16 rows come through the second
+  // buffers, whole lines at a time (32 rows of the wave fill half of one).
+  u32x4 q[QV];
+  if (kBf && KW == 1 && a.D == DP) {
+    constexpr int QLOADS = 32 / FIRST;
+    E* place = (w < 2 ? s.k[1] : s.v[1]) + (w & 1) * 32 * DP;
+    const char* from = reinterpret_cast<const char*>(static_cast<const E*>(a.q) + (long)(t.start + t.row0) * a.q_t + h * a.q_h);
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const long row = t.start + min(q0 + 32 * qt + c, t.len - 1);
-    const E* p = static_cast<const E*>(a.q) + row * a.q_t + h * a.q_h;
+    for (int i = 0; i < QLOADS; i += 4) {
+      uint32_t off[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int row = (i + x) * FIRST + lane / R::CHUNKS;
+        off[x] = (uint32_t)min(w * 32 + row, t.len - 1 - t.row0) * (uint32_t)(a.q_t * ES) + (((lane % R::CHUNKS) ^ R::swizzle(row)) * 16);
+      }
+      async_loads<4, 1024>(from, lds_address(place) + i * 1024, off);
+    }
+    wait_loads();
+#pragma unroll
+    for (int kb = 0; kb < QV; ++kb) q[kb] = *reinterpret_cast<const u32x4*>(place + R::at(c, (kb * 2 + hf) * R::V));
+  } else {
+    const E* p = static_cast<const E*>(a.q) + (t.start + min(q0 + c, t.len - 1)) * a.q_t + h * a.q_h;
 #pragma unroll
     for (int kb = 0; kb < QV; ++kb) {
       const int col = (kb * 2 + hf) * R::V;
-      q[qt][kb] = col < a.D ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{0, 0, 0, 0};
+      q[kb] = col < a.D ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{0, 0, 0, 0};
     }
   }
 
-  floatx16 o[QT][DT];
-  float m[QT], l[QT];
+  floatx16 o[DT];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    m[qt] = -INFINITY;
-    l[qt] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[qt][dt] = zero16();
-  }
+  for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
+  float m = -INFINITY, l = 0.f;
   const float sc = a.scale_log2;
 
   const auto step = [&](const int tile, auto parity) {
@@ -256,34 +317,34 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
     if (tile + 1 < n_tiles) load(tile + 1, buf ^ 1);
     const E* ks = s.k[buf];
     const E* vs = s.v[buf];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      const int qa = q0 + 32 * qt;
-      if (j0 > qa + 31) continue;                    // nothing of the tile is visible to these queries
+    const int jw = j0 + kw * (BN / KW), kv0 = kw * (BN / KW);
+    if (jw > q0 + 31) return;                        // nothing of the tile is visible to these queries
+    {
       floatx16 st[KT];
 #pragma unroll
       for (int kt2 = 0; kt2 < KT; ++kt2) {
         st[kt2] = zero16();
 #pragma unroll
         for (int kb = 0; kb < QV; ++kb) {
-          const u32x4 f = *reinterpret_cast<const u32x4*>(ks + R::at(32 * kt2 + c, (kb * 2 + hf) * R::V));
+          const u32x4 f = *reinterpret_cast<const u32x4*>(ks + R::at(kv0 + 32 * kt2 + c, (kb * 2 + hf) * R::V));
           if constexpr (kBf) {
-            st[kt2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, q[qt][kb]),
+            st[kt2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, q[kb]),
                                                               st[kt2], 0, 0, 0);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              st[kt2] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f[i]), __uint_as_float(q[qt][kb][i]), st[kt2], 0, 0, 0);
+              st[kt2] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f[i]), __uint_as_float(q[kb][i]), st[kt2], 0, 0, 0);
           }
         }
       }
-      const bool masked = j0 + BN - 1 > qa;
+      const bool masked = jw + 32 * KT - 1 > q0;
       if (masked) {
+        const int lim = q0 + c - jw - 4 * hf;        // the last key that the query sees, from the lane's first
 #pragma unroll
         for (int kt2 = 0; kt2 < KT; ++kt2)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (j0 + 32 * kt2 + 8 * (i / 4) + 4 * hf + i % 4 > qa + c) st[kt2][i] = -INFINITY;
+            if (32 * kt2 + 8 * (i / 4) + i % 4 > lim) st[kt2][i] = -INFINITY;
       }
       float top = st[0][0];
 #pragma unroll
@@ -291,22 +352,22 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, st[kt2][i]);
       top = half_max(top);
-      if (__ballot((top - m[qt]) * sc > kAttnRescale)) {       // (-inf - -inf is no number and asks for nothing)
-        const float up = fmaxf(top, m[qt]);
-        const float f = m[qt] == -INFINITY ? 0.f : pow2((m[qt] - up) * sc);
-        m[qt] = up;
-        l[qt] *= f;
+      if (__ballot((top - m) * sc > kAttnRescale)) {       // (-inf - -inf is no number and asks for nothing)
+        const float up = fmaxf(top, m);
+        const float f = m == -INFINITY ? 0.f : pow2((m - up) * sc);
+        m = up;
+        l *= f;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[qt][dt] *= f;
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
       }
-      const float off = m[qt] == -INFINITY ? 0.f : m[qt] * sc;
+      const float off = m == -INFINITY ? 0.f : m * sc;
       float p[KT][16];
 #pragma unroll
       for (int kt2 = 0; kt2 < KT; ++kt2)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           p[kt2][i] = pow2(__builtin_fmaf(st[kt2][i], sc, -off));
-          l[qt] += p[kt2][i];
+          l += p[kt2][i];
         }
 #pragma unroll
       for (int kt2 = 0; kt2 < KT; ++kt2) {
@@ -316,7 +377,7 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
             bf16x8 pb;
 #pragma unroll
             for (int i = 0; i < 8; ++i) pb[i] = (bf16)p[kt2][8 * j + i];
-            const int row = 32 * kt2 + 16 * j + 4 * hf + ((lane & 15) >> 2);
+            const int row = kv0 + 32 * kt2 + 16 * j + 4 * hf + ((lane & 15) >> 2);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
               const int col = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -325,30 +386,30 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
 #pragma unroll
                 for (int i = 0; i < 8; ++i) vf[i] = __builtin_isfinite((float)vf[i]) ? vf[i] : (bf16)0.f;
               }
-              o[qt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[qt][dt], 0, 0, 0);
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[dt], 0, 0, 0);
             }
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int row = 32 * kt2 + 8 * (i / 4) + 4 * hf + i % 4;
+            const int row = kv0 + 32 * kt2 + 8 * (i / 4) + 4 * hf + i % 4;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
               float vf = vs[R::at(row, 32 * dt + c)];
               if (AGAIN && masked) vf = __builtin_isfinite(vf) ? vf : 0.f;
-              o[qt][dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, p[kt2][i], o[qt][dt], 0, 0, 0);
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, p[kt2][i], o[dt], 0, 0, 0);
             }
           }
         }
       }
       if (AGAIN && masked) {
-        for (int j = 0; j < BN; ++j)
+        for (int j = 0; j < BN / KW; ++j)
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float x = to_f32(vs[R::at(j, 32 * dt + 8 * (i / 4) + 4 * hf + i % 4)]);
-              if (!__builtin_isfinite(x) && j0 + j <= qa + c) o[qt][dt][i] += x;
+              const float x = to_f32(vs[R::at(kv0 + j, 32 * dt + 8 * (i / 4) + 4 * hf + i % 4)]);
+              if (!__builtin_isfinite(x) && jw + j <= q0 + c) o[dt][i] += x;
             }
       }
     }
@@ -358,37 +419,81 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
     if (tile + 1 < n_tiles) step(tile + 1, std::integral_constant<int, 1>{});
   }
 
-  bool bad = false;
+  // Waves that share the rows: their sums at one bound, in the first of them.
+  lds_barrier();
+  l = half_sum(l);
+  if constexpr (KW > 1) {
+    floatx4* const sums = reinterpret_cast<floatx4*>(&s);
+    static_assert((KW - 1) * RW * DT * 4 * 64 * 16 <= (int)sizeof(s) - (int)sizeof(s.bounds), "the sums fit");
+    if (kw > 0) {
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int row = q0 + 32 * qt + c;
-    const float total = half_sum(l[qt]);
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (row >= t.extent || (row >= t.len && !a.zero_rest)) continue;
-    E* p = static_cast<E*>(a.o) + (long)(t.start + row) * a.o_t + h * a.o_h;
-    typedef typename VecAny<E, 4>::T Out;
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+        for (int i4 = 0; i4 < 4; ++i4)
+          sums[(((w - RW) * DT + dt) * 4 + i4) * 64 + lane] = floatx4{o[dt][4 * i4], o[dt][4 * i4 + 1], o[dt][4 * i4 + 2], o[dt][4 * i4 + 3]};
+      s.bounds[w][0][lane] = m;
+      s.bounds[w][1][lane] = l;
+    }
+    lds_barrier();
+    if (kw == 0) {
+      float up = m;
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        const int col = 32 * dt + 8 * i4 + 4 * hf;
-        if (col >= a.D) continue;
-        Out out;
+      for (int k = 1; k < KW; ++k) up = fmaxf(up, s.bounds[k * RW + w][0][lane]);
+      const float own = m == -INFINITY ? 1.f : pow2((m - up) * sc);
+      l *= own;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = row < t.len ? o[qt][dt][4 * i4 + i] * inv : 0.f;
-          bad |= !__builtin_isfinite(x);
-          out[i] = from_f32<E>(x);
-        }
-        *reinterpret_cast<Out*>(p + col) = out;
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= own;
+#pragma unroll
+      for (int k = 1; k < KW; ++k) {
+        const float mk = s.bounds[k * RW + w][0][lane], f = mk == -INFINITY ? 1.f : pow2((mk - up) * sc);
+        l += s.bounds[k * RW + w][1][lane] * f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const floatx4 x = sums[((((k - 1) * RW + w) * DT + dt) * 4 + i4) * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[dt][4 * i4 + i] = __builtin_fmaf(x[i], f, o[dt][4 * i4 + i]);
+          }
       }
+    }
+    lds_barrier();
+    if (kw > 0) return false;
+  }
+  // The output by way of LDS, where each wave has a quarter, so that it is stored in whole rows.
+  E* const place = reinterpret_cast<E*>(&s) + w * BN * DP;
+  static_assert(BN >= 32, "a wave's rows fit a buffer");
+  typedef typename VecAny<E, R::V>::T Out;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float spoilt = inv * 0.f;                          // 0 of finite values, else NaN
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = o[dt][4 * i4 + i] * inv;
+        spoilt = __builtin_fmaf(x[i], 0.f, spoilt);
+      }
+      store4(place + R::at(c, 32 * dt + 8 * i4 + 4 * hf), x[0], x[1], x[2], x[3]);
+    }
+  const bool bad = q0 + c < t.len && spoilt != 0.f;  // (NaN is unequal)
+  const int rows = min(32, (a.zero_rest ? t.extent : t.len) - q0), live = t.len - q0;
+  E* const to = static_cast<E*>(a.o) + (long)(t.start + q0) * a.o_t + h * a.o_h;
+#pragma unroll
+  for (int i = 0; i < 32 / FIRST; ++i) {
+    const int r = i * FIRST + lane / R::CHUNKS, col = lane % R::CHUNKS * R::V;
+    u32x4 x = *reinterpret_cast<const u32x4*>(place + R::at(r, col));
+    if (r >= live) x = u32x4{0, 0, 0, 0};
+    if (r < rows && col < a.D) *reinterpret_cast<Out*>(to + r * a.o_t + col) = __builtin_bit_cast(Out, x);
   }
   return bad;
 }
 
-template <typename E, int DP, int QT, int BN>
-__global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
-  constexpr int BM = 128 * QT;
+template <typename E, int DP, int KW, int BN>
+__global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : 2) void attn_kernel(AttnArgs a) {
+  constexpr int BM = 128 / KW;
   __shared__ AttnLds<E, DP, BN> s;
   __shared__ int again;
   // Heads vary fastest, those of keys before those that share one, and go round robin over the eight XCDs: the workgroups that
@@ -397,13 +502,12 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   if (tile >= (uint32_t)a.tiles) return;
   const int h = wave_int(hi % (uint32_t)a.G * (a.H / a.G) + hi / (uint32_t)a.G);
   const AttnTile t = find_tile<BM>(a, wave_int(tile));
-  if (!t.found) {
-    if (!a.zero_rest) return;
+  if (t.past && a.zero_rest) {
     const long each = 64, step = (long)(a.tiles - ((int)tile - t.excess)) * each;
     zero_rows<E>(a, h, t.excess * each, t.first, step, each);
     zero_rows<E>(a, h, t.last + t.excess * each, a.N, step, each);
-    return;
   }
+  if (!t.found) return;
   if (t.row0 >= t.len) {
     if (a.zero_rest) {
       const long r = t.start + t.row0, n = min(t.extent - t.row0, BM);
@@ -417,9 +521,9 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   }
   if (threadIdx.x == 0) again = 0;
   __syncthreads();
-  if (attn_walk<E, DP, QT, BN, false>(a, s, t, h)) again = 1;
+  if (attn_walk<E, DP, KW, BN, false>(a, s, t, h)) again = 1;
   __syncthreads();
-  if (again) attn_walk<E, DP, QT, BN, true>(a, s, t, h);
+  if (again) attn_walk<E, DP, KW, BN, true>(a, s, t, h);
 }
 
 }  // namespace pf

@@ -34,15 +34,37 @@ bool grid_of(double workgroups, dim3& grid) {
 }
 
 // ---- prompts -------------------------------------------------------------------------------
-template <typename E, int DP, int QT, int BN>
+template <typename E, int DP, int KW, int BN>
 int attn_launch(pf::AttnArgs& a, hipStream_t s) {
-  constexpr int BM = 128 * QT;
+  constexpr int BM = 128 / KW;
   a.tiles = a.N / BM + a.B + 1;        // a prompt's last tile is ragged; and one that finds none
   dim3 grid;
   if ((double)a.tiles * a.H >= 2147483648.0 || !grid_of((double)a.tiles * a.H, grid)) return PF_ERR_ARG;
   pf::LaunchScope scope;
-  pf::attn_kernel<E, DP, QT, BN><<<grid, dim3(256), 0, s>>>(a);
+  pf::attn_kernel<E, DP, KW, BN><<<grid, dim3(256), 0, s>>>(a);
   return scope.status();
+}
+
+// Waves that share a query row, each with a part of every tile's keys.  Alone they read each key once for 128 queries; sharing
+// makes two or four times as many workgroups, of as many times fewer steps each, for calls whose workgroups are few or whose
+// longest one is what is waited for.  By the number of workgroups without sharing (prompts x rows x heads; us alone / two / four):
+//   bf16, D = 128: 1 x 2048 x 16 (256) 42.7 / 33.9 / 67, 1 x 4096 x 16 (512) 92 / 88 / 206, 24 x 512 x 16 (1536) 49 / 66 / 237,
+//                  2 x 2048 x 32 (1024) 81 / 93 / 261; four have 133 KB of LDS and a wave a SIMD: 1 x 1024 x 8 (64) 23.3 / 18.2 / 17.2
+//   bf16, D = 64:  1 x 1024 x 16 (128) 18.2 / 14.0 / 11.9, 1 x 1536 x 16 (192) 24.3 / 18.7 / 19.6, 1 x 4096 x 16 60 / 51 / 69,
+//                  1 x 6144 x 16 (768) 100.9 / 103.0 / 137
+//   fp32, D = 128: 1 x 2048 x 16 277 / 171, 3 x 2048 x 8 (384) 277 / 270, 1 x 4096 x 16 593 / 629
+//   fp32, D = 64:  1 x 1024 x 16 75 / 42 / 36, 3 x 512 x 16 (192) 41.6 / 30.2 / 38.0, 1 x 1536 x 16 111.8 / 73.6 / 72.4, a padded
+//                  batch of 3 x 1471 x 6 with 61 % live rows (207) 106 / 72 / 54, 1 x 6144 x 16 640 / 614 / 845, 4 x 4096 x 16 1062 / 1072
+template <typename E, int DP>
+int attn_width(pf::AttnArgs& a, hipStream_t s) {
+  constexpr bool kBf = sizeof(E) == 2;
+  const double alone = (double)a.N / 128 * a.H;
+  if (alone > (kBf ? 512 : DP == 64 ? 768 : 384)) return attn_launch<E, DP, 1, kBf ? 64 : 32>(a, s);
+  if constexpr (DP == 64) {
+    const bool long_ones = !kBf && a.B > 0 && a.N / a.B >= 1024;
+    if (alone <= (long_ones ? 224 : 128)) return attn_launch<E, DP, 4, 128>(a, s);
+  }
+  return attn_launch<E, DP, 2, 64>(a, s);
 }
 
 // ---- single tokens -------------------------------------------------------------------------
@@ -98,8 +120,8 @@ int pf_attn_exec(const pf_attn_args* p, void* stream) {
   a.N = p->N; a.B = p->B; a.H = p->H; a.G = p->G; a.D = p->D; a.zero_rest = p->zero_rest;
   a.scale_log2 = p->scale * 1.44269504088896340736f;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p->dtype == PF_DTYPE_BF16) return p->D <= 64 ? attn_launch<bf16, 64, 1, 64>(a, s) : attn_launch<bf16, 128, 1, 64>(a, s);
-  return p->D <= 64 ? attn_launch<float, 64, 1, 32>(a, s) : attn_launch<float, 128, 1, 32>(a, s);
+  if (p->dtype == PF_DTYPE_BF16) return p->D <= 64 ? attn_width<bf16, 64>(a, s) : attn_width<bf16, 128>(a, s);
+  return p->D <= 64 ? attn_width<float, 64>(a, s) : attn_width<float, 128>(a, s);
 }
 
 size_t pf_attn_step_workspace_bytes(int B, int H, int G, int D, int M, int page, int dtype) {

@@ -45,9 +45,7 @@ __device__ __forceinline__ int units_of(int len) { return max((len - 1) / kStepU
 __device__ __forceinline__ int units_before(const AttnStepArgs& a, int b) {
   int sum = 0;
   for (int i = threadIdx.x & 63; i < b; i += 64) sum += units_of(cached(a, i));
-#pragma unroll
-  for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-  return wave_int(sum) * a.G * a.blocks;
+  return wave_sum(sum) * a.G * a.blocks;
 }
 // The sequence that unit x lies in, and how many units come before that.
 __device__ __forceinline__ int sequence_at(const AttnStepArgs& a, int x, int& before) {
@@ -56,12 +54,7 @@ __device__ __forceinline__ int sequence_at(const AttnStepArgs& a, int x, int& be
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
     const int n = b < a.B ? units_of(cached(a, b)) * a.G * a.blocks : 0;
-    int upto = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int other = __shfl_up(upto, d);
-      if (lane >= d) upto += other;
-    }
+    const int upto = wave_sums(n);
     const unsigned long long behind = __ballot(before + upto > x);
     if (behind) {
       const int l = __builtin_ctzll(behind);

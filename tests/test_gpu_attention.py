@@ -61,6 +61,36 @@ def test_prompts(dtype, lens, H, G, D):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lens,H,G,D", [
+    ([1100, 37], 64, 8, 64), ([900], 80, 16, 128), ([1] * 100 + [700, 0, 65], 64, 4, 128), ([700, 500], 24, 3, 64), ([1025], 32, 2, 128),
+    ([130] * 9, 16, 4, 72)])
+def test_many_workgroups(dtype, lens, H, G, D):
+    """Sizes at which a row is one wave's, two waves' and four waves', up to 64 prompts and more of them; some heads of each."""
+    announce(f"causal_attention {dtype} {lens[-2:]} of {len(lens)} H{H} G{G} D{D}")
+    q, k, v = _qkv(lens, H, G, D, dtype, sum(lens) + H)
+    o = causal_attention(q, k, v, _cu(lens))
+    r = H // G
+    for h in (0, r - 1, H - 1):
+        g = h // r
+        _check_prompts(o[:, h:h + 1], q[:, h:h + 1], k[:, g:g + 1], v[:, g:g + 1], lens, f"head {h}")
+
+
+@pytest.mark.parametrize("H", [2, 64])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_many_prompts_that_share_a_buffer_with_others(dtype, H):
+    """70 prompts, some of no rows, behind rows of none and before others: each is itself, and the rest is zero."""
+    announce(f"causal_attention 70 prompts {dtype} H{H}")
+    lens = [(i * 37) % 150 for i in range(70)]
+    starts = [11 + sum(lens[:i]) for i in range(71)]
+    N = starts[-1] + 500
+    q, k, v = _qkv([N], H, 2, 64, dtype, 41)
+    o = causal_attention(q, k, v, _ints(starts))
+    assert not o[:11].any() and not o[starts[-1]:].any()
+    inside = slice(11, starts[-1])
+    _check_prompts(o[inside, H - 1:], q[inside, H - 1:], k[inside, 1:], v[inside, 1:], lens, "o")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("D,extra,at", [(64, 8, 8), (128, 5, 1), (80, 16, 8), (96, 3, 2)])
 def test_prompts_of_views(dtype, D, extra, at):
     """Rows inside wider rows, on 16-byte vectors and off them; heads stored before tokens; an output that is a view."""
@@ -153,12 +183,12 @@ def test_scores_that_rise_along_the_keys():
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("what", [NAN, INF])
-def test_values_that_are_not_finite(dtype, D, what):
+@pytest.mark.parametrize("what,H,G", [(NAN, 4, 2), (INF, 4, 2), (NAN, 256, 2), (INF, 80, 2)])
+def test_values_that_are_not_finite(dtype, D, what, H, G):
     """In v they reach their own column from their own token on, in a key the tokens from it on, in a query its own row;
     the next prompt and the other heads stay as they are."""
-    announce(f"causal_attention not finite {dtype} D{D} {what}")
-    n, H, G = 330, 4, 2
+    announce(f"causal_attention not finite {dtype} D{D} {what} H{H}")
+    n = 330
     lens = [n, 100]
     clean = _qkv(lens, H, G, D, dtype, 13)
     good = ref.f64(causal_attention(*clean, _cu(lens)))
@@ -166,7 +196,7 @@ def test_values_that_are_not_finite(dtype, D, what):
         q, k, v = (x.clone() for x in clean)
         v[t, 1, 3] = what
         bad = torch.zeros(sum(lens), H, D, dtype=torch.bool)
-        bad[t:n, 2:, 3] = True
+        bad[t:n, H // 2:, 3] = True
         o = ref.f64(causal_attention(q, k, v, _cu(lens)))
         assert torch.equal(~torch.isfinite(o), bad), t
         assert torch.equal(o[~bad], good[~bad]), t
@@ -174,7 +204,7 @@ def test_values_that_are_not_finite(dtype, D, what):
         q, k, v = (x.clone() for x in clean)
         k[t, 0, 5] = NAN
         bad = torch.zeros(sum(lens), H, D, dtype=torch.bool)
-        bad[t:n, :2] = True
+        bad[t:n, :H // 2] = True
         o = ref.f64(causal_attention(q, k, v, _cu(lens)))
         assert torch.equal(~torch.isfinite(o), bad) and torch.equal(o[~bad], good[~bad]), t
         q, k, v = (x.clone() for x in clean)
