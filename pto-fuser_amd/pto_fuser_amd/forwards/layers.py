@@ -1,13 +1,16 @@
-"""Recurrent layers as they are served: a prompt (or a ragged batch of them), then single tokens from its state.
+"""Layers as they are served: a prompt (or a ragged batch of them), then single tokens from its state.
 
-Two layers over the package's operators, with torch's library products for the projections:
+Three layers over the package's operators, with torch's library products for the projections:
 
 * a state space layer — norm with the residual's addition, one projection to z, x, B, C and dt, the short convolution
   over x, B and C in place, the scan, the norm of its output in 8 bits with a scale a token, and the projection of those;
-* a gated delta rule layer — the same around the chunked forward (``gdn_chunk_forward``) and ``gdn_step``.
+* a gated delta rule layer — the same around the chunked forward (``gdn_chunk_forward``) and ``gdn_step``;
+* an attention layer, as models put one after every few recurrent ones — norm, one projection to q, k and v, their storing in a
+  paged cache, attention over the prompts or one token over the cache, the norm of its output in 8 bits, the projection.
 
-``prefill`` returns the states after each prompt; ``step`` moves states in a pool on, which its ``slots`` name.  No
-counterpart in the reference, whose path ends at the chunked forward.
+``prefill`` of the recurrent layers returns the states after each prompt; ``step`` moves states in a pool on, which its ``slots``
+name.  Where an attention layer's tokens go is planned once for all of them (``assign_pages``): its ``prefill`` and ``step`` take
+that plan.  No counterpart in the reference, whose path ends at the chunked forward.
 """
 from __future__ import annotations
 
@@ -16,11 +19,13 @@ from typing import Optional, Tuple
 
 import torch
 
+from ..attention import PagePlan, attention_step, causal_attention, store_kv
 from ..ops import gdn_chunk_forward
 from ..serving import (add_rms_norm, add_rms_norm_fp8, causal_conv, causal_conv_step, gdn_step, ssm_chunk_forward,
                        ssm_step)
 
-__all__ = ["LayerCache", "SsmLayer", "GdnLayer", "make_ssm_layer", "make_gdn_layer"]
+__all__ = ["LayerCache", "SsmLayer", "GdnLayer", "AttentionLayer", "KvCache", "make_ssm_layer", "make_gdn_layer",
+           "make_attention_layer"]
 
 _FP8_MAX = 448.0
 
@@ -168,6 +173,56 @@ class GdnLayer:
         return self._project(o.flatten(-2)), hidden if stream is None else stream
 
 
+@dataclass
+class KvCache:
+    """The keys and values of one attention layer in pages; which page is whose is in the tables that the layers share."""
+    k: torch.Tensor       # [pages, page, G, D]
+    v: torch.Tensor
+
+
+@dataclass
+class AttentionLayer:
+    norm_w: torch.Tensor        # [D]
+    in_w: torch.Tensor          # [D, (H + 2 G) head]: q, k, v
+    out_norm_w: torch.Tensor    # [H head]
+    out: _Projection8
+    H: int
+    G: int
+    head: int
+
+    def cache(self, pages: int, page_size: int) -> KvCache:
+        shape = (pages, page_size, self.G, self.head)
+        return KvCache(*(torch.zeros(shape, device=self.in_w.device, dtype=self.in_w.dtype) for _ in range(2)))
+
+    def _operands(self, rows):
+        """q [N, H, head], k and v [N, G, head] of rows [N, D]."""
+        q, k, v = (rows @ self.in_w).split([self.H * self.head, self.G * self.head, self.G * self.head], dim=-1)
+        return q.unflatten(-1, (self.H, self.head)), *(t.unflatten(-1, (self.G, self.head)) for t in (k, v))
+
+    def _project(self, o):
+        codes, scales, _ = add_rms_norm_fp8(o.flatten(-2), self.out_norm_w)
+        return self.out(codes, scales)
+
+    def prefill(self, hidden: torch.Tensor, residual: Optional[torch.Tensor], cache: KvCache,
+                plan: PagePlan) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Whole prompts, packed: hidden, residual [N,D] with N the plan's capacity -> (output [N,D], the residual stream).
+        Their keys and values go to the plan's rows; a prompt that it did not serve is computed and not stored."""
+        y, stream = add_rms_norm(hidden, self.norm_w, residual)
+        q, k, v = self._operands(y)
+        store_kv(k, v, cache.k, cache.v, plan.rows)
+        out = self._project(causal_attention(q, k, v, plan.cu_seqlens))
+        return out, hidden if stream is None else stream
+
+    def step(self, hidden: torch.Tensor, residual: Optional[torch.Tensor], cache: KvCache, plan: PagePlan,
+             tables: torch.Tensor, slots: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """One token of each sequence: hidden, residual [B,D]; ``slots`` names the sequences' tables."""
+        y, stream = add_rms_norm(hidden, self.norm_w, residual)
+        q, k, v = self._operands(y)
+        store_kv(k, v, cache.k, cache.v, plan.rows)
+        out = self._project(attention_step(q, cache.k, cache.v, tables, plan.lengths, slots=slots))
+        return out, hidden if stream is None else stream
+
+
 def make_ssm_layer(D: int, H: int, P: int = 64, G: int = 1, N: int = 128, K: int = 4, *, seed: int = 0,
                    device="cuda") -> SsmLayer:
     """Seeded weights with the usual scales: steps between 1e-3 and 1e-1, A between -16 and -1."""
@@ -189,3 +244,11 @@ def make_gdn_layer(D: int, H: int, K: int = 4, *, seed: int = 0, device="cuda") 
     bf = lambda t: t.to(device, torch.bfloat16)  # noqa: E731
     return GdnLayer(bf(1 + 0.1 * randn(D)), bf(randn(D, 3 * inner + 2 * H) * D ** -0.5), bf((2 * rand(3 * inner, K) - 1) * K ** -0.5),
                     (1 + 0.1 * randn(inner)).to(device), _Projection8((randn(D, inner) * inner ** -0.5).to(device)), H)
+
+
+def make_attention_layer(D: int, H: int, G: int, head: int = 128, *, seed: int = 0, device="cuda") -> AttentionLayer:
+    gen = torch.Generator().manual_seed(seed)
+    randn, inner = (lambda *s: torch.randn(*s, generator=gen)), H * head
+    bf = lambda t: t.to(device, torch.bfloat16)  # noqa: E731
+    return AttentionLayer(bf(1 + 0.1 * randn(D)), bf(randn(D, inner + 2 * G * head) * D ** -0.5), bf(1 + 0.1 * randn(inner)),
+                          _Projection8((randn(D, inner) * inner ** -0.5).to(device)), H, G, head)
