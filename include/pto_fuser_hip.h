@@ -411,7 +411,7 @@ int pf_attn_step_exec(const pf_attn_step_args* args, void* stream);
  * 2^30) or the capacity, or whose pages are more than free (F entries) has left is not served: its rows are -1, its length
  * stays; after one that lacked pages, none that needs any is served.
  * rows [capacity]: the cache row of each new token, -1 of none; cu [B+1]: the requests' new tokens in them (cut at capacity);
- * lengths_out [B], taken_out [1]: lengths and taken after the call (they may not be lengths and taken).  place [B]: scratch. */
+ * lengths_out [B], taken_out [1]: lengths and taken after the call (they may not be lengths and taken). */
 typedef struct pf_assign_args {
   size_t size;
   int* tables;
@@ -424,7 +424,6 @@ typedef struct pf_assign_args {
   int* cu;
   int* lengths_out;
   int* taken_out;
-  int* place;
   int B, S, M, F, capacity, page;
 } pf_assign_args;
 int pf_assign_exec(const pf_assign_args* args, void* stream);

@@ -8,6 +8,8 @@
 
 #include "pf_serving.h"
 
+#include <type_traits>
+
 namespace pf {
 
 struct AssignArgs {
@@ -21,125 +23,122 @@ struct AssignArgs {
   int* cu;                 // [B + 1]
   int* lengths_out;        // [B]
   int* taken_out;          // [1]
-  int* place;              // [B] scratch: the first of a request's new pages in free; -1: it is not served
   int B, S, M, F, capacity, page_log;
-  int fill;                // the first kernel's workgroup fills the rows too
 };
 
-__device__ __forceinline__ int pages_of(long tokens, int page_log) { return (int)((tokens + (1L << page_log) - 1) >> page_log); }
-
-// Sums of two values over a workgroup's threads before each, and of all.
-template <int THREADS>
-__device__ __forceinline__ void scan2(long& x, long& y, long& all_x, long& all_y, long (*s)[THREADS / 64]) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  long ux = x, uy = y;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const long ox = __shfl_up(ux, d), oy = __shfl_up(uy, d);
-    if (lane >= d) {
-      ux += ox;
-      uy += oy;
-    }
-  }
-  if (lane == 63) {
-    s[0][w] = ux;
-    s[1][w] = uy;
-  }
-  __syncthreads();
-  long bx = 0, by = 0;
-  all_x = all_y = 0;
-#pragma unroll
-  for (int i = 0; i < THREADS / 64; ++i) {
-    if (i < w) {
-      bx += s[0][i];
-      by += s[1][i];
-    }
-    all_x += s[0][i];
-    all_y += s[1][i];
-  }
-  __syncthreads();
-  x = bx + ux - x;
-  y = by + uy - y;
+// (tokens up to 2^31)
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, int page_log) {
+  return (tokens >> page_log) + ((tokens & ((1u << page_log) - 1)) != 0);
 }
 
-// The row of new token t, and the entry of a page that begins with it.
-__device__ __forceinline__ void fill_row(const AssignArgs& a, int t) {
-  long row = -1;
-  if (t < a.cu[a.B]) {
-    int lo = 0, hi = a.B;                            // the last request that begins at t or before has it
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      (a.cu[mid] <= t ? lo : hi) = mid;
-    }
-    const int place = a.place[lo];
-    if (place >= 0) {
-      const int c = max(a.lengths[lo], 0), at = c + t - a.cu[lo], index = at >> a.page_log, have = pages_of(c, a.page_log);
-      const int off = at & ((1 << a.page_log) - 1);
-      int* entry = a.tables + (long)(a.slots ? a.slots[lo] : lo) * a.M + index;
-      int page;
-      if (index >= have) {
-        page = a.free[place + index - have];
-        if (off == 0) *entry = page;
-      } else {
-        page = *entry;
-      }
-      if (page >= 0) row = ((long)page << a.page_log) + off;
-    }
+// Sums that stay at 2^32 - 1 once they reach it, which is past every capacity and pool.
+__device__ __forceinline__ uint32_t sat_add(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
+
+// A value's sum over the threads before each, added to `carry`, which then takes them all in.
+__device__ __forceinline__ uint32_t block_sums(uint32_t v, uint32_t& carry, uint32_t (&s)[4]) {
+  const int w = threadIdx.x >> 6;
+  const auto moved = [](uint32_t x, auto ctrl, auto rows) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, decltype(rows)::value == 0xf);
+  };
+  uint32_t u = v;
+  u = sat_add(u, moved(u, std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{}));
+  u = sat_add(u, moved(u, std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{}));
+  u = sat_add(u, moved(u, std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{}));
+  u = sat_add(u, moved(u, std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{}));
+  u = sat_add(u, moved(u, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));   // from row to row of 16
+  u = sat_add(u, moved(u, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) s[w] = u;
+  __syncthreads();
+  // (the lane before's inclusive sum: a saturated sum less its own value would not be one)
+  uint32_t before = (uint32_t)__shfl_up((int)u, 1);
+  if ((threadIdx.x & 63) == 0) before = 0;
+  uint32_t sum = carry;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i == w) before = sat_add(sum, before);
+    sum = sat_add(sum, s[i]);
   }
-  a.rows[t] = row;
+  carry = sum;
+  return before;
 }
 
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void assign_kernel(AssignArgs a) {
-  __shared__ long s[2][THREADS / 64];
+constexpr int kAssignTokens = 512;       // of a workgroup
+
+// Every workgroup goes through all requests, 256 at a time, and fills the rows of its own tokens from them; the first also
+// writes what is of requests.  So there is one launch, and none waits for another.
+__global__ __launch_bounds__(256) void assign_kernel(AssignArgs a) {
+  __shared__ uint32_t sums[4];
+  __shared__ int s_cu[257], s_place[256], s_c[256], s_slot[256];
   const int tid = threadIdx.x;
-  const long taken = min(max(a.taken[0], 0), a.F);
-  long rows = 0, pages = 0, used = 0;                // new tokens and pages of the requests so far; pages that were given
-  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+  const uint32_t taken = (uint32_t)min(max(a.taken[0], 0), a.F), left = a.F - taken;
+  const long mine = block_id() * kAssignTokens;
+  const int t0 = (int)min(mine, (long)a.capacity), t1 = (int)min(mine + kAssignTokens, (long)a.capacity);
+  const bool leads = blockIdx.x == 0 && blockIdx.y == 0;
+  uint32_t rows = 0, pages = 0, used = 0;            // new tokens and pages of the requests so far; pages that were given
+  for (int b0 = 0; b0 < a.B; b0 += 256) {
     const int b = b0 + tid;
-    long c = 0, n = 0, need = 0, limit = 0;
+    uint32_t c = 0, n = 0;
+    int slot = -1;
     if (b < a.B) {
-      c = max(a.lengths[b], 0);
-      n = a.tokens ? max(a.tokens[b], 0) : 1;
-      limit = (long)a.M << a.page_log;
-      const int slot = a.slots ? a.slots[b] : b;
-      if (slot < 0 || slot >= a.S || c + n > limit) limit = -1;
-      need = limit < 0 ? 0 : pages_of(c + n, a.page_log) - pages_of(c, a.page_log);
+      c = (uint32_t)max(a.lengths[b], 0);
+      n = a.tokens ? (uint32_t)max(a.tokens[b], 0) : 1u;
+      slot = a.slots ? a.slots[b] : b;
     }
-    // (a request that its rows' capacity cuts off is not served either, and its need does not count: all that come before it
-    // within the capacity are known from the first sum alone)
-    long first = n, none = 0, all_n, all_none;
-    scan2<THREADS>(first, none, all_n, all_none, s);
-    first += rows;
-    const bool fits = b < a.B && limit >= 0 && first + n <= a.capacity;
-    long before = fits ? need : 0, given = 0, all_need, all_given;
-    scan2<THREADS>(before, given, all_need, all_given, s);
-    before += pages;
-    const bool served = fits && (need == 0 || taken + before + need <= a.F);
-    given = served ? need : 0;
-    none = 0;
-    scan2<THREADS>(given, none, all_given, all_none, s);
-    used += all_given;
-    if (b < a.B) {
-      a.cu[b] = (int)min(first, (long)a.capacity);
-      a.lengths_out[b] = (int)(served ? c + n : c);
-      a.place[b] = served ? (int)(taken + min(before, a.F - taken)) : -1;
+    const uint32_t first = block_sums(n, rows, sums);
+    const bool fits = slot >= 0 && slot < a.S && c + n <= (uint32_t)a.M << a.page_log && sat_add(first, n) <= (uint32_t)a.capacity;
+    const uint32_t need = fits ? pages_of(c + n, a.page_log) - pages_of(c, a.page_log) : 0;
+    const uint32_t before = block_sums(need, pages, sums);
+    const bool served = fits && (need == 0 || sat_add(before, need) <= left);
+    if (served && need) used = before + need;
+    const int start = (int)min(first, (uint32_t)a.capacity), after = (int)(served ? c + n : c);
+    s_cu[tid] = start;
+    s_place[tid] = served ? (int)(taken + min(before, left)) : -1;
+    s_c[tid] = (int)c;
+    s_slot[tid] = slot;
+    if (tid == 0) s_cu[256] = (int)min(rows, (uint32_t)a.capacity);
+    if (leads && b < a.B) {
+      a.cu[b] = start;
+      a.lengths_out[b] = after;
     }
-    rows += all_n;
-    pages += all_need;
+    __syncthreads();
+    for (int t = max(t0, s_cu[0]) + tid; t < min(t1, s_cu[256]); t += 256) {
+      int lo = 0, hi = 256;                          // the last request that begins at t or before has it
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int mid = (lo + hi) / 2;
+        (s_cu[mid] <= t ? lo : hi) = mid;
+      }
+      long row = -1;
+      const int place = s_place[lo];
+      if (place >= 0) {
+        const int at = s_c[lo] + t - s_cu[lo], index = at >> a.page_log, have = (int)pages_of((uint32_t)s_c[lo], a.page_log);
+        const int off = at & ((1 << a.page_log) - 1);
+        int* entry = a.tables + (long)s_slot[lo] * a.M + index;
+        int page;
+        if (index >= have) {
+          page = a.free[place + index - have];
+          if (off == 0) *entry = page;               // (every new page begins with a new token)
+        } else {
+          page = *entry;
+        }
+        if (page >= 0) row = ((long)page << a.page_log) + off;
+      }
+      a.rows[t] = row;
+    }
   }
-  if (tid == 0) {
-    a.cu[a.B] = (int)min(rows, (long)a.capacity);
-    a.taken_out[0] = (int)(taken + used);
-  }
-  if (!a.fill) return;
+  for (int t = max(t0, (int)min(rows, (uint32_t)a.capacity)) + tid; t < t1; t += 256) a.rows[t] = -1;
+  if (!leads) return;
+  // (pages given: up to the end of the last request that got any)
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) used = max(used, (uint32_t)__shfl_xor((int)used, d));
   __syncthreads();
-  for (int t = tid; t < a.capacity; t += THREADS) fill_row(a, t);
-}
-
-__global__ __launch_bounds__(256) void assign_rows_kernel(AssignArgs a) {
-  const long t = block_id() * 256 + threadIdx.x;
-  if (t < a.capacity) fill_row(a, (int)t);
+  if ((tid & 63) == 0) sums[tid >> 6] = used;
+  __syncthreads();
+  if (tid == 0) {
+    a.cu[a.B] = (int)min(rows, (uint32_t)a.capacity);
+    a.taken_out[0] = (int)(taken + max(max(sums[0], sums[1]), max(sums[2], sums[3])));
+  }
 }
 
 struct ReleaseArgs {
@@ -153,40 +152,35 @@ struct ReleaseArgs {
 };
 
 // Request b's pages go back to free[taken - 1 - those of all before it ..] downwards; one that more pages come before than
-// were taken (a request released twice) keeps them.  A workgroup a request.
+// were taken (a request released twice) keeps them.  A workgroup a request, and one for what all give back.
 __global__ __launch_bounds__(256) void release_kernel(ReleaseArgs a) {
-  __shared__ long s[2][4];
-  const int mine = (int)block_id();
-  const long taken = min(max(a.taken[0], 0), a.F);
+  __shared__ uint32_t sums[4];
+  const int mine = (int)block_id(), tid = threadIdx.x;
+  if (mine > a.B) return;
+  const uint32_t taken = (uint32_t)min(max(a.taken[0], 0), a.F);
   const auto pages = [&](int b) {
     const int slot = a.slots ? a.slots[b] : b;
-    return slot < 0 || slot >= a.S ? 0L : (long)min(pages_of(max(a.lengths[b], 0), a.page_log), a.M);
+    return slot < 0 || slot >= a.S ? 0u : min(pages_of((uint32_t)max(a.lengths[b], 0), a.page_log), (uint32_t)a.M);
   };
-  // Of the requests up to this one (the last workgroup: of all, and of those that are released).
-  long before = 0, n = 0;
-  const bool last = mine == a.B;
+  uint32_t before = 0, back = 0;                     // pages of the requests before this one; of those, that go back
   for (int b0 = 0; b0 < mine; b0 += 256) {
-    const int b = b0 + threadIdx.x;
-    long x = b < mine ? pages(b) : 0, y = 0, all, none;
-    const long own = x;
-    scan2<256>(x, y, all, none, s);
-    if (last) {
-      y = before + x + own <= taken ? own : 0;
-      x = 0;
-      long all_x;
-      scan2<256>(x, y, all_x, none, s);
-      n += none;
-    }
-    before += all;
+    const uint32_t own = b0 + tid < mine ? pages(b0 + tid) : 0;
+    const uint32_t x = block_sums(own, before, sums);
+    if (own && sat_add(x, own) <= taken) back = x + own;
   }
-  if (last) {
-    if (threadIdx.x == 0) a.taken_out[0] = (int)(taken - n);
+  if (mine == a.B) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) back = max(back, (uint32_t)__shfl_xor((int)back, d));
+    __syncthreads();
+    if ((tid & 63) == 0) sums[tid >> 6] = back;
+    __syncthreads();
+    if (tid == 0) a.taken_out[0] = (int)(taken - max(max(sums[0], sums[1]), max(sums[2], sums[3])));
     return;
   }
-  n = pages(mine);
-  if (before + n > taken) return;
+  const uint32_t n = pages(mine);
+  if (sat_add(before, n) > taken) return;
   const int* row = a.tables + (long)(a.slots ? a.slots[mine] : mine) * a.M;
-  for (long i = threadIdx.x; i < n; i += 256) a.free[taken - 1 - before - i] = row[i];
+  for (uint32_t i = tid; i < n; i += 256) a.free[taken - 1 - before - i] = row[i];
 }
 
 struct StoreArgs {

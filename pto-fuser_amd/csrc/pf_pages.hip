@@ -21,8 +21,6 @@ bool grid_of(double workgroups, dim3& grid) {
   return true;
 }
 
-constexpr int kAssignThreads = 1024;
-
 }  // namespace
 
 extern "C" {
@@ -32,19 +30,16 @@ int pf_assign_exec(const pf_assign_args* p, void* stream) {
   if (p->B < 0 || p->S < 0 || p->M < 0 || p->F < 0 || p->capacity < 0 || (!p->slots && p->B > p->S)) return PF_ERR_ARG;
   if ((double)p->M * p->page > (double)(1 << 30) || p->B == 0x7fffffff) return PF_ERR_ARG;
   if (!p->cu || !p->taken || !p->taken_out || (p->capacity > 0 && !p->rows)) return PF_ERR_ARG;
-  if (p->B > 0 && (!p->lengths || !p->lengths_out || !p->place)) return PF_ERR_ARG;
+  if (p->B > 0 && (!p->lengths || !p->lengths_out)) return PF_ERR_ARG;
   if ((p->F > 0 && !p->free) || (p->S > 0 && p->M > 0 && !p->tables)) return PF_ERR_ARG;
   pf::AssignArgs a{};
   a.tables = p->tables; a.lengths = p->lengths; a.tokens = p->tokens; a.slots = p->slots; a.free = p->free; a.taken = p->taken;
-  a.rows = p->rows; a.cu = p->cu; a.lengths_out = p->lengths_out; a.taken_out = p->taken_out; a.place = p->place;
+  a.rows = p->rows; a.cu = p->cu; a.lengths_out = p->lengths_out; a.taken_out = p->taken_out;
   a.B = p->B; a.S = p->S; a.M = p->M; a.F = p->F; a.capacity = p->capacity; a.page_log = log2_of(p->page);
-  a.fill = a.capacity <= 4 * kAssignThreads;
   dim3 grid;
-  if (!grid_of(((double)a.capacity + 255) / 256, grid)) return PF_ERR_ARG;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!grid_of(a.capacity ? ((double)a.capacity + pf::kAssignTokens - 1) / pf::kAssignTokens : 1, grid)) return PF_ERR_ARG;
   pf::LaunchScope scope;
-  pf::assign_kernel<kAssignThreads><<<1, kAssignThreads, 0, s>>>(a);
-  if (!a.fill) pf::assign_rows_kernel<<<grid, 256, 0, s>>>(a);
+  pf::assign_kernel<<<grid, 256, 0, static_cast<hipStream_t>(stream)>>>(a);
   return scope.status();
 }
 

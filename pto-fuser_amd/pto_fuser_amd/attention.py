@@ -26,7 +26,7 @@ from .serving import _apart, _device_of, _dim, _exec, _pool, _ptr, _require_view
 
 _ATTN = struct.Struct("@N6P8q7if")
 _ATTN_STEP = struct.Struct("@N8PN10q9if")
-_ASSIGN = struct.Struct("@N11P6i")
+_ASSIGN = struct.Struct("@N10P6i")
 _RELEASE = struct.Struct("@N6P5i")
 _STORE = struct.Struct("@N5P10q6i")
 _ATTN_SIZE, _ATTN_STEP_SIZE, _ASSIGN_SIZE, _RELEASE_SIZE, _STORE_SIZE = (
@@ -253,11 +253,10 @@ def assign_pages(tables: torch.Tensor, lengths: torch.Tensor, tokens: Optional[t
         raise ValueError(f"capacity must be 0 to {MAX_TOKENS}, got {capacity}")
     _clear("tables", tables, lengths=lengths, tokens=tokens, free=free, taken=taken, slots=slots)
     rows = torch.empty(capacity, device=dev, dtype=torch.int64)
-    ints = torch.empty(3 * B + 2, device=dev, dtype=torch.int32)
-    cu, after, taken_after, place = ints.split([B + 1, B, 1, B])
+    cu, after, taken_after = torch.empty(2 * B + 2, device=dev, dtype=torch.int32).split_with_sizes([B + 1, B, 1])
     _exec("pf_assign_exec", dev, _ASSIGN, _ASSIGN_SIZE, tables.data_ptr(), lengths.data_ptr(), _ptr(tokens), _ptr(slots),
           free.data_ptr(), taken.data_ptr(), rows.data_ptr(), cu.data_ptr(), after.data_ptr(), taken_after.data_ptr(),
-          place.data_ptr(), B, S, M, F, capacity, page_size)
+          B, S, M, F, capacity, page_size)
     return PagePlan(rows, cu, after, taken_after)
 
 

@@ -85,14 +85,14 @@ def test_step_workspaces(lib):
 
 def _assign(**kw):
     f = dict(size=attention._ASSIGN_SIZE)
-    f.update({n: 64 for n in ("tables", "lengths", "tokens", "slots", "free", "taken", "rows", "cu", "after", "taken_out", "place")})
+    f.update({n: 64 for n in ("tables", "lengths", "tokens", "slots", "free", "taken", "rows", "cu", "after", "taken_out")})
     f.update(B=2, S=2, M=4, F=9, capacity=5, page=16)
     assert not set(kw) - set(f)
     return attention._ASSIGN.pack(*{**f, **kw}.values())
 
 
 @pytest.mark.parametrize("bad", [dict(size=0), dict(tables=0), dict(lengths=0), dict(free=0), dict(taken=0), dict(rows=0), dict(cu=0),
-                                 dict(after=0), dict(taken_out=0), dict(place=0), dict(B=-1), dict(B=3, slots=0), dict(S=-1), dict(M=-1),
+                                 dict(after=0), dict(taken_out=0), dict(B=-1), dict(B=3, slots=0), dict(S=-1), dict(M=-1),
                                  dict(F=-1), dict(capacity=-1), dict(page=12), dict(M=1 << 27)])
 def test_assign_statuses(lib, bad):
     assert lib.pf_assign_exec(_assign(**bad), None) == _hip.PF_ERR_ARG

@@ -161,3 +161,20 @@ def test_store_past_32_bits():
     for cache, x in ((kc, k), (vc, v)):
         assert torch.equal(cache.view(-1, 8, 128)[rows], x)
         assert int(cache.view(torch.int32).count_nonzero()) <= 3 * 8 * 64
+
+
+def test_assign_of_numbers_at_their_limits():
+    """Sums of tokens past 32 bits, lengths at a table's end: refused requests stay refused, and the rest is served."""
+    announce("assign_pages at the limits")
+    page, big = 65536, 2 ** 31 - 1
+    M = (1 << 30) // page
+    for lengths, tokens, capacity in (([0, 0, 0, 5], [big, big, big, 1], 40), ([(1 << 30) - 1, (1 << 30) - 1, 3], [1, 2, 4], 90),
+                                      ([7, 0, 0], [3, big, 2], 10)):
+        B = len(lengths)
+        tables = [[b * 3 + i for i in range(3)] + [5] * (M - 3) for b in range(B)]
+        _assign(tables, lengths, tokens, list(range(50, 90)), 2, page, capacity)
+    lengths = _ints([-3, 4])
+    tables = torch.zeros(2, 2, dtype=torch.int32, device=DEV)
+    plan = assign_pages(tables, lengths, _ints([-7, 2]), _ints([9]), _ints([-1]), page_size=16, capacity=5)
+    assert plan.cu_seqlens.tolist() == [0, 0, 2] and plan.rows.tolist() == [4, 5, -1, -1, -1] and plan.lengths.tolist() == [0, 6]
+    assert plan.taken.tolist() == [0]
