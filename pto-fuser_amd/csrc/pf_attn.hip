@@ -72,7 +72,7 @@ constexpr int kStepWgs = 512;          // workgroups that share a walk: two a CU
 
 struct StepPlan {
   int rows, wgs, blocks;
-  size_t bytes;
+  size_t parts, bytes;
 };
 
 bool step_plan(int B, int H, int G, int D, int M, int page, StepPlan& p) {
@@ -83,7 +83,8 @@ bool step_plan(int B, int H, int G, int D, int M, int page, StepPlan& p) {
   p.rows = (int)rows;
   const double wgs = D <= 64 ? 2 * kStepWgs : kStepWgs;
   p.wgs = tokens <= 512 ? 0 : (int)(units < wgs ? units : wgs);
-  p.bytes = (size_t)p.wgs * 2 * 16 * ((D <= 64 ? 64 : 128) + 4) * sizeof(float);
+  p.parts = (size_t)p.wgs * 2 * 16 * ((D <= 64 ? 64 : 128) + 4);
+  p.bytes = p.wgs ? p.parts * sizeof(float) + (size_t)p.rows * 4 * sizeof(int) : 0;
   return true;
 }
 
@@ -145,6 +146,7 @@ int pf_attn_step_exec(const pf_attn_step_args* p, void* stream) {
   pf::AttnStepArgs a{};
   a.q = p->q; a.k = p->k; a.v = p->v; a.o = p->o; a.tables = p->tables; a.lengths = p->lengths; a.slots = p->slots;
   a.part = static_cast<float*>(p->workspace);
+  a.spread = reinterpret_cast<int*>(a.part + pl.parts);
   a.q_b = p->q_b; a.q_h = p->q_h; a.o_b = p->o_b; a.o_h = p->o_h;
   a.k_p = p->k_p; a.k_r = p->k_r; a.k_h = p->k_h; a.v_p = p->v_p; a.v_r = p->v_r; a.v_h = p->v_h;
   a.B = p->B; a.S = p->S; a.H = p->H; a.G = p->G; a.D = p->D; a.M = p->M; a.pages = p->pages; a.page_log = log2_of(p->page);

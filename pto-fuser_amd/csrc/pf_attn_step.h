@@ -22,7 +22,8 @@ struct AttnStepArgs {
   const int* tables;       // [S, M]: a sequence's pages
   const int* lengths;      // [B]
   const int* slots;        // [B] or null
-  float* part;             // [2 wgs][16][DP + 2]: sums, then the bound and the weights' sum
+  float* part;             // [2 wgs][16][DP + 4]: sums, then the bound and the weights' sum
+  int* spread;             // [rows][4]: of a (sequence, head, block) its first part, the workgroups of the first and last one
   long q_b, q_h, o_b, o_h, k_p, k_r, k_h, v_p, v_r, v_h;
   int B, S, H, G, D, M, pages, page_log;
   int blocks;              // of 16 of a group's query heads
@@ -41,32 +42,46 @@ __device__ __forceinline__ int cached(const AttnStepArgs& a, int b) {
 // Its units, one of them of an empty sequence, whose output somebody has to write.
 __device__ __forceinline__ int units_of(int len) { return max((len - 1) / kStepUnit + 1, 1); }
 
-// The sequences' units on the line, 64 sequences at a time by each wave.  (The host keeps the line under 2^31 units.)
-__device__ __forceinline__ int units_before(const AttnStepArgs& a, int b) {
-  int sum = 0;
-  for (int i = threadIdx.x & 63; i < b; i += 64) sum += units_of(cached(a, i));
-  return wave_sum(sum) * a.G * a.blocks;
-}
-// The sequence that unit x lies in, and how many units come before that.
-__device__ __forceinline__ int sequence_at(const AttnStepArgs& a, int x, int& before) {
-  const int lane = threadIdx.x & 63;
-  before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
-    const int n = b < a.B ? units_of(cached(a, b)) * a.G * a.blocks : 0;
-    const int upto = wave_sums(n);
+// A workgroup's run on the line of units, and where it begins.  (The host keeps the line under 2^31 units.)
+struct StepRun {
+  int per, begin, end;     // units of a run; this one's
+  int b, before, len;      // the sequence that the first of them lies in, the units before that, its tokens
+};
+// Up to 64 sequences, a lane each: their lengths are asked for once.  More: once for all, then 64 at a time up to the one.
+__device__ __forceinline__ StepRun find_run(const AttnStepArgs& a, int wg) {
+  const int lane = threadIdx.x & 63, each = a.G * a.blocks;
+  StepRun r{};
+  int len = lane < a.B ? cached(a, lane) : 0;
+  int n = lane < a.B ? units_of(len) : 0, upto = wave_sums(n), total = __builtin_amdgcn_readlane(upto, 63);
+  if (a.B > 64) {
+    int rest = 0;
+#pragma unroll 4
+    for (int b = 64 + lane; b < a.B; b += 64) rest += units_of(cached(a, b));
+    total += wave_sum(rest);
+  }
+  total *= each;
+  r.per = (total + a.wgs - 1) / a.wgs;
+  if ((long)wg * r.per >= total) return r;
+  r.begin = wg * r.per;
+  r.end = min(r.begin + r.per, total);
+  const int x = r.begin / each;                      // in units of all heads
+  int before = 0;
+  for (int b0 = 0;;) {
     const unsigned long long behind = __ballot(before + upto > x);
     if (behind) {
       const int l = __builtin_ctzll(behind);
-      before += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
-      return b0 + l;
+      r.b = b0 + l;
+      r.before = (before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l)) * each;
+      r.len = __builtin_amdgcn_readlane(len, l);
+      return r;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
+    b0 += 64;
+    len = b0 + lane < a.B ? cached(a, b0 + lane) : 0;
+    n = b0 + lane < a.B ? units_of(len) : 0;
+    upto = wave_sums(n);
   }
-  return a.B;
 }
-// Units of a workgroup's run.
-__device__ __forceinline__ int run_of(const AttnStepArgs& a, int total) { return (total + a.wgs - 1) / a.wgs; }
 
 template <typename E, int DP> struct StepLds {
   static constexpr int KEYS = sizeof(E) == 2 ? 32 : 16;    // of a wave's step
@@ -308,20 +323,25 @@ __global__ __launch_bounds__(64 * kStepWaves) void attn_step_kernel(AttnStepArgs
     return;
   }
   if (wg >= a.wgs) return;
-  const int total = units_before(a, a.B), per = run_of(a, total);
-  if ((long)wg * per >= total) return;
-  int x = wg * per, before;
-  const int begin = x, end = min(x + per, total);
-  int b = sequence_at(a, x, before), off = x - before;
-  while (x < end) {
-    const int len = wave_int(cached(a, b)), n = units_of(len), u = off / n, i0 = off % n, count = min(n - i0, end - x);
-    float* part = count == n ? nullptr : part_of<DP>(a, 2 * wg + (x == begin ? 0 : 1));
+  const StepRun run = find_run(a, wg);
+  int x = run.begin, b = run.b, len = run.len, off = x - run.before;
+  while (x < run.end) {
+    const int n = units_of(len), u = off / n, i0 = off % n, count = min(n - i0, run.end - x);
+    const int mine = 2 * wg + (x == run.begin ? 0 : 1);
+    float* part = count == n ? nullptr : part_of<DP>(a, mine);
+    if (i0 == 0 && threadIdx.x == 0) {               // (for the kernel that joins)
+      int* to = a.spread + 4L * (b * each + u);
+      to[0] = mine;
+      to[1] = wg;
+      to[2] = (x + n - 1) / run.per;
+    }
     step_segment<E, DP>(a, s, b, u / a.blocks, u % a.blocks, len, i0 * kStepUnit, min(len, (i0 + count) * kStepUnit), part);
     x += count;
     off += count;
     if (off == n * each) {
       off = 0;
       ++b;
+      if (x < run.end) len = wave_int(cached(a, b));
     }
   }
 }
@@ -336,13 +356,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnStepArgs a) {
   const int share = a.H / a.G, each = a.G * a.blocks;
   const int head = (int)block_id(), b = head / a.H, g = head % a.H / share, hr = head % share, hb = hr / 16, r = hr % 16;
   if (b >= a.B) return;
-  const int n = units_of(wave_int(cached(a, b)));
-  const int per = run_of(a, units_before(a, a.B));
-  const int x0 = units_before(a, b) + (g * a.blocks + hb) * n, w0 = x0 / per, w1 = (x0 + n - 1) / per;
+  // The first part is its workgroup's last piece, unless it begins that run; in the others it is the first.
+  const int* spread = a.spread + 4L * (b * each + g * a.blocks + hb);
+  const int p0 = spread[0], w0 = spread[1], w1 = spread[2], grp = threadIdx.x / LANES, col = threadIdx.x % LANES * 4;
   if (w0 == w1) return;
   const float sc = a.scale_log2;
-  // The first of them is its workgroup's last piece, unless it begins that run; in the others it is the first.
-  const int p0 = 2 * w0 + (w0 * per == x0 ? 0 : 1), grp = threadIdx.x / LANES, col = threadIdx.x % LANES * 4;
   floatx4 sum = zero4();
   float up = -INFINITY, weight = 0.f;
 #pragma unroll 4
