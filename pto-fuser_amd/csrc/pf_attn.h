@@ -2,7 +2,8 @@
 //   o_i = sum_j 2^{c (q_i . k_j - m_i)} v_j / l_i,     m_i a bound of q_i . k_j so far,  l_i = sum_j 2^{..}
 // in one pass over the keys: m_i, l_i and o_i are carried, and o_i and l_i are scaled down when m_i has to grow.
 //
-// A workgroup owns BM query rows of one head and walks the keys up to its last row in tiles.  The products are made
+// A workgroup's four waves own 32 query rows each: of four heads that share keys where there are as many, so that all four see
+// as many keys, else of two heads or one; it walks the keys up to its last row in tiles.  The products are made
 // transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane holds ONE query's column of S^T: the maximum and the sum over
 // keys are sums over its registers (and one swap with the other half of the wave), and the registers of P^T are at once the
 // operand of the second product (permuted K: see pf_device.h).  K and V tiles go from global memory to LDS directly, double
@@ -27,7 +28,9 @@ struct AttnArgs {
   const int* lengths;      // [B] or null: live rows of each
   long q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h;
   int N, B, H, G, D;
-  int tiles;               // of BM rows, at most, plus one or more that find none
+  int heads_log;           // log2 of the heads, that share one of keys, of a workgroup
+  int rows_log;            // log2 of its query rows
+  int tiles;               // of those rows, at most, plus one or more that find none
   int zero_rest;           // rows of no live token are written zero
   float scale_log2;
 };
@@ -134,16 +137,15 @@ struct AttnTile {
 
 // The longest tiles are to come first, and the shortest last, when the chip runs empty.  Up to 64 prompts, a lane each: the
 // tiles are numbered by their place in the prompt, the last place first, over all prompts, and a search over places finds the
-// tile.  More prompts: prompt b has tiles from cu[b] / BM + b on, which leaves it as many as it needs and one too many at most,
+// tile.  More prompts: prompt b has tiles from cu[b] / rows + b on, which leaves it as many as it needs and one too many at most,
 // so that a search in cu finds it.  (Offsets that fall find some prompt or none, inside the rows.)
-template <int BM>
 __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int tile) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, log = a.rows_log, up = (1 << log) - 1;
   AttnTile t{};
   int b, place;
   if (a.B <= 64) {
     const int start = min(max(a.cu[min(lane, a.B)], 0), a.N), end = min(max(a.cu[min(lane + 1, a.B)], start), a.N);
-    const int n = lane < a.B ? (end - start + BM - 1) / BM : 0;
+    const int n = lane < a.B ? (end - start + up) >> log : 0;
     const auto from = [&](int p) { return wave_sum(max(n - p, 0)); };     // tiles at place p and later
     const int all = from(0);
     t.excess = tile - all;
@@ -153,7 +155,7 @@ __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int tile) {
       t.last = max(min(max(wave_int(a.cu[a.B]), 0), a.N), t.first);
       return t;
     }
-    int lo = 0, hi = a.N / BM + 1, behind = 0;       // tiles from lo on are more than this one's number, from hi on `behind`
+    int lo = 0, hi = (a.N >> log) + 1, behind = 0;       // tiles from lo on are more than this one's number, from hi on `behind`
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2, count = from(mid);
       if (count > tile) {
@@ -176,12 +178,12 @@ __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int tile) {
     int lo = 0, count = a.B + 1;                     // entries of cu, the last of which at or before the tile is sought
     while (count > 1) {
       const int run = (count + 63) / 64, i = lo + min(lane * run, count - 1);
-      const unsigned long long before = __ballot(min(max(a.cu[i], 0), a.N) / BM + i <= tile && lane * run < count);
+      const unsigned long long before = __ballot((min(max(a.cu[i], 0), a.N) >> log) + i <= tile && lane * run < count);
       const int l = before ? 63 - __builtin_clzll(before) : 0;
       lo += l * run;
       count = min(run, count - l * run);
     }
-    const int start = min(max(wave_int(a.cu[lo]), 0), a.N), rank = tile - (start / BM + lo);
+    const int start = min(max(wave_int(a.cu[lo]), 0), a.N), rank = tile - ((start >> log) + lo);
     if (lo == a.B) {
       t.past = true;
       t.excess = max(rank, 0);
@@ -192,25 +194,27 @@ __device__ __forceinline__ AttnTile find_tile(const AttnArgs& a, int tile) {
     b = lo;
     t.start = start;
     t.extent = min(max(wave_int(a.cu[lo + 1]), start), a.N) - start;
-    const int tiles = (t.extent + BM - 1) / BM;
+    const int tiles = (t.extent + up) >> log;
     t.found = rank >= 0 && rank < tiles;
     place = tiles - 1 - rank;
   }
-  t.row0 = place * BM;
+  t.row0 = place << log;
   t.len = t.extent;
   if (a.lengths) t.len = min(max(wave_int(a.lengths[b]), 0), t.extent);
   return t;
 }
 
-// Zeros in rows [from, to) of the output's head h, by a workgroup.
+// Zeros in rows [from, to) of the output's heads from h on, by a workgroup.
 template <typename E>
 __device__ __forceinline__ void zero_rows(const AttnArgs& a, int h, long from, long to, long step, long rows) {
 #pragma unroll 1
   for (long r0 = from; r0 < to; r0 += step) {
     const long n = min(to - r0, rows);
 #pragma unroll 1
-    for (long i = threadIdx.x; i < n * a.D; i += blockDim.x)
-      static_cast<E*>(a.o)[(r0 + i / a.D) * a.o_t + h * a.o_h + i % a.D] = from_f32<E>(0.f);
+    for (long i = threadIdx.x; i < n * a.D << a.heads_log; i += blockDim.x) {
+      const long r = i / a.D;
+      static_cast<E*>(a.o)[(r0 + (r >> a.heads_log)) * a.o_t + (h + (r & ((1 << a.heads_log) - 1))) * a.o_h + i % a.D] = from_f32<E>(0.f);
+    }
   }
 }
 
@@ -223,21 +227,22 @@ template <typename E, int DP, int BN> struct AttnLds {
 // before it through the products with the zeros above the diagonal: the walk is then made AGAIN, which leaves such values of
 // the diagonal's tiles out of the products and adds them to the queries that see them.
 template <typename E, int DP, int KW, int BN, bool AGAIN>
-__device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>& s, const AttnTile& t, const int h) {
+__device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>& s, const AttnTile& t, const int h0) {
   using R = Rows<E, DP>;
   constexpr bool kBf = sizeof(E) == 2;
-  constexpr int NW = 4, RW = NW / KW, BM = RW * 32, KT = BN / KW / 32, DT = DP / 32, ES = sizeof(E);
+  constexpr int NW = 4, RW = NW / KW, KT = BN / KW / 32, DT = DP / 32, ES = sizeof(E);
   constexpr int LOADS = BN * R::RB / 1024 / NW;      // 1 KiB each, of a wave and operand
   constexpr int QV = DP / (kBf ? 16 : 8);            // 16-byte vectors of a lane's query
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hf = lane >> 5;
-  const int g = wave_int(h / (a.H / a.G));
-  const int kw = w / RW, q0 = t.row0 + w % RW * 32;  // the wave's part of a tile's keys, its first query
+  const int g = wave_int(h0 / (a.H / a.G));
+  // The wave's part of a tile's keys, its head and its first query.
+  const int kw = w / RW, h = h0 + (w % RW & ((1 << a.heads_log) - 1)), q0 = t.row0 + (w % RW >> a.heads_log) * 32;
 
   const char* kg = reinterpret_cast<const char*>(static_cast<const E*>(a.k) + (long)t.start * a.k_t + g * a.k_h);
   const char* vg = reinterpret_cast<const char*>(static_cast<const E*>(a.v) + (long)t.start * a.v_t + g * a.v_h);
   const uint32_t kt = (uint32_t)a.k_t * ES, vt = (uint32_t)a.v_t * ES;
-  const int rows_end = min(t.row0 + BM, t.len);      // keys that any query here sees
+  const int rows_end = min(t.row0 + (1 << a.rows_log), t.len);      // keys that any query here sees
   const int n_tiles = (rows_end + BN - 1) / BN;
 
   // A lane's place in the loads of a tile: row and (swizzled) chunk, the same chunk for all LOADS.  Rows past the last live one
@@ -279,14 +284,14 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
   if (kBf && KW == 1 && a.D == DP) {
     constexpr int QLOADS = 32 / FIRST;
     E* place = (w < 2 ? s.k[1] : s.v[1]) + (w & 1) * 32 * DP;
-    const char* from = reinterpret_cast<const char*>(static_cast<const E*>(a.q) + (long)(t.start + t.row0) * a.q_t + h * a.q_h);
+    const char* from = reinterpret_cast<const char*>(static_cast<const E*>(a.q) + (long)(t.start + min(q0, t.len - 1)) * a.q_t + h * a.q_h);
 #pragma unroll
     for (int i = 0; i < QLOADS; i += 4) {
       uint32_t off[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int row = (i + x) * FIRST + lane / R::CHUNKS;
-        off[x] = (uint32_t)min(w * 32 + row, t.len - 1 - t.row0) * (uint32_t)(a.q_t * ES) + (((lane % R::CHUNKS) ^ R::swizzle(row)) * 16);
+        off[x] = (uint32_t)min(row, max(t.len - 1 - q0, 0)) * (uint32_t)(a.q_t * ES) + (((lane % R::CHUNKS) ^ R::swizzle(row)) * 16);
       }
       async_loads<4, 1024>(from, lds_address(place) + i * 1024, off);
     }
@@ -493,15 +498,14 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
 
 template <typename E, int DP, int KW, int BN>
 __global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : 2) void attn_kernel(AttnArgs a) {
-  constexpr int BM = 128 / KW;
   __shared__ AttnLds<E, DP, BN> s;
   __shared__ int again;
   // Heads vary fastest, those of keys before those that share one, and go round robin over the eight XCDs: the workgroups that
   // read the same keys at the same time meet in few L2s.
-  const uint32_t bid = block_id(), hi = bid % (uint32_t)a.H, tile = bid / (uint32_t)a.H;
+  const uint32_t sets = (uint32_t)a.H >> a.heads_log, bid = block_id(), hi = bid % sets, tile = bid / sets;
   if (tile >= (uint32_t)a.tiles) return;
-  const int h = wave_int(hi % (uint32_t)a.G * (a.H / a.G) + hi / (uint32_t)a.G);
-  const AttnTile t = find_tile<BM>(a, wave_int(tile));
+  const int h = wave_int(hi % (uint32_t)a.G * (a.H / a.G) + (hi / (uint32_t)a.G << a.heads_log));
+  const AttnTile t = find_tile(a, wave_int(tile));
   if (t.past && a.zero_rest) {
     const long each = 64, step = (long)(a.tiles - ((int)tile - t.excess)) * each;
     zero_rows<E>(a, h, t.excess * each, t.first, step, each);
@@ -510,7 +514,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : 2) void attn
   if (!t.found) return;
   if (t.row0 >= t.len) {
     if (a.zero_rest) {
-      const long r = t.start + t.row0, n = min(t.extent - t.row0, BM);
+      const long r = t.start + t.row0, n = min(t.extent - t.row0, 1 << a.rows_log);
       zero_rows<E>(a, h, r, r + n, n, n);
     }
     return;
@@ -518,12 +522,14 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : 2) void attn
   if (a.D < DP) {                                    // columns past D
     u32x4* z = reinterpret_cast<u32x4*>(&s);
     for (int i = threadIdx.x; i < (int)(sizeof(s) / 16); i += 256) z[i] = u32x4{0, 0, 0, 0};
+    lds_barrier();
   }
-  if (threadIdx.x == 0) again = 0;
-  __syncthreads();
+  if (threadIdx.x == 0) again = 0;                   // (the walk's barriers lie between this and the next line)
   if (attn_walk<E, DP, KW, BN, false>(a, s, t, h)) again = 1;
+  lds_barrier();                                     // (the stores are under way: nobody waits for them)
+  if (!again) return;
   __syncthreads();
-  if (again) attn_walk<E, DP, KW, BN, true>(a, s, t, h);
+  attn_walk<E, DP, KW, BN, true>(a, s, t, h);
 }
 
 }  // namespace pf

@@ -36,10 +36,14 @@ bool grid_of(double workgroups, dim3& grid) {
 // ---- prompts -------------------------------------------------------------------------------
 template <typename E, int DP, int KW, int BN>
 int attn_launch(pf::AttnArgs& a, hipStream_t s) {
-  constexpr int BM = 128 / KW;
-  a.tiles = a.N / BM + a.B + 1;        // a prompt's last tile is ragged; and one that finds none
+  const int share = a.H / a.G;
+  a.heads_log = KW <= 1 && share % 4 == 0 ? 2 : KW <= 2 && share % 2 == 0 ? 1 : 0;
+  a.rows_log = (KW == 1 ? 7 : KW == 2 ? 6 : 5) - a.heads_log;
+  const double tiles = (double)(a.N >> a.rows_log) + a.B + 1;      // a prompt's last tile is ragged; and one that finds none
+  const double workgroups = tiles * (a.H >> a.heads_log);
   dim3 grid;
-  if ((double)a.tiles * a.H >= 2147483648.0 || !grid_of((double)a.tiles * a.H, grid)) return PF_ERR_ARG;
+  if (workgroups >= 2147483648.0 || !grid_of(workgroups, grid)) return PF_ERR_ARG;
+  a.tiles = (int)tiles;
   pf::LaunchScope scope;
   pf::attn_kernel<E, DP, KW, BN><<<grid, dim3(256), 0, s>>>(a);
   return scope.status();

@@ -233,11 +233,22 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
         p[t][i] = pow2(__builtin_fmaf(st[t][i], sc, -off));
         l += p[t][i];
       }
+    bf16x8 hi, lo;                                   // the weights in two terms of bf16
+    if constexpr (kBf) {
+      hi = pack8(p[0], p[KG - 1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[0][i] -= (float)hi[i];
+        p[KG - 1][i] -= (float)hi[4 + i];
+      }
+      lo = pack8(p[0], p[KG - 1]);
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       if constexpr (kBf) {
         const int row = 4 * gr + (c >> 2), col = 16 * dt + 4 * (c & 3);
-        o[dt] = mfma_bf16(cat8(lds_read_tr(vs + R::at(row, col)), lds_read_tr(vs + R::at(row + 16, col))), pack8(p[0], p[KG - 1]), o[dt]);
+        const bf16x8 f = cat8(lds_read_tr(vs + R::at(row, col)), lds_read_tr(vs + R::at(row + 16, col)));
+        o[dt] = mfma_bf16(f, hi, mfma_bf16(f, lo, o[dt]));
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
