@@ -67,25 +67,26 @@ def _vectors(t: torch.Tensor, strides) -> bool:
 
 def _strides(t: torch.Tensor):
     """Strides of all but the last dimension; 0 where there is nothing to step to, whatever the tensor says."""
-    s = t.stride()[:-1]
-    return s if 1 not in t.shape else tuple(0 if n == 1 else x for x, n in zip(s, t.shape))
+    s, n = t.stride()[:-1], t.shape
+    return s if 1 not in n else tuple([0 if m == 1 else x for x, m in zip(s, n)])
 
 
-def _bytes(t: torch.Tensor) -> int:
-    return t.numel() * t.element_size() if t.is_contiguous() else _span(t)
+def _ends(t: torch.Tensor):
+    """The address of a tensor's first byte and that after its last."""
+    lo = t.data_ptr()
+    return lo, lo + (t.numel() * t.element_size() if t.is_contiguous() else _span(t))
 
 
 def _clear(name: str, t: torch.Tensor, **others) -> None:
-    """``t``, which a call writes, overlaps neither itself nor ``others``: by their ends, and where that does not say, by
+    """``t``, which a call writes, overlaps neither itself nor ``others``: by their ends, and where those do not say, by
     :func:`serving._apart`."""
     if not t.is_contiguous():
         return _apart(name, t, **others)
-    lo = t.data_ptr()
-    hi = lo + t.numel() * t.element_size()
+    lo, hi = _ends(t)
     for u in others.values():
         if u is not None:
             at = u.data_ptr()
-            if at < hi and (at >= lo or at + _bytes(u) > lo):
+            if at < hi and (at >= lo or _ends(u)[1] > lo):
                 return _apart(name, t, **others)
 
 
@@ -102,7 +103,8 @@ def _tables(tables, slots, B: int, dev):
     _dim(tables, "tables", 2, "[S,M]")
     shape = tables.shape
     _require(tables, "tables", shape, torch.int32, dev)
-    _pool(tables, slots, B, dev)
+    if slots is not None or shape[0] != B:
+        _pool(tables, slots, B, dev)
     return shape
 
 
