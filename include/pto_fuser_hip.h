@@ -367,7 +367,7 @@ int pf_norm_exec(const pf_norm_args* args, void* stream);
  *   o_i = sum_{j <= i} softmax_j(scale q_i . k_j) v_j
  * q, o [N,H,D], k, v [N,G,D].  Rows of no live token are written zero (zero_rest) or not written.  A value that is not finite
  * reaches its own token and later ones of its prompt, as in the formula, and nothing before.
- * q, k, v: 16-byte aligned with strides of whole 16-byte vectors; token strides of k and v up to 2^22 elements. */
+ * q, k, v: 16-byte aligned with strides of whole 16-byte vectors; token strides up to 2^22 elements. */
 typedef struct pf_attn_args {
   size_t size;
   const void* q;         /* E */

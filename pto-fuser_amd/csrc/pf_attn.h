@@ -519,16 +519,19 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : 2) void attn
     }
     return;
   }
-  if (a.D < DP) {                                    // columns past D
+  const auto clear = [&] {                           // columns past D: no load writes them
+    if (a.D == DP) return;
     u32x4* z = reinterpret_cast<u32x4*>(&s);
     for (int i = threadIdx.x; i < (int)(sizeof(s) / 16); i += 256) z[i] = u32x4{0, 0, 0, 0};
     lds_barrier();
-  }
+  };
+  clear();
   if (threadIdx.x == 0) again = 0;                   // (the walk's barriers lie between this and the next line)
   if (attn_walk<E, DP, KW, BN, false>(a, s, t, h)) again = 1;
   lds_barrier();                                     // (the stores are under way: nobody waits for them)
   if (!again) return;
   __syncthreads();
+  clear();
   attn_walk<E, DP, KW, BN, true>(a, s, t, h);
 }
 

@@ -118,7 +118,7 @@ int pf_attn_exec(const pf_attn_args* p, void* stream) {
   if (!p->q || !p->k || !p->v || !p->o) return PF_ERR_ARG;
   if (!vectors(p->dtype, p->q, p->q_t, p->q_h) || !vectors(p->dtype, p->k, p->k_t, p->k_h) || !vectors(p->dtype, p->v, p->v_t, p->v_h))
     return PF_ERR_ARG;
-  if (p->k_t > kMaxRowStride || p->v_t > kMaxRowStride || p->o_t < 0 || p->o_h < 0) return PF_ERR_ARG;
+  if (p->q_t > kMaxRowStride || p->k_t > kMaxRowStride || p->v_t > kMaxRowStride || p->o_t < 0 || p->o_h < 0) return PF_ERR_ARG;
   pf::AttnArgs a{};
   a.q = p->q; a.k = p->k; a.v = p->v; a.o = p->o; a.cu = p->cu; a.lengths = p->lengths;
   a.q_t = p->q_t; a.q_h = p->q_h; a.k_t = p->k_t; a.k_h = p->k_h; a.v_t = p->v_t; a.v_h = p->v_h; a.o_t = p->o_t; a.o_h = p->o_h;

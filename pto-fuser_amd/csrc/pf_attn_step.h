@@ -62,14 +62,14 @@ __device__ __forceinline__ StepRun find_run(const AttnStepArgs& a, int wg) {
   total *= each;
   r.per = (total + a.wgs - 1) / a.wgs;
   if ((long)wg * r.per >= total) return r;
-  r.begin = wg * r.per;
-  r.end = min(r.begin + r.per, total);
-  const int x = r.begin / each;                      // in units of all heads
+  const int x = wg * r.per / each;                   // in units of all heads
   int before = 0;
-  for (int b0 = 0;;) {
+  for (int b0 = 0; b0 < a.B;) {
     const unsigned long long behind = __ballot(before + upto > x);
     if (behind) {
       const int l = __builtin_ctzll(behind);
+      r.begin = wg * r.per;
+      r.end = min(r.begin + r.per, total);
       r.b = b0 + l;
       r.before = (before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l)) * each;
       r.len = __builtin_amdgcn_readlane(len, l);
@@ -81,6 +81,7 @@ __device__ __forceinline__ StepRun find_run(const AttnStepArgs& a, int wg) {
     n = b0 + lane < a.B ? units_of(len) : 0;
     upto = wave_sums(n);
   }
+  return r;
 }
 
 template <typename E, int DP> struct StepLds {
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void attn_step_kernel(AttnStepArgs
   if (wg >= a.wgs) return;
   const StepRun run = find_run(a, wg);
   int x = run.begin, b = run.b, len = run.len, off = x - run.before;
-  while (x < run.end) {
+  while (x < run.end && b < a.B) {
     const int n = units_of(len), u = off / n, i0 = off % n, count = min(n - i0, run.end - x);
     const int mine = 2 * wg + (x == run.begin ? 0 : 1);
     float* part = count == n ? nullptr : part_of<DP>(a, mine);
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void attn_step_kernel(AttnStepArgs
     if (off == n * each) {
       off = 0;
       ++b;
-      if (x < run.end) len = wave_int(cached(a, b));
+      if (x < run.end && b < a.B) len = wave_int(cached(a, b));
     }
   }
 }

@@ -44,8 +44,8 @@ def _heads(H: int, G: int, D: int) -> None:
 
 def _scale(scale: Optional[float], D: int) -> float:
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 1e-30 < scale < 1e30:
+        raise ValueError(f"scale must be positive and between 1e-30 and 1e30, got {scale}")
     return scale
 
 

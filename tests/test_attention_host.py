@@ -50,7 +50,7 @@ def _attn(**kw):
 @pytest.mark.parametrize("bad", [dict(size=8), dict(dtype=2), dict(H=3), dict(H=0), dict(G=0), dict(D=12), dict(D=136), dict(D=0),
                                  dict(N=-1), dict(N=(1 << 30) + 1), dict(B=-1), dict(cu=0), dict(q=0), dict(k=0), dict(v=0), dict(o=0),
                                  dict(q=66), dict(k=72), dict(v=8), dict(s0=4), dict(s2=-8), dict(s3=12), dict(s4=1 << 23),
-                                 dict(s7=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+                                 dict(s0=1 << 23), dict(s7=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
                                  dict(N=1 << 30, H=65536, G=1)])
 def test_attention_statuses(lib, bad):
     assert lib.pf_attn_exec(_attn(**bad), None) == _hip.PF_ERR_ARG
@@ -162,7 +162,7 @@ def test_attention_checks(on_cpu):
                       ("cu_seqlens has dtype", dict(cu_seqlens=torch.zeros(3, dtype=torch.int64))),
                       ("an entry more", dict(cu_seqlens=torch.zeros(0, dtype=I32))), ("cu_seqlens must be", dict(cu_seqlens=None)),
                       ("lengths has shape", dict(lengths=torch.zeros(3, dtype=I32))), ("scale", dict(scale=0.0)),
-                      ("scale", dict(scale=float("inf"))), ("out has shape", dict(out=q[:9])), ("out may not be q", dict(q=q, out=q))):
+                      ("scale", dict(scale=float("inf"))), ("scale", dict(scale=1e39)), ("scale", dict(scale=-0.1)), ("out has shape", dict(out=q[:9])), ("out may not be q", dict(q=q, out=q))):
         with pytest.raises(ValueError, match=match):
             _attn_call(**kw)
     with pytest.raises((ValueError, TypeError)):

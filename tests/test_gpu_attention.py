@@ -182,8 +182,8 @@ def test_scores_that_rise_along_the_keys():
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("what,H,G", [(NAN, 4, 2), (INF, 4, 2), (NAN, 256, 2), (INF, 80, 2)])
+@pytest.mark.parametrize("what,H,G,D", [(NAN, 4, 2, 64), (INF, 4, 2, 128), (NAN, 256, 2, 64), (INF, 80, 2, 128), (NAN, 6, 2, 40),
+                                        (INF, 256, 2, 96), (NAN, 80, 2, 120), (INF, 96, 2, 32)])
 def test_values_that_are_not_finite(dtype, D, what, H, G):
     """In v they reach their own column from their own token on, in a key the tokens from it on, in a query its own row;
     the next prompt and the other heads stay as they are."""
@@ -200,6 +200,12 @@ def test_values_that_are_not_finite(dtype, D, what, H, G):
         o = ref.f64(causal_attention(q, k, v, _cu(lens)))
         assert torch.equal(~torch.isfinite(o), bad), t
         assert torch.equal(o[~bad], good[~bad]), t
+    q, k, v = (x.clone() for x in clean)                 # a later token's, and another's of the same tile
+    v[300, 0, D - 1], v[302, 0, 0] = what, -INF
+    bad = torch.zeros(sum(lens), H, D, dtype=torch.bool)
+    bad[300:n, :H // 2, D - 1] = bad[302:n, :H // 2, 0] = True
+    o = ref.f64(causal_attention(q, k, v, _cu(lens)))
+    assert torch.equal(~torch.isfinite(o), bad) and torch.equal(o[~bad], good[~bad])
     for t in (0, 70, 329):
         q, k, v = (x.clone() for x in clean)
         k[t, 0, 5] = NAN
