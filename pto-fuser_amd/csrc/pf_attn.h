@@ -218,7 +218,8 @@ __device__ __forceinline__ void zero_rows(const AttnArgs& a, int h, long from, l
   }
 }
 
-template <typename E, int DP, int BN> struct AttnLds {
+template <typename E, int DP, int KW> struct AttnLds {
+  static constexpr int BN = 32 * KW;                 // keys of a tile
   E k[2][BN * DP], v[2][BN * DP];
   float bounds[4][2][64];                            // of waves that share rows
 };
@@ -226,11 +227,11 @@ template <typename E, int DP, int BN> struct AttnLds {
 // One workgroup's walk.  Returns whether an output came out not finite.  A value of v that is not finite reaches the queries
 // before it through the products with the zeros above the diagonal: the walk is then made AGAIN, which leaves such values of
 // the diagonal's tiles out of the products and adds them to the queries that see them.
-template <typename E, int DP, int KW, int BN, bool AGAIN>
-__device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>& s, const AttnTile& t, const int h0) {
+template <typename E, int DP, int KW, bool AGAIN>
+__device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>& s, const AttnTile& t, const int h0) {
   using R = Rows<E, DP>;
   constexpr bool kBf = sizeof(E) == 2;
-  constexpr int NW = 4, RW = NW / KW, KT = BN / KW / 32, DT = DP / 32, ES = sizeof(E);
+  constexpr int NW = 4, BN = AttnLds<E, DP, KW>::BN, RW = NW / KW, DT = DP / 32, ES = sizeof(E);
   constexpr int LOADS = BN * R::RB / 1024 / NW;      // 1 KiB each, of a wave and operand
   constexpr int QV = DP / (kBf ? 16 : 8);            // 16-byte vectors of a lane's query
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -278,33 +279,13 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
 
   if (n_tiles > 0) load(0, 0);
 
-  // Q: a lane has row q0 + 32 qt + c; columns 16 kb + 8 hf .. (fp32: 8 kb + 4 hf ..).  Whole bf16 rows come through the second
-  // buffers, whole lines at a time (32 rows of the wave fill half of one).
+  // Q: a lane has row q0 + c; columns 16 kb + 8 hf .. (fp32: 8 kb + 4 hf ..)
   u32x4 q[QV];
-  if (kBf && KW == 1 && a.D == DP) {
-    constexpr int QLOADS = 32 / FIRST;
-    E* place = (w < 2 ? s.k[1] : s.v[1]) + (w & 1) * 32 * DP;
-    const char* from = reinterpret_cast<const char*>(static_cast<const E*>(a.q) + (long)(t.start + min(q0, t.len - 1)) * a.q_t + h * a.q_h);
+  const E* qp = static_cast<const E*>(a.q) + (t.start + min(q0 + c, t.len - 1)) * a.q_t + h * a.q_h;
 #pragma unroll
-    for (int i = 0; i < QLOADS; i += 4) {
-      uint32_t off[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int row = (i + x) * FIRST + lane / R::CHUNKS;
-        off[x] = (uint32_t)min(row, max(t.len - 1 - q0, 0)) * (uint32_t)(a.q_t * ES) + (((lane % R::CHUNKS) ^ R::swizzle(row)) * 16);
-      }
-      async_loads<4, 1024>(from, lds_address(place) + i * 1024, off);
-    }
-    wait_loads();
-#pragma unroll
-    for (int kb = 0; kb < QV; ++kb) q[kb] = *reinterpret_cast<const u32x4*>(place + R::at(c, (kb * 2 + hf) * R::V));
-  } else {
-    const E* p = static_cast<const E*>(a.q) + (t.start + min(q0 + c, t.len - 1)) * a.q_t + h * a.q_h;
-#pragma unroll
-    for (int kb = 0; kb < QV; ++kb) {
-      const int col = (kb * 2 + hf) * R::V;
-      q[kb] = col < a.D ? *reinterpret_cast<const u32x4*>(p + col) : u32x4{0, 0, 0, 0};
-    }
+  for (int kb = 0; kb < QV; ++kb) {
+    const int col = (kb * 2 + hf) * R::V;
+    q[kb] = col < a.D ? *reinterpret_cast<const u32x4*>(qp + col) : u32x4{0, 0, 0, 0};
   }
 
   floatx16 o[DT];
@@ -322,101 +303,106 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
     if (tile + 1 < n_tiles) load(tile + 1, buf ^ 1);
     const E* ks = s.k[buf];
     const E* vs = s.v[buf];
-    const int jw = j0 + kw * (BN / KW), kv0 = kw * (BN / KW);
-    if (jw > q0 + 31) return;                        // nothing of the tile is visible to these queries
-    {
-      floatx16 st[KT];
+    const int row0 = 32 * kw, jw = j0 + row0;        // the wave's keys of the tile
+    if (jw > q0) return;                             // (both are multiples of 32: nothing of them is visible to its queries)
+    // Where a wave or two share a SIMD nobody else hides LDS: the operands are asked for AHEAD of the products, those of V
+    // before the weights.  Three waves hide it for each other, and have no registers for that.
+    constexpr bool AHEAD = kBf && (KW > 1 || DP == 64);
+    const auto k_at = [&](int kb) { return *reinterpret_cast<const u32x4*>(ks + R::at(row0 + c, (kb * 2 + hf) * R::V)); };
+    const int v_row = row0 + 4 * hf + ((lane & 15) >> 2), v_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const auto v_at = [&](int j, int dt) {
+      const bf16* v = reinterpret_cast<const bf16*>(vs);
+      return cat8(lds_read_tr(v + R::at(v_row + 16 * j, v_col + 32 * dt)), lds_read_tr(v + R::at(v_row + 16 * j + 8, v_col + 32 * dt)));
+    };
+    floatx16 st = zero16();
+    u32x4 kf[AHEAD ? QV : 1];
+    bf16x8 vf[AHEAD ? 2 : 1][AHEAD ? DT : 1];
+    if constexpr (AHEAD) {
 #pragma unroll
-      for (int kt2 = 0; kt2 < KT; ++kt2) {
-        st[kt2] = zero16();
+      for (int kb = 0; kb < QV; ++kb) kf[kb] = k_at(kb);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-        for (int kb = 0; kb < QV; ++kb) {
-          const u32x4 f = *reinterpret_cast<const u32x4*>(ks + R::at(kv0 + 32 * kt2 + c, (kb * 2 + hf) * R::V));
-          if constexpr (kBf) {
-            st[kt2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, q[kb]),
-                                                              st[kt2], 0, 0, 0);
-          } else {
+    for (int kb = 0; kb < QV; ++kb) {
+      const u32x4 f = AHEAD ? kf[AHEAD ? kb : 0] : k_at(kb);
+      if constexpr (kBf) {
+        st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, q[kb]), st, 0, 0, 0);
+      } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              st[kt2] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f[i]), __uint_as_float(q[kb][i]), st[kt2], 0, 0, 0);
+        for (int i = 0; i < 4; ++i)
+          st = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f[i]), __uint_as_float(q[kb][i]), st, 0, 0, 0);
+      }
+    }
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) vf[j][dt] = v_at(j, dt);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const bool masked = jw == q0;                    // on the diagonal
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + i % 4 > c - 4 * hf) st[i] = -INFINITY;
+    }
+    float top = st[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, st[i]);
+    top = half_max(top);
+    if (__ballot((top - m) * sc > kAttnRescale)) {   // (-inf - -inf is no number and asks for nothing)
+      const float up = fmaxf(top, m);
+      const float f = m == -INFINITY ? 0.f : pow2((m - up) * sc);
+      m = up;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+    }
+    const float off = m == -INFINITY ? 0.f : m * sc;
+    float p[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[i] = pow2(__builtin_fmaf(st[i], sc, -off));
+      l += p[i];
+    }
+    if constexpr (kBf) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        bf16x8 pb;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pb[i] = (bf16)p[8 * j + i];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          bf16x8 f = AHEAD ? vf[AHEAD ? j : 0][AHEAD ? dt : 0] : v_at(j, dt);
+          if (AGAIN && masked) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __builtin_isfinite((float)f[i]) ? f[i] : (bf16)0.f;
           }
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, pb, o[dt], 0, 0, 0);
         }
       }
-      const bool masked = jw + 32 * KT - 1 > q0;
-      if (masked) {
-        const int lim = q0 + c - jw - 4 * hf;        // the last key that the query sees, from the lane's first
+    } else {
 #pragma unroll
-        for (int kt2 = 0; kt2 < KT; ++kt2)
+      for (int i = 0; i < 16; ++i) {
+        const int row = row0 + 8 * (i / 4) + 4 * hf + i % 4;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * kt2 + 8 * (i / 4) + i % 4 > lim) st[kt2][i] = -INFINITY;
-      }
-      float top = st[0][0];
-#pragma unroll
-      for (int kt2 = 0; kt2 < KT; ++kt2)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, st[kt2][i]);
-      top = half_max(top);
-      if (__ballot((top - m) * sc > kAttnRescale)) {       // (-inf - -inf is no number and asks for nothing)
-        const float up = fmaxf(top, m);
-        const float f = m == -INFINITY ? 0.f : pow2((m - up) * sc);
-        m = up;
-        l *= f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
-      }
-      const float off = m == -INFINITY ? 0.f : m * sc;
-      float p[KT][16];
-#pragma unroll
-      for (int kt2 = 0; kt2 < KT; ++kt2)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          p[kt2][i] = pow2(__builtin_fmaf(st[kt2][i], sc, -off));
-          l += p[kt2][i];
+        for (int dt = 0; dt < DT; ++dt) {
+          float f = vs[R::at(row, 32 * dt + c)];
+          if (AGAIN && masked) f = __builtin_isfinite(f) ? f : 0.f;
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(f, p[i], o[dt], 0, 0, 0);
         }
+      }
+    }
+    if (AGAIN && masked) {
+#pragma unroll 1
+      for (int j = 0; j < 32; ++j)
 #pragma unroll
-      for (int kt2 = 0; kt2 < KT; ++kt2) {
-        if constexpr (kBf) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            bf16x8 pb;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pb[i] = (bf16)p[kt2][8 * j + i];
-            const int row = kv0 + 32 * kt2 + 16 * j + 4 * hf + ((lane & 15) >> 2);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-              const int col = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-              bf16x8 vf = cat8(lds_read_tr(vs + R::at(row, col)), lds_read_tr(vs + R::at(row + 8, col)));
-              if (AGAIN && masked) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) vf[i] = __builtin_isfinite((float)vf[i]) ? vf[i] : (bf16)0.f;
-              }
-              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[dt], 0, 0, 0);
-            }
-          }
-        } else {
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int row = kv0 + 32 * kt2 + 8 * (i / 4) + 4 * hf + i % 4;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-              float vf = vs[R::at(row, 32 * dt + c)];
-              if (AGAIN && masked) vf = __builtin_isfinite(vf) ? vf : 0.f;
-              o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, p[kt2][i], o[dt], 0, 0, 0);
-            }
+            const float x = to_f32(vs[R::at(row0 + j, 32 * dt + 8 * (i / 4) + 4 * hf + i % 4)]);
+            if (!__builtin_isfinite(x) && j <= c) o[dt][i] += x;
           }
-        }
-      }
-      if (AGAIN && masked) {
-        for (int j = 0; j < BN / KW; ++j)
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float x = to_f32(vs[R::at(kv0 + j, 32 * dt + 8 * (i / 4) + 4 * hf + i % 4)]);
-              if (!__builtin_isfinite(x) && jw + j <= q0 + c) o[dt][i] += x;
-            }
-      }
     }
   };
   for (int tile = 0; tile < n_tiles; tile += 2) {    // (twice, so that the buffers' addresses are constants)
@@ -467,7 +453,6 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
   }
   // The output by way of LDS, where each wave has a quarter, so that it is stored in whole rows.
   E* const place = reinterpret_cast<E*>(&s) + w * BN * DP;
-  static_assert(BN >= 32, "a wave's rows fit a buffer");
   typedef typename VecAny<E, R::V>::T Out;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float spoilt = inv * 0.f;                          // 0 of finite values, else NaN
@@ -496,9 +481,9 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, BN>&
   return bad;
 }
 
-template <typename E, int DP, int KW, int BN>
-__global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : 2) void attn_kernel(AttnArgs a) {
-  __shared__ AttnLds<E, DP, BN> s;
+template <typename E, int DP, int KW>
+__global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : KW > 1 ? 2 : 3) void attn_kernel(AttnArgs a) {
+  __shared__ AttnLds<E, DP, KW> s;
   __shared__ int again;
   // Heads vary fastest, those of keys before those that share one, and go round robin over the eight XCDs: the workgroups that
   // read the same keys at the same time meet in few L2s.
@@ -527,12 +512,12 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : 2) void attn
   };
   clear();
   if (threadIdx.x == 0) again = 0;                   // (the walk's barriers lie between this and the next line)
-  if (attn_walk<E, DP, KW, BN, false>(a, s, t, h)) again = 1;
+  if (attn_walk<E, DP, KW, false>(a, s, t, h)) again = 1;
   lds_barrier();                                     // (the stores are under way: nobody waits for them)
   if (!again) return;
   __syncthreads();
   clear();
-  attn_walk<E, DP, KW, BN, true>(a, s, t, h);
+  attn_walk<E, DP, KW, true>(a, s, t, h);
 }
 
 }  // namespace pf

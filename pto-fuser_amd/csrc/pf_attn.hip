@@ -34,7 +34,7 @@ bool grid_of(double workgroups, dim3& grid) {
 }
 
 // ---- prompts -------------------------------------------------------------------------------
-template <typename E, int DP, int KW, int BN>
+template <typename E, int DP, int KW>
 int attn_launch(pf::AttnArgs& a, hipStream_t s) {
   const int share = a.H / a.G;
   a.heads_log = KW <= 1 && share % 4 == 0 ? 2 : KW <= 2 && share % 2 == 0 ? 1 : 0;
@@ -45,30 +45,31 @@ int attn_launch(pf::AttnArgs& a, hipStream_t s) {
   if (workgroups >= 2147483648.0 || !grid_of(workgroups, grid)) return PF_ERR_ARG;
   a.tiles = (int)tiles;
   pf::LaunchScope scope;
-  pf::attn_kernel<E, DP, KW, BN><<<grid, dim3(256), 0, s>>>(a);
+  pf::attn_kernel<E, DP, KW><<<grid, dim3(256), 0, s>>>(a);
   return scope.status();
 }
 
-// Waves that share a query row, each with a part of every tile's keys.  Alone they read each key once for 128 queries; sharing
-// makes two or four times as many workgroups, of as many times fewer steps each, for calls whose workgroups are few or whose
-// longest one is what is waited for.  By the number of workgroups without sharing (prompts x rows x heads; us alone / two / four):
-//   bf16, D = 128: 1 x 2048 x 16 (256) 42.7 / 33.9 / 67, 1 x 4096 x 16 (512) 92 / 88 / 206, 24 x 512 x 16 (1536) 49 / 66 / 237,
-//                  2 x 2048 x 32 (1024) 81 / 93 / 261; four have 133 KB of LDS and a wave a SIMD: 1 x 1024 x 8 (64) 23.3 / 18.2 / 17.2
-//   bf16, D = 64:  1 x 1024 x 16 (128) 18.2 / 14.0 / 11.9, 1 x 1536 x 16 (192) 24.3 / 18.7 / 19.6, 1 x 4096 x 16 60 / 51 / 69,
-//                  1 x 6144 x 16 (768) 100.9 / 103.0 / 137
-//   fp32, D = 128: 1 x 2048 x 16 277 / 171, 3 x 2048 x 8 (384) 277 / 270, 1 x 4096 x 16 593 / 629
-//   fp32, D = 64:  1 x 1024 x 16 75 / 42 / 36, 3 x 512 x 16 (192) 41.6 / 30.2 / 38.0, 1 x 1536 x 16 111.8 / 73.6 / 72.4, a padded
-//                  batch of 3 x 1471 x 6 with 61 % live rows (207) 106 / 72 / 54, 1 x 6144 x 16 640 / 614 / 845, 4 x 4096 x 16 1062 / 1072
+// Waves that share a query row, each with a part of every tile's keys.  Alone a wave walks all of them, and three workgroups a CU
+// hide each other's waiting; sharing makes two or four times as many workgroups of as many times fewer steps, which is better
+// where workgroups are few, or where the longest one is what is waited for.  By the number of workgroups without sharing (rows x
+// heads / 128) and the prompts' mean length; us alone / two / four, prompts x rows x heads, 4 (fp32 ragged: 3) heads to one of keys:
+//   bf16, D = 128: 1 x 2048 x 16 (256) 55 / 32.3, 4 x 512 x 16 (256) 19.0 / 13.8, 6 x 512 (384) 21.1 / 22.1, 2 x 2048 (512) 61 / 54,
+//                  8 x 512 (512) 23.5 / 26, 1 x 6144 (768) 188 / 178, 3 x 2048 (768) 69 / 72, 1 x 8192 (1024) 288 / 306;
+//                  four, with 133 KB of LDS, are nowhere faster than two by more than a twentieth
+//   bf16, D = 64:  1 x 1024 x 16 (128) 20.2 / 13.0 / 11.3, 1 x 1536 (192) 27.7 / 17.8 / 18.8, 4 x 512 12.7 / 11.1 / 14.4, 12 x 512
+//                  (768) 14.8 / 18.5, 1 x 6144 110 / 100
+//   fp32, D = 128: 1 x 2048 x 16 274 / 169, 3 x 2048 x 8 (384) 274 / 270, 1 x 4096 x 16 (512) 580 / 620
+//   fp32, D = 64:  1 x 1024 x 16 73 / 41 / 35, 3 x 512 (192) 40.3 / 29.7 / 36.7, 1 x 1536 108 / 72.6 / 69.7, a padded batch of
+//                  3 x 1471 x 6 with 61 % live rows (207) 103 / 71 / 52, 12 x 512 72 / 74, 2 x 4096 (1024) 562 / 542, 4 x 4096 1026 / 1067
 template <typename E, int DP>
 int attn_width(pf::AttnArgs& a, hipStream_t s) {
   constexpr bool kBf = sizeof(E) == 2;
-  const double alone = (double)a.N / 128 * a.H;
-  if (alone > (kBf ? 512 : DP == 64 ? 768 : 384)) return attn_launch<E, DP, 1, kBf ? 64 : 32>(a, s);
+  const double alone = (double)a.N / 128 * a.H, mean = a.B > 0 ? (double)a.N / a.B : 0;
+  if (alone > (kBf ? 384 + mean / 16 : DP == 64 ? 768 + mean / 16 : 384)) return attn_launch<E, DP, 1>(a, s);
   if constexpr (DP == 64) {
-    const bool long_ones = !kBf && a.B > 0 && a.N / a.B >= 1024;
-    if (alone <= (long_ones ? 224 : 128)) return attn_launch<E, DP, 4, 128>(a, s);
+    if (alone <= (!kBf && mean >= 1024 ? 224 : 128)) return attn_launch<E, DP, 4>(a, s);
   }
-  return attn_launch<E, DP, 2, 64>(a, s);
+  return attn_launch<E, DP, 2>(a, s);
 }
 
 // ---- single tokens -------------------------------------------------------------------------
