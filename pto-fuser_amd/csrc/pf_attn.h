@@ -220,7 +220,8 @@ __device__ __forceinline__ void zero_rows(const AttnArgs& a, int h, long from, l
 
 template <typename E, int DP, int KW> struct AttnLds {
   static constexpr int BN = 32 * KW;                 // keys of a tile
-  E k[2][BN * DP], v[2][BN * DP];
+  static constexpr int BUFS = KW == 4 ? 1 : 2;
+  E k[BUFS][BN * DP], v[BUFS][BN * DP];
   float bounds[4][2][64];                            // of waves that share rows
 };
 
@@ -277,7 +278,30 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>&
     }
   };
 
-  if (n_tiles > 0) load(0, 0);
+  // Four waves that share rows read nothing of each other's keys: each loads its own, K again as soon as the scores are made
+  // and V as soon as the products are, into the one buffer of it, and there is no barrier.  Columns past D repeat the first.
+  constexpr int OWN = KW == 4 ? 32 * R::RB / 1024 : 1;     // loads of a wave's 32 keys
+  const int own_tiles = q0 >= 32 * kw ? (q0 - 32 * kw) / BN + 1 : 0;
+  const auto own_load = [&](const char* from, uint32_t pitch, E* to, int tile) {
+    const int j0 = tile * BN + 32 * kw, last = t.len - 1 - j0;
+    uint32_t off[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int row = i * FIRST + lane / R::CHUNKS, chunk = (lane % R::CHUNKS) ^ R::swizzle(row);
+      off[i] = (uint32_t)min(row, last) * pitch + (chunk * R::V < a.D ? chunk * 16 : 0);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);              // this wave's reads of the buffer
+    async_loads<OWN, 1024>(from + (long)j0 * pitch, lds_address(to + 32 * kw * DP), off);
+  };
+
+  if constexpr (KW == 4) {
+    if (own_tiles > 0) {
+      own_load(kg, kt, s.k[0], 0);
+      own_load(vg, vt, s.v[0], 0);
+    }
+  } else {
+    load(0, 0);
+  }
 
   // Q: a lane has row q0 + c; columns 16 kb + 8 hf .. (fp32: 8 kb + 4 hf ..)
   u32x4 q[QV];
@@ -294,21 +318,18 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>&
   float m = -INFINITY, l = 0.f;
   const float sc = a.scale_log2;
 
-  const auto step = [&](const int tile, auto parity) {
-    constexpr int buf = decltype(parity)::value;
-    const int j0 = tile * BN;
-    wait_loads();
-    __builtin_amdgcn_s_barrier();
-    __asm__ __volatile__("" ::: "memory");
-    if (tile + 1 < n_tiles) load(tile + 1, buf ^ 1);
-    const E* ks = s.k[buf];
-    const E* vs = s.v[buf];
-    const int row0 = 32 * kw, jw = j0 + row0;        // the wave's keys of the tile
-    if (jw > q0) return;                             // (both are multiples of 32: nothing of them is visible to its queries)
+  // The wave's keys from jw on, in rows 32 kw .. of a tile; the hooks stand where its reads of K are made, before those of V
+  // and after them.
+  const auto work = [&](const int jw, const E* ks, const E* vs, auto k_read, auto v_next, auto v_read) {
+    const int row0 = 32 * kw;
     // Where a wave or two share a SIMD nobody else hides LDS: the operands are asked for AHEAD of the products, those of V
     // before the weights.  Three waves hide it for each other, and have no registers for that.
     constexpr bool AHEAD = kBf && (KW > 1 || DP == 64);
-    const auto k_at = [&](int kb) { return *reinterpret_cast<const u32x4*>(ks + R::at(row0 + c, (kb * 2 + hf) * R::V)); };
+    const auto k_at = [&](int kb) {
+      const int col = (kb * 2 + hf) * R::V;
+      const u32x4 f = *reinterpret_cast<const u32x4*>(ks + R::at(row0 + c, col));
+      return KW == 4 && col >= a.D ? u32x4{0, 0, 0, 0} : f;
+    };
     const int v_row = row0 + 4 * hf + ((lane & 15) >> 2), v_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     const auto v_at = [&](int j, int dt) {
       const bf16* v = reinterpret_cast<const bf16*>(vs);
@@ -333,7 +354,9 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>&
           st = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f[i]), __uint_as_float(q[kb][i]), st, 0, 0, 0);
       }
     }
+    k_read();
     if constexpr (AHEAD) {
+      v_next();
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -365,6 +388,7 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>&
       p[i] = pow2(__builtin_fmaf(st[i], sc, -off));
       l += p[i];
     }
+    if constexpr (!AHEAD) v_next();
     if constexpr (kBf) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -404,10 +428,32 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>&
             if (!__builtin_isfinite(x) && j <= c) o[dt][i] += x;
           }
     }
+    v_read();
   };
-  for (int tile = 0; tile < n_tiles; tile += 2) {    // (twice, so that the buffers' addresses are constants)
-    step(tile, std::integral_constant<int, 0>{});
-    if (tile + 1 < n_tiles) step(tile + 1, std::integral_constant<int, 1>{});
+  if constexpr (KW == 4) {
+    wait_loads();                                    // (the query: the compiler counts its own loads)
+    for (int tile = 0; tile < own_tiles; ++tile) {
+      const bool more = tile + 1 < own_tiles;
+      wait_all_but<OWN>();                           // V is under way
+      work(tile * BN + 32 * kw, s.k[0], s.v[0], [&] { if (more) own_load(kg, kt, s.k[0], tile + 1); },
+           [&] { if (more) wait_all_but<OWN>(); else wait_all_but<0>(); },
+           [&] { if (more) own_load(vg, vt, s.v[0], tile + 1); });
+    }
+  } else {
+    const auto step = [&](const int tile, auto parity) {
+      constexpr int buf = decltype(parity)::value;
+      wait_loads();
+      __builtin_amdgcn_s_barrier();
+      __asm__ __volatile__("" ::: "memory");
+      if (tile + 1 < n_tiles) load(tile + 1, buf ^ 1);
+      const int jw = tile * BN + 32 * kw;
+      const auto nothing = [] {};
+      if (jw <= q0) work(jw, s.k[buf], s.v[buf], nothing, nothing, nothing);   // (multiples of 32: else nothing is visible)
+    };
+    for (int tile = 0; tile < n_tiles; tile += 2) {  // (twice, so that the buffers' addresses are constants)
+      step(tile, std::integral_constant<int, 0>{});
+      if (tile + 1 < n_tiles) step(tile + 1, std::integral_constant<int, 1>{});
+    }
   }
 
   // Waves that share the rows: their sums at one bound, in the first of them.

@@ -55,19 +55,20 @@ int attn_launch(pf::AttnArgs& a, hipStream_t s) {
 // heads / 128) and the prompts' mean length; us alone / two / four, prompts x rows x heads, 4 (fp32 ragged: 3) heads to one of keys:
 //   bf16, D = 128: 1 x 2048 x 16 (256) 55 / 32.3, 4 x 512 x 16 (256) 19.0 / 13.8, 6 x 512 (384) 21.1 / 22.1, 2 x 2048 (512) 61 / 54,
 //                  8 x 512 (512) 23.5 / 26, 1 x 6144 (768) 188 / 178, 3 x 2048 (768) 69 / 72, 1 x 8192 (1024) 288 / 306;
-//                  four, with 133 KB of LDS, are nowhere faster than two by more than a twentieth
-//   bf16, D = 64:  1 x 1024 x 16 (128) 20.2 / 13.0 / 11.3, 1 x 1536 (192) 27.7 / 17.8 / 18.8, 4 x 512 12.7 / 11.1 / 14.4, 12 x 512
-//                  (768) 14.8 / 18.5, 1 x 6144 110 / 100
+//                  four are not built: they were nowhere faster than two by more than a twentieth
+//   bf16, D = 64:  1 x 1024 x 16 (128) 20.2 / 13.8 / 11.7, 1 x 1536 (192) 27.7 / 18.3 / 15.0, 1 x 2048 35.5 / 22.4 / 24.8, 3 x 512
+//                  (192) 12.5 / 11.1 / 11.3, 4 x 512 12.7 / 11.2 / 15.0, 12 x 512 (768) 14.8 / 18.5, 1 x 6144 110 / 100
 //   fp32, D = 128: 1 x 2048 x 16 274 / 169, 3 x 2048 x 8 (384) 274 / 270, 1 x 4096 x 16 (512) 580 / 620
-//   fp32, D = 64:  1 x 1024 x 16 73 / 41 / 35, 3 x 512 (192) 40.3 / 29.7 / 36.7, 1 x 1536 108 / 72.6 / 69.7, a padded batch of
-//                  3 x 1471 x 6 with 61 % live rows (207) 103 / 71 / 52, 12 x 512 72 / 74, 2 x 4096 (1024) 562 / 542, 4 x 4096 1026 / 1067
+//   fp32, D = 64:  1 x 1024 x 16 73 / 41 / 34, 3 x 512 (192) 40.3 / 29.8 / 30.5, 1 x 2048 143 / 104 / 93, 3 x 2048 x 8 178 / 124 / 127, a
+//                  padded batch of 3 x 1471 x 6 with 61 % live rows (207) 103 / 71.6 / 50.3, 12 x 512 72 / 74, 2 x 4096 (1024) 562 / 542,
+//                  4 x 4096 1026 / 1067
 template <typename E, int DP>
 int attn_width(pf::AttnArgs& a, hipStream_t s) {
   constexpr bool kBf = sizeof(E) == 2;
   const double alone = (double)a.N / 128 * a.H, mean = a.B > 0 ? (double)a.N / a.B : 0;
   if (alone > (kBf ? 384 + mean / 16 : DP == 64 ? 768 + mean / 16 : 384)) return attn_launch<E, DP, 1>(a, s);
   if constexpr (DP == 64) {
-    if (alone <= (!kBf && mean >= 1024 ? 224 : 128)) return attn_launch<E, DP, 4>(a, s);
+    if (alone <= (mean < 1024 ? 128 : kBf ? 192 : 256)) return attn_launch<E, DP, 4>(a, s);
   }
   return attn_launch<E, DP, 2>(a, s);
 }
