@@ -8,6 +8,20 @@
 // keys are sums over its registers (and one swap with the other half of the wave), and the registers of P^T are at once the
 // operand of the second product (permuted K: see pf_device.h).  K and V tiles go from global memory to LDS directly, double
 // buffered, one barrier a tile.
+//
+// Rounding: scores, bounds, sums and outputs are fp32; with bf16 operands the weights enter the second product in bf16 (one
+// rounding of 2^-9 to 2^-8 each: the output is 2.0e-3 of its norm off, 1.7e-3 by its own rounding alone).  A second term for
+// them would cost half of that product again, which bounds the kernel; single tokens have it (pf_attn_step.h).
+//
+// Measured, bf16, D = 128: 1 prompt of 32768, 32 heads over 8 of keys, 7.57 to 7.72 ms, 1140 to 1160 TFLOP/s; the library's
+// product of 8192^3 reaches 1213 to 1224 on the same card.  Under it the shader clock falls to 1.6 GHz (12.3 million cycles a
+// pass), of which the matrix pipes work 8.4 million, the vector port 7.4; L2 answers 96 % of the tiles.  4 x 4096 x 16 heads
+// 262 to 270 us (1020 to 1050 TFLOP/s): the diagonal's tiles and each workgroup's start and end.  D = 64: 2.2 ms for 1 x 32768 x
+// 16, 1000 TFLOP/s: the vector port, with as many weights to half the products.  fp32, D = 128: 1.13 ms for 2 x 4096 x 16, 121 of
+// the library's 154 TFLOP/s.  Tried on the way (4 x 4096 x 16, us): one wave a SIMD 603, two 297, loads in flight past the
+// compiler's waits 274, tiles of 32 keys and three waves 262; the diagonal's second half left out by a branch (spills, 310),
+// the weights' sum by dot products of bf16 pairs (no gain), 128 rows of one head a workgroup instead of 32 of four (the
+// same here, 48 prompts of up to 512 tokens 48 to 43).
 #pragma once
 
 #include "pf_gfx950.h"

@@ -4,6 +4,10 @@
 // Requests are served in order.  With c tokens in the cache and n new ones, request b needs ceil((c + n) / page) - ceil(c /
 // page) pages: free[taken + those of all before it ..].  One that the rest of the pool does not hold gets none, and no later
 // one that needs any does; so the ones served are a prefix, and a sum over the requests before gives each its place.
+//
+// Latency, not bytes: 64 prompts of up to 1024 tokens 4.4 us, 256 requests of a token each 3.4 us (a launch of nothing takes 2.4);
+// as one workgroup and a second launch for the rows they took 9.4 and 7.3.  Storing: 16384 tokens of 4 heads of 128, 67 MB
+// 11.4 us, 5.9 TB/s (what the last pass wrote is partly still in the memory-side cache).
 #pragma once
 
 #include "pf_serving.h"
