@@ -358,7 +358,7 @@ int pf_norm_exec(const pf_norm_args* args, void* stream);
 /* ------------------------------------------------------------------------------------------
  * Attention of a served model: causal attention over prompts, one token over a cache of keys and values in pages, and the
  * cache's bookkeeping.  Conventions as above.  H query heads share G heads of keys and values (head h reads h / (H / G));
- * D is a multiple of 8 up to 128; scale > 0.  A row whose tokens are none, or whose scores are all minus infinity, is zero.
+ * D is a multiple of 8 up to 256; scale > 0.  A row whose tokens are none, or whose scores are all minus infinity, is zero.
  * A page holds `page` rows, a power of two from 16 to 65536; a row of the cache is page_index * page + offset.
  * ------------------------------------------------------------------------------------------ */
 

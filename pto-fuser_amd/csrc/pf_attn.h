@@ -18,7 +18,7 @@
 // pass), of which the matrix pipes work 8.4 million, the vector port 7.4; L2 answers 96 % of the tiles.  4 x 4096 x 16 heads
 // 262 to 270 us (1020 to 1050 TFLOP/s): the diagonal's tiles and each workgroup's start and end.  D = 64: 2.2 ms for 1 x 32768 x
 // 16, 1000 TFLOP/s: the vector port, with as many weights to half the products.  fp32, D = 128: 1.13 ms for 2 x 4096 x 16, 121 of
-// the library's 154 TFLOP/s.  Tried on the way (4 x 4096 x 16, us): one wave a SIMD 603, two 297, loads in flight past the
+// the library's 154 TFLOP/s.  D = 256, a wave a SIMD (492 registers): bf16 700 TFLOP/s, fp32 100.  Tried on the way (4 x 4096 x 16, us): one wave a SIMD 603, two 297, loads in flight past the
 // compiler's waits 274, tiles of 32 keys and three waves 262; the diagonal's second half left out by a branch (spills, 310),
 // the weights' sum by dot products of bf16 pairs (no gain), 128 rows of one head a workgroup instead of 32 of four (the
 // same here, 48 prompts of up to 512 tokens 48 to 43).
@@ -121,7 +121,8 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 template <typename E, int DP> struct Rows {
   static constexpr int V = 16 / (int)sizeof(E), RB = DP * (int)sizeof(E), CHUNKS = RB / 16;
   __device__ __forceinline__ static constexpr int swizzle(int row) {
-    if constexpr (RB > 256) return ((row & 3) << 2) | ((row >> 2) & 1);     // (fp32: twice is no loss beside its products)
+    if constexpr (RB > 512) return (row & 3) << 2;
+    if constexpr (RB > 256) return ((row & 3) << 2) | ((row >> 2) & 1);     // (wide rows: two or four of 16 meet, beside products enough)
     if constexpr (RB == 256) return ((row & 3) << 2) | ((row >> 2) & 3);
     else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
   }
@@ -335,10 +336,11 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>&
   // The wave's keys from jw on, in rows 32 kw .. of a tile; the hooks stand where its reads of K are made, before those of V
   // and after them.
   const auto work = [&](const int jw, const E* ks, const E* vs, auto k_read, auto v_next, auto v_read) {
-    const int row0 = 32 * kw;
+    int row0 = 32 * kw;
+    if constexpr (!kBf && DP == 256) __asm__ __volatile__("" : "+v"(row0));     // (places in LDS made anew: kept, they would spill)
     // Where a wave or two share a SIMD nobody else hides LDS: the operands are asked for AHEAD of the products, those of V
     // before the weights.  Three waves hide it for each other, and have no registers for that.
-    constexpr bool AHEAD = kBf && (KW > 1 || DP == 64);
+    constexpr bool AHEAD = kBf && DP <= 128 && (KW > 1 || DP == 64);
     const auto k_at = [&](int kb) {
       const int col = (kb * 2 + hf) * R::V;
       const u32x4 f = *reinterpret_cast<const u32x4*>(ks + R::at(row0 + c, col));
@@ -542,7 +544,7 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>&
 }
 
 template <typename E, int DP, int KW>
-__global__ __launch_bounds__(256, sizeof(E) == 4 && DP == 128 ? 1 : KW > 1 ? 2 : 3) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP == 256 || (sizeof(E) == 4 && DP == 128) ? 1 : KW > 1 ? 2 : 3) void attn_kernel(AttnArgs a) {
   __shared__ AttnLds<E, DP, KW> s;
   __shared__ int again;
   // Heads vary fastest, those of keys before those that share one, and go round robin over the eight XCDs: the workgroups that

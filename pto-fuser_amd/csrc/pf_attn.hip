@@ -15,7 +15,7 @@ constexpr int kMaxRows = 1 << 30;
 constexpr long long kMaxRowStride = 1LL << 22;   // elements: offsets inside a tile are 32-bit
 
 bool heads_ok(int H, int G, int D, int dtype) {
-  return H > 0 && G > 0 && H % G == 0 && H <= 65536 && D > 0 && D <= 128 && D % 8 == 0 &&
+  return H > 0 && G > 0 && H % G == 0 && H <= 65536 && D > 0 && D <= 256 && D % 8 == 0 &&
          (dtype == PF_DTYPE_F32 || dtype == PF_DTYPE_BF16);
 }
 
@@ -56,6 +56,7 @@ int attn_launch(pf::AttnArgs& a, hipStream_t s) {
 //   bf16, D = 128: 1 x 2048 x 16 (256) 55 / 32.3, 4 x 512 x 16 (256) 19.0 / 13.8, 6 x 512 (384) 21.1 / 22.1, 2 x 2048 (512) 61 / 54,
 //                  8 x 512 (512) 23.5 / 26, 1 x 6144 (768) 188 / 178, 3 x 2048 (768) 69 / 72, 1 x 8192 (1024) 288 / 306;
 //                  four are not built: they were nowhere faster than two by more than a twentieth
+//   bf16, D = 256: 1 x 1024 x 8 (64) 58.5 / 40.3, 1 x 2048 x 16 (256) 107 / 83, 4 x 512 (256) 36 / 38, 8 x 512 45 / 72, 1 x 4096 226 / 276
 //   bf16, D = 64:  1 x 1024 x 16 (128) 20.2 / 13.8 / 11.7, 1 x 1536 (192) 27.7 / 18.3 / 15.0, 1 x 2048 35.5 / 22.4 / 24.8, 3 x 512
 //                  (192) 12.5 / 11.1 / 11.3, 4 x 512 12.7 / 11.2 / 15.0, 12 x 512 (768) 14.8 / 18.5, 1 x 6144 110 / 100
 //   fp32, D = 128: 1 x 2048 x 16 274 / 169, 3 x 2048 x 8 (384) 274 / 270, 1 x 4096 x 16 (512) 580 / 620
@@ -66,15 +67,24 @@ template <typename E, int DP>
 int attn_width(pf::AttnArgs& a, hipStream_t s) {
   constexpr bool kBf = sizeof(E) == 2;
   const double alone = (double)a.N / 128 * a.H, mean = a.B > 0 ? (double)a.N / a.B : 0;
-  if (alone > (kBf ? 384 + mean / 16 : DP == 64 ? 768 + mean / 16 : 384)) return attn_launch<E, DP, 1>(a, s);
+  if (DP == 256 && !kBf) return attn_launch<E, DP, 1>(a, s);      // (two would have 256 KB of LDS)
+  if (alone > (DP == 256 ? 128 + mean / 16 : kBf ? 384 + mean / 16 : DP == 64 ? 768 + mean / 16 : 384)) return attn_launch<E, DP, 1>(a, s);
   if constexpr (DP == 64) {
     if (alone <= (mean < 1024 ? 128 : kBf ? 192 : 256)) return attn_launch<E, DP, 4>(a, s);
   }
-  return attn_launch<E, DP, 2>(a, s);
+  if constexpr (kBf || DP < 256) return attn_launch<E, DP, 2>(a, s);
+  return PF_ERR_ARG;
 }
 
+// The kernels' widths: a head's columns up to the next are zero.
+template <typename E>
+int attn_heads(pf::AttnArgs& a, hipStream_t s) {
+  return a.D <= 64 ? attn_width<E, 64>(a, s) : a.D <= 128 ? attn_width<E, 128>(a, s) : attn_width<E, 256>(a, s);
+}
+int padded(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
 // ---- single tokens -------------------------------------------------------------------------
-constexpr int kStepWgs = 512;          // workgroups that share a walk: two a CU, which their LDS fills (heads up to 64: four)
+constexpr int kStepWgs = 512;          // workgroups that share a walk: two a CU, which their LDS fills (heads up to 64: four; past 128: one)
 
 struct StepPlan {
   int rows, wgs, blocks;
@@ -87,9 +97,9 @@ bool step_plan(int B, int H, int G, int D, int M, int page, StepPlan& p) {
   const double units = rows * ((tokens + pf::kStepUnit - 1) / pf::kStepUnit + 1);
   if (tokens > kMaxRows || units >= 2147483648.0) return false;
   p.rows = (int)rows;
-  const double wgs = D <= 64 ? 2 * kStepWgs : kStepWgs;
+  const double wgs = (double)kStepWgs * 128 / padded(D);
   p.wgs = tokens <= 512 ? 0 : (int)(units < wgs ? units : wgs);
-  p.parts = (size_t)p.wgs * 2 * 16 * ((D <= 64 ? 64 : 128) + 4);
+  p.parts = (size_t)p.wgs * 2 * 16 * (padded(D) + 4);
   p.bytes = p.wgs ? p.parts * sizeof(float) + (size_t)p.rows * 4 * sizeof(int) : 0;
   return true;
 }
@@ -102,6 +112,11 @@ int step_launch(const pf::AttnStepArgs& a, const StepPlan& p, hipStream_t s) {
   pf::attn_step_kernel<E, DP><<<grid, dim3(64 * pf::kStepWaves), 0, s>>>(a);
   if (p.wgs) pf::attn_join_kernel<E, DP><<<rows, dim3(256), 0, s>>>(a);
   return scope.status();
+}
+
+template <typename E>
+int step_heads(const pf::AttnStepArgs& a, const StepPlan& p, hipStream_t s) {
+  return a.D <= 64 ? step_launch<E, 64>(a, p, s) : a.D <= 128 ? step_launch<E, 128>(a, p, s) : step_launch<E, 256>(a, p, s);
 }
 
 int log2_of(int page) {
@@ -127,8 +142,7 @@ int pf_attn_exec(const pf_attn_args* p, void* stream) {
   a.N = p->N; a.B = p->B; a.H = p->H; a.G = p->G; a.D = p->D; a.zero_rest = p->zero_rest;
   a.scale_log2 = p->scale * 1.44269504088896340736f;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p->dtype == PF_DTYPE_BF16) return p->D <= 64 ? attn_width<bf16, 64>(a, s) : attn_width<bf16, 128>(a, s);
-  return p->D <= 64 ? attn_width<float, 64>(a, s) : attn_width<float, 128>(a, s);
+  return p->dtype == PF_DTYPE_BF16 ? attn_heads<bf16>(a, s) : attn_heads<float>(a, s);
 }
 
 size_t pf_attn_step_workspace_bytes(int B, int H, int G, int D, int M, int page, int dtype) {
@@ -159,8 +173,7 @@ int pf_attn_step_exec(const pf_attn_step_args* p, void* stream) {
   a.blocks = pl.blocks; a.wgs = pl.wgs;
   a.scale_log2 = p->scale * 1.44269504088896340736f;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p->dtype == PF_DTYPE_BF16) return p->D <= 64 ? step_launch<bf16, 64>(a, pl, s) : step_launch<bf16, 128>(a, pl, s);
-  return p->D <= 64 ? step_launch<float, 64>(a, pl, s) : step_launch<float, 128>(a, pl, s);
+  return p->dtype == PF_DTYPE_BF16 ? step_heads<bf16>(a, pl, s) : step_heads<float>(a, pl, s);
 }
 
 }  // extern "C"

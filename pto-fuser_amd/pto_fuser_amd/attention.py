@@ -32,7 +32,7 @@ _STORE = struct.Struct("@N5P10q6i")
 _ATTN_SIZE, _ATTN_STEP_SIZE, _ASSIGN_SIZE, _RELEASE_SIZE, _STORE_SIZE = (
     _size(s) for s in (_ATTN, _ATTN_STEP, _ASSIGN, _RELEASE, _STORE))
 
-HEAD_MAX = 128
+HEAD_MAX = 256
 ROW_MAX_STRIDE = 1 << 22
 MAX_TOKENS = 1 << 30
 
@@ -122,7 +122,7 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention over prompts packed in one buffer: o_i = Σ_{j≤i} softmax_j(scale · q_i·k_j) v_j within each prompt.
 
-    q [N,H,D], k and v [N,G,D], float32 or bfloat16, D a multiple of 8 up to 128, query head h reading head h // (H // G) of
+    q [N,H,D], k and v [N,G,D], float32 or bfloat16, D a multiple of 8 up to 256, query head h reading head h // (H // G) of
     keys and values; token and head strides are free (operands whose rows are not whole 16-byte vectors, or whose tokens lie
     more than 2^22 elements apart, are copied first).  ``cu_seqlens`` [B+1] int32, rising: prompt b has rows cu_seqlens[b] up
     to cu_seqlens[b+1], of which the first ``lengths[b]`` (int32; None: all) are live; a padded batch [B,T] has cu_seqlens of

@@ -205,8 +205,9 @@ class AttentionLayer:
 
     def prefill(self, hidden: torch.Tensor, residual: Optional[torch.Tensor], cache: KvCache,
                 plan: PagePlan) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Whole prompts, packed: hidden, residual [N,D] with N the plan's capacity -> (output [N,D], the residual stream).
-        Their keys and values go to the plan's rows; a prompt that it did not serve is computed and not stored."""
+        """Whole prompts, packed, of requests that the cache held nothing of: hidden, residual [N,D] with N the plan's
+        capacity -> (output [N,D], the residual stream).  Their keys and values go to the plan's rows; a prompt that it did
+        not serve is computed and not stored."""
         y, stream = add_rms_norm(hidden, self.norm_w, residual)
         q, k, v = self._operands(y)
         store_kv(k, v, cache.k, cache.v, plan.rows)

@@ -47,7 +47,7 @@ def _attn(**kw):
     return attention._ATTN.pack(*{**f, **kw}.values())
 
 
-@pytest.mark.parametrize("bad", [dict(size=8), dict(dtype=2), dict(H=3), dict(H=0), dict(G=0), dict(D=12), dict(D=136), dict(D=0),
+@pytest.mark.parametrize("bad", [dict(size=8), dict(dtype=2), dict(H=3), dict(H=0), dict(G=0), dict(D=12), dict(D=264), dict(D=0),
                                  dict(N=-1), dict(N=(1 << 30) + 1), dict(B=-1), dict(cu=0), dict(q=0), dict(k=0), dict(v=0), dict(o=0),
                                  dict(q=66), dict(k=72), dict(v=8), dict(s0=4), dict(s2=-8), dict(s3=12), dict(s4=1 << 23),
                                  dict(s0=1 << 23), dict(s7=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),

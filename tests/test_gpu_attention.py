@@ -52,7 +52,8 @@ def _check_prompts(o, q, k, v, lens, what, scale=None):
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("lens,H,G,D", [
     ([1], 1, 1, 8), ([2, 0, 1], 2, 1, 64), ([31, 33, 64, 65], 4, 2, 64), ([127, 128, 129], 2, 2, 128), ([300], 6, 1, 40),
-    ([5, 0, 0, 257, 3], 5, 5, 80), ([200, 56], 8, 2, 120), ([513], 3, 3, 128), ([1] * 70 + [90], 2, 1, 32), ([0, 0], 2, 1, 64)])
+    ([5, 0, 0, 257, 3], 5, 5, 80), ([200, 56], 8, 2, 120), ([513], 3, 3, 128), ([1] * 70 + [90], 2, 1, 32), ([0, 0], 2, 1, 64),
+    ([1, 65, 0, 130], 4, 2, 256), ([33, 300], 3, 1, 200), ([64], 2, 2, 136)])
 def test_prompts(dtype, lens, H, G, D):
     announce(f"causal_attention {dtype} {lens[:5]} H{H} G{G} D{D}")
     q, k, v = _qkv(lens, H, G, D, dtype, sum(lens) + D)
@@ -63,7 +64,7 @@ def test_prompts(dtype, lens, H, G, D):
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("lens,H,G,D", [
     ([1100, 37], 64, 8, 64), ([900], 80, 16, 128), ([1] * 100 + [700, 0, 65], 64, 4, 128), ([700, 500], 24, 3, 64), ([1025], 32, 2, 128),
-    ([130] * 9, 16, 4, 72)])
+    ([130] * 9, 16, 4, 72), ([1100, 37], 64, 8, 256), ([500, 129], 64, 16, 168)])
 def test_many_workgroups(dtype, lens, H, G, D):
     """Sizes at which a row is one wave's, two waves' and four waves', up to 64 prompts and more of them; some heads of each."""
     announce(f"causal_attention {dtype} {lens[-2:]} of {len(lens)} H{H} G{G} D{D}")
@@ -183,7 +184,7 @@ def test_scores_that_rise_along_the_keys():
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("what,H,G,D", [(NAN, 4, 2, 64), (INF, 4, 2, 128), (NAN, 256, 2, 64), (INF, 80, 2, 128), (NAN, 6, 2, 40),
-                                        (INF, 256, 2, 96), (NAN, 80, 2, 120), (INF, 96, 2, 32)])
+                                        (INF, 256, 2, 96), (NAN, 80, 2, 120), (INF, 96, 2, 32), (NAN, 4, 2, 256), (INF, 160, 2, 144)])
 def test_values_that_are_not_finite(dtype, D, what, H, G):
     """In v they reach their own column from their own token on, in a key the tokens from it on, in a query its own row;
     the next prompt and the other heads stay as they are."""
@@ -283,7 +284,8 @@ def _check_step(o, q, rows, lens, what, scale=None):
 @pytest.mark.parametrize("lens,H,G,D,page", [
     ([1], 1, 1, 8, 16), ([0, 1, 2, 15, 16, 17], 4, 2, 64, 16), ([127, 128, 129, 31, 33], 8, 1, 128, 16), ([600], 16, 1, 64, 32),
     ([700, 3], 20, 1, 80, 16), ([5, 900], 40, 2, 128, 64), ([1023, 0, 1], 6, 2, 64, 128), ([4097], 5, 5, 128, 16),
-    ([64] * 70 + [2000], 2, 1, 64, 16), ([300, 40], 2, 2, 120, 256)])
+    ([64] * 70 + [2000], 2, 1, 64, 16), ([300, 40], 2, 2, 120, 256),
+    ([1, 0, 700, 33], 8, 2, 256, 16), ([2500], 6, 1, 192, 64), ([90, 600], 20, 1, 136, 16)])
 def test_step(dtype, lens, H, G, D, page):
     announce(f"attention_step {dtype} {lens[:5]} H{H} G{G} D{D} page{page}")
     (k, v), tables, rows = _paged(lens, G, D, page, dtype, sum(lens) + D)
