@@ -95,7 +95,7 @@ bool step_plan(int B, int H, int G, int D, int M, int page, StepPlan& p) {
   p.blocks = (H / G + 15) / 16;
   const double rows = (double)B * G * p.blocks, tokens = (double)M * page;
   const double units = rows * ((tokens + pf::kStepUnit - 1) / pf::kStepUnit + 1);
-  if (tokens > kMaxRows || units >= 2147483648.0) return false;
+  if (tokens > kMaxRows || units > kMaxRows) return false;       // (a run's end stays an int)
   p.rows = (int)rows;
   const double wgs = (double)kStepWgs * 128 / padded(D);
   p.wgs = tokens <= 512 ? 0 : (int)(units < wgs ? units : wgs);

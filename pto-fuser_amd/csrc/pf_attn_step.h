@@ -50,7 +50,7 @@ __device__ __forceinline__ int cached(const AttnStepArgs& a, int b) {
 // Its units, one of them of an empty sequence, whose output somebody has to write.
 __device__ __forceinline__ int units_of(int len) { return max((len - 1) / kStepUnit + 1, 1); }
 
-// A workgroup's run on the line of units, and where it begins.  (The host keeps the line under 2^31 units.)
+// A workgroup's run on the line of units, and where it begins.  (The host keeps the line to 2^30 units.)
 struct StepRun {
   int per, begin, end;     // units of a run; this one's
   int b, before, len;      // the sequence that the first of them lies in, the units before that, its tokens

@@ -15,6 +15,7 @@ names each request's row of it as it names states elsewhere (no two the same; on
 """
 from __future__ import annotations
 
+import functools
 import struct
 from typing import NamedTuple, Optional
 
@@ -40,6 +41,12 @@ MAX_TOKENS = 1 << 30
 def _heads(H: int, G: int, D: int) -> None:
     if H == 0 or G == 0 or H % G or not 0 < D <= HEAD_MAX or D % 8:
         raise ValueError(f"unsupported shape H={H} G={G} D={D} (H a multiple of G, D of 8 up to {HEAD_MAX})")
+
+
+def _needed(t, name: str, shape, dtype, dev) -> None:
+    if t is None:
+        raise ValueError(f"{name} must be a tensor")
+    _require(t, name, shape, dtype, dev)
 
 
 def _scale(scale: Optional[float], D: int) -> float:
@@ -164,6 +171,11 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     return o
 
 
+@functools.lru_cache(maxsize=1024)
+def _step_workspace(*sizes: int) -> int:
+    return _hip.load().pf_attn_step_workspace_bytes(*sizes)
+
+
 def attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tables: torch.Tensor,
                    lengths: torch.Tensor, *, slots: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -185,7 +197,7 @@ def attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _heads(H, G, D)
     _require_view(q, "q", (B, H, D), dtype, dev)
     S, M = _tables(tables, slots, B, dev)
-    _require(lengths, "lengths", (B,), torch.int32, dev)
+    _needed(lengths, "lengths", (B,), torch.int32, dev)
     if M * page > MAX_TOKENS:
         raise ValueError(f"tables hold {M} pages of {page} (up to {MAX_TOKENS} tokens)")
     sk, sv = _strides(k_cache), _strides(v_cache)
@@ -200,10 +212,11 @@ def attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         _clear("out", out, q=q, k_cache=k_cache, v_cache=v_cache, tables=tables, lengths=lengths, slots=slots)
         o = out
     q, sq = _rows(q)
-    need = _hip.load().pf_attn_step_workspace_bytes(B, H, G, D, M, page, code)
+    need = _step_workspace(B, H, G, D, M, page, code)
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     _exec("pf_attn_step_exec", dev, _ATTN_STEP, _ATTN_STEP_SIZE, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-          o.data_ptr(), tables.data_ptr(), lengths.data_ptr(), _ptr(slots), _ptr(ws), need, *sq, *_strides(o), *sk, *sv, B, S, H, G, D, M, pages, page, code, scale)
+          o.data_ptr(), tables.data_ptr(), lengths.data_ptr(), _ptr(slots), _ptr(ws), need, *sq, *_strides(o), *sk, *sv,
+          B, S, H, G, D, M, pages, page, code, scale)
     return o
 
 
@@ -225,7 +238,7 @@ def _pool_state(tables, lengths, free, taken, slots, page_size: int, dev):
         raise ValueError(f"tables hold {M} pages of {page_size} (up to {MAX_TOKENS} tokens)")
     _dim(free, "free", 1, "[F]")
     _require(free, "free", free.shape, torch.int32, dev)
-    _require(taken, "taken", (1,), torch.int32, dev)
+    _needed(taken, "taken", (1,), torch.int32, dev)
     return B, S, M, free.shape[0]
 
 
@@ -293,7 +306,7 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     pages, page, Gc, Dc = _cache(k_cache, v_cache, dtype, dev)
     if (Gc, Dc) != (G, D):
         raise ValueError(f"k_cache has {Gc} heads of {Dc}, expected {G} of {D}")
-    _require(rows, "rows", (N,), torch.int64, dev)
+    _needed(rows, "rows", (N,), torch.int64, dev)
     _clear("k_cache", k_cache, k=k, v=v, v_cache=v_cache, rows=rows)
     _clear("v_cache", v_cache, k=k, v=v, rows=rows)
     _exec("pf_store_exec", dev, _STORE, _STORE_SIZE, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),

@@ -194,7 +194,7 @@ def test_step_checks(on_cpu):
                       ("heads of 32", dict(k_cache=c[..., :32], v_cache=c[..., :32])), ("unsupported shape", dict(q=torch.zeros(3, 5, 64))),
                       ("tables must be", dict(tables=None)), ("tables has dtype", dict(tables=torch.zeros(3, 7))),
                       ("state holds 2", dict(tables=torch.zeros(2, 7, dtype=I32))),
-                      ("lengths has shape", dict(lengths=torch.zeros(2, dtype=I32))), ("slots has dtype", dict(slots=torch.zeros(3))),
+                      ("lengths has shape", dict(lengths=torch.zeros(2, dtype=I32))), ("lengths must be", dict(lengths=None)), ("slots has dtype", dict(slots=torch.zeros(3))),
                       ("whole 16-byte", dict(k_cache=torch.zeros(5, 16, 2, 65)[..., 1:])),
                       ("out may not be", dict(q=c[:3, 0, :].repeat(1, 2, 1), out=c[:3, :4, 0], v_cache=c))):
         with pytest.raises(ValueError, match=match):
@@ -218,7 +218,7 @@ def test_pages_checks(on_cpu):
     assert call(tokens=None, capacity=None).rows.shape == (3,)
     z = torch.zeros(3, dtype=I32)
     for match, kw in (("tables must be", dict(tables=z)), ("lengths must be", dict(lengths=None)), ("tokens has shape", dict(tokens=z[:2])),
-                      ("free has dtype", dict(free=z.long())), ("taken has shape", dict(taken=z)), ("power of two", dict(page_size=48)),
+                      ("free has dtype", dict(free=z.long())), ("taken has shape", dict(taken=z)), ("taken must be", dict(taken=None)), ("free must be", dict(free=None)), ("power of two", dict(page_size=48)),
                       ("capacity must be given", dict(capacity=None)), ("capacity must be 0", dict(capacity=-1)),
                       ("state holds 2", dict(tables=torch.zeros(2, 7, dtype=I32))), ("slots has shape", dict(slots=z[:2]))):
         with pytest.raises(ValueError, match=match):
@@ -240,7 +240,8 @@ def test_store_checks(on_cpu):
     call()
     c = torch.zeros(5, 16, 2, 64)
     for match, kw in (("k must be", dict(k=c)), ("v has shape", dict(v=torch.zeros(3, 2, 64))), ("rows has dtype", dict(rows=torch.zeros(4, dtype=I32))),
-                      ("rows has shape", dict(rows=torch.zeros(5, dtype=torch.int64))), ("expected 2 of 64", dict(k_cache=c[:, :, :1], v_cache=c[:, :, :1])),
+                      ("rows has shape", dict(rows=torch.zeros(5, dtype=torch.int64))), ("rows must be", dict(rows=None)), ("v must be", dict(v=None)),
+                      ("k_cache must be", dict(k_cache=None)), ("v_cache must be", dict(v_cache=None)), ("expected 2 of 64", dict(k_cache=c[:, :, :1], v_cache=c[:, :, :1])),
                       ("power of two", dict(k_cache=c[:, :12], v_cache=c[:, :12])), ("v_cache has shape", dict(v_cache=c[1:])),
                       ("k_cache may not be v_cache", dict(k_cache=c, v_cache=c)),
                       ("k_cache has overlapping rows", dict(k_cache=c[:, :1].expand(5, 16, 2, 64)))):
