@@ -249,6 +249,37 @@ def test_store_checks(on_cpu):
             call(**kw)
 
 
+@pytest.mark.parametrize("swap", [False, True])
+def test_store_operands_that_share_memory(on_cpu, swap):
+    n, rows = 2 * 16 * 2 * 64, torch.zeros(4, dtype=torch.int64)          # elements of a cache of two pages
+
+    def call(at_k, at_v, at_first, at_second, rows=rows):
+        """Operands at these elements of one buffer: keys and values are 4 tokens of 2 heads, 512 elements."""
+        buf = torch.zeros(4 * n)
+        k, v = (buf[at:at + 512].view(4, 2, 64) for at in (at_k, at_v))
+        caches = [buf[at:at + n].view(2, 16, 2, 64) for at in (at_first, at_second)]
+        return attention.store_kv(k, v, *(caches[::-1] if swap else caches), rows)
+
+    for k, v, first, second in ((0, 512, 1024, 1024 + n), (0, n + 512, 512, n + 1024), (n, n + 512, 0, n + 1024),
+                                (3 * n, 2 * n, 0, n), (0, 0, 512, 512 + n)):
+        call(k, v, first, second)
+    assert len(on_cpu) == 5
+    for k, v, first, second in ((0, 511, 512, 512 + n), (1022, 0, 1024, 1024 + n), (n - 1, n + 511, 0, n + 1023), (n, n + 512, 0, n + 511),
+                                (2 * n - 1, 3 * n, 0, n), (3 * n, 0, 0, n), (3 * n, 2 * n + 8, 0, n + 16), (3 * n, 3 * n, 0, n - 1)):
+        with pytest.raises(ValueError, match="may not be"):
+            call(k, v, first, second)
+    # Views whose ends cross but whose elements do not: two halves of one cache's heads.
+    both = torch.zeros(2, 16, 4, 64)
+    call_views = lambda k, v: attention.store_kv(k, v, both[:, :, :2], both[:, :, 2:], rows)
+    call_views(torch.zeros(4, 2, 64), torch.zeros(4, 2, 64))
+    with pytest.raises(ValueError, match="k_cache may not be k"):
+        call_views(both[0, :4, :2], torch.zeros(4, 2, 64))
+    with pytest.raises(ValueError, match="v_cache may not be rows"):
+        words = torch.zeros(2 * 16 * 2 * 64)
+        attention.store_kv(torch.zeros(4, 2, 64), torch.zeros(4, 2, 64), torch.zeros(2, 16, 2, 64), words.view(2, 16, 2, 64),
+                           words.view(torch.int64)[-4:])
+
+
 def test_pages_by_hand():
     """The definitions that the device is held to, at sizes worked out by hand."""
     rows, cu, after, taken, tables = att.assign([[7, -1, -1], [-1] * 3, [5, 6, -1]], [15, 0, 32], [3, 2, 1], [0, 0, 0, 9, 4, 2], 3, 16, 7)
