@@ -385,8 +385,9 @@ int pf_attn_exec(const pf_attn_args* args, void* stream);
 /* One new token of each of B sequences, q, o [B,H,D], over its lengths[b] tokens (the new one among them) in a cache
  * k, v [pages,page,G,D].  Sequence b's pages are tables[slots[b]] (tables [S,M] contiguous; slots NULL: tables[b]); entries
  * past its length are not read; a page outside the pool holds no tokens, nor does a slot outside it.  lengths are cut at
- * M * page, at most 2^30.  The walk is shared out over workgroups by the lengths of all B: the same sequence alone and in a
- * batch may differ by rounding.  workspace: pf_attn_step_workspace_bytes (arithmetic; 0: none needed, or not supported),
+ * M * page, at most 2^30.  A value of v that is not finite reaches its own column, as in the formula.  The
+ * walk is shared out over workgroups by the lengths of all B: the same sequence alone and in a batch may differ by rounding.
+ * workspace: pf_attn_step_workspace_bytes (arithmetic; 0: none needed, or not supported),
  * 16-byte aligned, used by the launches of the call only.  q, k, v as above; row strides of k and v up to 2^22 elements. */
 typedef struct pf_attn_step_args {
   size_t size;

@@ -6,7 +6,8 @@
 // of all sequences and heads, in units of 64, are one line of which each workgroup takes an equal run.  A (sequence, head)
 // that ends up in several workgroups leaves partial sums there, which a second kernel joins.  Each wave walks its own 32 keys
 // of a unit, through buffers of its own, the next ones under way to LDS; waves meet only at a segment's end.  With bf16
-// operands the weights enter the second product in two terms of bf16, which costs nothing beside the memory (1 %).
+// operands the weights enter the second product in two terms of bf16, which costs nothing beside the memory (1 %).  Sums that
+// are not finite are made again (step_keys); that they are looked for costs a short call 0.1 to 0.3 us, a long one nothing.
 //
 // Measured, bf16, D = 128: 64 sequences of up to 8192, 4 heads of keys, 504 MB, 99 to 104 us and 4.5 to 5.7 the join (4.6 to 4.8
 // TB/s together; a copy moves 5.05); 1 of 131072, 8 heads, 537 MB, 101 to 105 and 4.8.  Two workgroups of two waves a CU;
@@ -100,12 +101,16 @@ template <typename E, int DP> struct StepLds {
     float o[kStepWaves][16 * (DP + 4)];                      // the waves' sums
   };
   float m[kStepWaves][16], l[kStepWaves][16];
+  int again;                                                 // a sum came out not finite
 };
 
-// The keys [k0, k1) of one (sequence, head, block) by a workgroup; len: the sequence's.
-template <typename E, int DP>
-__device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, DP>& s, const int b, const int g, const int hb,
-                                             const int len, const int k0, const int k1, float* part) {
+// The keys [k0, k1) of one (sequence, head, block) by a workgroup; len: the sequence's.  Returns whether a sum came out not
+// finite.  A value of v that is not finite meets weights that are no token's (0 times it is no number), and the second term of
+// a weight, which may have the other sign (inf - inf): the keys are then walked AGAIN, where keys that are no token's have
+// no values, and the second term no value that is not finite.
+template <typename E, int DP, bool AGAIN>
+__device__ __forceinline__ bool step_keys(const AttnStepArgs& a, StepLds<E, DP>& s, const int b, const int g, const int hb,
+                                          const int len, const int k0, const int k1, float* part) {
   using R = Rows<E, DP>;
   constexpr bool kBf = sizeof(E) == 2;
   constexpr int ES = sizeof(E), KEYS = StepLds<E, DP>::KEYS, KG = KEYS / 16, DT = DP / 16;
@@ -195,6 +200,7 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
     }
   };
 
+  const auto is_token = [&](const Stage& stage, int t, int i) { return stage.ok[t] && stage.j + 16 * t + 4 * gr + i < len; };
   const auto compute = [&](const Stage& stage, int buf) {
     if (!stage.any) return;
     const E* ks = s.k[w][buf];
@@ -217,7 +223,7 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (!stage.ok[t] || stage.j + 16 * t + 4 * gr + i >= len) st[t][i] = -INFINITY;
+        if (!is_token(stage, t, i)) st[t][i] = -INFINITY;
     }
     float top = st[0][0];
 #pragma unroll
@@ -256,12 +262,22 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
     for (int dt = 0; dt < DT; ++dt) {
       if constexpr (kBf) {
         const int row = 4 * gr + (c >> 2), col = 16 * dt + 4 * (c & 3);
-        const bf16x8 f = cat8(lds_read_tr(vs + R::at(row, col)), lds_read_tr(vs + R::at(row + 16, col)));
-        o[dt] = mfma_bf16(f, hi, mfma_bf16(f, lo, o[dt]));
+        bf16x8 f = cat8(lds_read_tr(vs + R::at(row, col)), lds_read_tr(vs + R::at(row + 16, col))), finite = f;
+        if constexpr (AGAIN) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (!is_token(stage, i / 4, i % 4)) f[i] = (bf16)0.f;
+            finite[i] = __builtin_isfinite((float)f[i]) ? f[i] : (bf16)0.f;
+          }
+        }
+        o[dt] = mfma_bf16(f, hi, mfma_bf16(finite, lo, o[dt]));
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vs[R::at(4 * gr + i, 16 * dt + c)], p[0][i], o[dt], 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+          float f = vs[R::at(4 * gr + i, 16 * dt + c)];
+          if (AGAIN && !is_token(stage, 0, i)) f = 0.f;
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(f, p[0][i], o[dt], 0, 0, 0);
+        }
       }
     }
   };
@@ -300,7 +316,9 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
   }
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<floatx4*>(&s.o[w][c * (DP + 4) + 16 * dt + 4 * gr]) = o[dt];
+  if (tid == 0) s.again = 0;
   __syncthreads();
+  float spoilt = 0.f;                                // 0 of finite sums, else NaN
   for (int i = tid; i < heads * (DP / 4); i += 64 * kStepWaves) {
     const int r = i / (DP / 4), col = i % (DP / 4) * 4;
     float up = s.m[0][r];
@@ -314,6 +332,8 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
       sum += *reinterpret_cast<const floatx4*>(&s.o[k][r * (DP + 4) + col]) * f;
       weight += s.l[k][r] * f;
     }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) spoilt = __builtin_fmaf(sum[x], 0.f, spoilt);
     if (part) {
       *reinterpret_cast<floatx4*>(part + r * (DP + 4) + col) = sum;
       if (col == 0) {
@@ -326,7 +346,15 @@ __device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, D
       store_vec<4>(static_cast<E*>(a.o) + b * a.o_b + (g * share + 16 * hb + r) * a.o_h + col, out);
     }
   }
+  if (spoilt != 0.f) s.again = 1;                    // (NaN is unequal)
   __syncthreads();
+  return s.again;                                    // (set to 0 next behind another barrier)
+}
+
+template <typename E, int DP>
+__device__ __forceinline__ void step_segment(const AttnStepArgs& a, StepLds<E, DP>& s, const int b, const int g, const int hb,
+                                             const int len, const int k0, const int k1, float* part) {
+  if (step_keys<E, DP, false>(a, s, b, g, hb, len, k0, k1, part)) step_keys<E, DP, true>(a, s, b, g, hb, len, k0, k1, part);
 }
 
 template <int DP> __device__ __forceinline__ float* part_of(const AttnStepArgs& a, long i) { return a.part + i * 16 * (DP + 4); }

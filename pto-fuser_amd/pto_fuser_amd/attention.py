@@ -184,8 +184,9 @@ def attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
     q [B,H,D] float32 or bfloat16; k_cache, v_cache [pages,page,G,D] in its type, whole 16-byte vectors; D, H and G as in
     :func:`causal_attention`.  Sequence b's pages are ``tables[slots[b]]``; entries past its length are not read, and a page
-    outside the cache holds no tokens.  lengths [B] int32, cut at M · page.  A sequence of no tokens gives zeros.  The keys
-    of all sequences are shared out evenly over the chip, so the same sequence alone and in a batch may differ by rounding.
+    outside the cache holds no tokens.  lengths [B] int32, cut at M · page.  A sequence of no tokens gives zeros.  An infinity
+    or NaN in v reaches its own column, as in the formula; what lies behind a sequence's tokens reaches nothing.  The keys of all
+    sequences are shared out evenly over the chip, so the same sequence alone and in a batch may differ by rounding.
     Returns o [B,H,D] in q's type."""
     dev = _device_of(q, "q")
     _dim(q, "q", 3, "[B,H,D]")
