@@ -443,6 +443,20 @@ typedef struct pf_release_args {
 } pf_release_args;
 int pf_release_exec(const pf_release_args* args, void* stream);
 
+/* For attention over the new tokens of a plan of pf_assign_exec alone (cu, lengths, rows: what it wrote, N its capacity), which is
+ * wrong for requests that held tokens before: the first of k's [N,G,D] new keys of each such request becomes NaN, in every head, so
+ * that all rows of it come out as NaN.  Other requests' keys stay as they are. */
+typedef struct pf_refuse_args {
+  size_t size;
+  const int* cu;
+  const int* lengths;
+  const long long* rows;
+  void* k;
+  long long k_t, k_h;
+  int N, B, G, dtype;
+} pf_refuse_args;
+int pf_refuse_exec(const pf_refuse_args* args, void* stream);
+
 /* k, v [N,G,D] into rows[t] of k_cache, v_cache [pages,page,G,D]; a row outside the cache is skipped, no two may be the same.
  * D a multiple of 8 up to 65536; addresses need an element's alignment. */
 typedef struct pf_store_args {

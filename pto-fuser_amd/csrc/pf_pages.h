@@ -187,6 +187,26 @@ __global__ __launch_bounds__(256) void release_kernel(ReleaseArgs a) {
   for (uint32_t i = tid; i < n; i += 256) a.free[taken - 1 - before - i] = row[i];
 }
 
+struct RefuseArgs {
+  const int* cu;           // [B + 1]
+  const int* lengths;      // [B]: after the plan
+  const long long* rows;   // [N]
+  void* k;
+  long k_t, k_h;
+  int N, B, G;
+};
+
+// A request held tokens before a plan where more are in the cache after it than the plan brought: all its new ones if its
+// first has a row, else none.  Its first new key becomes NaN, in every head, which reaches each of its rows.
+template <typename E>
+__global__ __launch_bounds__(256) void refuse_kernel(RefuseArgs a) {
+  const long b = block_id() * 256 + threadIdx.x;
+  if (b >= a.B) return;
+  const int first = a.cu[b], end = a.cu[b + 1];
+  if (first < 0 || first >= min(end, a.N) || a.lengths[b] <= (a.rows[first] >= 0 ? end - first : 0)) return;
+  for (int g = 0; g < a.G; ++g) static_cast<E*>(a.k)[first * a.k_t + g * a.k_h] = from_f32<E>(__builtin_nanf(""));
+}
+
 struct StoreArgs {
   const void* k;
   const void* v;

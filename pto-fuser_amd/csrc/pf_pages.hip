@@ -58,6 +58,23 @@ int pf_release_exec(const pf_release_args* p, void* stream) {
   return scope.status();
 }
 
+int pf_refuse_exec(const pf_refuse_args* p, void* stream) {
+  if (!p || p->size != sizeof *p || (p->dtype != PF_DTYPE_F32 && p->dtype != PF_DTYPE_BF16)) return PF_ERR_ARG;
+  if (p->N < 0 || p->B < 0 || p->B == 0x7fffffff || p->G <= 0 || p->G > 65536 || p->k_t < 0 || p->k_h < 0) return PF_ERR_ARG;
+  if (p->N == 0 || p->B == 0) return PF_OK;
+  if (!p->cu || !p->lengths || !p->rows || !p->k) return PF_ERR_ARG;
+  pf::RefuseArgs a{};
+  a.cu = p->cu; a.lengths = p->lengths; a.rows = p->rows; a.k = p->k; a.k_t = p->k_t; a.k_h = p->k_h;
+  a.N = p->N; a.B = p->B; a.G = p->G;
+  dim3 grid;
+  if (!grid_of(((double)a.B + 255) / 256, grid)) return PF_ERR_ARG;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  pf::LaunchScope scope;
+  if (p->dtype == PF_DTYPE_BF16) pf::refuse_kernel<bf16><<<grid, 256, 0, s>>>(a);
+  else pf::refuse_kernel<float><<<grid, 256, 0, s>>>(a);
+  return scope.status();
+}
+
 int pf_store_exec(const pf_store_args* p, void* stream) {
   if (!p || p->size != sizeof *p || log2_of(p->page) < 0 || (p->dtype != PF_DTYPE_F32 && p->dtype != PF_DTYPE_BF16)) return PF_ERR_ARG;
   if (p->N < 0 || p->G <= 0 || p->G > 65536 || p->D <= 0 || p->D > 65536 || p->D % 8 || p->pages < 0) return PF_ERR_ARG;

@@ -71,6 +71,7 @@ SIGNATURES = {
     "pf_attn_step_exec": (c_int, [c_void_p, c_void_p]),
     "pf_assign_exec": (c_int, [c_void_p, c_void_p]),
     "pf_release_exec": (c_int, [c_void_p, c_void_p]),
+    "pf_refuse_exec": (c_int, [c_void_p, c_void_p]),
     "pf_store_exec": (c_int, [c_void_p, c_void_p]),
 }
 

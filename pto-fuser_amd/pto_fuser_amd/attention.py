@@ -29,9 +29,10 @@ _ATTN = struct.Struct("@N6P8q7if")
 _ATTN_STEP = struct.Struct("@N8PN10q9if")
 _ASSIGN = struct.Struct("@N10P6i")
 _RELEASE = struct.Struct("@N6P5i")
+_REFUSE = struct.Struct("@N4P2q4i")
 _STORE = struct.Struct("@N5P10q6i")
-_ATTN_SIZE, _ATTN_STEP_SIZE, _ASSIGN_SIZE, _RELEASE_SIZE, _STORE_SIZE = (
-    _size(s) for s in (_ATTN, _ATTN_STEP, _ASSIGN, _RELEASE, _STORE))
+_ATTN_SIZE, _ATTN_STEP_SIZE, _ASSIGN_SIZE, _RELEASE_SIZE, _REFUSE_SIZE, _STORE_SIZE = (
+    _size(s) for s in (_ATTN, _ATTN_STEP, _ASSIGN, _RELEASE, _REFUSE, _STORE))
 
 HEAD_MAX = 256
 ROW_MAX_STRIDE = 1 << 22
@@ -289,6 +290,36 @@ def release_pages(tables: torch.Tensor, lengths: torch.Tensor, free: torch.Tenso
     _exec("pf_release_exec", dev, _RELEASE, _RELEASE_SIZE, tables.data_ptr(), lengths.data_ptr(), _ptr(slots),
           free.data_ptr(), taken.data_ptr(), after.data_ptr(), B, S, M, F, page_size)
     return after
+
+
+def _outside(at: int, size: int, other: int, other_size: int) -> bool:
+    return other + other_size <= at or at + size <= other
+
+
+def refuse_held(k: torch.Tensor, plan: PagePlan) -> None:
+    """Makes attention over a plan's new tokens alone give NaN for requests that held tokens before it, which those tokens would
+    have to see: their first key in k [N,G,D], N the plan's capacity, becomes NaN (in place; k is stored before).  Nothing on
+    the host knows which those are."""
+    dev = _device_of(k, "k")
+    _dim(k, "k", 3, "[N,G,D]")
+    N, G, D = k.shape
+    code = _dtype_code(k.dtype)
+    if not 0 < G <= 65536 or D == 0:
+        raise ValueError(f"unsupported shape G={G} D={D} (G up to 65536)")
+    _require_view(k, "k", (N, G, D), k.dtype, dev)
+    rows, cu, lengths = plan.rows, plan.cu_seqlens, plan.lengths
+    _dim(lengths, "lengths", 1, "[B]")
+    B = lengths.shape[0]
+    _needed(rows, "rows", (N,), torch.int64, dev)
+    _needed(cu, "cu_seqlens", (B + 1,), torch.int32, dev)
+    _needed(lengths, "lengths", (B,), torch.int32, dev)
+    at, at_rows, at_cu, at_lengths, (st, sh) = k.data_ptr(), rows.data_ptr(), cu.data_ptr(), lengths.data_ptr(), k.stride()[:2]
+    span = ((N - 1) * st + (G - 1) * sh + D) * k.element_size()
+    # (by their ends where those say enough, as in store_kv: 4 us less of the host)
+    if not (0 < D <= sh and (G - 1) * sh + D <= st and _outside(at, span, at_rows, 8 * N) and _outside(at, span, at_cu, 4 * B + 4)
+            and _outside(at, span, at_lengths, 4 * B)):
+        _apart("k", k, rows=rows, cu_seqlens=cu, lengths=lengths)
+    _exec("pf_refuse_exec", dev, _REFUSE, _REFUSE_SIZE, at_cu, at_lengths, at_rows, at, st, sh, N, B, G, code)
 
 
 def _caches_clear(k_cache, v_cache, held: int, others) -> bool:

@@ -19,7 +19,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ..attention import PagePlan, attention_step, causal_attention, store_kv
+from ..attention import PagePlan, attention_step, causal_attention, refuse_held, store_kv
 from ..ops import gdn_chunk_forward
 from ..serving import (add_rms_norm, add_rms_norm_fp8, causal_conv, causal_conv_step, gdn_step, ssm_chunk_forward,
                        ssm_step)
@@ -207,10 +207,12 @@ class AttentionLayer:
                 plan: PagePlan) -> Tuple[torch.Tensor, torch.Tensor]:
         """Whole prompts, packed, of requests that the cache held nothing of: hidden, residual [N,D] with N the plan's
         capacity -> (output [N,D], the residual stream).  Their keys and values go to the plan's rows; a prompt that it did
-        not serve is computed and not stored."""
+        not serve is computed and not stored.  New tokens of a request that the cache held some of are not attended with those:
+        their output is NaN."""
         y, stream = add_rms_norm(hidden, self.norm_w, residual)
         q, k, v = self._operands(y)
         store_kv(k, v, cache.k, cache.v, plan.rows)
+        refuse_held(k, plan)
         out = self._project(causal_attention(q, k, v, plan.cu_seqlens))
         return out, hidden if stream is None else stream
 
