@@ -91,14 +91,28 @@ struct StepPlan {
   size_t parts, bytes;
 };
 
-bool step_plan(int B, int H, int G, int D, int M, int page, StepPlan& p) {
+// Whether the walk is shared out, by what the host knows: the tables' width in tokens, and the rows, (sequence, head, block).
+// Whole rows need no second kernel, so they are faster where a row is a few steps; from there on a row is a chain of steps that
+// sharing cuts, while rows are few.  us as nodes of a graph, a workgroup a row / shared, rows x tokens, all of them in use:
+//   bf16, D = 128: 4 x 128 6.3 / 8.9, 4 x 256 8.9 / 9.0, 4 x 512 14.3 / 9.1, 64 x 512 14.9 / 11.8, 128 x 512 15.6 / 15.6, 256 x 512 16.6 / 19.9
+//   bf16, D = 64:  4 x 256 7.2 / 8.2, 4 x 512 11.5 / 8.4, 128 x 512 12.2 / 11.9, 256 x 512 12.9 / 14.8 (uneven lengths 11.8 / 11.2)
+//   bf16, D = 256: 4 x 256 12.7 / 10.4, 4 x 512 20.8 / 10.8, 64 x 512 21.7 / 16.5, 128 x 512 22.4 / 21.9, 256 x 512 26.4 / 32.0
+//   fp32, D = 64:  4 x 128 8.0 / 9.8, 4 x 256 12.9 / 9.8, 128 x 256 13.5 / 13.3, 256 x 256 14.1 / 15.7, 256 x 512 24.6 / 21.6
+//   fp32, D = 128: 4 x 128 12.4 / 12.7, 4 x 256 20.9 / 12.7, 128 x 256 21.6 / 17.9, 128 x 512 38.7 / 24.0, 256 x 512 40.0 / 35.7
+// Past 512 tokens hundreds of even rows are 2 to 16 % faster whole (512 x 2048, bf16, D = 128: 98.5 / 103.4), few rows up to
+// ten times slower (4 x 2048 45.4 / 9.4), and one long row among many short ones alone takes as long as it does whole: shared.
+bool step_shares(double rows, double tokens, double wgs, int dtype) {
+  return tokens > 512 || (tokens > (dtype == PF_DTYPE_BF16 ? 256 : 128) && rows * 4 <= wgs);
+}
+
+bool step_plan(int B, int H, int G, int D, int M, int page, int dtype, StepPlan& p) {
   p.blocks = (H / G + 15) / 16;
   const double rows = (double)B * G * p.blocks, tokens = (double)M * page;
   const double units = rows * ((tokens + pf::kStepUnit - 1) / pf::kStepUnit + 1);
   if (tokens > kMaxRows || units > kMaxRows) return false;       // (a run's end stays an int)
   p.rows = (int)rows;
   const double wgs = (double)kStepWgs * 128 / padded(D);
-  p.wgs = tokens <= 512 ? 0 : (int)(units < wgs ? units : wgs);
+  p.wgs = step_shares(rows, tokens, wgs, dtype) ? (int)(units < wgs ? units : wgs) : 0;
   p.parts = (size_t)p.wgs * 2 * 16 * (padded(D) + 4);
   p.bytes = p.wgs ? p.parts * sizeof(float) + (size_t)p.rows * 4 * sizeof(int) : 0;
   return true;
@@ -147,7 +161,7 @@ int pf_attn_exec(const pf_attn_args* p, void* stream) {
 
 size_t pf_attn_step_workspace_bytes(int B, int H, int G, int D, int M, int page, int dtype) {
   StepPlan pl;
-  if (B <= 0 || M < 0 || !heads_ok(H, G, D, dtype) || log2_of(page) < 0 || !step_plan(B, H, G, D, M, page, pl)) return 0;
+  if (B <= 0 || M < 0 || !heads_ok(H, G, D, dtype) || log2_of(page) < 0 || !step_plan(B, H, G, D, M, page, dtype, pl)) return 0;
   return pl.bytes;
 }
 
@@ -155,7 +169,7 @@ int pf_attn_step_exec(const pf_attn_step_args* p, void* stream) {
   if (!p || p->size != sizeof *p || !heads_ok(p->H, p->G, p->D, p->dtype) || log2_of(p->page) < 0) return PF_ERR_ARG;
   if (p->B < 0 || p->S < 0 || p->M < 0 || p->pages < 0 || !(p->scale > 0.f) || (!p->slots && p->B > p->S)) return PF_ERR_ARG;
   StepPlan pl;
-  if (!step_plan(p->B, p->H, p->G, p->D, p->M, p->page, pl)) return PF_ERR_ARG;
+  if (!step_plan(p->B, p->H, p->G, p->D, p->M, p->page, p->dtype, pl)) return PF_ERR_ARG;
   if (p->B == 0) return PF_OK;
   if (!p->q || !p->o || !p->lengths || (p->pages > 0 && (!p->k || !p->v)) || (!p->tables && p->S > 0 && p->M > 0)) return PF_ERR_ARG;
   if (!vectors(p->dtype, p->q, p->q_b, p->q_h) || !vectors(p->dtype, p->k, p->k_p, p->k_r, p->k_h) ||

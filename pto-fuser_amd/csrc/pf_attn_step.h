@@ -12,8 +12,7 @@
 // Measured, bf16, D = 128: 64 sequences of up to 8192, 4 heads of keys, 504 MB, 99 to 104 us and 4.5 to 5.7 the join (4.6 to 4.8
 // TB/s together; a copy moves 5.05); 1 of 131072, 8 heads, 537 MB, 101 to 105 and 4.8.  Two workgroups of two waves a CU;
 // one of four: 114 and 130.  A short call is a chain of latencies: 1 of 512 tokens 6.4 us and 2.9 us the join, and 13.4 us
-// in one workgroup a head.  Whole rows without the join are faster where there are hundreds of even length (64 x 2048: 51 for 59 us)
-// and take twice the time where one is long, which the host cannot know.
+// in one workgroup a head.  When a walk is shared out: step_shares in pf_attn.hip.
 #pragma once
 
 #include "pf_attn.h"
