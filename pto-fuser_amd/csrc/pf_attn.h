@@ -13,13 +13,14 @@
 // rounding of 2^-9 to 2^-8 each: the output is 2.0e-3 of its norm off, 1.7e-3 by its own rounding alone).  A second term for
 // them would cost half of that product again, which bounds the kernel; single tokens have it (pf_attn_step.h).
 //
-// Measured, bf16, D = 128: 1 prompt of 32768, 32 heads over 8 of keys, 7.57 to 7.72 ms, 1140 to 1160 TFLOP/s; the library's
+// Measured, bf16, D = 128: 1 prompt of 32768, 32 heads over 8 of keys, 7.57 to 8.12 ms by machine, 1085 to 1160 TFLOP/s; the library's
 // product of 8192^3 reaches 1213 to 1224 on the same card.  Under it the shader clock falls to 1.6 GHz (12.3 million cycles a
 // pass), of which the matrix pipes work 8.4 million, the vector port 7.4; L2 answers 96 % of the tiles.  4 x 4096 x 16 heads
-// 262 to 270 us (1020 to 1050 TFLOP/s): the diagonal's tiles and each workgroup's start and end.  D = 64: 2.2 ms for 1 x 32768 x
+// 262 to 281 us (980 to 1050 TFLOP/s): the diagonal's tiles and each workgroup's start and end.  D = 64: 2.2 ms for 1 x 32768 x
 // 16, 1000 TFLOP/s: the vector port, with as many weights to half the products.  fp32, D = 128: 1.13 ms for 2 x 4096 x 16, 121 of
-// the library's 154 TFLOP/s.  D = 256, a wave a SIMD (492 registers): bf16 700 TFLOP/s, fp32 100.  Tried on the way (4 x 4096 x 16, us): one wave a SIMD 603, two 297, loads in flight past the
-// compiler's waits 274, tiles of 32 keys and three waves 262; the diagonal's second half left out by a branch (spills, 310),
+// the library's 154 TFLOP/s.  D = 256, a wave a SIMD (492 registers; fp32 512 and 36 spilled): bf16 610 TFLOP/s for 1 x 4096 x 16,
+// 630 for 4 x 4096, 705 for 1 x 32768, fp32 103 to 107.  Tried on the way (4 x 4096 x 16, us): one wave a SIMD 603, two 297, loads
+// in flight past the compiler's waits 274, tiles of 32 keys and three waves (168 registers, 9 spilled) 262; the diagonal's second half left out by a branch (spills, 310),
 // the weights' sum by dot products of bf16 pairs (no gain), 128 rows of one head a workgroup instead of 32 of four (the
 // same here, 48 prompts of up to 512 tokens 48 to 43).
 #pragma once
@@ -338,8 +339,9 @@ __device__ __forceinline__ bool attn_walk(const AttnArgs& a, AttnLds<E, DP, KW>&
   const auto work = [&](const int jw, const E* ks, const E* vs, auto k_read, auto v_next, auto v_read) {
     int row0 = 32 * kw;
     if constexpr (!kBf && DP == 256) __asm__ __volatile__("" : "+v"(row0));     // (places in LDS made anew: kept, they would spill)
-    // Where a wave or two share a SIMD nobody else hides LDS: the operands are asked for AHEAD of the products, those of V
-    // before the weights.  Three waves hide it for each other, and have no registers for that.
+    // With bf16 the operands are asked for AHEAD of the products, those of V before the weights, where registers allow it: at
+    // D = 64, and at D = 128 where two waves share rows.  Else at D = 128 three waves a SIMD hide LDS for each other and
+    // have no registers for that.  Past 128 columns it is not done (nor tried), nor with fp32, whose products outlast LDS.
     constexpr bool AHEAD = kBf && DP <= 128 && (KW > 1 || DP == 64);
     const auto k_at = [&](int kb) {
       const int col = (kb * 2 + hf) * R::V;

@@ -7,7 +7,8 @@
 //
 // Latency, not bytes: 64 prompts of up to 1024 tokens 4.4 us, 256 requests of a token each 3.4 us (a launch of nothing takes 2.4);
 // as one workgroup and a second launch for the rows they took 9.4 and 7.3.  Storing: 16384 tokens of 4 heads of 128, 67 MB
-// 11.4 us, 5.9 TB/s (what the last pass wrote is partly still in the memory-side cache).
+// 11.4 us, 5.9 TB/s (what the last pass wrote is partly still in the memory-side cache).  Marking requests that held tokens: 1.4 us
+// for 64.
 #pragma once
 
 #include "pf_serving.h"

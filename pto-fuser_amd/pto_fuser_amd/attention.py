@@ -4,6 +4,7 @@
 * :func:`attention_step` — one new token of each running sequence over a cache of keys and values in pages.
 * :func:`assign_pages`, :func:`release_pages` — which pages of the cache new tokens take and which row each has, and back.
 * :func:`store_kv` — keys and values into those rows.
+* :func:`refuse_held` — marks the requests of a plan for which attention over its new tokens alone would be wrong.
 
 No counterpart in the reference.  Forward only.  As in ``serving``: operands may be views whose innermost dimension is
 contiguous, every operator raises ``ValueError`` before launching for what it does not support, works on the current stream of

@@ -218,7 +218,8 @@ class AttentionLayer:
 
     def step(self, hidden: torch.Tensor, residual: Optional[torch.Tensor], cache: KvCache, plan: PagePlan,
              tables: torch.Tensor, slots: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-        """One token of each sequence: hidden, residual [B,D]; ``slots`` names the sequences' tables."""
+        """One token of each sequence: hidden, residual [B,D]; ``slots`` names the sequences' tables.  A token that the plan gave
+        no row is not stored and sees only those that the cache held."""
         y, stream = add_rms_norm(hidden, self.norm_w, residual)
         q, k, v = self._operands(y)
         store_kv(k, v, cache.k, cache.v, plan.rows)
